@@ -18,7 +18,8 @@ from ._lib import HKError, call, lib  # noqa: F401
 __all__ = [
     "HKError", "gelu_forward", "gelu_backward", "layer_norm_forward", "ln_backward_input",
     "ln_backward_gamma_beta", "layer_norm_backward", "sparse_ce_forward", "sparse_ce_backward",
-    "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "ReductionLayout",
+    "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "Adam8Plan", "ADAM8_BLOCK",
+    "adam8_states", "adam8_quantize", "adam8_dequantize", "ReductionLayout",
     "unified_reduce_sum", "reduce_generic", "REDUCE_INNER", "REDUCE_OUTER", "REDUCE_GENERIC",
 ]
 
@@ -263,6 +264,117 @@ class AdamPlan:
     def close(self):
         if self._plan:
             call("hk_adam_plan_destroy", self._plan)
+            self._plan = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ----------------------------------------------------------------------------------------------
+# Multi-tensor AdamW with both moments in 8 bits (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+ADAM8_BLOCK = 256
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HK_TYPE_*
+
+
+def _here(fn: str, *ts: torch.Tensor | None) -> None:
+    """Device tensors of the current device, whose stream the launch goes to."""
+    cur = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.get_device() != cur:
+            raise ValueError(f"{fn}: tensors of the current device (cuda:{cur}) only")
+
+
+def _adam8_check(fn: str, m, v, m_scale, v_scale, blocks: int) -> None:
+    _dev(m, v, m_scale, v_scale)
+    _here(fn, m, v, m_scale, v_scale)
+    if m.dtype != torch.int8 or v.dtype != torch.uint8 or m_scale.dtype != torch.float32 or (
+            v_scale.dtype != torch.float32):
+        raise ValueError(f"{fn}: m int8, v uint8, m_scale and v_scale fp32")
+    if m.numel() != blocks * ADAM8_BLOCK or v.numel() != m.numel() or not (
+            m_scale.numel() == v_scale.numel() == blocks):
+        raise ValueError(f"{fn}: {blocks} blocks need {blocks * ADAM8_BLOCK} codes and {blocks} "
+                         "scales of each moment")
+
+
+def adam8_states(sizes: Sequence[int], device="cuda"):
+    """(m, v, m_scale, v_scale), moments of zero for tensors of these sizes: the codes of all tensors
+    one behind the other, each tensor from a block's first element on."""
+    blocks = sum(-(-int(n) // ADAM8_BLOCK) for n in sizes)
+    z = lambda n, dt: torch.zeros(n, device=device, dtype=dt)  # noqa: E731
+    return (z(blocks * ADAM8_BLOCK, torch.int8), z(blocks * ADAM8_BLOCK, torch.uint8),
+            z(blocks, torch.float32), z(blocks, torch.float32))
+
+
+def adam8_quantize(m, v, states=None):
+    """8-bit states (m, v, m_scale, v_scale) of fp32 moments of one tensor (or of several that each
+    begin on a block)."""
+    _dev(m, v)
+    _here("adam8_quantize", m, v)
+    if m.dtype != torch.float32 or v.dtype != torch.float32 or m.numel() != v.numel():
+        raise ValueError("adam8_quantize: fp32 moments of equal size")
+    states = adam8_states([m.numel()], m.device) if states is None else states
+    _adam8_check("adam8_quantize", *states, -(-m.numel() // ADAM8_BLOCK))
+    call("hk_adam8_quantize", _ptr(m), _ptr(v), m.numel(), *map(_ptr, states), _stream())
+    return tuple(states)
+
+
+def adam8_dequantize(m, v, m_scale, v_scale, m_out=None, v_out=None):
+    """The fp32 moments (m, v) that 8-bit states stand for, of all their elements or of as many as
+    m_out and v_out hold."""
+    n = m.numel() if m_out is None else m_out.numel()
+    _adam8_check("adam8_dequantize", m, v, m_scale, v_scale, -(-n // ADAM8_BLOCK))
+    m_out = torch.empty(n, device=m.device, dtype=torch.float32) if m_out is None else m_out
+    v_out = torch.empty(n, device=m.device, dtype=torch.float32) if v_out is None else v_out
+    _dev(m_out, v_out)
+    _here("adam8_dequantize", m_out, v_out)
+    if m_out.dtype != torch.float32 or v_out.dtype != torch.float32 or v_out.numel() != n:
+        raise ValueError("adam8_dequantize: fp32 outputs of equal size")
+    call("hk_adam8_dequantize", _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), n, _ptr(m_out),
+         _ptr(v_out), _stream())
+    return m_out, v_out
+
+
+class Adam8Plan:
+    """AdamPlan with both moments in 8 bits: fp32 parameters, gradients of one type (fp32, bf16 or
+    fp16), states as adam8_states lays them out, and optionally bf16 copies of the updated parameters
+    (one tensor or None for each)."""
+
+    def __init__(self, params, grads, m, v, m_scale, v_scale, copies=None):
+        n = len(params)
+        copies = [None] * n if copies is None else list(copies)
+        if not (n == len(grads) == len(copies)):
+            raise ValueError("Adam8Plan: equal list lengths")
+        types = {g.dtype for g in grads} or {torch.float32}
+        if len(types) != 1 or not types <= set(_TYPE):
+            raise ValueError("Adam8Plan: the gradients share one type (fp32, bf16 or fp16)")
+        for p, g, c in zip(params, grads, copies):
+            _dev(p, g, c)
+            _here("Adam8Plan", p, g, c)
+            if p.dtype != torch.float32 or g.numel() != p.numel():
+                raise ValueError("Adam8Plan: fp32 parameters, gradients of equal size")
+            if c is not None and (c.dtype != torch.bfloat16 or c.numel() != p.numel()):
+                raise ValueError("Adam8Plan: copies are bf16 of the parameters' size")
+        _adam8_check("Adam8Plan", m, v, m_scale, v_scale,
+                     sum(-(-p.numel() // ADAM8_BLOCK) for p in params))
+        arr = lambda ts: (ctypes.c_void_p * n)(*[_ptr(t) for t in ts])  # noqa: E731
+        self._keep = (list(params), list(grads), copies, m, v, m_scale, v_scale)
+        sizes = (ctypes.c_int64 * n)(*[p.numel() for p in params])
+        self._plan = ctypes.c_void_p()
+        call("hk_adam8_plan_create", n, arr(params), arr(grads), _TYPE[types.pop()], arr(copies),
+             sizes, _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), ctypes.byref(self._plan))
+        self.num_blocks = lib().hk_adam8_plan_num_blocks(self._plan)
+
+    def step(self, lr, beta1, beta2, eps, weight_decay, bias_correction1, bias_correction2):
+        call("hk_adam8_plan_step", self._plan, lr, beta1, beta2, eps, weight_decay,
+             bias_correction1, bias_correction2, _stream())
+
+    def close(self):
+        if self._plan:
+            call("hk_adam8_plan_destroy", self._plan)
             self._plan = ctypes.c_void_p()
 
     def __del__(self):

@@ -221,6 +221,53 @@ HK_API hipError_t hk_adam_plan_destroy(hk_adam_plan* plan);
 HK_API int64_t hk_adam_plan_num_chunks(const hk_adam_plan* plan);
 
 /* ------------------------------------------------------------------------------------------
+ * Multi-tensor AdamW with both moments in 8 bits. No counterpart in the reference. The update is
+ * hk_adam_plan_step's, on moments that are kept in blocks of HK_ADAM8_BLOCK elements of one tensor,
+ * each block with one fp32 scale per moment, each element with one code per moment:
+ *   m = m_scale c |c| / 127^2 (c = -127 .. 127),  v = v_scale (c / 255)^4 (c = 0 .. 255).
+ * A step reads the moments, applies the step's gradient, updates the parameter from the moments as
+ * they are then, and rounds them to codes: the scale is the block's largest |m| (v) in fp32, the code
+ * the one whose value is nearest (of two equally near the larger; a v > 0 keeps code 1 at least).
+ * Codes of zero with scales of zero are moments of zero, so cleared memory starts a run.
+ * hk_adam8_plan_create: host arrays of num_tensors device pointers, as for hk_adam_plan_create;
+ *   grad_type HK_TYPE_* is the gradients' element type. copies may be NULL, and so may each of its
+ *   elements: otherwise the updated parameter is stored there in bf16 too (rounded to nearest even).
+ *   The states of all tensors lie one behind the other, each tensor from a block's first element on:
+ *   tensor t has ceil(sizes[t] / HK_ADAM8_BLOCK) blocks behind those of the tensors before it.
+ *   m_codes and v_codes hold HK_ADAM8_BLOCK bytes a block, m_scales and v_scales one float a block
+ *   (hk_adam8_plan_num_blocks gives the count); codes behind a tensor's end are written as 0.
+ *   Parameters and gradients may have any alignment of their element type, the codes need 4 bytes.
+ * hk_adam8_plan_step: on the device that was current at creation; steps of plans that share memory
+ *   have to be ordered. It takes no workspace and can be captured into a graph.
+ * A gradient that is not finite, or a moment past fp32, leaves the block's scales NaN, and with them
+ *   all its moments from then on (the step's parameters: those of the elements themselves).
+ * hk_adam8_quantize / hk_adam8_dequantize convert between fp32 moments and these states (a 32-bit run
+ *   that goes on in 8 bits, a checkpoint): numel elements of whole blocks, but for the last one. v is
+ *   taken as 0 where it is negative.
+ * ---------------------------------------------------------------------------------------- */
+#define HK_TYPE_F32 0
+#define HK_TYPE_BF16 1
+#define HK_TYPE_F16 2
+#define HK_ADAM8_BLOCK 256
+typedef struct hk_adam8_plan hk_adam8_plan;
+HK_API hipError_t hk_adam8_plan_create(int num_tensors, float* const* params,
+                                       const void* const* grads, int grad_type,
+                                       hk_bf16* const* copies, const int64_t* sizes,
+                                       int8_t* m_codes, uint8_t* v_codes, float* m_scales,
+                                       float* v_scales, hk_adam8_plan** plan_out);
+HK_API hipError_t hk_adam8_plan_step(const hk_adam8_plan* plan, float lr, float beta1, float beta2,
+                                     float eps, float weight_decay, float bias_correction1,
+                                     float bias_correction2, hipStream_t stream);
+HK_API hipError_t hk_adam8_plan_destroy(hk_adam8_plan* plan);
+HK_API int64_t hk_adam8_plan_num_blocks(const hk_adam8_plan* plan);
+HK_API hipError_t hk_adam8_quantize(const float* m, const float* v, int64_t numel, int8_t* m_codes,
+                                    uint8_t* v_codes, float* m_scales, float* v_scales,
+                                    hipStream_t stream);
+HK_API hipError_t hk_adam8_dequantize(const int8_t* m_codes, const uint8_t* v_codes,
+                                      const float* m_scales, const float* v_scales, int64_t numel,
+                                      float* m, float* v, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Unified sum reduction, fp32 in / fp32 out.
  * Replaces detail::ReductionLayout + build_reduce_config + launch_reduce_kernel
  *   (kernels/reduction/unified_reduce_standalone.cu:46-56, 151-221, 702-804).
