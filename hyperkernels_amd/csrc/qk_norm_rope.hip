@@ -1,0 +1,495 @@
+// qk_norm_rope.hip - RMS norm of each query and key head with the position rotation, in one pass.
+//
+// Per token and head, x its head_dim elements:
+//   n = x r, r = (mean(x^2) + eps)^(-1/2),  z = n w,  y = z with pair i of its first rotary_dim elements
+//   (z_i, z_{i + rotary_dim / 2}), or (z_2i, z_2i+1) where interleaved, turned by the angle of the
+//   token's position: (a cos - b sin, b cos + a sin).
+// Backward, from dy: g = dy turned back by the same angles, and
+//   dw = sum over tokens and heads of g n,   dx = r (g w - n mean(g w n)).
+// All arithmetic is fp32, with one rounding where an output has 16 bits. r is not kept between the
+// passes: the backward pass reads x anyway and forms it again.
+//
+// Bound: HBM, each row read once and written once (the table's rows and w are shared by the heads of a
+// token and come from the caches). A row is held by 2^k lanes, each with a unit of V pairs: the two
+// vectors of V elements that its rotation combines sit in one lane, so the only exchange between
+// lanes is the sum of squares (and of g w n), a register butterfly over the row's lanes. Vectors are
+// 16 bytes where head_dim and rotary_dim allow (multiples of 2 V elements), at any element alignment.
+// Rows go to lane groups token by token, heads innermost, so that the groups of a wave read the same
+// table rows. Elements behind rotary_dim are units of two neighbouring vectors with an angle of zero.
+//
+// The gradients of the two weight vectors are summed in registers over the rows of a lane group, over
+// a workgroup through LDS, and over the workgroups by a second kernel, all in a fixed order.
+#include "hk_device.h"
+#include "hk_host.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / HK_WAVE;
+constexpr int kMaxDim = 256;
+// Workgroups of the backward pass for queries (and for keys): each leaves one row of partial sums.
+constexpr int kMostPartials = 1024;
+constexpr int kRowsPerGroup = 4;  // rows that a lane group of the backward pass takes at least
+
+// Vectors of V elements at any alignment of the element type.
+template <typename S, int V>
+__device__ __forceinline__ void load_vec(const S* p, S (&f)[V]) {
+  __builtin_memcpy(f, p, V * sizeof(S));
+}
+template <typename S, int V>
+__device__ __forceinline__ void store_vec(S* p, const S (&f)[V]) {
+  __builtin_memcpy(p, f, V * sizeof(S));
+}
+template <class F, int V>
+__device__ __forceinline__ void load_f32(const typename F::storage* p, float (&f)[V]) {
+  typename F::storage s[V];
+  load_vec(p, s);
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] = F::load(s, e);
+}
+template <class F, int V>
+__device__ __forceinline__ void store_f32(typename F::storage* p, const float (&f)[V]) {
+  typename F::storage s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) F::store(s, e, f[e]);
+  store_vec(p, s);
+}
+
+struct Shape {
+  int d, rot, half, units, lanes;  // half: rot / 2; lanes: of a row, a power of two
+  bool interleaved;
+};
+
+// Where the two vectors of unit u lie in a row, and whether the second exists (a head of odd size,
+// V == 1).
+template <int V>
+struct Unit {
+  int a, b, angle;  // angle: first pair of the table row, -1: not rotated
+  bool on, pairs;   // pairs: neighbouring elements are rotated together
+  __device__ Unit(const Shape& s, int u) {
+    const int rotated = s.half / V;
+    on = u < s.units;
+    pairs = u < rotated && s.interleaved;
+    angle = u < rotated ? u * V : -1;
+    if (u < rotated) {
+      a = s.interleaved ? 2 * u * V : u * V;
+      b = s.interleaved ? a + V : s.half + u * V;
+    } else {
+      a = 2 * u * V;  // rot is 2 V rotated
+      b = a + V;
+    }
+  }
+};
+
+// x as the pairs (a[j], b[j]) of a unit.
+template <class F, int V>
+__device__ __forceinline__ void load_unit(const typename F::storage* row, const Unit<V>& u, int d,
+                                          float (&a)[V], float (&b)[V]) {
+  load_f32<F, V>(row + u.a, a);
+  if (V > 1 || u.b < d) {
+    load_f32<F, V>(row + u.b, b);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) b[e] = 0.f;
+  }
+  if (V > 1 && u.pairs) {
+    float t[2 * V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[e] = a[e], t[V + e] = b[e];
+#pragma unroll
+    for (int e = 0; e < V; ++e) a[e] = t[2 * e], b[e] = t[2 * e + 1];
+  }
+}
+template <class F, int V>
+__device__ __forceinline__ void store_unit(typename F::storage* row, const Unit<V>& u, int d,
+                                           const float (&a)[V], const float (&b)[V]) {
+  if (V > 1 && u.pairs) {
+    float t[2 * V], lo[V], hi[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[2 * e] = a[e], t[2 * e + 1] = b[e];
+#pragma unroll
+    for (int e = 0; e < V; ++e) lo[e] = t[e], hi[e] = t[V + e];
+    store_f32<F, V>(row + u.a, lo);
+    store_f32<F, V>(row + u.b, hi);
+  } else {
+    store_f32<F, V>(row + u.a, a);
+    if (V > 1 || u.b < d) store_f32<F, V>(row + u.b, b);
+  }
+}
+
+// Sum over the `lanes` lanes of a row (a power of two, aligned groups).
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  using namespace hk::detail;
+  if (lanes > 1) v += dpp<kDppXor1>(v);
+  if (lanes > 2) v += dpp<kDppXor2>(v);
+  if (lanes > 4) v += dpp<kDppHalfMirror>(v);
+  if (lanes > 8) v += dpp<kDppMirror>(v);
+  if (lanes > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (lanes > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// Queries or keys: a strided [B, heads, T, d] tensor and what belongs to it.
+struct Side {
+  const void* x;
+  const void* w;   // NULL: 1
+  const void* dy;  // backward
+  void* out;       // forward: y, backward: dx
+  float* part;     // backward: partial sums of dw, one row of d a workgroup (NULL: none asked for)
+  int heads, rows, blocks;
+  int64_t xB, xM, xH, yB, yM, yH, oB, oM, oH;  // strides of x, dy and out
+};
+struct Args {
+  Side side[2];
+  Shape s;
+  const float* cos;
+  const float* sin;
+  int64_t table_stride, table_rows;
+  const int64_t* positions;  // NULL: the token's index
+  int64_t pos_stride;
+  int T;
+  float eps, inv_d;
+};
+
+// The cosines and sines of a unit for a token; NaN where the table has no such position.
+template <int V>
+__device__ __forceinline__ void angles(const Args& g, const Unit<V>& u, int b, int t, float (&c)[V],
+                                       float (&s)[V]) {
+  const int64_t pos = g.positions ? g.positions[b * g.pos_stride + t] : t;
+  if (pos < 0 || pos >= g.table_rows) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) c[e] = s[e] = NAN;
+  } else if (u.angle >= 0) {
+    load_vec(g.cos + pos * g.table_stride + u.angle, c);
+    load_vec(g.sin + pos * g.table_stride + u.angle, s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) c[e] = 1.f, s[e] = 0.f;
+  }
+}
+
+template <class F, int V>
+__device__ __forceinline__ void weights(const void* w, const Unit<V>& u, int d, float (&a)[V],
+                                        float (&b)[V]) {
+  if (w && u.on) {
+    load_unit<F, V>(static_cast<const typename F::storage*>(w), u, d, a, b);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) a[e] = b[e] = 1.f;
+  }
+}
+
+// U: units a lane holds (more than one only where a row needs more than 64 of them, V == 1).
+template <class FI, class FO, int V, int U>
+__global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
+  const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
+  const Side& sd = g.side[which];
+  const int block = blockIdx.x - (which ? g.side[0].blocks : 0);
+  const int per_block = kThreads / g.s.lanes;
+  const int row = block * per_block + threadIdx.x / g.s.lanes;
+  const int j = threadIdx.x & (g.s.lanes - 1);
+  if (row >= sd.rows) return;  // whole lane groups: the butterflies below stay inside a group
+  const int token = row / sd.heads, head = row - token * sd.heads;
+  const int b = token / g.T, t = token - b * g.T;
+  const auto* x = static_cast<const typename FI::storage*>(sd.x) + b * sd.xB + t * sd.xM + head * sd.xH;
+  auto* y = static_cast<typename FO::storage*>(sd.out) + b * sd.oB + t * sd.oM + head * sd.oH;
+  float xa[U][V], xb[U][V], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const Unit<V> u(g.s, j + k * HK_WAVE);
+    if (!u.on) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) xa[k][e] = xb[k][e] = 0.f;
+      continue;
+    }
+    load_unit<FI, V>(x, u, g.s.d, xa[k], xb[k]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum += xa[k][e] * xa[k][e] + xb[k][e] * xb[k][e];
+  }
+  const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const Unit<V> u(g.s, j + k * HK_WAVE);
+    if (!u.on) continue;
+    float wa[V], wb[V], c[V], s[V], ya[V], yb[V];
+    weights<FI, V>(sd.w, u, g.s.d, wa, wb);
+    angles<V>(g, u, b, t, c, s);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float a = xa[k][e] * r * wa[e], bb = xb[k][e] * r * wb[e];
+      ya[e] = a * c[e] - bb * s[e];
+      yb[e] = bb * c[e] + a * s[e];
+    }
+    store_unit<FO, V>(y, u, g.s.d, ya, yb);
+  }
+}
+
+template <class FI, class FO, int V, int U>
+__global__ __launch_bounds__(kThreads) void qk_backward(Args g) {
+  __shared__ float lds[kWaves][kMaxDim];
+  const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
+  const Side& sd = g.side[which];
+  const int block = blockIdx.x - (which ? g.side[0].blocks : 0);
+  const int per_block = kThreads / g.s.lanes;
+  const int j = threadIdx.x & (g.s.lanes - 1);
+  float wa[U][V], wb[U][V], da[U][V], db[U][V];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    weights<FI, V>(sd.w, Unit<V>(g.s, j + k * HK_WAVE), g.s.d, wa[k], wb[k]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) da[k][e] = db[k][e] = 0.f;
+  }
+  for (int row = block * per_block + threadIdx.x / g.s.lanes; row < sd.rows;
+       row += sd.blocks * per_block) {
+    const int token = row / sd.heads, head = row - token * sd.heads;
+    const int b = token / g.T, t = token - b * g.T;
+    const auto* x = static_cast<const typename FI::storage*>(sd.x) + b * sd.xB + t * sd.xM + head * sd.xH;
+    const auto* dy = static_cast<const typename FO::storage*>(sd.dy) + b * sd.yB + t * sd.yM + head * sd.yH;
+    auto* dx = static_cast<typename FI::storage*>(sd.out) + b * sd.oB + t * sd.oM + head * sd.oH;
+    float xa[U][V], xb[U][V], ga[U][V], gb[U][V], sum = 0.f, dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const Unit<V> u(g.s, j + k * HK_WAVE);
+      if (!u.on) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) xa[k][e] = xb[k][e] = ga[k][e] = gb[k][e] = 0.f;
+        continue;
+      }
+      float c[V], s[V], ya[V], yb[V];
+      load_unit<FI, V>(x, u, g.s.d, xa[k], xb[k]);
+      load_unit<FO, V>(dy, u, g.s.d, ya, yb);
+      angles<V>(g, u, b, t, c, s);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        ga[k][e] = ya[e] * c[e] + yb[e] * s[e];
+        gb[k][e] = yb[e] * c[e] - ya[e] * s[e];
+        sum += xa[k][e] * xa[k][e] + xb[k][e] * xb[k][e];
+        dot += ga[k][e] * wa[k][e] * xa[k][e] + gb[k][e] * wb[k][e] * xb[k][e];
+      }
+    }
+    const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
+    // mean(g w n) = r mean(g w x)
+    const float m = lanes_sum(dot, g.s.lanes) * g.inv_d * r;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const Unit<V> u(g.s, j + k * HK_WAVE);
+      float oa[V], ob[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float na = xa[k][e] * r, nb = xb[k][e] * r;
+        da[k][e] += ga[k][e] * na;
+        db[k][e] += gb[k][e] * nb;
+        oa[e] = r * (ga[k][e] * wa[k][e] - na * m);
+        ob[e] = r * (gb[k][e] * wb[k][e] - nb * m);
+      }
+      if (u.on) store_unit<FI, V>(dx, u, g.s.d, oa, ob);
+    }
+  }
+  if (!sd.part) return;
+  // the row groups of a wave, then the waves of the workgroup, in a fixed order
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const Unit<V> u(g.s, j + k * HK_WAVE);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      for (int step = g.s.lanes; step < HK_WAVE; step *= 2) {
+        da[k][e] += __shfl_xor(da[k][e], step);
+        db[k][e] += __shfl_xor(db[k][e], step);
+      }
+    }
+    if (u.on && (threadIdx.x & 63) < g.s.lanes) {
+      store_unit<hk::F32, V>(lds[threadIdx.x / HK_WAVE], u, g.s.d, da[k], db[k]);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < g.s.d; i += kThreads) {
+    float v = lds[0][i];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) v += lds[k][i];
+    sd.part[static_cast<int64_t>(block) * g.s.d + i] = v;
+  }
+}
+
+// dw[i] (+)= the sum over n rows of part[n][d]; blockIdx.y: queries, keys. Each workgroup sums 16
+// columns, its 16 row groups take every 16th row.
+struct Weights {
+  const float* part[2];
+  float* dw[2];
+  int n[2];
+};
+__global__ __launch_bounds__(256) void qk_weight_sums(Weights a, int d, int accumulate) {
+  __shared__ float lds[16][17];
+  const int which = blockIdx.y, col = blockIdx.x * 16 + (threadIdx.x & 15), grp = threadIdx.x >> 4;
+  if (!a.dw[which]) return;
+  float v = 0.f;
+  if (col < d)
+    for (int i = grp; i < a.n[which]; i += 16) v += a.part[which][static_cast<int64_t>(i) * d + col];
+  lds[grp][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (grp == 0 && col < d) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x];
+    a.dw[which][col] = accumulate ? a.dw[which][col] + s : s;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+size_t elem_size(int type) { return type == HK_TYPE_F32 ? 4 : 2; }
+bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+hipError_t check(const hk_qk_norm_rope_params* p, int type, bool backward) {
+  HK_CHECK_ARG(p != nullptr && type >= HK_TYPE_F32 && type <= HK_TYPE_F16);
+  HK_CHECK_ARG(p->B >= 0 && p->T >= 0 && p->q_heads >= 0 && p->k_heads >= 0);
+  HK_CHECK_ARG(p->head_dim >= 1 && p->head_dim <= kMaxDim);
+  HK_CHECK_ARG(p->rotary_dim >= 0 && p->rotary_dim <= p->head_dim && p->rotary_dim % 2 == 0);
+  const int64_t tokens = static_cast<int64_t>(p->B) * p->T;
+  HK_CHECK_ARG(tokens <= INT32_MAX / 2 && tokens * p->q_heads <= INT32_MAX / 2 &&
+               tokens * p->k_heads <= INT32_MAX / 2);
+  const size_t ei = elem_size(type), eo = p->f32_io ? 4 : ei;
+  if (tokens == 0) return hipSuccess;
+  if (p->rotary_dim > 0) {
+    HK_CHECK_ARG(p->cos && p->sin && aligned_to(p->cos, 4) && aligned_to(p->sin, 4));
+    HK_CHECK_ARG(p->table_rows >= 0 && p->table_stride >= p->rotary_dim / 2);
+    HK_CHECK_ARG(p->positions != nullptr || p->T <= p->table_rows);
+    HK_CHECK_ARG(aligned_to(p->positions, 8));
+  }
+  const void* x[2] = {p->q, p->k};
+  const void* w[2] = {p->q_weight, p->k_weight};
+  const void* y[2] = {backward ? p->dq_out : p->q_out, backward ? p->dk_out : p->k_out};
+  const void* dx[2] = {p->dq, p->dk};
+  const int heads[2] = {p->q_heads, p->k_heads};
+  for (int i = 0; i < 2; ++i) {
+    if (heads[i] == 0) continue;
+    HK_CHECK_ARG(x[i] && y[i] && aligned_to(x[i], ei) && aligned_to(w[i], ei) && aligned_to(y[i], eo));
+    HK_CHECK_ARG(!backward || (dx[i] && aligned_to(dx[i], ei)));
+  }
+  HK_CHECK_ARG(!backward || (aligned_to(p->dq_weight, 4) && aligned_to(p->dk_weight, 4)));
+  return hipSuccess;
+}
+
+// Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it.
+int unit_pairs(int type, int d, int rot) {
+  for (int v = type == HK_TYPE_F32 ? 4 : 8; v > 1; v /= 2)
+    if (v != 2 && d % (2 * v) == 0 && rot % (2 * v) == 0) return v;
+  return 1;
+}
+
+Args make_args(const hk_qk_norm_rope_params* p, int v, bool backward) {
+  Args g{};
+  g.s = Shape{p->head_dim, p->rotary_dim, p->rotary_dim / 2, (p->head_dim + 2 * v - 1) / (2 * v), 1,
+              p->interleaved};
+  while (g.s.lanes < g.s.units && g.s.lanes < HK_WAVE) g.s.lanes *= 2;
+  g.cos = p->cos, g.sin = p->sin;
+  g.table_stride = p->table_stride;
+  // without a rotation no position is out of the table
+  g.table_rows = p->rotary_dim > 0 ? p->table_rows : INT64_MAX;
+  g.positions = p->rotary_dim > 0 ? p->positions : nullptr;
+  g.pos_stride = p->pos_strideB;
+  g.T = p->T;
+  g.eps = p->eps;
+  g.inv_d = 1.0f / static_cast<float>(p->head_dim);
+  const int tokens = p->B * p->T;
+  Side& q = g.side[0];
+  q.x = p->q, q.w = p->q_weight, q.dy = p->dq_out, q.out = backward ? p->dq : p->q_out;
+  q.heads = p->q_heads, q.rows = tokens * p->q_heads;
+  q.xB = p->q_strideB, q.xM = p->q_strideM, q.xH = p->q_strideH;
+  q.yB = p->qo_strideB, q.yM = p->qo_strideM, q.yH = p->qo_strideH;
+  q.oB = backward ? p->dq_strideB : q.yB, q.oM = backward ? p->dq_strideM : q.yM;
+  q.oH = backward ? p->dq_strideH : q.yH;
+  Side& k = g.side[1];
+  k.x = p->k, k.w = p->k_weight, k.dy = p->dk_out, k.out = backward ? p->dk : p->k_out;
+  k.heads = p->k_heads, k.rows = tokens * p->k_heads;
+  k.xB = p->k_strideB, k.xM = p->k_strideM, k.xH = p->k_strideH;
+  k.yB = p->ko_strideB, k.yM = p->ko_strideM, k.yH = p->ko_strideH;
+  k.oB = backward ? p->dk_strideB : k.yB, k.oM = backward ? p->dk_strideM : k.yM;
+  k.oH = backward ? p->dk_strideH : k.yH;
+  const int per_block = kThreads / g.s.lanes;
+  for (Side& s : g.side) {
+    s.blocks = static_cast<int>(hk::ceil_div(s.rows, backward ? kRowsPerGroup * per_block : per_block));
+    if (backward && s.blocks > kMostPartials) s.blocks = kMostPartials;
+  }
+  return g;
+}
+
+template <class FI, class FO, int V, int U>
+hipError_t launch(const Args& g, bool backward, hipStream_t stream) {
+  const unsigned blocks = g.side[0].blocks + g.side[1].blocks;
+  if (backward)
+    hipLaunchKernelGGL((qk_backward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+  else
+    hipLaunchKernelGGL((qk_forward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+  return hk::launch_status();
+}
+template <class FI, class FO>
+hipError_t by_unit(const Args& g, int v, bool backward, hipStream_t stream) {
+  if constexpr (FI::kPerVec == 8)
+    if (v == 8) return launch<FI, FO, 8, 1>(g, backward, stream);
+  if (v == 4) return launch<FI, FO, 4, 1>(g, backward, stream);
+  return g.s.units > HK_WAVE ? launch<FI, FO, 1, 2>(g, backward, stream)
+                             : launch<FI, FO, 1, 1>(g, backward, stream);
+}
+hipError_t by_type(const Args& g, int type, bool f32_io, int v, bool backward, hipStream_t stream) {
+  using namespace hk;
+  if (type == HK_TYPE_F32) return by_unit<F32, F32>(g, v, backward, stream);
+  if (type == HK_TYPE_BF16)
+    return f32_io ? by_unit<BF16, F32>(g, v, backward, stream) : by_unit<BF16, BF16>(g, v, backward, stream);
+  return f32_io ? by_unit<F16, F32>(g, v, backward, stream) : by_unit<F16, F16>(g, v, backward, stream);
+}
+
+size_t partial_bytes(const Args& g) {
+  return static_cast<size_t>(g.side[0].blocks + g.side[1].blocks) * g.s.d * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" hipError_t hk_qk_norm_rope_forward(const hk_qk_norm_rope_params* p, int type,
+                                              hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(p, type, false));
+  const int v = unit_pairs(type, p->head_dim, p->rotary_dim);
+  const Args g = make_args(p, v, false);
+  if (g.side[0].rows + g.side[1].rows == 0) return hipSuccess;
+  return by_type(g, type, p->f32_io, v, false, stream);
+}
+
+extern "C" int64_t hk_qk_norm_rope_workspace(const hk_qk_norm_rope_params* p, int type) {
+  if (check(p, type, true) != hipSuccess) return -1;
+  if (!p->dq_weight && !p->dk_weight) return 0;
+  return static_cast<int64_t>(
+      partial_bytes(make_args(p, unit_pairs(type, p->head_dim, p->rotary_dim), true)));
+}
+
+extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, int type,
+                                               void* workspace, int64_t workspace_bytes,
+                                               hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(p, type, true));
+  const int v = unit_pairs(type, p->head_dim, p->rotary_dim);
+  Args g = make_args(p, v, true);
+  Weights w{{nullptr, nullptr},
+            {p->q_heads ? p->dq_weight : nullptr, p->k_heads ? p->dk_weight : nullptr},
+            {g.side[0].blocks, g.side[1].blocks}};
+  const bool sums = w.dw[0] || w.dw[1];
+  if (sums && g.side[0].rows + g.side[1].rows > 0) {
+    const size_t bytes = partial_bytes(g);
+    void* ws = workspace;
+    if (ws) HK_CHECK_ARG(workspace_bytes >= static_cast<int64_t>(bytes) && aligned_to(ws, 4));
+    else HK_RETURN_IF_ERROR(hk::device_workspace(bytes, stream, &ws));
+    float* part = static_cast<float*>(ws);
+    for (int i = 0; i < 2; ++i) {
+      if (w.dw[i]) w.part[i] = g.side[i].part = part;
+      part += static_cast<int64_t>(g.side[i].blocks) * g.s.d;
+    }
+  }
+  if (g.side[0].rows + g.side[1].rows > 0)
+    HK_RETURN_IF_ERROR(by_type(g, type, p->f32_io, v, true, stream));
+  if (!sums || (p->accumulate && g.side[0].rows + g.side[1].rows == 0)) return hipSuccess;
+  // without rows the sums are zero
+  hipLaunchKernelGGL(qk_weight_sums, dim3(static_cast<unsigned>((g.s.d + 15) / 16), 2), dim3(256), 0,
+                     stream, w, g.s.d, p->accumulate ? 1 : 0);
+  return hk::launch_status();
+}

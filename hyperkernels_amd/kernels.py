@@ -19,7 +19,8 @@ __all__ = [
     "HKError", "gelu_forward", "gelu_backward", "layer_norm_forward", "ln_backward_input",
     "ln_backward_gamma_beta", "layer_norm_backward", "sparse_ce_forward", "sparse_ce_backward",
     "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "Adam8Plan", "ADAM8_BLOCK",
-    "adam8_states", "adam8_quantize", "adam8_dequantize", "ReductionLayout",
+    "adam8_states", "adam8_quantize", "adam8_dequantize", "qk_norm_rope_forward",
+    "qk_norm_rope_backward", "ReductionLayout",
     "unified_reduce_sum", "reduce_generic", "REDUCE_INNER", "REDUCE_OUTER", "REDUCE_GENERIC",
 ]
 
@@ -45,6 +46,20 @@ def _dev(*ts: torch.Tensor | None) -> None:
             raise ValueError("hyperkernels_amd kernels take device tensors only")
         if not t.is_contiguous():
             raise ValueError("hyperkernels_amd kernels take contiguous tensors")
+
+
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HK_TYPE_*
+
+
+def _here(fn: str, *ts: torch.Tensor | None) -> None:
+    """Device tensors of the current device, whose stream the launch goes to."""
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{fn}: device tensors only")
+    cur = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.get_device() != cur:
+            raise ValueError(f"{fn}: tensors of the current device (cuda:{cur}) only")
 
 
 # ----------------------------------------------------------------------------------------------
@@ -277,15 +292,6 @@ class AdamPlan:
 # Multi-tensor AdamW with both moments in 8 bits (no counterpart in the reference)
 # ----------------------------------------------------------------------------------------------
 ADAM8_BLOCK = 256
-_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HK_TYPE_*
-
-
-def _here(fn: str, *ts: torch.Tensor | None) -> None:
-    """Device tensors of the current device, whose stream the launch goes to."""
-    cur = torch._C._cuda_getDevice()
-    for t in ts:
-        if t is not None and t.get_device() != cur:
-            raise ValueError(f"{fn}: tensors of the current device (cuda:{cur}) only")
 
 
 def _adam8_check(fn: str, m, v, m_scale, v_scale, blocks: int) -> None:
@@ -488,6 +494,116 @@ def attn_backward(q, k, v, do, lse, D, causal: bool, scale: float | None = None,
     p = _bwd_params(q, k, v, o, do, lse, D, dq, dk, dv, causal, scale)
     call(fn, ctypes.byref(p), Dh, _stream())
     return dq, dk, dv
+
+
+# ----------------------------------------------------------------------------------------------
+# RMS norm of query and key heads with the position rotation (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+class QkNormRopeParams(ctypes.Structure):
+    """hk_qk_norm_rope_params (hk.h), field for field."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "q_weight", "k_weight", "cos", "sin", "positions", "q_out", "k_out", "dq_out",
+        "dk_out", "dq", "dk", "dq_weight", "dk_weight")] + [
+        (n, ctypes.c_int) for n in ("B", "T", "q_heads", "k_heads", "head_dim", "rotary_dim")] + [
+        ("eps", ctypes.c_float)] + [
+        (n, ctypes.c_bool) for n in ("interleaved", "f32_io", "accumulate")] + [
+        (n, _I64) for n in ("table_rows", "table_stride", "pos_strideB")] + [
+        (f"{t}_stride{s}", _I64) for t in ("q", "k", "qo", "ko", "dq", "dk")
+        for s in ("B", "M", "H")]
+
+
+def _qk_params(fn, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved, qo, ko,
+               backward=False, dq=None, dk=None, dqw=None, dkw=None, accumulate=False):
+    """The parameter block; qo, ko: the outputs, or in the backward pass their gradients."""
+    x = q if q is not None else k
+    if x is None or x.dim() != 4 or x.dtype not in _TYPE:
+        raise ValueError(f"{fn}: q or k, [B, heads, T, head_dim], fp32, bf16 or fp16")
+    _here(fn, q, k, cos, sin, positions, q_weight, k_weight, qo, ko, dq, dk, dqw, dkw)
+    (B, _, T, d), out = x.shape, (qo if qo is not None else ko).dtype
+    for t, o, w, g, gw in ((q, qo, q_weight, dq, dqw), (k, ko, k_weight, dk, dkw)):
+        if t is None:
+            if o is not None or g is not None or gw is not None:
+                raise ValueError(f"{fn}: outputs and gradients of a tensor that is not passed")
+            continue
+        if t.dim() != 4 or t.dtype != x.dtype or t.shape[0] != B or t.shape[2:] != x.shape[2:]:
+            raise ValueError(f"{fn}: q and k share type, batch, length and head_dim")
+        if o is None or o.shape != t.shape or o.dtype != out or out not in (x.dtype, torch.float32):
+            raise ValueError(f"{fn}: outputs have their input's shape, and its type or fp32")
+        if w is not None and (w.dtype != x.dtype or w.shape != (d,) or not w.is_contiguous()):
+            raise ValueError(f"{fn}: weights are [head_dim] of the inputs' type")
+        if g is not None and (g.shape != t.shape or g.dtype != x.dtype):
+            raise ValueError(f"{fn}: gradients have their input's shape and type")
+        if gw is not None and (gw.dtype != torch.float32 or gw.shape != (d,)
+                               or not gw.is_contiguous()):
+            raise ValueError(f"{fn}: gradients of the weights are fp32 [head_dim]")
+    rows = stride = rot = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or not (
+                cos.dtype == sin.dtype == torch.float32) or cos.stride() != sin.stride() or (
+                cos.stride(1) != 1 and cos.shape[1] > 1):
+            raise ValueError(f"{fn}: cos and sin are fp32 [rows, rotary_dim / 2], laid out alike")
+        rows, stride, rot = cos.shape[0], cos.stride(0), 2 * cos.shape[1]
+        if rows == 1:
+            stride = max(stride, cos.shape[1])
+    pos_stride = 0
+    if positions is not None:
+        if positions.dtype != torch.int64 or positions.shape not in ((B, T), (T,)) or (
+                positions.stride(-1) != 1 and T > 1):
+            raise ValueError(f"{fn}: positions are int64 [B, T] or [T]")
+        pos_stride = positions.stride(0) if positions.dim() == 2 else 0
+    return QkNormRopeParams(
+        _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(positions),
+        None if backward else _ptr(qo), None if backward else _ptr(ko),
+        _ptr(qo) if backward else None, _ptr(ko) if backward else None, _ptr(dq), _ptr(dk),
+        _ptr(dqw), _ptr(dkw), B, T, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1],
+        d, rot, eps, bool(interleaved), out != x.dtype, bool(accumulate), rows, stride, pos_stride,
+        *_strides(q), *_strides(k), *_strides(qo), *_strides(ko), *_strides(dq), *_strides(dk))
+
+
+def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None,
+                         eps: float = 1e-6, interleaved: bool = False, q_out=None, k_out=None,
+                         out_dtype=None):
+    """RMS norm of each head of q and k (either may be None) over its last dimension, times its weight,
+    then the rotation of its first 2 * cos.shape[1] elements by the table rows of the tokens'
+    positions (None: token t at position t). Returns (q_out, k_out) of q's type or out_dtype, which
+    may be fp32 for 16-bit inputs. q_out and k_out may be q and k themselves."""
+    make = lambda t: None if t is None else torch.empty(  # noqa: E731
+        t.shape, device=t.device, dtype=out_dtype or t.dtype)
+    q_out = make(q) if q_out is None else q_out
+    k_out = make(k) if k_out is None else k_out
+    p = _qk_params("qk_norm_rope_forward", q, k, cos, sin, positions, q_weight, k_weight, eps,
+                   interleaved, q_out, k_out)
+    call("hk_qk_norm_rope_forward", ctypes.byref(p), _TYPE[(q if q is not None else k).dtype],
+         _stream())
+    return q_out, k_out
+
+
+def _by_token(t):
+    """An empty [B, heads, T, d] tensor with the heads of a token together, as a projection has them."""
+    B, H, T, d = t.shape
+    return torch.empty(B, T, H, d, device=t.device, dtype=t.dtype).transpose(1, 2)
+
+
+def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=None, q_weight=None,
+                          k_weight=None, eps: float = 1e-6, interleaved: bool = False,
+                          grad_q_weight=None, grad_k_weight=None, dq=None, dk=None,
+                          accumulate: bool = True):
+    """Gradients of qk_norm_rope_forward's inputs from those of its outputs: returns (dq, dk), which
+    may be q, k or gradients of the same type passed in. grad_q_weight and grad_k_weight (fp32
+    [head_dim]) are added to, or written where accumulate is False; None: not wanted."""
+    dq = _by_token(q) if dq is None and q is not None else dq
+    dk = _by_token(k) if dk is None and k is not None else dk
+    p = _qk_params("qk_norm_rope_backward", q, k, cos, sin, positions, q_weight, k_weight, eps,
+                   interleaved, dq_out, dk_out, True, dq, dk, grad_q_weight, grad_k_weight,
+                   accumulate)
+    x, ws, n = (q if q is not None else k), None, 0
+    if grad_q_weight is not None or grad_k_weight is not None:
+        # the call's own partial sums: captured graphs and other streams have theirs
+        n = max(0, lib().hk_qk_norm_rope_workspace(ctypes.byref(p), _TYPE[x.dtype]))
+        ws = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
+    call("hk_qk_norm_rope_backward", ctypes.byref(p), _TYPE[x.dtype], _ptr(ws), n, _stream())
+    return dq, dk
 
 
 # ----------------------------------------------------------------------------------------------

@@ -39,6 +39,11 @@ extern "C" {
 typedef uint16_t hk_bf16;
 typedef uint16_t hk_f16; /* IEEE binary16 bit pattern (__half) */
 
+/* Element types, where an entry point takes tensors of more than one as an argument. */
+#define HK_TYPE_F32 0
+#define HK_TYPE_BF16 1
+#define HK_TYPE_F16 2
+
 /* ------------------------------------------------------------------------------------------
  * Library
  * ---------------------------------------------------------------------------------------- */
@@ -245,9 +250,6 @@ HK_API int64_t hk_adam_plan_num_chunks(const hk_adam_plan* plan);
  *   that goes on in 8 bits, a checkpoint): numel elements of whole blocks, but for the last one. v is
  *   taken as 0 where it is negative.
  * ---------------------------------------------------------------------------------------- */
-#define HK_TYPE_F32 0
-#define HK_TYPE_BF16 1
-#define HK_TYPE_F16 2
 #define HK_ADAM8_BLOCK 256
 typedef struct hk_adam8_plan hk_adam8_plan;
 HK_API hipError_t hk_adam8_plan_create(int num_tensors, float* const* params,
@@ -580,6 +582,69 @@ HK_API hipError_t hk_attn_backward(const hk_attn_bwd_params* params, int head_di
  * not accumulate: dQ is written, whatever it held before, without a clearing launch of its own. */
 HK_API hipError_t hk_attn_backward_set(const hk_attn_bwd_params* params, int head_dim,
                                        hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * RMS norm of each query and key head with the position rotation, in one pass: what lies between a
+ * query / key / value projection and the attention. No counterpart in the reference.
+ * Per token and head, x its head_dim elements (1 .. 256):
+ *   n = x / sqrt(mean(x^2) + eps),  z = n * weight,
+ *   and pair i < rotary_dim / 2 of z turned by the angle of the token's position:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), (a, b) = (z[i], z[i + rotary_dim / 2]), or
+ *   (z[2 i], z[2 i + 1]) where interleaved. Elements from rotary_dim on (even, 0 .. head_dim) stay.
+ * cos and sin are fp32 [table_rows, rotary_dim / 2], rows table_stride elements apart: row p holds the
+ * angles of position p (any frequencies, any scaling of them). positions is int64 [B, T], batches
+ * pos_strideB elements apart (0: the same for all), NULL for token t at position t (T <= table_rows
+ * then). A position outside the table makes the token's outputs and gradients NaN.
+ * q, k and the weights (head_dim elements each, NULL: all 1) are of the call's type, HK_TYPE_*; the
+ * outputs, and in the backward pass their gradients, are of that type too, or fp32 where f32_io is set
+ * (what the attention takes and returns). Tensors are [B, heads, T, head_dim] with any batch / row /
+ * head strides (elements; last-dim stride 1) and any alignment of their element type. q and k may have
+ * different numbers of heads; one of them with 0 is left out.
+ * hk_qk_norm_rope_forward reads q, k and writes q_out, k_out, which may be q and k themselves.
+ * hk_qk_norm_rope_backward reads q, k and the gradients dq_out, dk_out (strides qo_*, ko_*, like the
+ *   outputs') and writes dq, dk, which may be q, k or, with f32_io unset, dq_out and dk_out themselves.
+ *   dq_weight and dk_weight (fp32, NULL: not wanted) are written, or added to where accumulate is
+ *   set, summed over tokens and heads in a fixed order. The partial sums take
+ *   hk_qk_norm_rope_workspace bytes (0 where neither is wanted, -1 for invalid arguments): at
+ *   `workspace`, or in the stream's workspace where that is NULL. A call that is captured into a graph
+ *   should bring its own, since graphs captured on one stream share the stream's.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct hk_qk_norm_rope_params {
+  const void* q;
+  const void* k;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  void* q_out;
+  void* k_out;
+  const void* dq_out;
+  const void* dk_out;
+  void* dq;
+  void* dk;
+  float* dq_weight;
+  float* dk_weight;
+  int B, T;
+  int q_heads, k_heads;
+  int head_dim, rotary_dim;
+  float eps;
+  bool interleaved, f32_io, accumulate;
+  int64_t table_rows, table_stride, pos_strideB;
+  int64_t q_strideB, q_strideM, q_strideH;
+  int64_t k_strideB, k_strideM, k_strideH;
+  int64_t qo_strideB, qo_strideM, qo_strideH;
+  int64_t ko_strideB, ko_strideM, ko_strideH;
+  int64_t dq_strideB, dq_strideM, dq_strideH;
+  int64_t dk_strideB, dk_strideM, dk_strideH;
+} hk_qk_norm_rope_params;
+
+HK_API hipError_t hk_qk_norm_rope_forward(const hk_qk_norm_rope_params* params, int type,
+                                          hipStream_t stream);
+HK_API int64_t hk_qk_norm_rope_workspace(const hk_qk_norm_rope_params* params, int type);
+HK_API hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* params, int type,
+                                           void* workspace, int64_t workspace_bytes,
+                                           hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Measurement

@@ -3,6 +3,8 @@ work, and the torch front end what is no device tensor."""
 from __future__ import annotations
 
 import ctypes
+import pathlib
+import subprocess
 
 import pytest
 import torch
@@ -77,3 +79,75 @@ def test_adam8_front_end_refuses_host_tensors():
         hk.adam8_dequantize(*state)
     with pytest.raises(ValueError):
         hk.Adam8Plan([x], [x, x], *state)
+
+
+def _qk(**kw):
+    from hyperkernels_amd.kernels import QkNormRopeParams
+
+    base = dict(q=64, k=64, cos=64, sin=64, q_out=64, k_out=64, dq_out=64, dk_out=64, dq=64, dk=64,
+                B=1, T=4, q_heads=2, k_heads=1, head_dim=64, rotary_dim=64, eps=1e-6, table_rows=4,
+                table_stride=32)
+    return QkNormRopeParams(**{**base, **kw})
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_qk_norm_rope_refuses(L, backward):
+    def go(kind=0, **kw):
+        p = ctypes.byref(_qk(**kw))
+        if not backward:
+            return L.hk_qk_norm_rope_forward(p, kind, NULL)
+        assert L.hk_qk_norm_rope_workspace(p, kind) == -1
+        return L.hk_qk_norm_rope_backward(p, kind, NULL, 0, NULL)
+
+    bad = [dict(B=-1), dict(T=-1), dict(q_heads=-1), dict(k_heads=-1), dict(head_dim=0),
+           dict(head_dim=257), dict(rotary_dim=3), dict(rotary_dim=66), dict(rotary_dim=-2),
+           dict(kind=3), dict(kind=-1), dict(cos=0), dict(sin=0), dict(cos=66), dict(table_rows=3),
+           dict(table_stride=31), dict(positions=68), dict(q=0), dict(k=0), dict(q=66), dict(q=65, kind=1),
+           dict(q_weight=66), dict(B=1 << 20, T=1 << 20, positions=64)]
+    if backward:
+        bad += [dict(dq=0), dict(dk=0), dict(dq_out=0), dict(dq=66), dict(dq_weight=66),
+                dict(dk_out=66, kind=1, f32_io=True)]
+    else:
+        bad += [dict(q_out=0), dict(k_out=0), dict(q_out=66), dict(q_out=66, kind=1, f32_io=True)]
+    for kw in bad:
+        assert go(**kw) == INVALID, kw
+    if backward:
+        assert L.hk_qk_norm_rope_backward(NULL, 0, NULL, 0, NULL) == INVALID
+        assert L.hk_qk_norm_rope_workspace(ctypes.byref(_qk()), 0) == 0  # no weight gradients
+        p = _qk(dq_weight=64)
+        n = L.hk_qk_norm_rope_workspace(ctypes.byref(p), 0)
+        assert n > 0
+        assert L.hk_qk_norm_rope_backward(ctypes.byref(p), 0, 64, n - 1, NULL) == INVALID
+        assert L.hk_qk_norm_rope_backward(ctypes.byref(p), 0, 66, n, NULL) == INVALID
+    else:
+        assert L.hk_qk_norm_rope_forward(NULL, 0, NULL) == INVALID
+        assert L.hk_qk_norm_rope_forward(ctypes.byref(_qk(B=0, q=0, k=0)), 0, NULL) == 0
+
+
+def test_qk_front_end_refuses_host_tensors():
+    from hyperkernels_amd import kernels as hk
+
+    q = torch.zeros(1, 2, 4, 64)
+    with pytest.raises(ValueError):
+        hk.qk_norm_rope_forward(q, q)
+    with pytest.raises(ValueError):
+        hk.qk_norm_rope_backward(q, q, q, q)
+    with pytest.raises(ValueError):
+        hk.qk_norm_rope_forward(None, None)
+
+
+def test_qk_parameter_block_matches_the_header(tmp_path):
+    from hyperkernels_amd.kernels import QkNormRopeParams as P
+
+    root = pathlib.Path(__file__).resolve().parents[1]
+    fields = [n for n, _ in P._fields_]
+    src = tmp_path / "probe.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "hk.h"\nint main(void) {\n'
+                   '  printf("%zu", sizeof(hk_qk_norm_rope_params));\n' + "".join(
+                       f'  printf(" %zu", offsetof(hk_qk_norm_rope_params, {n}));\n'
+                       for n in fields) + "  return 0;\n}\n")
+    subprocess.run(["gcc", "-D__HIP_PLATFORM_AMD__", f"-I{root / 'include'}", "-I/opt/rocm/include",
+                    str(src), "-o", str(tmp_path / "probe")], check=True)
+    got = list(map(int, subprocess.run([str(tmp_path / "probe")], capture_output=True, text=True,
+                                       check=True).stdout.split()))
+    assert got == [ctypes.sizeof(P)] + [getattr(P, n).offset for n in fields]
