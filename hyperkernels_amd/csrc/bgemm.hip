@@ -45,6 +45,7 @@
 // bgemm_flex.hip (make_plan); leading dimensions those do not take either, and K == 0, on a simple
 // fp32-accumulating kernel.
 #include "bgemm_flex.h"
+#include "bgemm_plan.h"
 #include "bgemm_wide.h"
 
 namespace {
@@ -197,16 +198,7 @@ int auto_split_k(int64_t work_tiles, int64_t ktiles, int64_t outputs, int most, 
 constexpr int kMostSplits = 8;      // of the library's own choice on the 256-wide tiles
 constexpr int kMaxGridZ = 65535;  // batches x k splits of one launch
 
-// What the rows of a product's matrices are, as the kernels see them.
-enum class Rows {
-  kAligned,  // whole 16-byte vectors: 8-element multiples for every contiguous extent, leading
-             // dimension and batch stride, 16-byte aligned bases
-  kRaggedC,  // A and B like that, C at any 2-byte address and any N
-  kRagged,   // any 2-byte address, any extent
-  kNone      // no MFMA path: no k, a leading dimension whose per-lane 32-bit byte offsets do not
-             // fit, or one under 8 (a vector could leave the matrix); more batches of unaligned
-             // rows than the tiles' grid takes
-};
+using Rows = hk::GemmRows;
 Rows row_kind(bool ta, bool tb, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc,
               int64_t sA, int64_t sB, int64_t sC, int batch, bool a16, bool b16, bool c16) {
   if (K <= 0 || lda >= (1 << 22) || ldb >= (1 << 22)) return Rows::kNone;
@@ -409,6 +401,36 @@ GemmPlan bgemm_plan(bool ta, bool tb, int M, int N, int K, int batch, int split_
 
 GemmPlan bgemm_lean_plan(bool ta, bool tb, int M, int N, int K, int batch, size_t held) {
   return lean_plan(ta, tb, M, N, K, batch, Rows::kAligned, held);
+}
+
+GemmRows bgemm_rows(bool ta, bool tb, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc,
+                    int64_t sA, int64_t sB, int64_t sC, int batch, bool a16, bool b16, bool c16) {
+  return row_kind(ta, tb, M, N, K, lda, ldb, ldc, sA, sB, sC, batch, a16, b16, c16);
+}
+
+GemmPlan bgemm_rows_plan(bool ta, bool tb, int M, int N, int K, int batch, GemmRows rows,
+                         bool may_split) {
+  const Plan p = make_plan(ta, tb, M, N, K, batch, 0, rows);
+  if (p.used == 1 || (may_split && static_cast<int64_t>(batch) * p.used <= kMaxGridZ)) return p;
+  return lean_plan(ta, tb, M, N, K, batch, rows, 0);
+}
+
+size_t bgemm_partial_bytes(int used, int M, int N, int batch) {
+  return partial_bytes(used, M, N, batch);
+}
+
+hipError_t bgemm_write_partials(bool ta, bool tb, int M, int N, int K, const hk_bf16* A, int64_t lda,
+                                int64_t sA, const hk_bf16* B, int64_t ldb, int64_t sB, int batch,
+                                const GemmPlan& plan, float* part, hipStream_t stream) {
+  HK_CHECK_ARG(plan.used > 1 && part != nullptr);
+  if (plan.flex)
+    return bgemm_flex_run(plan.flex,
+                          FlexCall{ta, tb, M, N, K, batch, A, lda, sA, B, ldb, sB, nullptr, 0, 0,
+                                   nullptr, plan.used, plan.kps, part, nullptr},
+                          stream);
+  const Epi ep{1.0f, 0.0f, nullptr, 0, 0, false};
+  return run_regions<true>(ta, tb, batch * plan.used, stream, M, N, K, ep, A, lda, sA, B, ldb, sB,
+                           nullptr, 0, 0, plan.used, plan.kps, part, F32Out{});
 }
 
 hipError_t bgemm_partials(bool ta, bool tb, int M, int N, int K, const hk_bf16* A, int64_t lda,

@@ -1,0 +1,210 @@
+// bgemm_act.h - the epilogue of the BF16 GEMM's tiles with bias, activation and residual, and the one of
+// its backward product (bgemm_act.hip).
+#pragma once
+
+#include "activation.h"
+#include "bgemm_tile.h"
+
+namespace hk {
+namespace gemm {
+
+// forward:  z = alpha acc + bias[col], stored in bf16 where z is not NULL; C = act(z) + residual
+// backward: d = alpha acc act'(z); C = d, and the column sums of d over each wave's rows where sums is
+//           not NULL: row (batch, wave row) of [batch][sum_rows][pitch]
+// Everything is fp32 until C and z are rounded, once each, to nearest even.
+struct ActEpi {
+  float alpha;
+  Activation act;
+  bool backward, ragged;  // ragged: C, z or residual are no whole number of aligned 16-byte vectors
+  const uint16_t* bias;
+  int64_t sBias;
+  const uint16_t* residual;
+  int64_t ldr, sR;
+  uint16_t* z;  // read in the backward pass
+  int64_t ldz, sZ;
+  float* sums;
+  int sum_rows, pitch;
+};
+
+// Eight bf16 of a row, n of them inside it. The whole vectors of rows that are not ragged are aligned.
+template <bool RAGGED>
+__device__ __forceinline__ uint4 load_row8(const uint16_t* p, int n) {
+  if (!RAGGED) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4];
+  if (n == 8) {
+    __builtin_memcpy(w, p, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = (2 * e < n ? p[2 * e] : 0u) |
+             (2 * e + 1 < n ? static_cast<uint32_t>(p[2 * e + 1]) << 16 : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Stores are non-temporal like those of the plain product: nothing here is read again by this one.
+template <bool RAGGED>
+__device__ __forceinline__ void store_row8(uint16_t* p, int n, const float (&f)[8]) {
+  const uint4 v = BF16::pack(f);
+  if (!RAGGED) {
+    st_nt(reinterpret_cast<uint4*>(p), v);
+  } else if (n == 8) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+// The epilogue of one lane: the 8 columns from col on of several rows, so the bias and the column sums stay
+// in registers. What it reads beside the sums (residual, or z in the backward pass) is fetched ahead
+// of the row's turn.
+template <bool RAGGED>
+struct ActLane {
+  const ActEpi& ep;
+  const WaveRows& w;
+  int col, n;          // n: columns inside N, 0 for none
+  const uint16_t* in;  // residual or z of row 0, column col; NULL: nothing to read
+  int64_t ld_in;
+  float reg[8];        // forward: bias, backward: column sums
+  __device__ ActLane(const ActEpi& e, const WaveRows& rows, int cc)
+      : ep(e), w(rows), col(rows.wcol0 + cc), n(min(8, max(0, rows.N - col))) {
+    const uint16_t* base = ep.backward ? (ep.act.kind == HK_ACT_NONE ? nullptr : ep.z) : ep.residual;
+    ld_in = ep.backward ? ep.ldz : ep.ldr;
+    in = base ? base + w.batch * (ep.backward ? ep.sZ : ep.sR) + col : nullptr;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      reg[i] = !ep.backward && ep.bias && i < n ? bf16_to_f32(ep.bias[w.batch * ep.sBias + col + i]) : 0.f;
+  }
+  __device__ bool has(int row) const { return row < w.M && n > 0; }
+  __device__ uint4 fetch(int row) const {
+    return in && has(row) ? load_row8<RAGGED>(in + row * ld_in, n) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ void row(int row, const uint4& extra, const f32x4_t& a, const f32x4_t& b) {
+    if (!has(row)) return;
+    float v[8], x[8];
+    BF16::unpack(extra, x);
+    if (ep.backward) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = ep.alpha * (e < 4 ? a[e] : b[e - 4]);
+      scale_by_grad(ep.act, x, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) reg[e] += v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(ep.alpha, e < 4 ? a[e] : b[e - 4], reg[e]);
+      if (ep.z) store_row8<RAGGED>(ep.z + w.batch * ep.sZ + row * ep.ldz + col, n, v);
+      activate(ep.act, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
+    store_row8<RAGGED>(w.C + w.batch * w.sC + row * w.ldc + col, n, v);
+  }
+  // Adds the lanes' column sums of one wave, in a fixed order, and stores its row of them. The LPR lanes
+  // of a row hold 8 columns each; a wave has 64 / LPR rows, the last lanes idle where LPR is no power
+  // of two.
+  template <int LPR>
+  __device__ void store_sums(int lane) {
+    if (!ep.sums || w.wrow0 >= w.M) return;  // a wave without rows is not counted in sum_rows
+    const int cc = (lane % LPR) * 8;
+    if constexpr ((LPR & (LPR - 1)) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int step = LPR; step < HK_WAVE; step *= 2) reg[e] += __shfl_xor(reg[e], step);
+    } else {
+      float HK_LDS* area = reinterpret_cast<float HK_LDS*>(w.area);
+      constexpr int kRows = HK_WAVE / LPR;
+      if (lane < kRows * LPR) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) area[(lane / LPR) * (8 * LPR) + cc + e] = reg[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        reg[e] = 0.f;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) reg[e] += area[r * (8 * LPR) + cc + e];
+      }
+    }
+    if (lane < LPR && n > 0) {
+      // pitch is a multiple of 8: a lane's columns past N lie in its padding
+      float4* dst = reinterpret_cast<float4*>(
+          ep.sums + (static_cast<int64_t>(w.batch) * ep.sum_rows + w.wave_row) * ep.pitch + col);
+      dst[0] = make_float4(reg[0], reg[1], reg[2], reg[3]);
+      dst[1] = make_float4(reg[4], reg[5], reg[6], reg[7]);
+    }
+  }
+};
+
+// The rows of a wave, as staged_rows: one 32-row MFMA block row at a time through LDS. The code of a row is
+// long, so the blocks are a loop (their accumulators are picked by uniform branches); the next
+// block's reads are in flight while a block is worked on.
+template <int kWaveN, int kBlkM, bool RAGGED>
+__device__ __forceinline__ void act_rows(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
+                                         const ActEpi& ep, const WaveRows& w) {
+  constexpr int kBlkN = kWaveN / 32;
+  constexpr int P = kWaveN * 4 + 16;  // staging pitch (bytes)
+  constexpr int LPR = kWaveN / 8;     // lanes per row
+  constexpr int RPP = 64 / LPR;       // rows per pass
+  constexpr int kPasses = 32 / RPP;
+  const int r = lane & 31, h = lane >> 5;
+  const int rr0 = lane / LPR, cc = (lane % LPR) * 8;
+  ActLane<RAGGED> out(ep, w, cc);
+  uint4 next[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) next[p] = out.fetch(w.wrow0 + p * RPP + rr0);
+#pragma unroll 1
+  for (int i = 0; i < kBlkM; ++i) {
+    uint4 extra[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      extra[p] = next[p];
+      if (i + 1 < kBlkM) next[p] = out.fetch(w.wrow0 + 32 * (i + 1) + p * RPP + rr0);
+    }
+#pragma unroll
+    for (int ii = 0; ii < kBlkM; ++ii)
+      if (i == ii) {
+#pragma unroll
+        for (int j = 0; j < kBlkN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4_t HK_LDS*>(w.area + r * P + (32 * j + 8 * q + 4 * h) * 4) =
+                f32x4_t{acc[ii][j][4 * q], acc[ii][j][4 * q + 1], acc[ii][j][4 * q + 2],
+                        acc[ii][j][4 * q + 3]};
+      }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int rr = p * RPP + rr0;
+      const f32x4_t a = *reinterpret_cast<const f32x4_t HK_LDS*>(w.area + rr * P + cc * 4);
+      const f32x4_t b = *reinterpret_cast<const f32x4_t HK_LDS*>(w.area + rr * P + cc * 4 + 16);
+      out.row(w.wrow0 + 32 * i + rr, extra[p], a, b);
+    }
+  }
+  if (ep.backward) out.template store_sums<LPR>(lane);
+}
+template <int kWaveN, int kBlkM>
+__device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
+                                           const ActEpi& ep, const WaveRows& w) {
+  if (ep.ragged) act_rows<kWaveN, kBlkM, true>(acc, lane, ep, w);
+  else act_rows<kWaveN, kBlkM, false>(acc, lane, ep, w);
+}
+
+// The same where the caller hands out the rows itself.
+template <int LPR, bool RAGGED, class Emit>
+__device__ __forceinline__ void emit_act(const ActEpi& ep, const WaveRows& w, int lane, Emit&& emit) {
+  ActLane<RAGGED> out(ep, w, (lane % LPR) * 8);
+  emit([&](int rr, int, const f32x4_t& a, const f32x4_t& b) {
+    out.row(w.wrow0 + rr, out.fetch(w.wrow0 + rr), a, b);
+  });
+  if (ep.backward) out.template store_sums<LPR>(lane);
+}
+template <int LPR, class Emit>
+__device__ __forceinline__ void emit_rows(const ActEpi& ep, const WaveRows& w, int lane,
+                                          Emit&& emit) {
+  if (ep.ragged) emit_act<LPR, true>(ep, w, lane, emit);
+  else emit_act<LPR, false>(ep, w, lane, emit);
+}
+
+}  // namespace gemm
+}  // namespace hk

@@ -1,0 +1,438 @@
+// bgemm_act.hip - the BF16 GEMM with bias, activation and residual in its epilogue, and the product of its
+// backward pass:
+//   forward   z = alpha op(A) op(B) + bias[col],  preact = bf16(z),  C = act(z) + residual
+//   backward  d = alpha op(A) op(B) act'(preact),  C = d,  dbias[col] (+)= the sum of d over rows
+// A feed-forward block's hidden layer is the first with A its input and B its weights, and d the
+// second with A the gradient behind the next layer and B that layer's weights: what would be passes
+// over [tokens, hidden] of their own (bias and activation 2 reads or writes of 2 bytes an element, the
+// gradient 3, the bias gradient 1) are part of the product's stores.
+//
+// The products are those of bgemm.hip and bgemm_flex.hip, on the same tiles by the same choice, with the
+// epilogue of bgemm_act.h in the tiles' place of the plain one; a product of one row runs on the kernels
+// of bgemv.hip. Where K is split, a second kernel adds the fp32 partials in split order and applies the
+// epilogue. The bias gradient is summed in fp32 from the values before their rounding: over the rows of
+// a wave in registers, over the waves of the grid by a further kernel, in a fixed order.
+#include "bgemm_act_tiles.h"
+#include "bgemm_plan.h"
+#include "bgemm_wide.h"
+
+namespace {
+
+using namespace hk::gemm;
+
+constexpr int kMaxGridZ = 65535;
+
+// One element's epilogue, for the kernels that hold one at a time: returns d in the backward pass.
+__device__ __forceinline__ float act_element(const ActEpi& ep, uint16_t* C, int64_t ldc, int64_t sC,
+                                             int b, int64_t row, int col, float acc) {
+  uint16_t* cp = C + b * sC + row * ldc + col;
+  float v[1];
+  if (ep.backward) {
+    v[0] = ep.alpha * acc;
+    if (ep.act.kind != HK_ACT_NONE) {
+      const float z[1] = {hk::bf16_to_f32(ep.z[b * ep.sZ + row * ep.ldz + col])};
+      hk::scale_by_grad(ep.act, z, v);
+    }
+  } else {
+    v[0] = __builtin_fmaf(ep.alpha, acc, ep.bias ? hk::bf16_to_f32(ep.bias[b * ep.sBias + col]) : 0.f);
+    if (ep.z) ep.z[b * ep.sZ + row * ep.ldz + col] = hk::f32_to_bf16(v[0]);
+    hk::activate(ep.act, v);
+    if (ep.residual) v[0] += hk::bf16_to_f32(ep.residual[b * ep.sR + row * ep.ldr + col]);
+  }
+  *cp = hk::f32_to_bf16(v[0]);
+  return v[0];
+}
+
+// The epilogue on the sums of the k splits (split order). A workgroup takes kFinalRows rows of 128
+// columns, a thread 8 columns of every 16th row.
+constexpr int kFinalRows = 32;
+__global__ __launch_bounds__(256) void act_finalize(const float* __restrict__ part, int split_k,
+                                                    int col_blocks, int M, int N, ActEpi ep,
+                                                    uint16_t* __restrict__ C, int64_t ldc,
+                                                    int64_t sC) {
+  __shared__ float lds[16][128 + 4];
+  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  const int b = blockIdx.z, batch = gridDim.z;
+  const int cc = (threadIdx.x & 15) * 8, ty = threadIdx.x >> 4;
+  const int64_t pitch = part_pitch(N);
+  const WaveRows w{C, ldc, sC, b, M, N, rb * kFinalRows, cb * 128, rb, nullptr};
+  auto rows = [&](auto&& out) {
+    constexpr int kRows = kFinalRows / 16;
+    uint4 extra[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) extra[i] = out.fetch(w.wrow0 + ty + 16 * i);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int row = w.wrow0 + ty + 16 * i;
+      if (!out.has(row)) continue;
+      f32x4_t lo{}, hi{};
+      for (int s = 0; s < split_k; ++s) {
+        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(
+            part + ((static_cast<int64_t>(s) * batch + b) * M + row) * pitch + out.col);
+        lo += p[0];
+        hi += p[1];
+      }
+      out.row(row, extra[i], lo, hi);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lds[ty][cc + e] = out.reg[e];
+  };
+  if (ep.ragged) rows(ActLane<true>(ep, w, cc));
+  else rows(ActLane<false>(ep, w, cc));
+  if (!ep.backward || !ep.sums) return;
+  __syncthreads();
+  if (threadIdx.x < 128 && w.wcol0 + static_cast<int>(threadIdx.x) < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) s += lds[t][threadIdx.x];
+    ep.sums[(static_cast<int64_t>(b) * ep.sum_rows + rb) * ep.pitch + w.wcol0 + threadIdx.x] = s;
+  }
+}
+
+// Fallback (K == 0, leading dimensions the tiles do not take): one thread per output and 16th row,
+// fp32 accumulation in k order.
+constexpr int kSimpleRows = 32;
+__global__ __launch_bounds__(256) void act_simple(int ta, int tb, int col_blocks, int M, int N, int K,
+                                                  ActEpi ep, const uint16_t* __restrict__ A,
+                                                  int64_t lda, int64_t sA,
+                                                  const uint16_t* __restrict__ B, int64_t ldb,
+                                                  int64_t sB, uint16_t* __restrict__ C, int64_t ldc,
+                                                  int64_t sC) {
+  __shared__ float lds[16][17];
+  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  const int b = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int col = cb * 16 + tx;
+  const uint16_t* Ab = A + b * sA;
+  const uint16_t* Bb = B + b * sB;
+  float sum = 0.f;
+  for (int i = 0; i < kSimpleRows / 16; ++i) {
+    const int row = rb * kSimpleRows + ty + 16 * i;
+    if (row >= M || col >= N) continue;
+    float acc = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const float a = hk::bf16_to_f32(ta ? Ab[static_cast<int64_t>(k) * lda + row]
+                                         : Ab[static_cast<int64_t>(row) * lda + k]);
+      const float v = hk::bf16_to_f32(tb ? Bb[static_cast<int64_t>(col) * ldb + k]
+                                         : Bb[static_cast<int64_t>(k) * ldb + col]);
+      acc += a * v;
+    }
+    sum += act_element(ep, C, ldc, sC, b, row, col, acc);
+  }
+  if (!ep.backward || !ep.sums) return;
+  lds[ty][tx] = sum;
+  __syncthreads();
+  if (ty == 0 && col < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) s += lds[t][tx];
+    ep.sums[(static_cast<int64_t>(b) * ep.sum_rows + rb) * ep.pitch + col] = s;
+  }
+}
+
+// The epilogue of a one-row product, on the partials [batch][nsplit][N] of bgemv_partials. dbias: its
+// bias gradient where that is this row alone (else ep.sums takes the row).
+__global__ __launch_bounds__(256) void act_row(const float* __restrict__ part, int nsplit, int N,
+                                               ActEpi ep, uint16_t* __restrict__ C, int64_t sC,
+                                               float* __restrict__ dbias, int64_t sD,
+                                               int accumulate) {
+  const int col = blockIdx.x * 256 + threadIdx.x, b = blockIdx.z;
+  if (col >= N) return;
+  const float* p = part + static_cast<int64_t>(b) * nsplit * N + col;
+  float s = 0.f;
+  // eight loads in flight, added in split order
+  for (int k = 0; k < nsplit; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = k + u < nsplit ? p[static_cast<int64_t>(k + u) * N] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
+  const float d = act_element(ep, C, 0, sC, b, 0, col, s);
+  if (!ep.backward) return;
+  if (dbias) {
+    float* dst = dbias + b * sD + col;
+    *dst = accumulate ? *dst + d : d;
+  } else if (ep.sums) {
+    ep.sums[static_cast<int64_t>(b) * ep.pitch + col] = d;
+  }
+}
+
+// dst[y * stride + col] (+)= the sum of `rows` rows of sums[y][rows][pitch]: 32 columns a workgroup, each
+// of its 8 groups of lanes every 8th row.
+__global__ __launch_bounds__(256) void act_column_sums(const float* __restrict__ sums, int64_t rows,
+                                                       int pitch, int N, float* __restrict__ dst,
+                                                       int64_t stride, int accumulate) {
+  __shared__ float lds[8][33];
+  const int tx = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + tx;
+  const float* p = sums + static_cast<int64_t>(blockIdx.y) * rows * pitch + col;
+  float v = 0.f;
+  if (col < N)
+    for (int64_t r = grp; r < rows; r += 8) v += p[r * pitch];
+  lds[grp][tx] = v;
+  __syncthreads();
+  if (grp == 0 && col < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) s += lds[t][tx];
+    float* d = dst + blockIdx.y * stride + col;
+    *d = accumulate ? *d + s : s;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+struct Call {
+  bool ta, tb;
+  int M, N, K, batch;
+  hk_bf16 alpha;
+  const hk_bf16* A;
+  int64_t lda, sA;
+  const hk_bf16* B;
+  int64_t ldb, sB;
+  ActEpi ep;
+  hk_bf16* C;
+  int64_t ldc, sC;
+  float* dbias;
+  int64_t sD;
+  bool accumulate;
+};
+
+// How a call runs, and what it needs: the column sums of `sum_rows` blocks of rows and matrix, and the
+// partials of its k splits.
+struct Plan {
+  enum Kind { kRow, kSimple, kTiles } kind;
+  hk::GemmPlan gemm{0, 1, 0};
+  hk::GemvPlan gemv{1, 0};
+  bool ragged = false;
+  int sum_rows = 0;
+  size_t sum_bytes = 0, part_bytes = 0;
+  size_t bytes() const { return sum_bytes + part_bytes; }
+};
+
+// may_split false: k splits only where the product needs them (one row).
+Plan make_plan(const Call& c, bool may_split) {
+  Plan p;
+  const bool sums = c.ep.backward && c.dbias;
+  if (c.M == 1 && c.K > 0) {
+    p.kind = Plan::kRow;
+    p.gemv = hk::bgemv_plan(c.tb, c.N, c.K, c.batch);
+    p.part_bytes = static_cast<size_t>(c.batch) * p.gemv.nsplit * c.N * sizeof(float);
+    p.sum_rows = sums && c.batch > 1 && c.sD == 0 ? 1 : 0;
+  } else {
+    using hk::aligned16;
+    hk::GemmRows rows = hk::bgemm_rows(c.ta, c.tb, c.M, c.N, c.K, c.lda, c.ldb, c.ldc, c.sA, c.sB,
+                                       c.sC, c.batch, aligned16(c.A), aligned16(c.B), aligned16(c.C));
+    if (rows == hk::GemmRows::kNone) {
+      p.kind = Plan::kSimple;
+      p.sum_rows = static_cast<int>(hk::ceil_div(c.M, kSimpleRows));
+    } else {
+      p.kind = Plan::kTiles;
+      p.ragged = rows != hk::GemmRows::kAligned ||
+                 (c.ep.z && (c.ep.ldz % 8 != 0 || c.ep.sZ % 8 != 0 || !aligned16(c.ep.z))) ||
+                 (c.ep.residual &&
+                  (c.ep.ldr % 8 != 0 || c.ep.sR % 8 != 0 || !aligned16(c.ep.residual)));
+      p.gemm = hk::bgemm_rows_plan(c.ta, c.tb, c.M, c.N, c.K, c.batch, rows, may_split);
+      int block = kFinalRows;
+      if (p.gemm.used > 1) {
+        p.part_bytes = hk::bgemm_partial_bytes(p.gemm.used, c.M, c.N, c.batch);
+      } else if (p.gemm.flex) {
+        block = hk::bgemm_flex_tile_rows(p.gemm.flex) / 2;  // two rows of waves
+      } else {
+        block = w160_plan(c.ta, c.tb, c.M, c.N, c.K, c.batch, 1) ? w160::kWaveM
+                                                                 : row_tile(c.ta, c.M, c.N, c.batch, 1) / 2;
+      }
+      p.sum_rows = static_cast<int>(hk::ceil_div(c.M, block));
+    }
+    if (!sums) p.sum_rows = 0;
+  }
+  // both parts begin on 16 bytes: the pitch is a multiple of 8 floats
+  p.sum_bytes = static_cast<size_t>(c.batch) * p.sum_rows * part_pitch(c.N) * sizeof(float);
+  return p;
+}
+
+hipError_t column_sums(const Call& c, const float* sums, int64_t rows, hipStream_t stream) {
+  const bool shared = c.sD == 0 || c.batch == 1;
+  if (rows == 0 && c.accumulate) return hipSuccess;
+  HK_CHECK_ARG(shared || c.batch <= 65535);
+  hipLaunchKernelGGL(act_column_sums, dim3((c.N + 31) / 32, shared ? 1 : c.batch), dim3(256), 0,
+                     stream, sums, shared ? rows * c.batch : rows, part_pitch(c.N), c.N, c.dbias,
+                     c.sD, c.accumulate ? 1 : 0);
+  return hk::launch_status();
+}
+
+hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (c.N == 0) return hipSuccess;
+  if (c.M == 0 || c.batch == 0)  // no rows: a bias gradient of zero
+    return c.ep.backward && c.dbias && (c.batch > 0 || c.sD == 0)
+               ? column_sums(c, nullptr, 0, stream)
+               : hipSuccess;
+  Plan p = make_plan(c, true);
+  char* ws = static_cast<char*>(workspace);
+  if (ws) {
+    HK_CHECK_ARG(workspace_bytes >= static_cast<int64_t>(p.bytes()) && hk::aligned16(ws));
+  } else if (p.bytes() > 0) {
+    // a graph would keep the stream's workspace, which other graphs and eager calls write too
+    if (hk::stream_capturing(stream)) return hipErrorStreamCaptureUnsupported;
+    void* got = nullptr;
+    hipError_t e = hk::device_workspace(p.bytes(), stream, &got);
+    if (e == hipErrorOutOfMemory && p.kind == Plan::kTiles && p.part_bytes > 0) {
+      (void)hipGetLastError();
+      p = make_plan(c, false);  // no memory for the partials
+      e = p.bytes() > 0 ? hk::device_workspace(p.bytes(), stream, &got) : hipSuccess;
+    }
+    HK_RETURN_IF_ERROR(e);
+    ws = static_cast<char*>(got);
+  }
+  float* part = reinterpret_cast<float*>(ws + p.sum_bytes);
+  ActEpi& ep = c.ep;
+  ep.ragged = p.ragged;
+  ep.sums = p.sum_bytes > 0 ? reinterpret_cast<float*>(ws) : nullptr;
+  ep.sum_rows = p.sum_rows;
+  ep.pitch = part_pitch(c.N);
+
+  if (p.kind == Plan::kRow) {
+    // C[0][n] = sum_k op(A)[0][k] op(B)[k][n]
+    HK_RETURN_IF_ERROR(hk::bgemv_partials(c.tb, c.N, c.K, c.B, c.ldb, c.sB, c.A, c.ta ? c.lda : 1,
+                                          c.sA, c.batch, p.gemv, part, stream));
+    float* direct = ep.sums ? nullptr : c.dbias;
+    hipLaunchKernelGGL(act_row, dim3((c.N + 255) / 256, 1, c.batch), dim3(256), 0, stream, part,
+                       p.gemv.nsplit, c.N, ep, c.C, c.sC, direct, c.sD, c.accumulate ? 1 : 0);
+    HK_RETURN_IF_ERROR(hk::launch_status());
+    return ep.sums ? column_sums(c, ep.sums, 1, stream) : hipSuccess;
+  }
+  if (p.kind == Plan::kSimple) {
+    const int cols = (c.N + 15) / 16;
+    const int64_t blocks = hk::ceil_div(c.M, kSimpleRows) * cols;
+    HK_CHECK_ARG(blocks <= INT32_MAX);
+    hipLaunchKernelGGL(act_simple, dim3(static_cast<unsigned>(blocks), 1, c.batch), dim3(256), 0,
+                       stream, c.ta ? 1 : 0, c.tb ? 1 : 0, cols, c.M, c.N, c.K, ep, c.A, c.lda, c.sA,
+                       c.B, c.ldb, c.sB, c.C, c.ldc, c.sC);
+    HK_RETURN_IF_ERROR(hk::launch_status());
+  } else if (p.gemm.used > 1) {
+    const int cols = (c.N + 127) / 128;
+    const int64_t blocks = hk::ceil_div(c.M, kFinalRows) * cols;
+    HK_CHECK_ARG(blocks <= INT32_MAX);
+    HK_RETURN_IF_ERROR(hk::bgemm_write_partials(c.ta, c.tb, c.M, c.N, c.K, c.A, c.lda, c.sA, c.B, c.ldb,
+                                                c.sB, c.batch, p.gemm, part, stream));
+    hipLaunchKernelGGL(act_finalize, dim3(static_cast<unsigned>(blocks), 1, c.batch), dim3(256), 0,
+                       stream, part, p.gemm.used, cols, c.M, c.N, ep, c.C, c.ldc, c.sC);
+    HK_RETURN_IF_ERROR(hk::launch_status());
+  } else if (p.gemm.flex) {
+    FlexArgs<ActEpi> g{};
+    g.M = c.M, g.N = c.N, g.K = c.K;
+    g.ep = ep;
+    g.a = Operand{c.A, c.lda, c.sA};
+    g.b = Operand{c.B, c.ldb, c.sB};
+    g.C = c.C, g.ldc = c.ldc, g.sC = c.sC;
+    g.split_k = 1, g.k_per_split = c.K;
+    HK_RETURN_IF_ERROR(act_flex_run(p.gemm.flex, c.ta, c.tb, g, c.batch, stream));
+  } else {
+    const int64_t tiles = hk::ceil_div(c.M, BM) * hk::ceil_div(c.N, BN);
+    HK_CHECK_ARG(2 * tiles <= INT32_MAX);
+    HK_RETURN_IF_ERROR(act_wide_run(c.ta, c.tb, c.batch, stream, c.M, c.N, c.K, ep, c.A, c.lda, c.sA,
+                                    c.B, c.ldb, c.sB, c.C, c.ldc, c.sC));
+  }
+  return ep.sums ? column_sums(c, ep.sums, p.sum_rows, stream) : hipSuccess;
+}
+
+float bf16_value(hk_bf16 h) {
+  const uint32_t u = static_cast<uint32_t>(h) << 16;
+  float f;
+  __builtin_memcpy(&f, &u, 4);
+  return f;
+}
+
+// The arguments that both entry points share.
+hipError_t check(int transA, int transB, int M, int N, int K, const void* A, int lda, const void* B,
+                 int ldb, int activation, const void* C, int ldc, int batchCount) {
+  HK_CHECK_ARG(transA >= 0 && transA <= 2 && transB >= 0 && transB <= 2);
+  HK_CHECK_ARG(M >= 0 && N >= 0 && K >= 0 && batchCount >= 0 && batchCount <= kMaxGridZ);
+  HK_CHECK_ARG(activation >= HK_ACT_NONE && activation <= HK_ACT_SILU);
+  if (M == 0 || N == 0 || batchCount == 0) return hipSuccess;
+  HK_CHECK_ARG(C != nullptr && ldc >= N);
+  HK_CHECK_ARG(K == 0 || (A != nullptr && B != nullptr));
+  HK_CHECK_ARG(lda >= (transA ? M : K) && ldb >= (transB ? K : N));
+  return hipSuccess;
+}
+
+Call forward_call(int transA, int transB, int M, int N, int K, hk_bf16 alpha, const hk_bf16* A, int lda,
+                  long long strideA, const hk_bf16* B, int ldb, long long strideB,
+                  const hk_bf16* bias, long long strideBias, int activation,
+                  const hk_bf16* residual, int ldr, long long strideR, hk_bf16* preact, int ldz,
+                  long long strideZ, hk_bf16* C, int ldc, long long strideC, int batchCount) {
+  ActEpi ep{};
+  ep.alpha = bf16_value(alpha);
+  ep.act = hk::make_activation(activation);
+  ep.bias = bias, ep.sBias = strideBias;
+  ep.residual = residual, ep.ldr = ldr, ep.sR = strideR;
+  ep.z = preact, ep.ldz = ldz, ep.sZ = strideZ;
+  return Call{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
+              ep, C, ldc, strideC, nullptr, 0, false};
+}
+
+}  // namespace
+
+extern "C" hipError_t hk_bgemm_act(int transA, int transB, int M, int N, int K, hk_bf16 alpha,
+                                   const hk_bf16* A, int lda, long long strideA, const hk_bf16* B,
+                                   int ldb, long long strideB, const hk_bf16* bias,
+                                   long long strideBias, int activation, const hk_bf16* residual,
+                                   int ldr, long long strideR, hk_bf16* preact, int ldz,
+                                   long long strideZ, hk_bf16* C, int ldc, long long strideC,
+                                   int batchCount, void* workspace, int64_t workspace_bytes,
+                                   hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, batchCount));
+  HK_CHECK_ARG(!residual || ldr >= N);
+  HK_CHECK_ARG(!preact || ldz >= N);
+  return run(forward_call(transA, transB, M, N, K, alpha, A, lda, strideA, B, ldb, strideB, bias,
+                          strideBias, activation, residual, ldr, strideR, preact, ldz, strideZ, C, ldc,
+                          strideC, batchCount),
+             workspace, workspace_bytes, stream);
+}
+
+extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N, int K, hk_bf16 alpha,
+                                            const hk_bf16* A, int lda, long long strideA,
+                                            const hk_bf16* B, int ldb, long long strideB,
+                                            int activation, const hk_bf16* preact, int ldz,
+                                            long long strideZ, hk_bf16* C, int ldc,
+                                            long long strideC, float* dbias, long long strideDbias,
+                                            int accumulate, int batchCount, void* workspace,
+                                            int64_t workspace_bytes, hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, batchCount));
+  const bool empty = M == 0 || N == 0 || batchCount == 0;
+  HK_CHECK_ARG(activation == HK_ACT_NONE || empty || (preact != nullptr && ldz >= N));
+  HK_CHECK_ARG((reinterpret_cast<uintptr_t>(dbias) & 3u) == 0);
+  ActEpi ep{};
+  ep.alpha = bf16_value(alpha);
+  ep.act = hk::make_activation(activation);
+  ep.backward = true;
+  ep.z = activation == HK_ACT_NONE ? nullptr : const_cast<hk_bf16*>(preact);
+  ep.ldz = ldz, ep.sZ = strideZ;
+  return run(Call{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
+                  ep, C, ldc, strideC, dbias, strideDbias, accumulate != 0},
+             workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t hk_bgemm_act_workspace(int transA, int transB, int M, int N, int K, int batchCount,
+                                          int dbias) {
+  if (transA < 0 || transA > 2 || transB < 0 || transB > 2 || M < 0 || N < 0 || K < 0 ||
+      batchCount < 0 || batchCount > kMaxGridZ)
+    return -1;
+  if (M == 0 || N == 0 || batchCount == 0) return 0;
+  // the most of what the rows' alignments make of the call
+  Call c{};
+  c.ta = transA != 0, c.tb = transB != 0;
+  c.M = M, c.N = N, c.K = K, c.batch = batchCount;
+  c.ep.backward = dbias != 0;
+  float none;
+  c.dbias = dbias ? &none : nullptr;  // compared with NULL only
+  size_t most = 0;
+  for (int odd = 0; odd < 4; ++odd) {
+    // aligned, unaligned C, unaligned A and B, and the fallback's leading dimensions
+    c.lda = (odd == 3 ? int64_t{1} << 22 : hk::ceil_div(c.ta ? M : K, 8) * 8) + (odd == 2 ? 1 : 0);
+    c.ldb = hk::ceil_div(c.tb ? K : N, 8) * 8;
+    c.ldc = hk::ceil_div(N, 8) * 8 + (odd == 1 ? 1 : 0);
+    const size_t bytes = make_plan(c, true).bytes();
+    if (bytes > most) most = bytes;
+  }
+  return static_cast<int64_t>(most);
+}

@@ -307,8 +307,9 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
         M, N, wrow0, wcol0);
     return;
   }
-  store_bf16<T::kWaveN, kBlkM>(acc, area, lane, g.ep, g.C + batch * g.sC, g.ldc, M, N, wrow0,
-                               wcol0);
+  store_bf16<T::kWaveN, kBlkM>(
+      acc, lane, g.ep,
+      WaveRows{g.C, g.ldc, g.sC, batch, M, N, wrow0, wcol0, tm * T::WM + wm, area});
 }
 
 template <class T, bool AK, bool BKM, bool RAGGED, class E>

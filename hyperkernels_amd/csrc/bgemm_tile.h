@@ -295,26 +295,36 @@ struct Bf16RowOut {
   }
 };
 
-// Writes a wave's accumulators to C through the form the call needs.
-template <int kWaveN, int kBlkM>
-__device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32],
-                                           unsigned char HK_LDS* area, int lane, const Epi& ep,
-                                           uint16_t* Cb, int64_t ldc, int M, int N, int wrow0,
-                                           int wcol0) {
+// Where a wave's rows of C lie: its first row and column, its index among the blocks of wave rows that cover
+// M, and the LDS area that staged its rows.
+struct WaveRows {
+  uint16_t* C;
+  int64_t ldc, sC;
+  int batch, M, N, wrow0, wcol0, wave_row;
+  unsigned char HK_LDS* area;
+};
+// Writes a wave's rows to C through the form the call needs: emit(out) hands every group of 8 columns to out;
+// LPR lanes hold a row.
+template <int LPR, class Emit>
+__device__ __forceinline__ void emit_rows(const Epi& ep, const WaveRows& w, int, Emit&& emit) {
+  uint16_t* Cb = w.C + static_cast<int64_t>(w.batch) * w.sC;
   if (ep.ragged) {
     if (ep.bias)
-      staged_rows<kWaveN, kBlkM>(acc, area, lane,
-                                 Bf16RowOut<true, true>{ep, Cb, ldc, M, N, wrow0, wcol0});
+      emit(Bf16RowOut<true, true>{ep, Cb, w.ldc, w.M, w.N, w.wrow0, w.wcol0});
     else
-      staged_rows<kWaveN, kBlkM>(acc, area, lane,
-                                 Bf16RowOut<false, true>{ep, Cb, ldc, M, N, wrow0, wcol0});
+      emit(Bf16RowOut<false, true>{ep, Cb, w.ldc, w.M, w.N, w.wrow0, w.wcol0});
   } else if (ep.bias) {
-    staged_rows<kWaveN, kBlkM>(acc, area, lane,
-                               Bf16RowOut<true>{ep, Cb, ldc, M, N, wrow0, wcol0});
+    emit(Bf16RowOut<true>{ep, Cb, w.ldc, w.M, w.N, w.wrow0, w.wcol0});
   } else {
-    staged_rows<kWaveN, kBlkM>(acc, area, lane,
-                               Bf16RowOut<false>{ep, Cb, ldc, M, N, wrow0, wcol0});
+    emit(Bf16RowOut<false>{ep, Cb, w.ldc, w.M, w.N, w.wrow0, w.wcol0});
   }
+}
+template <int kWaveN, int kBlkM>
+__device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
+                                           const Epi& ep, const WaveRows& w) {
+  emit_rows<kWaveN / 8>(ep, w, lane, [&](auto&& out) {
+    staged_rows<kWaveN, kBlkM>(acc, w.area, lane, out);
+  });
 }
 
 // fp32 output: C = alpha * acc + beta * C + bias_scale * bias (hk::F32Out), N % 8 == 0.

@@ -267,8 +267,8 @@ __device__ __forceinline__ void tile_body(
         N, wrow0, wcol0);
     return;
   }
-  uint16_t* Cb = C + static_cast<int64_t>(batch) * sC;
-  store_bf16<kWaveN, kBlkM>(acc, area, lane, ep, Cb, ldc, M, N, wrow0, wcol0);
+  store_bf16<kWaveN, kBlkM>(acc, lane, ep,
+                            WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 2 * tm + wm, area});
 }
 
 // One column region: workgroup x takes tile x.
@@ -489,7 +489,6 @@ __global__ __launch_bounds__(kThreads, 1) void bgemm_nt_w160(
   // bf16 outputs go out 16 bytes per lane in row segments.
   __syncthreads();
   unsigned char HK_LDS* area = lds + wave * (16 * kPitch);
-  uint16_t* Cb = C + static_cast<int64_t>(batch) * sC;
   const int wrow0 = m0 + wm * kWaveM, wcol0 = n0 + wn * kWaveN;
   auto emit = [&](auto&& out) {
 #pragma unroll
@@ -510,16 +509,8 @@ __global__ __launch_bounds__(kThreads, 1) void bgemm_nt_w160(
       }
     }
   };
-  if (ep.ragged) {
-    if (ep.bias)
-      emit(Bf16RowOut<true, true>{ep, Cb, ldc, M, N, wrow0, wcol0});
-    else
-      emit(Bf16RowOut<false, true>{ep, Cb, ldc, M, N, wrow0, wcol0});
-  } else if (ep.bias) {
-    emit(Bf16RowOut<true>{ep, Cb, ldc, M, N, wrow0, wcol0});
-  } else {
-    emit(Bf16RowOut<false>{ep, Cb, ldc, M, N, wrow0, wcol0});
-  }
+  emit_rows<kWaveN / 8>(ep, WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 4 * tm + wm, area}, lane,
+                        emit);
 }
 
 // BNT 256 or 128: one column region (bgemm_tiled); BNT 0: both regions (bgemm_mixed), with

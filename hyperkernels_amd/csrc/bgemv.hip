@@ -320,39 +320,13 @@ void pick_split(int64_t groups, int64_t target, int K, int min_k, int align, int
   *nsplit = static_cast<int>(K == 0 ? 1 : hk::ceil_div(K, chunk));
 }
 
-}  // namespace
-
-namespace hk {
-
-hipError_t bgemv_run(bool dot_form, int R, int K, hk_bf16 alpha, hk_bf16 beta,
-                     const hk_bf16* mtx, int64_t ld, int64_t sm, const hk_bf16* x, int64_t incx,
-                     int64_t sx, hk_bf16* y, int64_t incy, int64_t sy, int batch,
-                     hipStream_t stream) {
-  HK_CHECK_ARG(R >= 0 && K >= 0 && batch >= 0);
-  if (R == 0 || batch == 0) return hipSuccess;
-  HK_CHECK_ARG(y != nullptr && (K == 0 || (mtx != nullptr && x != nullptr)));
-  HK_CHECK_ARG(batch <= 65535);
-  Out out{bf16_bits_to_float(alpha), bf16_bits_to_float(beta), y, incy, sy, nullptr, 1};
+// The products of one plan, written as `out` says.
+hipError_t launch(bool dot_form, int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
+                  const hk_bf16* x, int64_t incx, int64_t sx, int batch, const hk::GemvPlan& plan,
+                  const Out& out, hipStream_t stream) {
   const int64_t strips = dot_form ? hk::ceil_div(R, kDotRows) : hk::ceil_div(R, kColsPerWave);
   HK_CHECK_ARG(strips <= INT32_MAX);
-  // Batches of one matrix launch fewer workgroups than are counted here (gemv_dot_shared). Counting
-  // those launched splits k further, which the finalize outweighs (MI355X, us: 20000 x 1024, two
-  // vectors 9.3 -> 11.2; 12000 x 1024, four 9.3 -> 11.1; the other way 5000 x 4096, four 17.8 -> 15.5).
-  int nsplit = 1, kchunk = K;
-  if (dot_form)
-    pick_split(strips * batch, kDotTargetGroups, K, 4 * kDotStep, kDotStep, &nsplit, &kchunk);
-  else
-    pick_split(strips * batch, kBcastTargetGroups, K, kUnroll * kWaves, kWaves, &nsplit,
-               &kchunk);
-  HK_CHECK_ARG(nsplit <= 65535);
-  if (nsplit > 1) {
-    void* ws = nullptr;
-    HK_RETURN_IF_ERROR(hk::device_workspace(
-        static_cast<size_t>(batch) * nsplit * R * sizeof(float), stream, &ws));
-    out.part = static_cast<float*>(ws);
-    out.nsplit = nsplit;
-  }
-  dim3 grid(static_cast<unsigned>(strips), static_cast<unsigned>(nsplit),
+  dim3 grid(static_cast<unsigned>(strips), static_cast<unsigned>(plan.nsplit),
             static_cast<unsigned>(batch));
   if (dot_form) {
     const bool vec = ld % 8 == 0 && sm % 8 == 0 && sx % 8 == 0 && hk::aligned16(mtx) &&
@@ -367,22 +341,70 @@ hipError_t bgemv_run(bool dot_form, int R, int K, hk_bf16 alpha, hk_bf16 beta,
       auto* k = rows == kElements  ? (two ? gemv_dot_shared<kElements, 2> : gemv_dot_shared<kElements, 4>)
                 : rows == kAligned ? (two ? gemv_dot_shared<kAligned, 2> : gemv_dot_shared<kAligned, 4>)
                                    : (two ? gemv_dot_shared<kAnywhere, 2> : gemv_dot_shared<kAnywhere, 4>);
-      hipLaunchKernelGGL(k, grid, dim3(kThreads), 0, stream, R, K, kchunk, batch, mtx, ld, x, incx,
+      hipLaunchKernelGGL(k, grid, dim3(kThreads), 0, stream, R, K, plan.kchunk, batch, mtx, ld, x, incx,
                          sx, out);
     } else {
       auto* k = rows == kElements  ? gemv_dot<kElements>
                 : rows == kAligned ? gemv_dot<kAligned>
                                    : gemv_dot<kAnywhere>;
-      hipLaunchKernelGGL(k, grid, dim3(kThreads), 0, stream, R, K, kchunk, mtx, ld, sm, x, incx, sx,
+      hipLaunchKernelGGL(k, grid, dim3(kThreads), 0, stream, R, K, plan.kchunk, mtx, ld, sm, x, incx, sx,
                          out);
     }
   } else {
     const bool vec = ld % 8 == 0 && sm % 8 == 0 && hk::aligned16(mtx);
     hipLaunchKernelGGL(vec ? gemv_bcast<kAligned> : gemv_bcast<kAnywhere>, grid, dim3(kBcastThreads), 0,
-                       stream, R, K, kchunk, mtx, ld, sm, x, incx, sx, out);
+                       stream, R, K, plan.kchunk, mtx, ld, sm, x, incx, sx, out);
   }
-  HK_RETURN_IF_ERROR(hk::launch_status());
-  if (nsplit > 1) {
+  return hk::launch_status();
+}
+
+}  // namespace
+
+namespace hk {
+
+GemvPlan bgemv_plan(bool dot_form, int R, int K, int batch) {
+  // Batches of one matrix launch fewer workgroups than are counted here (gemv_dot_shared). Counting
+  // those launched splits k further, which the finalize outweighs (MI355X, us: 20000 x 1024, two
+  // vectors 9.3 -> 11.2; 12000 x 1024, four 9.3 -> 11.1; the other way 5000 x 4096, four 17.8 -> 15.5).
+  const int64_t strips = dot_form ? hk::ceil_div(R, kDotRows) : hk::ceil_div(R, kColsPerWave);
+  GemvPlan p{1, K};
+  if (dot_form)
+    pick_split(strips * batch, kDotTargetGroups, K, 4 * kDotStep, kDotStep, &p.nsplit, &p.kchunk);
+  else
+    pick_split(strips * batch, kBcastTargetGroups, K, kUnroll * kWaves, kWaves, &p.nsplit,
+               &p.kchunk);
+  return p;
+}
+
+hipError_t bgemv_partials(bool dot_form, int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
+                          const hk_bf16* x, int64_t incx, int64_t sx, int batch,
+                          const GemvPlan& plan, float* part, hipStream_t stream) {
+  HK_CHECK_ARG(R > 0 && K >= 0 && batch > 0 && batch <= 65535 && part != nullptr);
+  HK_CHECK_ARG(plan.nsplit >= 1 && plan.nsplit <= 65535);
+  return launch(dot_form, R, K, mtx, ld, sm, x, incx, sx, batch, plan,
+                Out{1.0f, 0.0f, nullptr, 1, 0, part, plan.nsplit}, stream);
+}
+
+hipError_t bgemv_run(bool dot_form, int R, int K, hk_bf16 alpha, hk_bf16 beta,
+                     const hk_bf16* mtx, int64_t ld, int64_t sm, const hk_bf16* x, int64_t incx,
+                     int64_t sx, hk_bf16* y, int64_t incy, int64_t sy, int batch,
+                     hipStream_t stream) {
+  HK_CHECK_ARG(R >= 0 && K >= 0 && batch >= 0);
+  if (R == 0 || batch == 0) return hipSuccess;
+  HK_CHECK_ARG(y != nullptr && (K == 0 || (mtx != nullptr && x != nullptr)));
+  HK_CHECK_ARG(batch <= 65535);
+  Out out{bf16_bits_to_float(alpha), bf16_bits_to_float(beta), y, incy, sy, nullptr, 1};
+  const GemvPlan plan = bgemv_plan(dot_form, R, K, batch);
+  HK_CHECK_ARG(plan.nsplit <= 65535);
+  if (plan.nsplit > 1) {
+    void* ws = nullptr;
+    HK_RETURN_IF_ERROR(hk::device_workspace(
+        static_cast<size_t>(batch) * plan.nsplit * R * sizeof(float), stream, &ws));
+    out.part = static_cast<float*>(ws);
+    out.nsplit = plan.nsplit;
+  }
+  HK_RETURN_IF_ERROR(launch(dot_form, R, K, mtx, ld, sm, x, incx, sx, batch, plan, out, stream));
+  if (plan.nsplit > 1) {
     const int64_t total = static_cast<int64_t>(R) * batch;
     hipLaunchKernelGGL(gemv_finalize, dim3(static_cast<unsigned>(hk::ceil_div(total, kThreads))),
                        dim3(kThreads), 0, stream, R, batch, out);

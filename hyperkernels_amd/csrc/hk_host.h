@@ -48,6 +48,16 @@ hipError_t bgemv_run(bool dot_form, int R, int K, hk_bf16 alpha, hk_bf16 beta,
                      int64_t sx, hk_bf16* y, int64_t incy, int64_t sy, int batch,
                      hipStream_t stream);
 
+// The same product without its epilogue, for one of the caller's own: the sums of plan.nsplit k ranges as
+// fp32 partials part[batch][nsplit][R], to be added in split order.
+struct GemvPlan {
+  int nsplit, kchunk;
+};
+GemvPlan bgemv_plan(bool dot_form, int R, int K, int batch);
+hipError_t bgemv_partials(bool dot_form, int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
+                          const hk_bf16* x, int64_t incx, int64_t sx, int batch,
+                          const GemvPlan& plan, float* part, hipStream_t stream);
+
 // fp32 output written straight from the BF16 GEMM tiles when the product has one split:
 // C[b][row][col] = alpha * acc + beta * C (C not read when beta == 0) + bias_scale * bias, the
 // bias selected by bias_stride as hk_sgemm does (N: bias[col]; M*N: bias[(b % M) * N + col];

@@ -477,8 +477,13 @@ extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, 
   if (sums && g.side[0].rows + g.side[1].rows > 0) {
     const size_t bytes = partial_bytes(g);
     void* ws = workspace;
-    if (ws) HK_CHECK_ARG(workspace_bytes >= static_cast<int64_t>(bytes) && aligned_to(ws, 4));
-    else HK_RETURN_IF_ERROR(hk::device_workspace(bytes, stream, &ws));
+    if (ws) {
+      HK_CHECK_ARG(workspace_bytes >= static_cast<int64_t>(bytes) && aligned_to(ws, 4));
+    } else {
+      // a graph would keep the stream's workspace, which other graphs and eager calls write too
+      if (hk::stream_capturing(stream)) return hipErrorStreamCaptureUnsupported;
+      HK_RETURN_IF_ERROR(hk::device_workspace(bytes, stream, &ws));
+    }
     float* part = static_cast<float*>(ws);
     for (int i = 0; i < 2; ++i) {
       if (w.dw[i]) w.part[i] = g.side[i].part = part;

@@ -16,7 +16,7 @@ import torch
 from ._lib import HKError, call, lib  # noqa: F401
 
 __all__ = [
-    "HKError", "gelu_forward", "gelu_backward", "layer_norm_forward", "ln_backward_input",
+    "HKError", "gelu_forward", "gelu_backward", "bgemm_act", "bgemm_act_backward", "layer_norm_forward", "ln_backward_input",
     "ln_backward_gamma_beta", "layer_norm_backward", "sparse_ce_forward", "sparse_ce_backward",
     "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "Adam8Plan", "ADAM8_BLOCK",
     "adam8_states", "adam8_quantize", "adam8_dequantize", "qk_norm_rope_forward",
@@ -497,6 +497,109 @@ def attn_backward(q, k, v, do, lse, D, causal: bool, scale: float | None = None,
 
 
 # ----------------------------------------------------------------------------------------------
+# BF16 GEMM with bias, activation and residual in its epilogue, and its backward product (no
+# counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+_ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}  # HK_ACT_*
+
+
+def _matrix(fn: str, t: torch.Tensor, batch: int, rows: int, cols: int) -> tuple[int, int]:
+    """(leading dimension, batch stride) of a bf16 matrix [rows, cols], or [batch, rows, cols]."""
+    sh, st = t.shape, t.stride()
+    if t.dtype != torch.bfloat16 or sh not in ((rows, cols), (batch, rows, cols)) or (
+            len(sh) == 2 and batch != 1) or (st[-1] != 1 and cols > 1):
+        raise ValueError(f"{fn}: bf16 matrices of matching shapes with a unit last-dim stride; "
+                         f"[{batch}, {rows}, {cols}] expected, {tuple(sh)} given")
+    ld = st[-2] if rows > 1 else max(st[-2], cols)
+    return ld, st[0] if len(sh) == 3 and batch > 1 else 0
+
+
+def _product(fn: str, a, b, trans_a: bool, trans_b: bool, activation: str):
+    """(batch, M, N, K) of op(a) op(b)."""
+    if a.dim() != b.dim() or a.dim() not in (2, 3) or activation not in _ACT:
+        raise ValueError(f"{fn}: matrices or batches of them, and one of {', '.join(_ACT)}")
+    M, K = (a.shape[-1], a.shape[-2]) if trans_a else (a.shape[-2], a.shape[-1])
+    N = b.shape[-2] if trans_b else b.shape[-1]
+    return (a.shape[0] if a.dim() == 3 else 1), M, N, K
+
+
+def _own_workspace(need) -> tuple[torch.Tensor | None, int]:
+    """Under capture the bytes of need() in a tensor of the graph's; otherwise none: the library's."""
+    if not torch.cuda.is_current_stream_capturing():
+        return None, 0
+    n = max(0, need())
+    return (torch.empty(n, device="cuda", dtype=torch.uint8) if n else None), n
+
+
+def _bf16_bits(x: float) -> int:
+    return 0x3F80 if x == 1.0 else int(
+        torch.tensor(x, dtype=torch.bfloat16).view(torch.int16)) & 0xFFFF
+
+
+def bgemm_act(a, b, bias=None, activation: str = "none", residual=None, preact=None, out=None,
+              trans_a: bool = False, trans_b: bool = False, alpha: float = 1.0):
+    """act(alpha op(a) op(b) + bias) + residual for bf16 matrices [rows, cols] or batches of them; what
+    goes into the activation ("none", "relu", "gelu" or "silu") is stored in `preact` where that is
+    passed. bias is [N], or [batch, N]; residual may be `out` itself."""
+    fn = "bgemm_act"
+    batch, M, N, K = _product(fn, a, b, trans_a, trans_b, activation)
+    if out is None:
+        out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
+                          dtype=torch.bfloat16)
+    _here(fn, a, b, bias, residual, preact, out)
+    lda, sA = _matrix(fn, a, batch, K if trans_a else M, M if trans_a else K)
+    ldb, sB = _matrix(fn, b, batch, N if trans_b else K, K if trans_b else N)
+    ldc, sC = _matrix(fn, out, batch, M, N)
+    ldr, sR = (0, 0) if residual is None else _matrix(fn, residual, batch, M, N)
+    ldz, sZ = (0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
+    sbias = 0
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.shape not in ((N,), (batch, N)) or (
+                bias.stride(-1) != 1 and N > 1):
+            raise ValueError(f"{fn}: bias is bf16 [N] or [batch, N]")
+        sbias = bias.stride(0) if bias.dim() == 2 and batch > 1 else 0
+    ws, n = _own_workspace(lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch, 0))
+    call("hk_bgemm_act", trans_a, trans_b, M, N, K, _bf16_bits(alpha), a.data_ptr(), lda, sA,
+         b.data_ptr(), ldb, sB, _ptr(bias), sbias, _ACT[activation], _ptr(residual), ldr, sR,
+         _ptr(preact), ldz, sZ, out.data_ptr(), ldc, sC, batch, _ptr(ws), n, _stream())
+    return out
+
+
+def bgemm_act_backward(a, b, preact=None, activation: str = "none", dbias=None, out=None,
+                       trans_a: bool = False, trans_b: bool = False, alpha: float = 1.0,
+                       accumulate: bool = True):
+    """d = alpha op(a) op(b) * act'(preact) in bf16: the gradient of a layer's pre-activation, from the
+    gradient behind the next layer and that layer's weights. dbias (fp32 [N], or [batch, N]; None: not
+    wanted) is added to, or written where accumulate is False: the sums of d over rows (and, [N],
+    batches) before it is rounded."""
+    fn = "bgemm_act_backward"
+    batch, M, N, K = _product(fn, a, b, trans_a, trans_b, activation)
+    if out is None:
+        out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
+                          dtype=torch.bfloat16)
+    _here(fn, a, b, preact, dbias, out)
+    lda, sA = _matrix(fn, a, batch, K if trans_a else M, M if trans_a else K)
+    ldb, sB = _matrix(fn, b, batch, N if trans_b else K, K if trans_b else N)
+    ldc, sC = _matrix(fn, out, batch, M, N)
+    if preact is None and activation != "none":
+        raise ValueError(f"{fn}: the activation's derivative needs preact")
+    ldz, sZ = (0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
+    sD = 0
+    if dbias is not None:
+        if dbias.dtype != torch.float32 or dbias.shape not in ((N,), (batch, N)) or (
+                dbias.stride(-1) != 1 and N > 1) or (
+                dbias.dim() == 2 and batch > 1 and dbias.stride(0) < N):
+            raise ValueError(f"{fn}: dbias is fp32 [N] or [batch, N]")
+        sD = dbias.stride(0) if dbias.dim() == 2 and batch > 1 else 0
+    ws, n = _own_workspace(lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch,
+                                                                dbias is not None))
+    call("hk_bgemm_act_backward", trans_a, trans_b, M, N, K, _bf16_bits(alpha), a.data_ptr(), lda,
+         sA, b.data_ptr(), ldb, sB, _ACT[activation], _ptr(preact), ldz, sZ, out.data_ptr(), ldc,
+         sC, _ptr(dbias), sD, accumulate, batch, _ptr(ws), n, _stream())
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
 # RMS norm of query and key heads with the position rotation (no counterpart in the reference)
 # ----------------------------------------------------------------------------------------------
 class QkNormRopeParams(ctypes.Structure):
@@ -597,11 +700,8 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=No
     p = _qk_params("qk_norm_rope_backward", q, k, cos, sin, positions, q_weight, k_weight, eps,
                    interleaved, dq_out, dk_out, True, dq, dk, grad_q_weight, grad_k_weight,
                    accumulate)
-    x, ws, n = (q if q is not None else k), None, 0
-    if grad_q_weight is not None or grad_k_weight is not None:
-        # the call's own partial sums: captured graphs and other streams have theirs
-        n = max(0, lib().hk_qk_norm_rope_workspace(ctypes.byref(p), _TYPE[x.dtype]))
-        ws = torch.empty(n, device=x.device, dtype=torch.uint8) if n else None
+    x = q if q is not None else k
+    ws, n = _own_workspace(lambda: lib().hk_qk_norm_rope_workspace(ctypes.byref(p), _TYPE[x.dtype]))
     call("hk_qk_norm_rope_backward", ctypes.byref(p), _TYPE[x.dtype], _ptr(ws), n, _stream())
     return dq, dk
 

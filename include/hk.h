@@ -450,6 +450,50 @@ HK_API hipError_t hk_bgemm_core_bias(int layout, int splitK, int M, int N, int K
                                      long long strideC, int batchCount, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * BF16 GEMM with bias, activation and residual in its epilogue, and the product of its backward pass
+ * with the activation's derivative and the bias gradient in its own. No counterpart in the reference.
+ *   hk_bgemm_act           z = alpha * op(A) op(B) + bias[col];  preact = z;  C = act(z) + residual
+ *   hk_bgemm_act_backward  d = alpha * op(A) op(B) * act'(preact);  C = d;
+ *                          dbias[col] = the sum of d over rows (added to dbias where accumulate != 0)
+ * A hidden layer h = act(x W + b) is the first with A = x, B = W; the gradient of its pre-activation the
+ * second with A the gradient behind the next layer and B that layer's weights, transposed as needed.
+ * Layouts, extents, leading dimensions, strides and alignment as for hk_bgemm (at most 65,535 batches);
+ * bf16 everywhere but dbias (fp32). Everything is fp32 until C and preact are rounded, once each: the
+ * activation takes z and dbias takes d before that. bias (N elements a batch, strideBias apart, 0: one
+ * for all), residual and preact (M x N like C, leading dimensions ldr and ldz) may be NULL; preact is
+ * needed by hk_bgemm_act_backward unless the activation is HK_ACT_NONE. residual may be C itself.
+ * dbias may be NULL; strideDbias 0 sums over the batches too. GELU is the tanh form, as in
+ * hk_gelu_forward. Sums are in a fixed order.
+ * The k splits of some products and the bias gradient take device memory, hk_bgemm_act_workspace bytes
+ * at most (whatever the alignment of the rows; dbias: whether one is wanted; -1 for an invalid
+ * argument): at `workspace` (16-byte aligned), or, where that is NULL, in the stream's workspace. A
+ * call that needs some and is captured into a graph brings its own
+ * (hipErrorStreamCaptureUnsupported otherwise): graphs captured on one stream would share the stream's.
+ * ---------------------------------------------------------------------------------------- */
+#define HK_ACT_NONE 0
+#define HK_ACT_RELU 1
+#define HK_ACT_GELU 2
+#define HK_ACT_SILU 3
+HK_API hipError_t hk_bgemm_act(int transA, int transB, int M, int N, int K, hk_bf16 alpha,
+                               const hk_bf16* A, int lda, long long strideA, const hk_bf16* B,
+                               int ldb, long long strideB, const hk_bf16* bias,
+                               long long strideBias, int activation, const hk_bf16* residual,
+                               int ldr, long long strideR, hk_bf16* preact, int ldz,
+                               long long strideZ, hk_bf16* C, int ldc, long long strideC,
+                               int batchCount, void* workspace, int64_t workspace_bytes,
+                               hipStream_t stream);
+HK_API hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N, int K, hk_bf16 alpha,
+                                        const hk_bf16* A, int lda, long long strideA,
+                                        const hk_bf16* B, int ldb, long long strideB,
+                                        int activation, const hk_bf16* preact, int ldz,
+                                        long long strideZ, hk_bf16* C, int ldc, long long strideC,
+                                        float* dbias, long long strideDbias, int accumulate,
+                                        int batchCount, void* workspace, int64_t workspace_bytes,
+                                        hipStream_t stream);
+HK_API int64_t hk_bgemm_act_workspace(int transA, int transB, int M, int N, int K, int batchCount,
+                                      int dbias);
+
+/* ------------------------------------------------------------------------------------------
  * FP32 batched GEMM with fp32-class products (the reference uses single-pass TF32; gfx950 has no
  * TF32 MFMA): a bf16x3 split on the bf16 MFMA (x = hi + lo, a b = ah bh + ah bl + al bh, relative
  * error ~1e-5) when every dimension is a multiple of 8, exact fp32 MFMA products otherwise,
@@ -606,8 +650,8 @@ HK_API hipError_t hk_attn_backward_set(const hk_attn_bwd_params* params, int hea
  *   dq_weight and dk_weight (fp32, NULL: not wanted) are written, or added to where accumulate is
  *   set, summed over tokens and heads in a fixed order. The partial sums take
  *   hk_qk_norm_rope_workspace bytes (0 where neither is wanted, -1 for invalid arguments): at
- *   `workspace`, or in the stream's workspace where that is NULL. A call that is captured into a graph
- *   should bring its own, since graphs captured on one stream share the stream's.
+ *   `workspace`, or in the stream's workspace where that is NULL. A call that needs some and is captured
+ *   into a graph brings its own, as for hk_bgemm_act.
  * ---------------------------------------------------------------------------------------- */
 typedef struct hk_qk_norm_rope_params {
   const void* q;

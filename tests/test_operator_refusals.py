@@ -151,3 +151,44 @@ def test_qk_parameter_block_matches_the_header(tmp_path):
     got = list(map(int, subprocess.run([str(tmp_path / "probe")], capture_output=True, text=True,
                                        check=True).stdout.split()))
     assert got == [ctypes.sizeof(P)] + [getattr(P, n).offset for n in fields]
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_bgemm_act_refuses(L, backward):
+    def go(ta=0, tb=0, M=4, N=8, K=16, A=64, lda=16, B=64, ldb=8, act=2, res=64, ldr=8, Z=64, ldz=8,
+           C=64, ldc=8, dbias=64, batch=1, ws=0, ws_bytes=0):
+        if backward:
+            return L.hk_bgemm_act_backward(ta, tb, M, N, K, 0x3F80, A, lda, 0, B, ldb, 0, act, Z, ldz,
+                                           0, C, ldc, 0, dbias, 0, 0, batch, ws, ws_bytes, NULL)
+        return L.hk_bgemm_act(ta, tb, M, N, K, 0x3F80, A, lda, 0, B, ldb, 0, 64, 0, act, res, ldr, 0,
+                              Z, ldz, 0, C, ldc, 0, batch, ws, ws_bytes, NULL)
+
+    bad = [dict(ta=3), dict(ta=-1), dict(tb=3), dict(M=-1), dict(N=-1), dict(K=-1), dict(A=0),
+           dict(B=0), dict(C=0), dict(lda=15), dict(ldb=7), dict(ldc=7), dict(act=4), dict(act=-1),
+           dict(batch=-1), dict(batch=65536), dict(ldz=7), dict(ta=1, lda=3), dict(tb=1, ldb=15)]
+    bad += [dict(Z=0), dict(dbias=66)] if backward else [dict(ldr=7)]
+    for kw in bad:
+        assert go(**kw) == INVALID, kw
+    if not backward:
+        assert go(M=0, A=0, B=0, C=0) == 0 and go(N=0) == 0 and go(batch=0) == 0
+    for n in ((3, 0, 4, 8, 16, 1, 0), (0, -1, 4, 8, 16, 1, 0), (0, 0, -1, 8, 16, 1, 0),
+              (0, 0, 4, -8, 16, 1, 0), (0, 0, 4, 8, -1, 1, 0), (0, 0, 4, 8, 16, -1, 0),
+              (0, 0, 4, 8, 16, 65536, 0)):
+        assert L.hk_bgemm_act_workspace(*n) == -1
+    assert L.hk_bgemm_act_workspace(0, 0, 0, 8, 16, 1, 1) == 0
+    assert L.hk_bgemm_act_workspace(0, 0, 4, 8, 16, 1, 1) > 0
+
+
+def test_bgemm_act_front_end_refuses():
+    from hyperkernels_amd import kernels as hk
+
+    bf = torch.bfloat16
+    a, b = torch.zeros(4, 16, dtype=bf), torch.zeros(16, 8, dtype=bf)
+    with pytest.raises(ValueError):
+        hk.bgemm_act(a, b)  # host tensors
+    with pytest.raises(ValueError):
+        hk.bgemm_act(a, b, activation="tanh")
+    with pytest.raises(ValueError):
+        hk.bgemm_act(a[None], b)
+    with pytest.raises(ValueError):
+        hk.bgemm_act_backward(a, b)
