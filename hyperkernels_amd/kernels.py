@@ -9,11 +9,12 @@ path.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Sequence
 
 import torch
 
-from ._lib import HKError, call, lib  # noqa: F401
+from ._lib import HKError, _fns, call, lib  # noqa: F401
 
 __all__ = [
     "HKError", "gelu_forward", "gelu_backward", "bgemm_act", "bgemm_act_backward", "layer_norm_forward", "ln_backward_input",
@@ -53,13 +54,14 @@ _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HK_TYPE_*
 
 def _here(fn: str, *ts: torch.Tensor | None) -> None:
     """Device tensors of the current device, whose stream the launch goes to."""
+    cur = None
     for t in ts:
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"{fn}: device tensors only")
-    cur = torch._C._cuda_getDevice()
-    for t in ts:
-        if t is not None and t.get_device() != cur:
-            raise ValueError(f"{fn}: tensors of the current device (cuda:{cur}) only")
+        if t is not None:
+            d = t.get_device()  # -1: a host tensor
+            if d != cur:
+                if cur is not None or d < 0 or d != torch._C._cuda_getDevice():
+                    raise ValueError(f"{fn}: tensors of the current device only")
+                cur = d
 
 
 # ----------------------------------------------------------------------------------------------
@@ -295,15 +297,21 @@ ADAM8_BLOCK = 256
 
 
 def _adam8_check(fn: str, m, v, m_scale, v_scale, blocks: int) -> None:
-    _dev(m, v, m_scale, v_scale)
-    _here(fn, m, v, m_scale, v_scale)
-    if m.dtype != torch.int8 or v.dtype != torch.uint8 or m_scale.dtype != torch.float32 or (
-            v_scale.dtype != torch.float32):
+    if m.dtype is not torch.int8 or v.dtype is not torch.uint8 or (
+            m_scale.dtype is not torch.float32) or v_scale.dtype is not torch.float32:
         raise ValueError(f"{fn}: m int8, v uint8, m_scale and v_scale fp32")
-    if m.numel() != blocks * ADAM8_BLOCK or v.numel() != m.numel() or not (
-            m_scale.numel() == v_scale.numel() == blocks):
-        raise ValueError(f"{fn}: {blocks} blocks need {blocks * ADAM8_BLOCK} codes and {blocks} "
-                         "scales of each moment")
+    n = blocks * ADAM8_BLOCK
+    if m.numel() != n or v.numel() != n or m_scale.numel() != blocks or (
+            v_scale.numel() != blocks):
+        raise ValueError(f"{fn}: {blocks} blocks need {n} codes and {blocks} scales of each moment")
+
+
+def _flat(fn: str, *ts: torch.Tensor | None) -> None:
+    """Contiguous tensors of the current device."""
+    _here(fn, *ts)
+    for t in ts:
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{fn}: contiguous tensors only")
 
 
 def adam8_states(sizes: Sequence[int], device="cuda"):
@@ -318,13 +326,13 @@ def adam8_states(sizes: Sequence[int], device="cuda"):
 def adam8_quantize(m, v, states=None):
     """8-bit states (m, v, m_scale, v_scale) of fp32 moments of one tensor (or of several that each
     begin on a block)."""
-    _dev(m, v)
-    _here("adam8_quantize", m, v)
-    if m.dtype != torch.float32 or v.dtype != torch.float32 or m.numel() != v.numel():
+    n = m.numel()
+    if m.dtype is not torch.float32 or v.dtype is not torch.float32 or v.numel() != n:
         raise ValueError("adam8_quantize: fp32 moments of equal size")
-    states = adam8_states([m.numel()], m.device) if states is None else states
-    _adam8_check("adam8_quantize", *states, -(-m.numel() // ADAM8_BLOCK))
-    call("hk_adam8_quantize", _ptr(m), _ptr(v), m.numel(), *map(_ptr, states), _stream())
+    states = adam8_states([n], m.device) if states is None else states
+    _flat("adam8_quantize", m, v, *states)
+    _adam8_check("adam8_quantize", *states, -(-n // ADAM8_BLOCK))
+    call("hk_adam8_quantize", m.data_ptr(), v.data_ptr(), n, *map(_ptr, states), _stream())
     return tuple(states)
 
 
@@ -335,12 +343,11 @@ def adam8_dequantize(m, v, m_scale, v_scale, m_out=None, v_out=None):
     _adam8_check("adam8_dequantize", m, v, m_scale, v_scale, -(-n // ADAM8_BLOCK))
     m_out = torch.empty(n, device=m.device, dtype=torch.float32) if m_out is None else m_out
     v_out = torch.empty(n, device=m.device, dtype=torch.float32) if v_out is None else v_out
-    _dev(m_out, v_out)
-    _here("adam8_dequantize", m_out, v_out)
-    if m_out.dtype != torch.float32 or v_out.dtype != torch.float32 or v_out.numel() != n:
+    _flat("adam8_dequantize", m, v, m_scale, v_scale, m_out, v_out)
+    if m_out.dtype is not torch.float32 or v_out.dtype is not torch.float32 or v_out.numel() != n:
         raise ValueError("adam8_dequantize: fp32 outputs of equal size")
-    call("hk_adam8_dequantize", _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), n, _ptr(m_out),
-         _ptr(v_out), _stream())
+    call("hk_adam8_dequantize", m.data_ptr(), v.data_ptr(), m_scale.data_ptr(), v_scale.data_ptr(), n,
+         m_out.data_ptr(), v_out.data_ptr(), _stream())
     return m_out, v_out
 
 
@@ -357,9 +364,9 @@ class Adam8Plan:
         types = {g.dtype for g in grads} or {torch.float32}
         if len(types) != 1 or not types <= set(_TYPE):
             raise ValueError("Adam8Plan: the gradients share one type (fp32, bf16 or fp16)")
+        _flat("Adam8Plan", m, v, m_scale, v_scale)
         for p, g, c in zip(params, grads, copies):
-            _dev(p, g, c)
-            _here("Adam8Plan", p, g, c)
+            _flat("Adam8Plan", p, g, c)
             if p.dtype != torch.float32 or g.numel() != p.numel():
                 raise ValueError("Adam8Plan: fp32 parameters, gradients of equal size")
             if c is not None and (c.dtype != torch.bfloat16 or c.numel() != p.numel()):
@@ -503,32 +510,55 @@ def attn_backward(q, k, v, do, lse, D, causal: bool, scale: float | None = None,
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}  # HK_ACT_*
 
 
-def _matrix(fn: str, t: torch.Tensor, batch: int, rows: int, cols: int) -> tuple[int, int]:
-    """(leading dimension, batch stride) of a bf16 matrix [rows, cols], or [batch, rows, cols]."""
+def _matrix(fn: str, t: torch.Tensor, batch: int, rows: int, cols: int) -> tuple[int, int, int]:
+    """(address, leading dimension, batch stride) of a bf16 matrix [rows, cols], or
+    [batch, rows, cols]."""
     sh, st = t.shape, t.stride()
-    if t.dtype != torch.bfloat16 or sh not in ((rows, cols), (batch, rows, cols)) or (
-            len(sh) == 2 and batch != 1) or (st[-1] != 1 and cols > 1):
+    if len(sh) == 2:
+        ok, step = batch == 1 and sh[0] == rows and sh[1] == cols, 0
+    else:
+        ok = len(sh) == 3 and sh[0] == batch and sh[1] == rows and sh[2] == cols
+        step = st[0] if ok and batch > 1 else 0
+    if not ok or t.dtype is not torch.bfloat16 or (st[-1] != 1 and cols > 1):
         raise ValueError(f"{fn}: bf16 matrices of matching shapes with a unit last-dim stride; "
                          f"[{batch}, {rows}, {cols}] expected, {tuple(sh)} given")
-    ld = st[-2] if rows > 1 else max(st[-2], cols)
-    return ld, st[0] if len(sh) == 3 and batch > 1 else 0
+    ld = st[-2]
+    return t.data_ptr(), (ld if rows > 1 or ld > cols else cols), step
+
+
+def _vector(fn: str, t: torch.Tensor, dtype, batch: int, n: int) -> tuple[int, int]:
+    """(address, batch stride) of a vector [n], or [batch, n]."""
+    sh = t.shape
+    if t.dtype is not dtype or sh[-1:] != (n,) or (len(sh) == 2 and sh[0] != batch) or (
+            len(sh) > 2) or (t.stride(-1) != 1 and n > 1):
+        raise ValueError(f"{fn}: {dtype} vectors [{n}], or [{batch}, {n}]; {tuple(sh)} given")
+    return t.data_ptr(), t.stride(0) if len(sh) == 2 and batch > 1 else 0
 
 
 def _product(fn: str, a, b, trans_a: bool, trans_b: bool, activation: str):
-    """(batch, M, N, K) of op(a) op(b)."""
-    if a.dim() != b.dim() or a.dim() not in (2, 3) or activation not in _ACT:
+    """(batch, M, N, K, activation) of op(a) op(b)."""
+    ash, bsh = a.shape, b.shape
+    act = _ACT.get(activation)
+    if len(ash) != len(bsh) or not 2 <= len(ash) <= 3 or act is None:
         raise ValueError(f"{fn}: matrices or batches of them, and one of {', '.join(_ACT)}")
-    M, K = (a.shape[-1], a.shape[-2]) if trans_a else (a.shape[-2], a.shape[-1])
-    N = b.shape[-2] if trans_b else b.shape[-1]
-    return (a.shape[0] if a.dim() == 3 else 1), M, N, K
+    K, M = ash[-2:] if trans_a else ash[:-3:-1]
+    return (ash[0] if len(ash) == 3 else 1), M, bsh[-2] if trans_b else bsh[-1], K, act
 
 
-def _own_workspace(need) -> tuple[torch.Tensor | None, int]:
-    """Under capture the bytes of need() in a tensor of the graph's; otherwise none: the library's."""
-    if not torch.cuda.is_current_stream_capturing():
-        return None, 0
-    n = max(0, need())
-    return (torch.empty(n, device="cuda", dtype=torch.uint8) if n else None), n
+def _call_captured(name: str, need, *args) -> None:
+    """Calls an entry point whose arguments end in (workspace, bytes, stream), with the library's own
+    workspace; where the call is captured into a graph and needs one, with need() bytes of the graph's."""
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(lib(), name)
+    stream = _stream()
+    status = f(*args, None, 0, stream)
+    if status == 900:  # hipErrorStreamCaptureUnsupported
+        n = need()
+        ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+        status = f(*args, ws.data_ptr(), n, stream)
+    if status != 0:
+        raise HKError(name, status)
 
 
 def _bf16_bits(x: float) -> int:
@@ -542,26 +572,20 @@ def bgemm_act(a, b, bias=None, activation: str = "none", residual=None, preact=N
     goes into the activation ("none", "relu", "gelu" or "silu") is stored in `preact` where that is
     passed. bias is [N], or [batch, N]; residual may be `out` itself."""
     fn = "bgemm_act"
-    batch, M, N, K = _product(fn, a, b, trans_a, trans_b, activation)
+    batch, M, N, K, act = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
         out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
                           dtype=torch.bfloat16)
     _here(fn, a, b, bias, residual, preact, out)
-    lda, sA = _matrix(fn, a, batch, K if trans_a else M, M if trans_a else K)
-    ldb, sB = _matrix(fn, b, batch, N if trans_b else K, K if trans_b else N)
-    ldc, sC = _matrix(fn, out, batch, M, N)
-    ldr, sR = (0, 0) if residual is None else _matrix(fn, residual, batch, M, N)
-    ldz, sZ = (0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
-    sbias = 0
-    if bias is not None:
-        if bias.dtype != torch.bfloat16 or bias.shape not in ((N,), (batch, N)) or (
-                bias.stride(-1) != 1 and N > 1):
-            raise ValueError(f"{fn}: bias is bf16 [N] or [batch, N]")
-        sbias = bias.stride(0) if bias.dim() == 2 and batch > 1 else 0
-    ws, n = _own_workspace(lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch, 0))
-    call("hk_bgemm_act", trans_a, trans_b, M, N, K, _bf16_bits(alpha), a.data_ptr(), lda, sA,
-         b.data_ptr(), ldb, sB, _ptr(bias), sbias, _ACT[activation], _ptr(residual), ldr, sR,
-         _ptr(preact), ldz, sZ, out.data_ptr(), ldc, sC, batch, _ptr(ws), n, _stream())
+    A = _matrix(fn, a, batch, K, M) if trans_a else _matrix(fn, a, batch, M, K)
+    B = _matrix(fn, b, batch, N, K) if trans_b else _matrix(fn, b, batch, K, N)
+    C = _matrix(fn, out, batch, M, N)
+    R = (None, 0, 0) if residual is None else _matrix(fn, residual, batch, M, N)
+    Z = (None, 0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
+    v = (None, 0) if bias is None else _vector(fn, bias, torch.bfloat16, batch, N)
+    _call_captured("hk_bgemm_act",
+                   lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch, 0),
+                   trans_a, trans_b, M, N, K, _bf16_bits(alpha), *A, *B, *v, act, *R, *Z, *C, batch)
     return out
 
 
@@ -573,29 +597,25 @@ def bgemm_act_backward(a, b, preact=None, activation: str = "none", dbias=None, 
     wanted) is added to, or written where accumulate is False: the sums of d over rows (and, [N],
     batches) before it is rounded."""
     fn = "bgemm_act_backward"
-    batch, M, N, K = _product(fn, a, b, trans_a, trans_b, activation)
+    batch, M, N, K, act = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
         out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
                           dtype=torch.bfloat16)
     _here(fn, a, b, preact, dbias, out)
-    lda, sA = _matrix(fn, a, batch, K if trans_a else M, M if trans_a else K)
-    ldb, sB = _matrix(fn, b, batch, N if trans_b else K, K if trans_b else N)
-    ldc, sC = _matrix(fn, out, batch, M, N)
-    if preact is None and activation != "none":
+    A = _matrix(fn, a, batch, K, M) if trans_a else _matrix(fn, a, batch, M, K)
+    B = _matrix(fn, b, batch, N, K) if trans_b else _matrix(fn, b, batch, K, N)
+    C = _matrix(fn, out, batch, M, N)
+    if preact is None and act:
         raise ValueError(f"{fn}: the activation's derivative needs preact")
-    ldz, sZ = (0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
-    sD = 0
-    if dbias is not None:
-        if dbias.dtype != torch.float32 or dbias.shape not in ((N,), (batch, N)) or (
-                dbias.stride(-1) != 1 and N > 1) or (
-                dbias.dim() == 2 and batch > 1 and dbias.stride(0) < N):
-            raise ValueError(f"{fn}: dbias is fp32 [N] or [batch, N]")
-        sD = dbias.stride(0) if dbias.dim() == 2 and batch > 1 else 0
-    ws, n = _own_workspace(lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch,
-                                                                dbias is not None))
-    call("hk_bgemm_act_backward", trans_a, trans_b, M, N, K, _bf16_bits(alpha), a.data_ptr(), lda,
-         sA, b.data_ptr(), ldb, sB, _ACT[activation], _ptr(preact), ldz, sZ, out.data_ptr(), ldc,
-         sC, _ptr(dbias), sD, accumulate, batch, _ptr(ws), n, _stream())
+    Z = (None, 0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
+    v = (None, 0) if dbias is None else _vector(fn, dbias, torch.float32, batch, N)
+    if dbias is not None and dbias.dim() == 2 and batch > 1 and v[1] < N:
+        raise ValueError(f"{fn}: the rows of dbias overlap")
+    _call_captured("hk_bgemm_act_backward",
+                   lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch,
+                                                        dbias is not None),
+                   trans_a, trans_b, M, N, K, _bf16_bits(alpha), *A, *B, act, *Z, *C, *v, accumulate,
+                   batch)
     return out
 
 
@@ -616,52 +636,77 @@ class QkNormRopeParams(ctypes.Structure):
         for s in ("B", "M", "H")]
 
 
+# the same block, packed in one go (2 us; the ctypes structure takes 6)
+_QK_PACK = struct.Struct("@15P6if3?21q").pack
+_NO_SIDE = (0, 0, 0, 0, 0, 0), ((0, 0, 0),) * 3  # pointers x, w, out, dy, dx, dw; strides x, out, dx
+
+
+def _qk_side(fn, x, w, o, g, gw, like, out, backward):
+    """(pointers, strides, heads) of q or of k; o: the output, or in the backward pass its gradient."""
+    if x is None:
+        if o is not None or g is not None or gw is not None:
+            raise ValueError(f"{fn}: outputs and gradients of a tensor that is not passed")
+        return *_NO_SIDE, 0
+    sh, dt, d = x.shape, x.dtype, like[3]
+    if len(sh) != 4 or dt is not like[4] or sh[0] != like[0] or sh[2] != like[2] or sh[3] != d:
+        raise ValueError(f"{fn}: q and k share type, batch, length and head_dim")
+    if o is None or o.shape != sh or o.dtype is not out:
+        raise ValueError(f"{fn}: outputs have their input's shape, and its type or fp32")
+    strides = _strides(x), _strides(o), (0, 0, 0)
+    wp = gp = gwp = 0
+    if w is not None:
+        if w.dtype is not dt or w.shape != (d,) or (d > 1 and w.stride(0) != 1):
+            raise ValueError(f"{fn}: weights are [head_dim] of the inputs' type")
+        wp = w.data_ptr()
+    if g is not None:
+        if g.shape != sh or g.dtype is not dt:
+            raise ValueError(f"{fn}: gradients have their input's shape and type")
+        gp, strides = g.data_ptr(), (*strides[:2], _strides(g))
+    if gw is not None:
+        if gw.dtype is not torch.float32 or gw.shape != (d,) or (d > 1 and gw.stride(0) != 1):
+            raise ValueError(f"{fn}: gradients of the weights are fp32 [head_dim]")
+        gwp = gw.data_ptr()
+    op = o.data_ptr()
+    return ((x.data_ptr(), wp, 0 if backward else op, op if backward else 0, gp, gwp), strides, sh[1])
+
+
 def _qk_params(fn, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved, qo, ko,
-               backward=False, dq=None, dk=None, dqw=None, dkw=None, accumulate=False):
+               backward=False, dq=None, dk=None, dqw=None, dkw=None, accumulate=False) -> bytes:
     """The parameter block; qo, ko: the outputs, or in the backward pass their gradients."""
     x = q if q is not None else k
     if x is None or x.dim() != 4 or x.dtype not in _TYPE:
         raise ValueError(f"{fn}: q or k, [B, heads, T, head_dim], fp32, bf16 or fp16")
     _here(fn, q, k, cos, sin, positions, q_weight, k_weight, qo, ko, dq, dk, dqw, dkw)
-    (B, _, T, d), out = x.shape, (qo if qo is not None else ko).dtype
-    for t, o, w, g, gw in ((q, qo, q_weight, dq, dqw), (k, ko, k_weight, dk, dkw)):
-        if t is None:
-            if o is not None or g is not None or gw is not None:
-                raise ValueError(f"{fn}: outputs and gradients of a tensor that is not passed")
-            continue
-        if t.dim() != 4 or t.dtype != x.dtype or t.shape[0] != B or t.shape[2:] != x.shape[2:]:
-            raise ValueError(f"{fn}: q and k share type, batch, length and head_dim")
-        if o is None or o.shape != t.shape or o.dtype != out or out not in (x.dtype, torch.float32):
-            raise ValueError(f"{fn}: outputs have their input's shape, and its type or fp32")
-        if w is not None and (w.dtype != x.dtype or w.shape != (d,) or not w.is_contiguous()):
-            raise ValueError(f"{fn}: weights are [head_dim] of the inputs' type")
-        if g is not None and (g.shape != t.shape or g.dtype != x.dtype):
-            raise ValueError(f"{fn}: gradients have their input's shape and type")
-        if gw is not None and (gw.dtype != torch.float32 or gw.shape != (d,)
-                               or not gw.is_contiguous()):
-            raise ValueError(f"{fn}: gradients of the weights are fp32 [head_dim]")
-    rows = stride = rot = 0
+    B, _, T, d = x.shape
+    like, o = (B, 0, T, d, x.dtype), qo if qo is not None else ko
+    out = None if o is None else o.dtype
+    if out is not x.dtype and out is not torch.float32:
+        raise ValueError(f"{fn}: outputs have their input's type, or fp32")
+    (xq, wq, yq, dyq, gq, gwq), (sxq, syq, sgq), hq = _qk_side(fn, q, q_weight, qo, dq, dqw, like,
+                                                               out, backward)
+    (xk, wk, yk, dyk, gk, gwk), (sxk, syk, sgk), hk_ = _qk_side(fn, k, k_weight, ko, dk, dkw, like,
+                                                                out, backward)
+    cp = sp = pp = rows = stride = rot = pos_stride = 0
     if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or not (
-                cos.dtype == sin.dtype == torch.float32) or cos.stride() != sin.stride() or (
-                cos.stride(1) != 1 and cos.shape[1] > 1):
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or (
+                cos.dtype is not torch.float32) or sin.dtype is not torch.float32 or (
+                cos.stride() != sin.stride()) or (cos.stride(1) != 1 and cos.shape[1] > 1):
             raise ValueError(f"{fn}: cos and sin are fp32 [rows, rotary_dim / 2], laid out alike")
-        rows, stride, rot = cos.shape[0], cos.stride(0), 2 * cos.shape[1]
-        if rows == 1:
-            stride = max(stride, cos.shape[1])
-    pos_stride = 0
+        rows, half = cos.shape
+        stride, rot = cos.stride(0), 2 * half
+        if rows == 1 and stride < half:
+            stride = half
+        cp, sp = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        if positions.dtype != torch.int64 or positions.shape not in ((B, T), (T,)) or (
-                positions.stride(-1) != 1 and T > 1):
+        sh = positions.shape
+        if positions.dtype is not torch.int64 or sh[-1:] != (T,) or len(sh) > 2 or (
+                len(sh) == 2 and sh[0] != B) or (positions.stride(-1) != 1 and T > 1):
             raise ValueError(f"{fn}: positions are int64 [B, T] or [T]")
-        pos_stride = positions.stride(0) if positions.dim() == 2 else 0
-    return QkNormRopeParams(
-        _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), _ptr(positions),
-        None if backward else _ptr(qo), None if backward else _ptr(ko),
-        _ptr(qo) if backward else None, _ptr(ko) if backward else None, _ptr(dq), _ptr(dk),
-        _ptr(dqw), _ptr(dkw), B, T, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1],
-        d, rot, eps, bool(interleaved), out != x.dtype, bool(accumulate), rows, stride, pos_stride,
-        *_strides(q), *_strides(k), *_strides(qo), *_strides(ko), *_strides(dq), *_strides(dk))
+        pp = positions.data_ptr()
+        pos_stride = positions.stride(0) if len(sh) == 2 else 0
+    return _QK_PACK(xq, xk, wq, wk, cp, sp, pp, yq, yk, dyq, dyk, gq, gk, gwq, gwk, B, T, hq, hk_, d,
+                    rot, eps, interleaved, out is not x.dtype, accumulate, rows, stride, pos_stride,
+                    *sxq, *sxk, *syq, *syk, *sgq, *sgk)
 
 
 def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None,
@@ -671,21 +716,20 @@ def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None
     then the rotation of its first 2 * cos.shape[1] elements by the table rows of the tokens'
     positions (None: token t at position t). Returns (q_out, k_out) of q's type or out_dtype, which
     may be fp32 for 16-bit inputs. q_out and k_out may be q and k themselves."""
-    make = lambda t: None if t is None else torch.empty(  # noqa: E731
-        t.shape, device=t.device, dtype=out_dtype or t.dtype)
-    q_out = make(q) if q_out is None else q_out
-    k_out = make(k) if k_out is None else k_out
+    if q_out is None and q is not None:
+        q_out = torch.empty(q.shape, device=q.device, dtype=out_dtype or q.dtype)
+    if k_out is None and k is not None:
+        k_out = torch.empty(k.shape, device=k.device, dtype=out_dtype or k.dtype)
     p = _qk_params("qk_norm_rope_forward", q, k, cos, sin, positions, q_weight, k_weight, eps,
                    interleaved, q_out, k_out)
-    call("hk_qk_norm_rope_forward", ctypes.byref(p), _TYPE[(q if q is not None else k).dtype],
-         _stream())
+    call("hk_qk_norm_rope_forward", p, _TYPE[(q if q is not None else k).dtype], _stream())
     return q_out, k_out
 
 
 def _by_token(t):
     """An empty [B, heads, T, d] tensor with the heads of a token together, as a projection has them."""
     B, H, T, d = t.shape
-    return torch.empty(B, T, H, d, device=t.device, dtype=t.dtype).transpose(1, 2)
+    return torch.empty_strided((B, H, T, d), (T * H * d, d, H * d, 1), device=t.device, dtype=t.dtype)
 
 
 def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=None, q_weight=None,
@@ -700,9 +744,9 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=No
     p = _qk_params("qk_norm_rope_backward", q, k, cos, sin, positions, q_weight, k_weight, eps,
                    interleaved, dq_out, dk_out, True, dq, dk, grad_q_weight, grad_k_weight,
                    accumulate)
-    x = q if q is not None else k
-    ws, n = _own_workspace(lambda: lib().hk_qk_norm_rope_workspace(ctypes.byref(p), _TYPE[x.dtype]))
-    call("hk_qk_norm_rope_backward", ctypes.byref(p), _TYPE[x.dtype], _ptr(ws), n, _stream())
+    kind = _TYPE[(q if q is not None else k).dtype]
+    _call_captured("hk_qk_norm_rope_backward", lambda: lib().hk_qk_norm_rope_workspace(p, kind), p,
+                   kind)
     return dq, dk
 
 

@@ -137,7 +137,8 @@ class Data:
 LAYOUTS = [(0, 0), (0, 1), (1, 0), (1, 1)]
 SMALL = [(8, 8, 8), (64, 64, 64), (65, 63, 65), (63, 65, 127), (9, 200, 129), (200, 9, 321),
          (127, 129, 191), (333, 77, 1111), (2, 1000, 40), (500, 1, 77), (3, 5, 3), (1, 1, 1),
-         (1, 520, 129), (1, 1000, 1024), (1, 77, 5000), (17, 136, 1), (130, 264, 72)]
+         (1, 520, 129), (1, 1000, 1024), (1, 77, 5000), (1, 39, 9001), (1, 2000, 9001), (1, 31, 7),
+         (17, 136, 1), (130, 264, 72)]
 
 
 @pytest.mark.parametrize("ta,tb", LAYOUTS)
@@ -290,7 +291,7 @@ def test_two_graphs_captured_on_one_stream(hk):
     """Split products with a bias gradient: every graph has its own workspace, as the eager calls do."""
     s = torch.cuda.Stream()
     sets = []
-    for M, N, K in ((192, 384, 4096), (300, 299, 4001), (1, 1000, 2048)):
+    for M, N, K in ((192, 384, 4096), (300, 299, 4001), (1, 1000, 9000)):
         d = Data(M, N, K, 0, 0, 31 + M)
         assert M == 1 or hk.lib().hk_bgemm_split_count(0, 0, M, N, K, 1, 0) > 1
         db = torch.zeros(N, device=DEV)

@@ -336,7 +336,6 @@ def test_captured_calls_replay_as_they_ran(hk):
 
 def test_library_workspace_where_none_is_passed(hk):
     """The C entry with no workspace: the stream's own, the same bits."""
-    import ctypes
     gen = torch.Generator(device=DEV)
     gen.manual_seed(19)
     q, dy = _heads(gen, 2, 6, 50, 64, torch.float32, "token"), torch.randn(2, 6, 50, 64, generator=gen, device=DEV)
@@ -346,10 +345,10 @@ def test_library_workspace_where_none_is_passed(hk):
     d2 = torch.empty_like(dx)
     p = hk._qk_params("t", q, None, cos, sin, None, None, None, 1e-6, False, dy, None, True, d2, None,
                       g[1], None, False)
-    assert hk.lib().hk_qk_norm_rope_workspace(ctypes.byref(p), 0) > 0
-    hk.call("hk_qk_norm_rope_backward", ctypes.byref(p), 0, None, 0, hk._stream())
+    assert hk.lib().hk_qk_norm_rope_workspace(p, 0) > 0
+    hk.call("hk_qk_norm_rope_backward", p, 0, None, 0, hk._stream())
     assert torch.equal(dx, d2) and torch.equal(g[0], g[1])
     # one that is too small is refused
     small = torch.empty(4, device=DEV, dtype=torch.uint8)
     with pytest.raises(hk.HKError):
-        hk.call("hk_qk_norm_rope_backward", ctypes.byref(p), 0, small.data_ptr(), 4, hk._stream())
+        hk.call("hk_qk_norm_rope_backward", p, 0, small.data_ptr(), 4, hk._stream())

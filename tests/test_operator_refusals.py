@@ -192,3 +192,17 @@ def test_bgemm_act_front_end_refuses():
         hk.bgemm_act(a[None], b)
     with pytest.raises(ValueError):
         hk.bgemm_act_backward(a, b)
+
+
+def test_qk_packed_block_is_the_structure():
+    """The packed parameter block has the structure's layout, field by field."""
+    from hyperkernels_amd import kernels as hk
+
+    names = [n for n, _ in hk.QkNormRopeParams._fields_]
+    values = {n: i + 1 for i, n in enumerate(names)}
+    values |= dict(interleaved=True, f32_io=False, accumulate=True, eps=0.5)
+    got = hk.QkNormRopeParams.from_buffer_copy(
+        hk._QK_PACK(*values.values()).ljust(ctypes.sizeof(hk.QkNormRopeParams), b"\0"))
+    assert len(hk._QK_PACK(*values.values())) == ctypes.sizeof(hk.QkNormRopeParams)
+    for n in names:
+        assert getattr(got, n) == values[n], n
