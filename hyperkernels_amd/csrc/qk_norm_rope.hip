@@ -24,11 +24,10 @@
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / HK_WAVE;
+constexpr int kThreads = 256;      // forward
+constexpr int kBackThreads = 512, kBackWaves = kBackThreads / HK_WAVE;
+constexpr int kBackPerCu = 3;      // workgroups of the backward pass that a CU holds
 constexpr int kMaxDim = 256;
-// Workgroups of the backward pass for queries (and for keys): each leaves one row of partial sums.
-constexpr int kMostPartials = 1024;
-constexpr int kRowsPerGroup = 4;  // rows that a lane group of the backward pass takes at least
 
 // Vectors of V elements at any alignment of the element type.
 template <typename S, int V>
@@ -156,11 +155,13 @@ struct Args {
   float eps, inv_d;
 };
 
-// The cosines and sines of a unit for a token; NaN where the table has no such position.
+__device__ __forceinline__ int64_t position(const Args& g, int b, int t) {
+  return g.positions ? g.positions[b * g.pos_stride + t] : t;
+}
+// The cosines and sines of a unit at a position; NaN where the table has no such one.
 template <int V>
-__device__ __forceinline__ void angles(const Args& g, const Unit<V>& u, int b, int t, float (&c)[V],
+__device__ __forceinline__ void angles(const Args& g, const Unit<V>& u, int64_t pos, float (&c)[V],
                                        float (&s)[V]) {
-  const int64_t pos = g.positions ? g.positions[b * g.pos_stride + t] : t;
   if (pos < 0 || pos >= g.table_rows) {
 #pragma unroll
     for (int e = 0; e < V; ++e) c[e] = s[e] = NAN;
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
     if (!u.on) continue;
     float wa[V], wb[V], c[V], s[V], ya[V], yb[V];
     weights<FI, V>(sd.w, u, g.s.d, wa, wb);
-    angles<V>(g, u, b, t, c, s);
+    angles<V>(g, u, position(g, b, t), c, s);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float a = xa[k][e] * r * wa[e], bb = xb[k][e] * r * wb[e];
@@ -230,12 +231,12 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
 }
 
 template <class FI, class FO, int V, int U>
-__global__ __launch_bounds__(kThreads) void qk_backward(Args g) {
-  __shared__ float lds[kWaves][kMaxDim];
+__global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
+  __shared__ float lds[kBackWaves][kMaxDim];
   const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
   const Side& sd = g.side[which];
   const int block = blockIdx.x - (which ? g.side[0].blocks : 0);
-  const int per_block = kThreads / g.s.lanes;
+  const int per_block = kBackThreads / g.s.lanes;
   const int j = threadIdx.x & (g.s.lanes - 1);
   float wa[U][V], wb[U][V], da[U][V], db[U][V];
 #pragma unroll
@@ -251,6 +252,7 @@ __global__ __launch_bounds__(kThreads) void qk_backward(Args g) {
     const auto* x = static_cast<const typename FI::storage*>(sd.x) + b * sd.xB + t * sd.xM + head * sd.xH;
     const auto* dy = static_cast<const typename FO::storage*>(sd.dy) + b * sd.yB + t * sd.yM + head * sd.yH;
     auto* dx = static_cast<typename FI::storage*>(sd.out) + b * sd.oB + t * sd.oM + head * sd.oH;
+    const int64_t pos = position(g, b, t);
     float xa[U][V], xb[U][V], ga[U][V], gb[U][V], sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void qk_backward(Args g) {
       float c[V], s[V], ya[V], yb[V];
       load_unit<FI, V>(x, u, g.s.d, xa[k], xb[k]);
       load_unit<FO, V>(dy, u, g.s.d, ya, yb);
-      angles<V>(g, u, b, t, c, s);
+      angles<V>(g, u, pos, c, s);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         ga[k][e] = ya[e] * c[e] + yb[e] * s[e];
@@ -307,34 +309,39 @@ __global__ __launch_bounds__(kThreads) void qk_backward(Args g) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < g.s.d; i += kThreads) {
+  for (int i = threadIdx.x; i < g.s.d; i += kBackThreads) {
     float v = lds[0][i];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) v += lds[k][i];
+    for (int k = 1; k < kBackWaves; ++k) v += lds[k][i];
     sd.part[static_cast<int64_t>(block) * g.s.d + i] = v;
   }
 }
 
 // dw[i] (+)= the sum over n rows of part[n][d]; blockIdx.y: queries, keys. Each workgroup sums 16
-// columns, its 16 row groups take every 16th row.
+// columns, its 64 row groups take every 64th row.
 struct Weights {
   const float* part[2];
   float* dw[2];
   int n[2];
 };
-__global__ __launch_bounds__(256) void qk_weight_sums(Weights a, int d, int accumulate) {
+__global__ __launch_bounds__(1024) void qk_weight_sums(Weights a, int d, int accumulate) {
   __shared__ float lds[16][17];
-  const int which = blockIdx.y, col = blockIdx.x * 16 + (threadIdx.x & 15), grp = threadIdx.x >> 4;
+  const int which = blockIdx.y, tx = threadIdx.x & 15, col = blockIdx.x * 16 + tx;
+  const int grp = threadIdx.x >> 4, wave = threadIdx.x >> 6;
   if (!a.dw[which]) return;
   float v = 0.f;
-  if (col < d)
-    for (int i = grp; i < a.n[which]; i += 16) v += a.part[which][static_cast<int64_t>(i) * d + col];
-  lds[grp][threadIdx.x & 15] = v;
+  if (col < d) {
+#pragma unroll 4
+    for (int i = grp; i < a.n[which]; i += 64) v += a.part[which][static_cast<int64_t>(i) * d + col];
+  }
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  if ((threadIdx.x & 63) < 16) lds[wave][tx] = v;
   __syncthreads();
-  if (grp == 0 && col < d) {
+  if (threadIdx.x < 16 && col < d) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x];
+    for (int i = 0; i < 16; ++i) s += lds[i][tx];
     a.dw[which][col] = accumulate ? a.dw[which][col] + s : s;
   }
 }
@@ -373,10 +380,15 @@ hipError_t check(const hk_qk_norm_rope_params* p, int type, bool backward) {
   return hipSuccess;
 }
 
-// Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it.
-int unit_pairs(int type, int d, int rot) {
-  for (int v = type == HK_TYPE_F32 ? 4 : 8; v > 1; v /= 2)
-    if (v != 2 && d % (2 * v) == 0 && rot % (2 * v) == 0) return v;
+// Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it. 8 (16-byte
+// vectors of 16-bit elements) where a row is only read and written in 16 bits; 4 where outputs are fp32
+// (forward, 8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: 17.5 -> 16.2 us; bf16 -> bf16 the
+// other way: 11.7 and 12.6), and in the backward pass, which holds weights and their gradients beside
+// the row (110 registers a lane with 8: 25.4 us with dw, with 4 and three workgroups a CU 23.9;
+// 16 + 4 heads of 128, fp16: 46.3 and 36.8).
+int unit_pairs(int type, int d, int rot, bool wide) {
+  for (int v = type != HK_TYPE_F32 && wide ? 8 : 4; v > 1; v -= 4)
+    if (d % (2 * v) == 0 && rot % (2 * v) == 0) return v;
   return 1;
 }
 
@@ -409,26 +421,34 @@ Args make_args(const hk_qk_norm_rope_params* p, int v, bool backward) {
   k.yB = p->ko_strideB, k.yM = p->ko_strideM, k.yH = p->ko_strideH;
   k.oB = backward ? p->dk_strideB : k.yB, k.oM = backward ? p->dk_strideM : k.yM;
   k.oH = backward ? p->dk_strideH : k.yH;
-  const int per_block = kThreads / g.s.lanes;
-  for (Side& s : g.side) {
-    s.blocks = static_cast<int>(hk::ceil_div(s.rows, backward ? kRowsPerGroup * per_block : per_block));
-    if (backward && s.blocks > kMostPartials) s.blocks = kMostPartials;
-  }
+  const int64_t per_block = (backward ? kBackThreads : kThreads) / g.s.lanes;
+  // Backward: one round of workgroups, each of which leaves one row of partial sums, and as many rows for
+  // each of their lane groups as that takes.
+  int64_t passes = 1;
+  if (backward)
+    passes = hk::ceil_div(static_cast<int64_t>(q.rows) + k.rows,
+                          per_block * kBackPerCu * hk::device_cu_count());
+  for (Side& s : g.side)
+    s.blocks = static_cast<int>(hk::ceil_div(s.rows, per_block * (passes > 0 ? passes : 1)));
   return g;
 }
 
 template <class FI, class FO, int V, int U>
 hipError_t launch(const Args& g, bool backward, hipStream_t stream) {
   const unsigned blocks = g.side[0].blocks + g.side[1].blocks;
-  if (backward)
-    hipLaunchKernelGGL((qk_backward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
-  else
+  if constexpr (V == 8) {
+    if (backward) return hipErrorInvalidValue;  // unit_pairs
     hipLaunchKernelGGL((qk_forward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+  } else if (backward) {
+    hipLaunchKernelGGL((qk_backward<FI, FO, V, U>), dim3(blocks), dim3(kBackThreads), 0, stream, g);
+  } else {
+    hipLaunchKernelGGL((qk_forward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+  }
   return hk::launch_status();
 }
 template <class FI, class FO>
 hipError_t by_unit(const Args& g, int v, bool backward, hipStream_t stream) {
-  if constexpr (FI::kPerVec == 8)
+  if constexpr (FI::kPerVec == 8 && FO::kPerVec == 8)
     if (v == 8) return launch<FI, FO, 8, 1>(g, backward, stream);
   if (v == 4) return launch<FI, FO, 4, 1>(g, backward, stream);
   return g.s.units > HK_WAVE ? launch<FI, FO, 1, 2>(g, backward, stream)
@@ -451,7 +471,7 @@ size_t partial_bytes(const Args& g) {
 extern "C" hipError_t hk_qk_norm_rope_forward(const hk_qk_norm_rope_params* p, int type,
                                               hipStream_t stream) {
   HK_RETURN_IF_ERROR(check(p, type, false));
-  const int v = unit_pairs(type, p->head_dim, p->rotary_dim);
+  const int v = unit_pairs(type, p->head_dim, p->rotary_dim, !p->f32_io);
   const Args g = make_args(p, v, false);
   if (g.side[0].rows + g.side[1].rows == 0) return hipSuccess;
   return by_type(g, type, p->f32_io, v, false, stream);
@@ -461,14 +481,14 @@ extern "C" int64_t hk_qk_norm_rope_workspace(const hk_qk_norm_rope_params* p, in
   if (check(p, type, true) != hipSuccess) return -1;
   if (!p->dq_weight && !p->dk_weight) return 0;
   return static_cast<int64_t>(
-      partial_bytes(make_args(p, unit_pairs(type, p->head_dim, p->rotary_dim), true)));
+      partial_bytes(make_args(p, unit_pairs(type, p->head_dim, p->rotary_dim, false), true)));
 }
 
 extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, int type,
                                                void* workspace, int64_t workspace_bytes,
                                                hipStream_t stream) {
   HK_RETURN_IF_ERROR(check(p, type, true));
-  const int v = unit_pairs(type, p->head_dim, p->rotary_dim);
+  const int v = unit_pairs(type, p->head_dim, p->rotary_dim, false);
   Args g = make_args(p, v, true);
   Weights w{{nullptr, nullptr},
             {p->q_heads ? p->dq_weight : nullptr, p->k_heads ? p->dk_weight : nullptr},
@@ -494,7 +514,7 @@ extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, 
     HK_RETURN_IF_ERROR(by_type(g, type, p->f32_io, v, true, stream));
   if (!sums || (p->accumulate && g.side[0].rows + g.side[1].rows == 0)) return hipSuccess;
   // without rows the sums are zero
-  hipLaunchKernelGGL(qk_weight_sums, dim3(static_cast<unsigned>((g.s.d + 15) / 16), 2), dim3(256), 0,
+  hipLaunchKernelGGL(qk_weight_sums, dim3(static_cast<unsigned>((g.s.d + 15) / 16), 2), dim3(1024), 0,
                      stream, w, g.s.d, p->accumulate ? 1 : 0);
   return hk::launch_status();
 }
