@@ -37,15 +37,17 @@ __device__ __forceinline__ float gelu_grad(float x) {
 
 // An activation HK_ACT_* as a call's kernels evaluate it, the same for all of its elements. GELU and SiLU
 // are both x s with s = 1 / (1 + e^-q), q = x (c1 + c3 x^2): one code for the two, with the constants
-// of q and of t = -log2(e) q = x (k1 + k2 x^2) beside it. Derivative: s + x q' s (1 - s).
+// of t = -log2(e) q = x (k1 + k2 x^2) and of q'. Derivative: s + x q' s (1 - s). SiLU's cubic terms are 0;
+// 10^-30 in their place, which x^2 under 10^19 cannot raise to the last bit of k1, keeps an infinite
+// x^2 from meeting a 0.
 struct Activation {
-  int kind;  // HK_ACT_*
+  int kind;       // HK_ACT_*
   float k1, k2;   // of t
   float d1, d3;   // q' = d1 + d3 x^2
 };
 __host__ __device__ __forceinline__ Activation make_activation(int kind) {
   if (kind == HK_ACT_GELU) return Activation{kind, kK1, kK2, 2.0f * kC, 2.0f * kC3a};
-  return Activation{kind, -1.442695040888963f, 0.0f, 1.0f, 0.0f};  // SiLU
+  return Activation{kind, -1.442695040888963f, -1e-30f, 1.0f, 1e-30f};  // SiLU
 }
 // 2^t overflows to s = 0 and underflows to s = 1, the right limits. ReLU keeps a NaN.
 template <int N>
@@ -53,8 +55,7 @@ __device__ __forceinline__ void activate(const Activation& f, float (&x)[N]) {
   if (f.kind >= HK_ACT_GELU) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      // an infinite x^2 would meet SiLU's k2 = 0
-      const float t = x[e] * __builtin_fmaf(f.k2, __builtin_fminf(x[e] * x[e], 1e30f), f.k1);
+      const float t = x[e] * __builtin_fmaf(f.k2, x[e] * x[e], f.k1);
       x[e] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
     }
   } else if (f.kind == HK_ACT_RELU) {
@@ -68,17 +69,19 @@ __device__ __forceinline__ void scale_by_grad(const Activation& f, const float (
   if (f.kind >= HK_ACT_GELU) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      // past 128 the derivative is 0 or 1 to the last bit, and x^2 could overflow; NaN stays
-      const float y = __builtin_fabsf(x[e]) > 128.0f ? __builtin_copysignf(128.0f, x[e]) : x[e];
-      const float y2 = y * y;
+      const float x2 = x[e] * x[e];
       const float s = __builtin_amdgcn_rcpf(
-          1.0f + __builtin_amdgcn_exp2f(y * __builtin_fmaf(f.k2, y2, f.k1)));
-      const float yq = y * __builtin_fmaf(f.d3, y2, f.d1);
-      d[e] *= __builtin_fmaf(yq, __builtin_fmaf(-s, s, s), s);
+          1.0f + __builtin_amdgcn_exp2f(x[e] * __builtin_fmaf(f.k2, x2, f.k1)));
+      // s (1 - s) is 0 long before x q' overflows; a NaN in x is one in s
+      const float xq = __builtin_amdgcn_fmed3f(x[e] * __builtin_fmaf(f.d3, x2, f.d1), -1e30f, 1e30f);
+      d[e] *= __builtin_fmaf(xq, __builtin_fmaf(-s, s, s), s);
     }
   } else if (f.kind == HK_ACT_RELU) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) d[e] = x[e] > 0.0f ? d[e] : x[e] <= 0.0f ? 0.0f * d[e] : x[e];
+    for (int e = 0; e < N; ++e) {
+      const float s = x[e] > 0.0f ? 1.0f : 0.0f;
+      d[e] *= x[e] == x[e] ? s : x[e];
+    }
   }
 }
 

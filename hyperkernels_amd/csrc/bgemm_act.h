@@ -24,6 +24,7 @@ struct ActEpi {
   int64_t ldz, sZ;
   float* sums;
   int sum_rows, pitch;
+  static constexpr int kWideStage = 2;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
 // Eight bf16 of a row, n of them inside it. The whole vectors of rows that are not ragged are aligned.
@@ -57,6 +58,22 @@ __device__ __forceinline__ void store_row8(uint16_t* p, int n, const float (&f)[
   }
 }
 
+// What one lane reads beside the sums: the residual or, in the backward pass, z, from column col of row 0 on;
+// NULL where there is neither.
+struct ActInput {
+  const uint16_t* p;
+  int64_t ld;
+  __device__ ActInput(const ActEpi& ep, const WaveRows& w, int col) {
+    const uint16_t* base = ep.backward ? (ep.act.kind == HK_ACT_NONE ? nullptr : ep.z) : ep.residual;
+    ld = ep.backward ? ep.ldz : ep.ldr;
+    p = base ? base + w.batch * (ep.backward ? ep.sZ : ep.sR) + col : nullptr;
+  }
+};
+__device__ __forceinline__ uint4 load_bias8(const ActEpi& ep, const WaveRows& w, int col, int n) {
+  return !ep.backward && ep.bias && n > 0
+             ? load_row8<true>(ep.bias + w.batch * ep.sBias + col, n)
+             : make_uint4(0, 0, 0, 0);
+}
 // The epilogue of one lane: the 8 columns from col on of several rows, so the bias and the column sums stay
 // in registers. What it reads beside the sums (residual, or z in the backward pass) is fetched ahead
 // of the row's turn.
@@ -65,39 +82,48 @@ struct ActLane {
   const ActEpi& ep;
   const WaveRows& w;
   int col, n;          // n: columns inside N, 0 for none
-  const uint16_t* in;  // residual or z of row 0, column col; NULL: nothing to read
-  int64_t ld_in;
+  ActInput in;
   float reg[8];        // forward: bias, backward: column sums
-  __device__ ActLane(const ActEpi& e, const WaveRows& rows, int cc)
-      : ep(e), w(rows), col(rows.wcol0 + cc), n(min(8, max(0, rows.N - col))) {
-    const uint16_t* base = ep.backward ? (ep.act.kind == HK_ACT_NONE ? nullptr : ep.z) : ep.residual;
-    ld_in = ep.backward ? ep.ldz : ep.ldr;
-    in = base ? base + w.batch * (ep.backward ? ep.sZ : ep.sR) + col : nullptr;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      reg[i] = !ep.backward && ep.bias && i < n ? bf16_to_f32(ep.bias[w.batch * ep.sBias + col + i]) : 0.f;
+  __device__ ActLane(const ActEpi& e, const WaveRows& rows, int cc, const uint4& bias)
+      : ep(e), w(rows), col(rows.wcol0 + cc), n(min(8, max(0, rows.N - col))), in(e, rows, col) {
+    BF16::unpack(bias, reg);  // zeros in the backward pass
   }
+  __device__ ActLane(const ActEpi& e, const WaveRows& rows, int cc)
+      : ActLane(e, rows, cc,
+                load_bias8(e, rows, rows.wcol0 + cc, min(8, max(0, rows.N - rows.wcol0 - cc)))) {}
   __device__ bool has(int row) const { return row < w.M && n > 0; }
   __device__ uint4 fetch(int row) const {
-    return in && has(row) ? load_row8<RAGGED>(in + row * ld_in, n) : make_uint4(0, 0, 0, 0);
+    return in.p && has(row) ? load_row8<RAGGED>(in.p + row * in.ld, n) : make_uint4(0, 0, 0, 0);
   }
   __device__ void row(int row, const uint4& extra, const f32x4_t& a, const f32x4_t& b) {
     if (!has(row)) return;
+    // one VALU slot of an element is 1 us of 8192 x 5120 outputs: nothing is done that a call does not ask for
     float v[8], x[8];
-    BF16::unpack(extra, x);
     if (ep.backward) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = ep.alpha * (e < 4 ? a[e] : b[e - 4]);
-      scale_by_grad(ep.act, x, v);
+      for (int e = 0; e < 8; ++e) v[e] = e < 4 ? a[e] : b[e - 4];
+      if (ep.alpha != 1.0f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) reg[e] += v[e];
+        for (int e = 0; e < 8; ++e) v[e] *= ep.alpha;
+      }
+      if (in.p) {
+        BF16::unpack(extra, x);
+        scale_by_grad(ep.act, x, v);
+      }
+      if (ep.sums) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) reg[e] += v[e];
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(ep.alpha, e < 4 ? a[e] : b[e - 4], reg[e]);
       if (ep.z) store_row8<RAGGED>(ep.z + w.batch * ep.sZ + row * ep.ldz + col, n, v);
       activate(ep.act, v);
+      if (in.p) {
+        BF16::unpack(extra, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += x[e];
+        for (int e = 0; e < 8; ++e) v[e] += x[e];
+      }
     }
     store_row8<RAGGED>(w.C + w.batch * w.sC + row * w.ldc + col, n, v);
   }
@@ -137,57 +163,88 @@ struct ActLane {
   }
 };
 
-// The rows of a wave, as staged_rows: one 32-row MFMA block row at a time through LDS. The code of a row is
-// long, so the blocks are a loop (their accumulators are picked by uniform branches); the next
-// block's reads are in flight while a block is worked on.
-template <int kWaveN, int kBlkM, bool RAGGED>
+// The rows of a wave are worked on two passes of the wave at a time. The bias and the inputs of the first two
+// are read before the k loop: behind it they were a latency of memory that nothing hid (8192 x 1280 ->
+// 5120, bias: 103.5 us with the plain epilogue at 101.1, now the same to 0.4).
+template <int kWaveN>
+struct ActAhead {
+  static constexpr int LPR = kWaveN / 8;  // lanes per row
+  static constexpr int RPP = 64 / LPR;    // rows per pass
+  uint4 bias, first[2];
+};
+template <int kWaveN>
+__device__ __forceinline__ ActAhead<kWaveN> rows_ahead(const ActEpi& ep, const WaveRows& w, int lane) {
+  using A = ActAhead<kWaveN>;
+  A a;
+  const int col = w.wcol0 + (lane % A::LPR) * 8, n = min(8, max(0, w.N - col));
+  const ActInput in(ep, w, col);
+  a.bias = load_bias8(ep, w, col, n);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int row = w.wrow0 + p * A::RPP + lane / A::LPR;
+    a.first[p] = make_uint4(0, 0, 0, 0);
+    if (in.p && row < w.M && n > 0)
+      a.first[p] = ep.ragged ? load_row8<true>(in.p + row * in.ld, n)
+                             : load_row8<false>(in.p + row * in.ld, n);
+  }
+  return a;
+}
+
+// As staged_rows: 32-row MFMA block rows through LDS, kStage of them at a time (kStage x 32 rows of the wave's
+// staging area). The code of a row is long, so the blocks and passes are loops: the accumulators of a
+// block are picked by uniform branches, and the next passes' reads are in flight while two are worked on.
+template <int kWaveN, int kBlkM, bool RAGGED, int kStage>
 __device__ __forceinline__ void act_rows(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
-                                         const ActEpi& ep, const WaveRows& w) {
+                                         const ActEpi& ep, const WaveRows& w,
+                                         const ActAhead<kWaveN>& ahead) {
   constexpr int kBlkN = kWaveN / 32;
   constexpr int P = kWaveN * 4 + 16;  // staging pitch (bytes)
-  constexpr int LPR = kWaveN / 8;     // lanes per row
-  constexpr int RPP = 64 / LPR;       // rows per pass
-  constexpr int kPasses = 32 / RPP;
+  constexpr int LPR = ActAhead<kWaveN>::LPR, RPP = ActAhead<kWaveN>::RPP;
   const int r = lane & 31, h = lane >> 5;
   const int rr0 = lane / LPR, cc = (lane % LPR) * 8;
-  ActLane<RAGGED> out(ep, w, cc);
-  uint4 next[kPasses];
-#pragma unroll
-  for (int p = 0; p < kPasses; ++p) next[p] = out.fetch(w.wrow0 + p * RPP + rr0);
+  ActLane<RAGGED> out(ep, w, cc, ahead.bias);
+  uint4 next[2] = {ahead.first[0], ahead.first[1]};
 #pragma unroll 1
-  for (int i = 0; i < kBlkM; ++i) {
-    uint4 extra[kPasses];
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      extra[p] = next[p];
-      if (i + 1 < kBlkM) next[p] = out.fetch(w.wrow0 + 32 * (i + 1) + p * RPP + rr0);
-    }
+  for (int i = 0; i < kBlkM; i += kStage) {
 #pragma unroll
     for (int ii = 0; ii < kBlkM; ++ii)
-      if (i == ii) {
+      if (i == ii - ii % kStage) {
 #pragma unroll
         for (int j = 0; j < kBlkN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<f32x4_t HK_LDS*>(w.area + r * P + (32 * j + 8 * q + 4 * h) * 4) =
+            *reinterpret_cast<f32x4_t HK_LDS*>(w.area + (32 * (ii % kStage) + r) * P +
+                                              (32 * j + 8 * q + 4 * h) * 4) =
                 f32x4_t{acc[ii][j][4 * q], acc[ii][j][4 * q + 1], acc[ii][j][4 * q + 2],
                         acc[ii][j][4 * q + 3]};
       }
+    const int end = 32 * min(kBlkM - i, kStage);
+#pragma unroll 1
+    for (int s = 0; s < end; s += 2 * RPP) {
+      f32x4_t a[2], b[2];
+      uint4 extra[2];
+      const int row = w.wrow0 + 32 * i + s + rr0;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int rr = p * RPP + rr0;
-      const f32x4_t a = *reinterpret_cast<const f32x4_t HK_LDS*>(w.area + rr * P + cc * 4);
-      const f32x4_t b = *reinterpret_cast<const f32x4_t HK_LDS*>(w.area + rr * P + cc * 4 + 16);
-      out.row(w.wrow0 + 32 * i + rr, extra[p], a, b);
+      for (int p = 0; p < 2; ++p) {
+        const unsigned char HK_LDS* at = w.area + (s + p * RPP + rr0) * P + cc * 4;
+        a[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at);
+        b[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at + 16);
+        extra[p] = next[p];
+        // the rows behind the wave's last ones are the next wave's, or past M
+        next[p] = out.fetch(row + (2 + p) * RPP);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) out.row(row + p * RPP, extra[p], a[p], b[p]);
     }
   }
   if (ep.backward) out.template store_sums<LPR>(lane);
 }
-template <int kWaveN, int kBlkM>
+template <int kWaveN, int kBlkM, int kStage>
 __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
-                                           const ActEpi& ep, const WaveRows& w) {
-  if (ep.ragged) act_rows<kWaveN, kBlkM, true>(acc, lane, ep, w);
-  else act_rows<kWaveN, kBlkM, false>(acc, lane, ep, w);
+                                           const ActEpi& ep, const WaveRows& w,
+                                           const ActAhead<kWaveN>& ahead) {
+  if (ep.ragged) act_rows<kWaveN, kBlkM, true, kStage>(acc, lane, ep, w, ahead);
+  else act_rows<kWaveN, kBlkM, false, kStage>(acc, lane, ep, w, ahead);
 }
 
 // The same where the caller hands out the rows itself.

@@ -293,8 +293,15 @@ __global__ __launch_bounds__(256) void act_column_sums(const float* __restrict__
   const int col = blockIdx.x * 32 + tx;
   const float* p = sums + static_cast<int64_t>(blockIdx.y) * rows * pitch + col;
   float v = 0.f;
-  if (col < N)
-    for (int64_t r = grp; r < rows; r += 8) v += p[r * pitch];
+  if (col < N) {
+    for (int64_t r0 = grp; r0 < rows; r0 += 64) {  // eight loads in flight
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] = r0 + 8 * u < rows ? p[(r0 + 8 * u) * pitch] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += f[u];
+    }
+  }
   lds[grp][tx] = v;
   __syncthreads();
   if (grp == 0 && col < N) {

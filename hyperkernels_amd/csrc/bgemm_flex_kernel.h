@@ -196,6 +196,13 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
 #pragma unroll
     for (int j = 0; j < kBlkN; ++j) acc[i][j] = f32x16_t{};
 
+  // The wave's rows of C, staged for the stores at the start of the LDS. What the epilogue reads ahead is
+  // issued before the copies, so that the waits below, which count those, cover it.
+  const int wrow0 = m0 + wm * T::kWaveM, wcol0 = n0 + wn * T::kWaveN;
+  const WaveRows rows{g.C, g.ldc, g.sC, batch, M, N, wrow0, wcol0, tm * T::WM + wm,
+                      lds + wave * T::kStaging};
+  const auto ahead = rows_ahead<T::kWaveN>(g.ep, rows, lane);
+
   if constexpr (RAGGED) {
     if (ktiles > 0) {
       load(0);
@@ -294,22 +301,18 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
   if constexpr (T::KG > 1) {
     if (merge_groups<T>(acc, lds, group, wave, lane)) return;
   }
-  unsigned char HK_LDS* area = lds + wave * T::kStaging;
-  const int wrow0 = m0 + wm * T::kWaveM, wcol0 = n0 + wn * T::kWaveN;
   if (g.fo.C) {
-    store_f32<T::kWaveN, kBlkM>(acc, area, lane, g.fo, batch, M, N, wrow0, wcol0);
+    store_f32<T::kWaveN, kBlkM>(acc, rows.area, lane, g.fo, batch, M, N, wrow0, wcol0);
     return;
   }
   if (g.part) {
     store_partial<T::kWaveN, kBlkM>(
-        acc, area, lane,
+        acc, rows.area, lane,
         g.part + (static_cast<int64_t>(split) * (gridDim.z / g.split_k) + batch) * M * part_pitch(N),
         M, N, wrow0, wcol0);
     return;
   }
-  store_bf16<T::kWaveN, kBlkM>(
-      acc, lane, g.ep,
-      WaveRows{g.C, g.ldc, g.sC, batch, M, N, wrow0, wcol0, tm * T::WM + wm, area});
+  store_bf16<T::kWaveN, kBlkM, 1>(acc, lane, g.ep, rows, ahead);
 }
 
 template <class T, bool AK, bool BKM, bool RAGGED, class E>

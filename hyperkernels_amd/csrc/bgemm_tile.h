@@ -161,6 +161,7 @@ struct Epi {
   const uint16_t* bias;
   int64_t brow, bcol;
   bool ragged;  // rows of C that are no whole number of aligned 16-byte vectors
+  static constexpr int kWideStage = 1;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
 __device__ __forceinline__ float bias_at(const Epi& ep, int row, int col) {
@@ -319,9 +320,15 @@ __device__ __forceinline__ void emit_rows(const Epi& ep, const WaveRows& w, int,
     emit(Bf16RowOut<false>{ep, Cb, w.ldc, w.M, w.N, w.wrow0, w.wcol0});
   }
 }
-template <int kWaveN, int kBlkM>
+// What an epilogue reads ahead of the k loop: nothing here.
+struct NothingAhead {};
+template <int kWaveN>
+__device__ __forceinline__ NothingAhead rows_ahead(const Epi&, const WaveRows&, int) {
+  return {};
+}
+template <int kWaveN, int kBlkM, int kStage>
 __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
-                                           const Epi& ep, const WaveRows& w) {
+                                           const Epi& ep, const WaveRows& w, const NothingAhead&) {
   emit_rows<kWaveN / 8>(ep, w, lane, [&](auto&& out) {
     staged_rows<kWaveN, kBlkM>(acc, w.area, lane, out);
   });

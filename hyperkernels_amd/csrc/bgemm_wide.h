@@ -37,6 +37,11 @@ struct TileN {
   static constexpr int kLoadsB = kStageBytesB / 1024 / kWaves;
   static constexpr size_t kLdsBytes =
       static_cast<size_t>(kStages) * (TileM<BMT>::kStageBytes + kStageBytesB);
+  // the LDS of a kernel whose waves stage `blocks` block rows at a time
+  static constexpr size_t lds_bytes(int blocks) {
+    const size_t staging = static_cast<size_t>(kWaves) * blocks * 32 * (kWaveN * 4 + 16);
+    return staging > kLdsBytes ? staging : kLdsBytes;
+  }
 };
 
 // Main loop per k-tile kt (ring slot kt % 2), 4 k steps of 16 MFMAs each:
@@ -148,6 +153,13 @@ __device__ __forceinline__ void tile_body(
 #pragma unroll
     for (int j = 0; j < kBlkN; ++j) acc[i][j] = f32x16_t{};
 
+  // The wave's rows of C, staged for the stores at the start of the ring. What the epilogue reads ahead is
+  // issued before the copies, so that the waits below, which count those, cover it.
+  unsigned char HK_LDS* area = ldsA + wave * (E::kWideStage * 32 * (kWaveN * 4 + 16));
+  const int wrow0 = m0 + wm * kWaveM, wcol0 = n0 + wn * kWaveN;
+  const WaveRows rows{C, ldc, sC, batch, M, N, wrow0, wcol0, 2 * tm + wm, area};
+  const auto ahead = rows_ahead<kWaveN>(ep, rows, lane);
+
 #pragma unroll
   for (int p = 0; p < kStages; ++p)
     if (p < ktiles) {
@@ -251,10 +263,7 @@ __device__ __forceinline__ void tile_body(
   // wm*128 + 32 i + l % 32 and columns wn*kWaveN + 32 j + 8 q + 4 (l / 32) .. +3; the rows go
   // out through LDS (staged_rows).
   // every wave is done with the LDS ring: its start becomes the waves' staging areas
-  static_assert(kWaves * 32 * (kWaveN * 4 + 16) <= TileN<BNT, BMT>::kLdsBytes, "staging fits");
   __syncthreads();
-  unsigned char HK_LDS* area = ldsA + wave * (32 * (kWaveN * 4 + 16));
-  const int wrow0 = m0 + wm * kWaveM, wcol0 = n0 + wn * kWaveN;
   if (PARTIAL && fo.C) {
     // one split: fp32 C with alpha, beta and the bias applied here
     store_f32<kWaveN, kBlkM>(acc, area, lane, fo, batch, M, N, wrow0, wcol0);
@@ -267,8 +276,7 @@ __device__ __forceinline__ void tile_body(
         N, wrow0, wcol0);
     return;
   }
-  store_bf16<kWaveN, kBlkM>(acc, lane, ep,
-                            WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 2 * tm + wm, area});
+  store_bf16<kWaveN, kBlkM, E::kWideStage>(acc, lane, ep, rows, ahead);
 }
 
 // One column region: workgroup x takes tile x.
@@ -522,7 +530,8 @@ hipError_t launch_tiled(dim3 grid, hipStream_t stream, int M, int N, int K, cons
                         int64_t sC, int split_k, int kps, float* part, const hk::F32Out& fo,
                         int n_base, int n_end) {
   static_assert(BNT != 0 || BMT == 256, "the mixed-width launch uses 256-row tiles");
-  constexpr size_t kLds = TileN<BNT == 0 ? 256 : BNT, BMT>::kLdsBytes;
+  constexpr size_t kLds = TileN<BNT == 0 ? 256 : BNT, BMT>::lds_bytes(E::kWideStage);
+  static_assert(kLds <= 160 * 1024, "fits gfx950's 160 KiB of LDS");
   const void* fn;
   if constexpr (BNT == 0) fn = reinterpret_cast<const void*>(&bgemm_mixed<AK, BKM, P, E>);
   else fn = reinterpret_cast<const void*>(&bgemm_tiled<AK, BKM, P, BNT, BMT, E>);
