@@ -52,16 +52,25 @@ def _dev(*ts: torch.Tensor | None) -> None:
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # HK_TYPE_*
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
+def _device(fn: str, t: torch.Tensor) -> int:
+    """The device of a call's first tensor: the current one, whose stream the launch goes to."""
+    d = t.get_device()  # -1: a host tensor
+    if d < 0 or d != torch._C._cuda_getDevice():
+        raise ValueError(f"{fn}: tensors of the current device only")
+    return d
+
+
 def _here(fn: str, *ts: torch.Tensor | None) -> None:
-    """Device tensors of the current device, whose stream the launch goes to."""
+    """Device tensors of the current device."""
     cur = None
     for t in ts:
-        if t is not None:
-            d = t.get_device()  # -1: a host tensor
-            if d != cur:
-                if cur is not None or d < 0 or d != torch._C._cuda_getDevice():
-                    raise ValueError(f"{fn}: tensors of the current device only")
-                cur = d
+        if t is not None and t.get_device() != cur:
+            if cur is not None:
+                raise ValueError(f"{fn}: tensors of the current device only")
+            cur = _device(fn, t)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -308,10 +317,13 @@ def _adam8_check(fn: str, m, v, m_scale, v_scale, blocks: int) -> None:
 
 def _flat(fn: str, *ts: torch.Tensor | None) -> None:
     """Contiguous tensors of the current device."""
-    _here(fn, *ts)
+    cur = None
     for t in ts:
-        if t is not None and not t.is_contiguous():
-            raise ValueError(f"{fn}: contiguous tensors only")
+        if t is not None:
+            if cur is None:
+                cur = _device(fn, t)
+            if t.get_device() != cur or not t.is_contiguous():
+                raise ValueError(f"{fn}: contiguous tensors of the current device only")
 
 
 def adam8_states(sizes: Sequence[int], device="cuda"):
@@ -341,8 +353,8 @@ def adam8_dequantize(m, v, m_scale, v_scale, m_out=None, v_out=None):
     m_out and v_out hold."""
     n = m.numel() if m_out is None else m_out.numel()
     _adam8_check("adam8_dequantize", m, v, m_scale, v_scale, -(-n // ADAM8_BLOCK))
-    m_out = torch.empty(n, device=m.device, dtype=torch.float32) if m_out is None else m_out
-    v_out = torch.empty(n, device=m.device, dtype=torch.float32) if v_out is None else v_out
+    m_out = m_scale.new_empty(n) if m_out is None else m_out
+    v_out = m_scale.new_empty(n) if v_out is None else v_out
     _flat("adam8_dequantize", m, v, m_scale, v_scale, m_out, v_out)
     if m_out.dtype is not torch.float32 or v_out.dtype is not torch.float32 or v_out.numel() != n:
         raise ValueError("adam8_dequantize: fp32 outputs of equal size")
@@ -510,39 +522,49 @@ def attn_backward(q, k, v, do, lse, D, causal: bool, scale: float | None = None,
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}  # HK_ACT_*
 
 
-def _matrix(fn: str, t: torch.Tensor, batch: int, rows: int, cols: int) -> tuple[int, int, int]:
+def _matrix(fn: str, t: torch.Tensor, dev: int, batch: int, rows: int,
+            cols: int) -> tuple[int, int, int]:
     """(address, leading dimension, batch stride) of a bf16 matrix [rows, cols], or
     [batch, rows, cols]."""
-    sh, st = t.shape, t.stride()
-    if len(sh) == 2:
-        ok, step = batch == 1 and sh[0] == rows and sh[1] == cols, 0
-    else:
-        ok = len(sh) == 3 and sh[0] == batch and sh[1] == rows and sh[2] == cols
-        step = st[0] if ok and batch > 1 else 0
-    if not ok or t.dtype is not torch.bfloat16 or (st[-1] != 1 and cols > 1):
-        raise ValueError(f"{fn}: bf16 matrices of matching shapes with a unit last-dim stride; "
-                         f"[{batch}, {rows}, {cols}] expected, {tuple(sh)} given")
+    sh, st, step = t.shape, t.stride(), 0
+    if batch != 1 or len(sh) != 2:
+        if sh != (batch, rows, cols):
+            raise ValueError(f"{fn}: [{batch}, {rows}, {cols}] expected, {tuple(sh)} given")
+        step = st[0] if batch != 1 else 0
+    elif sh != (rows, cols):
+        raise ValueError(f"{fn}: [{rows}, {cols}] expected, {tuple(sh)} given")
+    if t.dtype is not _BF16 or t.get_device() != dev or (st[-1] != 1 and cols > 1):
+        raise ValueError(f"{fn}: bf16 matrices of one device with a unit last-dim stride")
     ld = st[-2]
-    return t.data_ptr(), (ld if rows > 1 or ld > cols else cols), step
+    if rows == 1 and ld < cols:
+        ld = cols
+    return t.data_ptr(), ld, step
 
 
-def _vector(fn: str, t: torch.Tensor, dtype, batch: int, n: int) -> tuple[int, int]:
+def _vector(fn: str, t: torch.Tensor, dtype, dev: int, batch: int, n: int) -> tuple[int, int]:
     """(address, batch stride) of a vector [n], or [batch, n]."""
-    sh = t.shape
-    if t.dtype is not dtype or sh[-1:] != (n,) or (len(sh) == 2 and sh[0] != batch) or (
-            len(sh) > 2) or (t.stride(-1) != 1 and n > 1):
+    sh, st = t.shape, t.stride()
+    if t.dtype is not dtype or t.get_device() != dev or (sh != (n,) and sh != (batch, n)) or (
+            st[-1] != 1 and n > 1):
         raise ValueError(f"{fn}: {dtype} vectors [{n}], or [{batch}, {n}]; {tuple(sh)} given")
-    return t.data_ptr(), t.stride(0) if len(sh) == 2 and batch > 1 else 0
+    return t.data_ptr(), st[0] if len(sh) == 2 and batch != 1 else 0
+
+
+_NO_MATRIX, _NO_VECTOR = (None, 0, 0), (None, 0)
 
 
 def _product(fn: str, a, b, trans_a: bool, trans_b: bool, activation: str):
-    """(batch, M, N, K, activation) of op(a) op(b)."""
+    """(batch, M, N, K, activation, device) of op(a) op(b)."""
     ash, bsh = a.shape, b.shape
     act = _ACT.get(activation)
-    if len(ash) != len(bsh) or not 2 <= len(ash) <= 3 or act is None:
+    if act is None or len(ash) != len(bsh) or not 2 <= len(ash) <= 3:
         raise ValueError(f"{fn}: matrices or batches of them, and one of {', '.join(_ACT)}")
-    K, M = ash[-2:] if trans_a else ash[:-3:-1]
-    return (ash[0] if len(ash) == 3 else 1), M, bsh[-2] if trans_b else bsh[-1], K, act
+    if trans_a:
+        K, M = ash[-2], ash[-1]
+    else:
+        M, K = ash[-2], ash[-1]
+    return (ash[0] if len(ash) == 3 else 1, M, bsh[-2] if trans_b else bsh[-1], K, act,
+            _device(fn, a))
 
 
 def _call_captured(name: str, need, *args) -> None:
@@ -562,8 +584,7 @@ def _call_captured(name: str, need, *args) -> None:
 
 
 def _bf16_bits(x: float) -> int:
-    return 0x3F80 if x == 1.0 else int(
-        torch.tensor(x, dtype=torch.bfloat16).view(torch.int16)) & 0xFFFF
+    return int(torch.tensor(x, dtype=torch.bfloat16).view(torch.int16)) & 0xFFFF
 
 
 def bgemm_act(a, b, bias=None, activation: str = "none", residual=None, preact=None, out=None,
@@ -572,20 +593,19 @@ def bgemm_act(a, b, bias=None, activation: str = "none", residual=None, preact=N
     goes into the activation ("none", "relu", "gelu" or "silu") is stored in `preact` where that is
     passed. bias is [N], or [batch, N]; residual may be `out` itself."""
     fn = "bgemm_act"
-    batch, M, N, K, act = _product(fn, a, b, trans_a, trans_b, activation)
+    batch, M, N, K, act, dev = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
-        out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
-                          dtype=torch.bfloat16)
-    _here(fn, a, b, bias, residual, preact, out)
-    A = _matrix(fn, a, batch, K, M) if trans_a else _matrix(fn, a, batch, M, K)
-    B = _matrix(fn, b, batch, N, K) if trans_b else _matrix(fn, b, batch, K, N)
-    C = _matrix(fn, out, batch, M, N)
-    R = (None, 0, 0) if residual is None else _matrix(fn, residual, batch, M, N)
-    Z = (None, 0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
-    v = (None, 0) if bias is None else _vector(fn, bias, torch.bfloat16, batch, N)
+        out = a.new_empty((M, N) if a.dim() == 2 else (batch, M, N))
+    A = _matrix(fn, a, dev, batch, K, M) if trans_a else _matrix(fn, a, dev, batch, M, K)
+    B = _matrix(fn, b, dev, batch, N, K) if trans_b else _matrix(fn, b, dev, batch, K, N)
+    C = _matrix(fn, out, dev, batch, M, N)
+    R = _NO_MATRIX if residual is None else _matrix(fn, residual, dev, batch, M, N)
+    Z = _NO_MATRIX if preact is None else _matrix(fn, preact, dev, batch, M, N)
+    v = _NO_VECTOR if bias is None else _vector(fn, bias, _BF16, dev, batch, N)
     _call_captured("hk_bgemm_act",
                    lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch, 0),
-                   trans_a, trans_b, M, N, K, _bf16_bits(alpha), *A, *B, *v, act, *R, *Z, *C, batch)
+                   trans_a, trans_b, M, N, K, 0x3F80 if alpha == 1.0 else _bf16_bits(alpha), *A, *B,
+                   *v, act, *R, *Z, *C, batch)
     return out
 
 
@@ -597,25 +617,23 @@ def bgemm_act_backward(a, b, preact=None, activation: str = "none", dbias=None, 
     wanted) is added to, or written where accumulate is False: the sums of d over rows (and, [N],
     batches) before it is rounded."""
     fn = "bgemm_act_backward"
-    batch, M, N, K, act = _product(fn, a, b, trans_a, trans_b, activation)
+    batch, M, N, K, act, dev = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
-        out = torch.empty((M, N) if a.dim() == 2 else (batch, M, N), device=a.device,
-                          dtype=torch.bfloat16)
-    _here(fn, a, b, preact, dbias, out)
-    A = _matrix(fn, a, batch, K, M) if trans_a else _matrix(fn, a, batch, M, K)
-    B = _matrix(fn, b, batch, N, K) if trans_b else _matrix(fn, b, batch, K, N)
-    C = _matrix(fn, out, batch, M, N)
+        out = a.new_empty((M, N) if a.dim() == 2 else (batch, M, N))
+    A = _matrix(fn, a, dev, batch, K, M) if trans_a else _matrix(fn, a, dev, batch, M, K)
+    B = _matrix(fn, b, dev, batch, N, K) if trans_b else _matrix(fn, b, dev, batch, K, N)
+    C = _matrix(fn, out, dev, batch, M, N)
     if preact is None and act:
         raise ValueError(f"{fn}: the activation's derivative needs preact")
-    Z = (None, 0, 0) if preact is None else _matrix(fn, preact, batch, M, N)
-    v = (None, 0) if dbias is None else _vector(fn, dbias, torch.float32, batch, N)
-    if dbias is not None and dbias.dim() == 2 and batch > 1 and v[1] < N:
+    Z = _NO_MATRIX if preact is None else _matrix(fn, preact, dev, batch, M, N)
+    v = _NO_VECTOR if dbias is None else _vector(fn, dbias, _F32, dev, batch, N)
+    if v[1] < N and dbias is not None and dbias.dim() == 2 and batch != 1:
         raise ValueError(f"{fn}: the rows of dbias overlap")
     _call_captured("hk_bgemm_act_backward",
                    lambda: lib().hk_bgemm_act_workspace(trans_a, trans_b, M, N, K, batch,
                                                         dbias is not None),
-                   trans_a, trans_b, M, N, K, _bf16_bits(alpha), *A, *B, act, *Z, *C, *v, accumulate,
-                   batch)
+                   trans_a, trans_b, M, N, K, 0x3F80 if alpha == 1.0 else _bf16_bits(alpha), *A, *B,
+                   act, *Z, *C, *v, accumulate, batch)
     return out
 
 
@@ -638,75 +656,88 @@ class QkNormRopeParams(ctypes.Structure):
 
 # the same block, packed in one go (2 us; the ctypes structure takes 6)
 _QK_PACK = struct.Struct("@15P6if3?21q").pack
-_NO_SIDE = (0, 0, 0, 0, 0, 0), ((0, 0, 0),) * 3  # pointers x, w, out, dy, dx, dw; strides x, out, dx
+_NO_SIDE = (0,) * 15  # x, weight, output, gradients of x and weight; strides; heads
 
 
-def _qk_side(fn, x, w, o, g, gw, like, out, backward):
+def _qk_side(fn, x, w, o, g, gw, dev, B, T, d, dt, out, backward):
     """(pointers, strides, heads) of q or of k; o: the output, or in the backward pass its gradient."""
     if x is None:
         if o is not None or g is not None or gw is not None:
             raise ValueError(f"{fn}: outputs and gradients of a tensor that is not passed")
-        return *_NO_SIDE, 0
-    sh, dt, d = x.shape, x.dtype, like[3]
-    if len(sh) != 4 or dt is not like[4] or sh[0] != like[0] or sh[2] != like[2] or sh[3] != d:
-        raise ValueError(f"{fn}: q and k share type, batch, length and head_dim")
-    if o is None or o.shape != sh or o.dtype is not out:
+        return _NO_SIDE
+    sh = x.shape
+    H = sh[1]
+    if sh != (B, H, T, d) or x.dtype is not dt or x.get_device() != dev:
+        raise ValueError(f"{fn}: q and k share type, device, batch, length and head_dim")
+    if o is None or o.shape != sh or o.dtype is not out or o.get_device() != dev:
         raise ValueError(f"{fn}: outputs have their input's shape, and its type or fp32")
-    strides = _strides(x), _strides(o), (0, 0, 0)
-    wp = gp = gwp = 0
+    xB, xH, xM, x1 = x.stride()
+    oB, oH, oM, o1 = o.stride()
+    if x1 != 1 or o1 != 1:
+        raise ValueError(f"{fn}: tensors are [B, heads, T, head_dim] with a unit last-dim stride")
+    wp = gp = gwp = gB = gM = gH = 0
     if w is not None:
-        if w.dtype is not dt or w.shape != (d,) or (d > 1 and w.stride(0) != 1):
+        if w.dtype is not dt or w.shape != (d,) or w.get_device() != dev or (
+                d > 1 and w.stride(0) != 1):
             raise ValueError(f"{fn}: weights are [head_dim] of the inputs' type")
         wp = w.data_ptr()
-    if g is not None:
-        if g.shape != sh or g.dtype is not dt:
+    if backward:
+        if g is None or g.shape != sh or g.dtype is not dt or g.get_device() != dev:
             raise ValueError(f"{fn}: gradients have their input's shape and type")
-        gp, strides = g.data_ptr(), (*strides[:2], _strides(g))
-    if gw is not None:
-        if gw.dtype is not torch.float32 or gw.shape != (d,) or (d > 1 and gw.stride(0) != 1):
-            raise ValueError(f"{fn}: gradients of the weights are fp32 [head_dim]")
-        gwp = gw.data_ptr()
-    op = o.data_ptr()
-    return ((x.data_ptr(), wp, 0 if backward else op, op if backward else 0, gp, gwp), strides, sh[1])
+        gB, gH, gM, g1 = g.stride()
+        if g1 != 1:
+            raise ValueError(f"{fn}: tensors are [B, heads, T, head_dim] with a unit last-dim stride")
+        gp = g.data_ptr()
+        if gw is not None:
+            if gw.dtype is not _F32 or gw.shape != (d,) or gw.get_device() != dev or (
+                    d > 1 and gw.stride(0) != 1):
+                raise ValueError(f"{fn}: gradients of the weights are fp32 [head_dim]")
+            gwp = gw.data_ptr()
+    return (x.data_ptr(), wp, o.data_ptr(), gp, gwp, xB, xM, xH, oB, oM, oH, gB, gM, gH, H)
 
 
 def _qk_params(fn, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved, qo, ko,
                backward=False, dq=None, dk=None, dqw=None, dkw=None, accumulate=False) -> bytes:
     """The parameter block; qo, ko: the outputs, or in the backward pass their gradients."""
-    x = q if q is not None else k
+    x, o = (q, qo) if q is not None else (k, ko)
     if x is None or x.dim() != 4 or x.dtype not in _TYPE:
         raise ValueError(f"{fn}: q or k, [B, heads, T, head_dim], fp32, bf16 or fp16")
-    _here(fn, q, k, cos, sin, positions, q_weight, k_weight, qo, ko, dq, dk, dqw, dkw)
-    B, _, T, d = x.shape
-    like, o = (B, 0, T, d, x.dtype), qo if qo is not None else ko
-    out = None if o is None else o.dtype
-    if out is not x.dtype and out is not torch.float32:
+    dev = _device(fn, x)
+    (B, _, T, d), dt, out = x.shape, x.dtype, None if o is None else o.dtype
+    if out is not dt and out is not _F32:
         raise ValueError(f"{fn}: outputs have their input's type, or fp32")
-    (xq, wq, yq, dyq, gq, gwq), (sxq, syq, sgq), hq = _qk_side(fn, q, q_weight, qo, dq, dqw, like,
-                                                               out, backward)
-    (xk, wk, yk, dyk, gk, gwk), (sxk, syk, sgk), hk_ = _qk_side(fn, k, k_weight, ko, dk, dkw, like,
-                                                                out, backward)
+    qp, qw, qy, qg, qgw, qB, qM, qH, qoB, qoM, qoH, qgB, qgM, qgH, hq = _qk_side(
+        fn, q, q_weight, qo, dq, dqw, dev, B, T, d, dt, out, backward)
+    kp, kw, ky, kg, kgw, kB, kM, kH, koB, koM, koH, kgB, kgM, kgH, nk = _qk_side(
+        fn, k, k_weight, ko, dk, dkw, dev, B, T, d, dt, out, backward)
     cp = sp = pp = rows = stride = rot = pos_stride = 0
     if cos is not None or sin is not None:
         if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or (
-                cos.dtype is not torch.float32) or sin.dtype is not torch.float32 or (
-                cos.stride() != sin.stride()) or (cos.stride(1) != 1 and cos.shape[1] > 1):
+                cos.dtype is not _F32) or sin.dtype is not _F32 or cos.stride() != sin.stride() or (
+                cos.get_device() != dev) or sin.get_device() != dev:
             raise ValueError(f"{fn}: cos and sin are fp32 [rows, rotary_dim / 2], laid out alike")
         rows, half = cos.shape
-        stride, rot = cos.stride(0), 2 * half
+        stride, one = cos.stride()
+        if one != 1 and half > 1:
+            raise ValueError(f"{fn}: cos and sin have a unit last-dim stride")
+        rot = 2 * half
         if rows == 1 and stride < half:
             stride = half
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        sh = positions.shape
-        if positions.dtype is not torch.int64 or sh[-1:] != (T,) or len(sh) > 2 or (
-                len(sh) == 2 and sh[0] != B) or (positions.stride(-1) != 1 and T > 1):
+        sh, st = positions.shape, positions.stride()
+        if positions.dtype is not torch.int64 or (sh != (B, T) and sh != (T,)) or (
+                st[-1] != 1 and T > 1) or positions.get_device() != dev:
             raise ValueError(f"{fn}: positions are int64 [B, T] or [T]")
         pp = positions.data_ptr()
-        pos_stride = positions.stride(0) if len(sh) == 2 else 0
-    return _QK_PACK(xq, xk, wq, wk, cp, sp, pp, yq, yk, dyq, dyk, gq, gk, gwq, gwk, B, T, hq, hk_, d,
-                    rot, eps, interleaved, out is not x.dtype, accumulate, rows, stride, pos_stride,
-                    *sxq, *sxk, *syq, *syk, *sgq, *sgk)
+        pos_stride = st[0] if len(sh) == 2 else 0
+    if backward:
+        outs, grads = (0, 0), (qy, ky)
+    else:
+        outs, grads = (qy, ky), (0, 0)
+    return _QK_PACK(qp, kp, qw, kw, cp, sp, pp, *outs, *grads, qg, kg, qgw, kgw, B, T, hq, nk, d, rot,
+                    eps, interleaved, out is not dt, accumulate, rows, stride, pos_stride, qB, qM, qH,
+                    kB, kM, kH, qoB, qoM, qoH, koB, koM, koH, qgB, qgM, qgH, kgB, kgM, kgH)
 
 
 def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None,
@@ -717,9 +748,9 @@ def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None
     positions (None: token t at position t). Returns (q_out, k_out) of q's type or out_dtype, which
     may be fp32 for 16-bit inputs. q_out and k_out may be q and k themselves."""
     if q_out is None and q is not None:
-        q_out = torch.empty(q.shape, device=q.device, dtype=out_dtype or q.dtype)
+        q_out = q.new_empty(q.shape, dtype=out_dtype)
     if k_out is None and k is not None:
-        k_out = torch.empty(k.shape, device=k.device, dtype=out_dtype or k.dtype)
+        k_out = k.new_empty(k.shape, dtype=out_dtype)
     p = _qk_params("qk_norm_rope_forward", q, k, cos, sin, positions, q_weight, k_weight, eps,
                    interleaved, q_out, k_out)
     call("hk_qk_norm_rope_forward", p, _TYPE[(q if q is not None else k).dtype], _stream())
@@ -729,7 +760,7 @@ def qk_norm_rope_forward(q, k, cos=None, sin=None, positions=None, q_weight=None
 def _by_token(t):
     """An empty [B, heads, T, d] tensor with the heads of a token together, as a projection has them."""
     B, H, T, d = t.shape
-    return torch.empty_strided((B, H, T, d), (T * H * d, d, H * d, 1), device=t.device, dtype=t.dtype)
+    return t.new_empty_strided((B, H, T, d), (T * H * d, d, H * d, 1))
 
 
 def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=None, q_weight=None,
