@@ -24,6 +24,7 @@ struct ActEpi {
   int64_t ldz, sZ;
   float* sums;
   int sum_rows, pitch;
+  static constexpr int kWideAhead = 4;  // passes whose inputs are in flight there
   static constexpr int kWideStage = 2;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
@@ -163,24 +164,28 @@ struct ActLane {
   }
 };
 
-// The rows of a wave are worked on two passes of the wave at a time. The bias and the inputs of the first two
-// are read before the k loop: behind it they were a latency of memory that nothing hid (8192 x 1280 ->
-// 5120, bias: 103.5 us with the plain epilogue at 101.1, now the same to 0.4).
-template <int kWaveN>
+// The rows of a wave are worked on two passes of the wave at a time, with the inputs of DEPTH in flight. Those of
+// the first, and the bias, are read before the k loop: behind it they were a latency of memory that
+// nothing hid (8192 x 1280 -> 5120, bias: 103.5 us with the plain epilogue at 101.1, now the same to
+// 0.4). One workgroup runs on a CU, so all tiles of a round read their inputs at once: two passes in
+// flight a wave are 16 KiB a CU, too little for the memory's latency, eight do not fit the registers
+// (8192 x 1280 -> 5120, residual: two 123, four 116, six 117, eight 126 us; GELU' 128, 125, 125, 134).
+template <int kWaveN, int DEPTH>
 struct ActAhead {
   static constexpr int LPR = kWaveN / 8;  // lanes per row
   static constexpr int RPP = 64 / LPR;    // rows per pass
-  uint4 bias, first[2];
+  uint4 bias, first[DEPTH];
 };
-template <int kWaveN>
-__device__ __forceinline__ ActAhead<kWaveN> rows_ahead(const ActEpi& ep, const WaveRows& w, int lane) {
-  using A = ActAhead<kWaveN>;
+template <int kWaveN, int DEPTH>
+__device__ __forceinline__ ActAhead<kWaveN, DEPTH> rows_ahead(const ActEpi& ep, const WaveRows& w,
+                                                              int lane) {
+  using A = ActAhead<kWaveN, DEPTH>;
   A a;
   const int col = w.wcol0 + (lane % A::LPR) * 8, n = min(8, max(0, w.N - col));
   const ActInput in(ep, w, col);
   a.bias = load_bias8(ep, w, col, n);
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int p = 0; p < DEPTH; ++p) {
     const int row = w.wrow0 + p * A::RPP + lane / A::LPR;
     a.first[p] = make_uint4(0, 0, 0, 0);
     if (in.p && row < w.M && n > 0)
@@ -193,17 +198,19 @@ __device__ __forceinline__ ActAhead<kWaveN> rows_ahead(const ActEpi& ep, const W
 // As staged_rows: 32-row MFMA block rows through LDS, kStage of them at a time (kStage x 32 rows of the wave's
 // staging area). The code of a row is long, so the blocks and passes are loops: the accumulators of a
 // block are picked by uniform branches, and the next passes' reads are in flight while two are worked on.
-template <int kWaveN, int kBlkM, bool RAGGED, int kStage>
+template <int kWaveN, int kBlkM, bool RAGGED, int kStage, int DEPTH>
 __device__ __forceinline__ void act_rows(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
                                          const ActEpi& ep, const WaveRows& w,
-                                         const ActAhead<kWaveN>& ahead) {
+                                         const ActAhead<kWaveN, DEPTH>& ahead) {
   constexpr int kBlkN = kWaveN / 32;
   constexpr int P = kWaveN * 4 + 16;  // staging pitch (bytes)
-  constexpr int LPR = ActAhead<kWaveN>::LPR, RPP = ActAhead<kWaveN>::RPP;
+  constexpr int LPR = ActAhead<kWaveN, DEPTH>::LPR, RPP = ActAhead<kWaveN, DEPTH>::RPP;
   const int r = lane & 31, h = lane >> 5;
   const int rr0 = lane / LPR, cc = (lane % LPR) * 8;
   ActLane<RAGGED> out(ep, w, cc, ahead.bias);
-  uint4 next[2] = {ahead.first[0], ahead.first[1]};
+  uint4 next[DEPTH];
+#pragma unroll
+  for (int p = 0; p < DEPTH; ++p) next[p] = ahead.first[p];
 #pragma unroll 1
   for (int i = 0; i < kBlkM; i += kStage) {
 #pragma unroll
@@ -230,8 +237,14 @@ __device__ __forceinline__ void act_rows(const f32x16_t (&acc)[kBlkM][kWaveN / 3
         a[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at);
         b[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at + 16);
         extra[p] = next[p];
-        // the rows behind the wave's last ones are the next wave's, or past M
-        next[p] = out.fetch(row + (2 + p) * RPP);
+      }
+#pragma unroll
+      for (int p = 0; p + 2 < DEPTH; ++p) next[p] = next[p + 2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        // not the rows behind the wave's last ones
+        const int at = 32 * i + s + (DEPTH + p) * RPP;
+        if (at < 32 * kBlkM) next[DEPTH - 2 + p] = out.fetch(w.wrow0 + at + rr0);
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) out.row(row + p * RPP, extra[p], a[p], b[p]);
@@ -239,12 +252,12 @@ __device__ __forceinline__ void act_rows(const f32x16_t (&acc)[kBlkM][kWaveN / 3
   }
   if (ep.backward) out.template store_sums<LPR>(lane);
 }
-template <int kWaveN, int kBlkM, int kStage>
+template <int kWaveN, int kBlkM, int kStage, int DEPTH>
 __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
                                            const ActEpi& ep, const WaveRows& w,
-                                           const ActAhead<kWaveN>& ahead) {
-  if (ep.ragged) act_rows<kWaveN, kBlkM, true, kStage>(acc, lane, ep, w, ahead);
-  else act_rows<kWaveN, kBlkM, false, kStage>(acc, lane, ep, w, ahead);
+                                           const ActAhead<kWaveN, DEPTH>& ahead) {
+  if (ep.ragged) act_rows<kWaveN, kBlkM, true, kStage, DEPTH>(acc, lane, ep, w, ahead);
+  else act_rows<kWaveN, kBlkM, false, kStage, DEPTH>(acc, lane, ep, w, ahead);
 }
 
 // The same where the caller hands out the rows itself.

@@ -201,7 +201,8 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
   const int wrow0 = m0 + wm * T::kWaveM, wcol0 = n0 + wn * T::kWaveN;
   const WaveRows rows{g.C, g.ldc, g.sC, batch, M, N, wrow0, wcol0, tm * T::WM + wm,
                       lds + wave * T::kStaging};
-  const auto ahead = rows_ahead<T::kWaveN>(g.ep, rows, lane);
+  // up to four passes of the wave over its rows
+  const auto ahead = rows_ahead<T::kWaveN, T::kWaveM * T::kWaveN >= 2048 ? 4 : 2>(g.ep, rows, lane);
 
   if constexpr (RAGGED) {
     if (ktiles > 0) {

@@ -161,6 +161,7 @@ struct Epi {
   const uint16_t* bias;
   int64_t brow, bcol;
   bool ragged;  // rows of C that are no whole number of aligned 16-byte vectors
+  static constexpr int kWideAhead = 0;
   static constexpr int kWideStage = 1;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
@@ -322,7 +323,7 @@ __device__ __forceinline__ void emit_rows(const Epi& ep, const WaveRows& w, int,
 }
 // What an epilogue reads ahead of the k loop: nothing here.
 struct NothingAhead {};
-template <int kWaveN>
+template <int kWaveN, int DEPTH>
 __device__ __forceinline__ NothingAhead rows_ahead(const Epi&, const WaveRows&, int) {
   return {};
 }

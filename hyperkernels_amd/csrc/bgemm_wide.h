@@ -158,7 +158,7 @@ __device__ __forceinline__ void tile_body(
   unsigned char HK_LDS* area = ldsA + wave * (E::kWideStage * 32 * (kWaveN * 4 + 16));
   const int wrow0 = m0 + wm * kWaveM, wcol0 = n0 + wn * kWaveN;
   const WaveRows rows{C, ldc, sC, batch, M, N, wrow0, wcol0, 2 * tm + wm, area};
-  const auto ahead = rows_ahead<kWaveN>(ep, rows, lane);
+  const auto ahead = rows_ahead<kWaveN, E::kWideAhead>(ep, rows, lane);
 
 #pragma unroll
   for (int p = 0; p < kStages; ++p)
