@@ -260,20 +260,40 @@ __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN /
   else act_rows<kWaveN, kBlkM, false, kStage, DEPTH>(acc, lane, ep, w, ahead);
 }
 
-// The same where the caller hands out the rows itself.
-template <int LPR, bool RAGGED, class Emit>
+// The same where the caller hands out the rows itself: the inputs of four passes are in flight.
+template <int LPR, int BLOCK, bool RAGGED>
+struct ActPasses {
+  static constexpr int RPP = HK_WAVE / LPR, kPerBlock = (BLOCK + RPP - 1) / RPP;
+  ActLane<RAGGED> lane_out;
+  int row0;  // of the lane in a pass
+  uint4 extra, next[4];
+  __device__ ActPasses(const ActEpi& ep, const WaveRows& w, int lane)
+      : lane_out(ep, w, (lane % LPR) * 8), row0(w.wrow0 + lane / LPR) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) next[n] = fetch(n);
+  }
+  __device__ uint4 fetch(int n) const {
+    return lane_out.fetch(row0 + BLOCK * (n / kPerBlock) + RPP * (n % kPerBlock));
+  }
+  __device__ void pass(int n) {
+    extra = next[n % 4];
+    next[n % 4] = fetch(n + 4);
+  }
+  __device__ void operator()(int rr, int, const f32x4_t& a, const f32x4_t& b) {
+    lane_out.row(lane_out.w.wrow0 + rr, extra, a, b);
+  }
+};
+template <int LPR, int BLOCK, bool RAGGED, class Emit>
 __device__ __forceinline__ void emit_act(const ActEpi& ep, const WaveRows& w, int lane, Emit&& emit) {
-  ActLane<RAGGED> out(ep, w, (lane % LPR) * 8);
-  emit([&](int rr, int, const f32x4_t& a, const f32x4_t& b) {
-    out.row(w.wrow0 + rr, out.fetch(w.wrow0 + rr), a, b);
-  });
-  if (ep.backward) out.template store_sums<LPR>(lane);
+  ActPasses<LPR, BLOCK, RAGGED> out(ep, w, lane);
+  emit(out);
+  if (ep.backward) out.lane_out.template store_sums<LPR>(lane);
 }
-template <int LPR, class Emit>
+template <int LPR, int BLOCK, class Emit>
 __device__ __forceinline__ void emit_rows(const ActEpi& ep, const WaveRows& w, int lane,
                                           Emit&& emit) {
-  if (ep.ragged) emit_act<LPR, true>(ep, w, lane, emit);
-  else emit_act<LPR, false>(ep, w, lane, emit);
+  if (ep.ragged) emit_act<LPR, BLOCK, true>(ep, w, lane, emit);
+  else emit_act<LPR, BLOCK, false>(ep, w, lane, emit);
 }
 
 }  // namespace gemm

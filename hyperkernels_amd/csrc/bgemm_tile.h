@@ -239,6 +239,7 @@ struct Bf16RowOut {
   uint16_t* Cb;
   int64_t ldc;
   int M, N, wrow0, wcol0;
+  __device__ void pass(int) const {}  // what comes before a pass of the wave
   __device__ void operator()(int rr, int cc, const f32x4_t& a, const f32x4_t& b) const {
     const int row = wrow0 + rr, col = wcol0 + cc;
     if (row >= M || col >= N) return;  // not RAGGED: N % 8 == 0, the 8 columns are all in or out
@@ -305,9 +306,9 @@ struct WaveRows {
   int batch, M, N, wrow0, wcol0, wave_row;
   unsigned char HK_LDS* area;
 };
-// Writes a wave's rows to C through the form the call needs: emit(out) hands every group of 8 columns to out;
-// LPR lanes hold a row.
-template <int LPR, class Emit>
+// Writes a wave's rows to C through the form the call needs: emit(out) hands every group of 8 columns to out,
+// behind out.pass(n) of the wave's n-th pass. LPR lanes hold a row, BLOCK rows are a block of passes.
+template <int LPR, int BLOCK, class Emit>
 __device__ __forceinline__ void emit_rows(const Epi& ep, const WaveRows& w, int, Emit&& emit) {
   uint16_t* Cb = w.C + static_cast<int64_t>(w.batch) * w.sC;
   if (ep.ragged) {
@@ -330,7 +331,7 @@ __device__ __forceinline__ NothingAhead rows_ahead(const Epi&, const WaveRows&, 
 template <int kWaveN, int kBlkM, int kStage>
 __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
                                            const Epi& ep, const WaveRows& w, const NothingAhead&) {
-  emit_rows<kWaveN / 8>(ep, w, lane, [&](auto&& out) {
+  emit_rows<kWaveN / 8, 32>(ep, w, lane, [&](auto&& out) {
     staged_rows<kWaveN, kBlkM>(acc, w.area, lane, out);
   });
 }

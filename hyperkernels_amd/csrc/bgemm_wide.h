@@ -508,6 +508,7 @@ __global__ __launch_bounds__(kThreads, 1) void bgemm_nt_w160(
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         const int rr = 6 * p + lane / 10, cc = (lane % 10) * 8;
+        out.pass(3 * i + p);
         if (lane < 60 && rr < 16) {
           const f32x4_t a = *reinterpret_cast<const f32x4_t HK_LDS*>(area + rr * kPitch + cc * 4);
           const f32x4_t b =
@@ -517,8 +518,8 @@ __global__ __launch_bounds__(kThreads, 1) void bgemm_nt_w160(
       }
     }
   };
-  emit_rows<kWaveN / 8>(ep, WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 4 * tm + wm, area}, lane,
-                        emit);
+  emit_rows<kWaveN / 8, 16>(ep, WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 4 * tm + wm, area},
+                            lane, emit);
 }
 
 // BNT 256 or 128: one column region (bgemm_tiled); BNT 0: both regions (bgemm_mixed), with
