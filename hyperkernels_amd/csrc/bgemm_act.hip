@@ -12,6 +12,8 @@
 // of bgemv.hip. Where K is split, a second kernel adds the fp32 partials in split order and applies the
 // epilogue. The bias gradient is summed in fp32 from the values before their rounding: over the rows of
 // a wave in registers, over the waves of the grid by a further kernel, in a fixed order.
+#include <algorithm>
+
 #include "bgemm_act_tiles.h"
 #include "bgemm_plan.h"
 #include "bgemm_wide.h"
@@ -21,6 +23,7 @@ namespace {
 using namespace hk::gemm;
 
 constexpr int kMaxGridZ = 65535;
+constexpr int kMaxSide = INT32_MAX - 0xFFFF;  // extents to which whole tiles can be added
 
 // One element's epilogue, for the kernels that hold one at a time: returns d in the backward pass.
 __device__ __forceinline__ float act_element(const ActEpi& ep, uint16_t* C, int64_t ldc, int64_t sC,
@@ -130,9 +133,9 @@ __global__ __launch_bounds__(256) void act_simple(int ta, int tb, int col_blocks
 }
 
 // ---- one row: a matrix that is read once, each of its elements for one product ---------------------
-// Both forms give a workgroup all of k for a few columns, so that it finishes them itself in the one launch
-// that a decoding step wants: 1280 -> 5120, bias and GELU, takes MEASURED. Loads are 16 bytes at any
-// alignment, eight in flight a lane.
+// A workgroup takes some columns of B over all of k and finishes them itself, in the one launch that a short
+// decoding step wants, or over a share of k, and a second kernel adds the shares (split_row says when).
+// Loads are 16 bytes at any alignment, eight in flight a lane.
 typedef uint32_t u32x4a2_t __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint4 load8_anywhere(const uint16_t* p) {
   const u32x4a2_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4a2_t*>(p));
@@ -159,34 +162,41 @@ struct RowOut {
   }
 };
 
-// B [K, N]: a workgroup takes 32 columns, a lane 8 of them in every 256th row of k; the 256 partial sums
-// of a column are added over the wave's lanes, then over the 16 waves through LDS. Neighbouring
-// workgroups share cache lines of B, so each XCD gets a run of them.
-constexpr int kNnWaves = 16, kNnCols = 32, kNnRows = kNnWaves * 16;
-__global__ __launch_bounds__(kNnWaves * HK_WAVE) void act_row_nn(int N, int K,
-                                                                 const uint16_t* __restrict__ B,
-                                                                 int64_t ldb, int64_t sB,
-                                                                 const uint16_t* __restrict__ x,
-                                                                 int64_t incx, int64_t sx,
-                                                                 RowOut out) {
-  __shared__ float lds[kNnWaves][kNnCols];
+// B [K, N]: a workgroup takes COLS columns and `share` rows of k, a lane 8 columns in every ROWS-th row; the
+// partial sums of a column are added over the wave's lanes, then over the waves through LDS. Neighbouring
+// workgroups of 32 columns share cache lines of B, so each XCD gets a run of them. With more than one
+// share (blockIdx.y) the sums go to part[batch][shares][N].
+template <int COLS, int WAVES>
+struct RowNn {
+  static constexpr int kLanes = COLS / 8, kRows = WAVES * (HK_WAVE / kLanes);
+};
+template <int COLS, int WAVES>
+__global__ __launch_bounds__(WAVES * HK_WAVE) void act_row_nn(int N, int K, int share,
+                                                              const uint16_t* __restrict__ B,
+                                                              int64_t ldb, int64_t sB,
+                                                              const uint16_t* __restrict__ x,
+                                                              int64_t incx, int64_t sx,
+                                                              float* __restrict__ part, RowOut out) {
+  constexpr int kLanes = RowNn<COLS, WAVES>::kLanes, kRows = RowNn<COLS, WAVES>::kRows;
+  __shared__ float lds[WAVES][COLS];
   const int b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned xcd = blockIdx.x & 7, total = gridDim.x;
   const int block = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
-  const int c = (lane & 3) * 8, col = block * kNnCols + c;
+  const int c = (lane % kLanes) * 8, col = block * COLS + c;
+  const unsigned k_begin = blockIdx.y * share, k_end = min(static_cast<unsigned>(K), k_begin + share);
   const int n = min(8, N - col);
   const uint16_t* xb = x + b * sx;
   const uint16_t* Bb = B + b * sB + col;
   float acc[8] = {};
-  for (int k0 = wave * 16 + (lane >> 2); k0 < K; k0 += kRowUnroll * kNnRows) {
+  for (unsigned k0 = k_begin + wave * (kRows / WAVES) + lane / kLanes; k0 < k_end; k0 += kRowUnroll * kRows) {
     uint4 m[kRowUnroll];
     float xv[kRowUnroll];
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u) {
-      const int k = k0 + u * kNnRows;
+      const unsigned k = k0 + u * kRows;
       m[u] = make_uint4(0, 0, 0, 0);
       xv[u] = 0.f;
-      if (k < K) {
+      if (k < k_end) {
         xv[u] = hk::bf16_to_f32(xb[k * incx]);
         if (n == 8) m[u] = load8_anywhere(Bb + k * ldb);
         else m[u] = load_row8<true>(Bb + k * ldb, n);
@@ -203,18 +213,19 @@ __global__ __launch_bounds__(kNnWaves * HK_WAVE) void act_row_nn(int N, int K,
 #pragma unroll
   for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int step = 4; step < HK_WAVE; step *= 2) acc[e] += __shfl_xor(acc[e], step);
-  if (lane < 4) {
+    for (int step = kLanes; step < HK_WAVE; step *= 2) acc[e] += __shfl_xor(acc[e], step);
+  if (lane < kLanes) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) lds[wave][c + e] = acc[e];
   }
   __syncthreads();
   const int i = threadIdx.x;
-  if (i < kNnCols && block * kNnCols + i < N) {
+  if (i < COLS && block * COLS + i < N) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kNnWaves; ++w) s += lds[w][i];
-    out(b, block * kNnCols + i, s);
+    for (int w = 0; w < WAVES; ++w) s += lds[w][i];
+    if (part) part[(static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * N + block * COLS + i] = s;
+    else out(b, block * COLS + i, s);
   }
 }
 
@@ -228,7 +239,7 @@ __global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* 
   const int col = blockIdx.x * kNtRows + (threadIdx.x >> 4);
   const uint16_t* xb = x + b * sx;
   const uint16_t* row = B + b * sB + static_cast<int64_t>(min(col, N - 1)) * ldb;
-  auto x8 = [&](int k) {
+  auto x8 = [&](unsigned k) {
     if (incx == 1) return load_row8<true>(xb + k, 8);
     uint32_t w[4];
 #pragma unroll
@@ -237,12 +248,12 @@ __global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* 
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
   float acc = 0.f;
-  const int kvec = K & ~7;
-  for (int k0 = 8 * j; k0 < kvec; k0 += kRowUnroll * kNtStep) {
+  const unsigned kvec = K & ~7;
+  for (unsigned k0 = 8 * j; k0 < kvec; k0 += kRowUnroll * kNtStep) {
     uint4 m[kRowUnroll], v[kRowUnroll];
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u) {
-      const int k = k0 + u * kNtStep;
+      const unsigned k = k0 + u * kNtStep;
       m[u] = v[u] = make_uint4(0, 0, 0, 0);
       if (k < kvec) {
         m[u] = load8_anywhere(row + k);
@@ -260,12 +271,12 @@ __global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* 
       acc += s;
     }
   }
-  if (kvec + j < K) acc += hk::bf16_to_f32(row[kvec + j]) * hk::bf16_to_f32(xb[(kvec + j) * incx]);
+  if (kvec + j < static_cast<unsigned>(K)) acc += hk::bf16_to_f32(row[kvec + j]) * hk::bf16_to_f32(xb[(kvec + j) * incx]);
   acc = hk::row16_sum(acc);
   if (j == 0 && col < N) out(b, col, acc);
 }
 
-// Where k is long and columns are few: the epilogue on the partials [batch][nsplit][N] of bgemv_partials.
+// The epilogue on the partials [batch][nsplit][N] of a product that is split over k.
 __global__ __launch_bounds__(256) void act_row_sum(const float* __restrict__ part, int nsplit, int N,
                                                    RowOut out) {
   const int col = blockIdx.x * 256 + threadIdx.x, b = blockIdx.z;
@@ -330,24 +341,47 @@ struct Call {
   bool accumulate;
 };
 
+// How a product of one row runs: over `splits` shares of k, and for B [K, N] on which workgroup.
+struct RowForm {
+  int splits;
+  int nn;  // 0: 32 columns, 16 waves; 1: 64 columns, 16 waves; 2: 64 columns, 8 waves
+};
+
 // How a call runs, and what it needs: the column sums of `sum_rows` blocks of rows and matrix, and the
 // partials of its k splits.
 struct Plan {
   enum Kind { kRow, kSimple, kTiles } kind;
   hk::GemmPlan gemm{0, 1, 0};
   hk::GemvPlan gemv{1, 0};
-  bool ragged = false, split_row = false;
+  RowForm row{1, 0};
+  bool ragged = false;
   int sum_rows = 0;
   size_t sum_bytes = 0, part_bytes = 0;
   size_t bytes() const { return sum_bytes + part_bytes; }
 };
 
-// Whether a one-row product is split over k.
-bool split_row(const Call& c) {
-  const int64_t groups = hk::ceil_div(c.N, c.tb ? kNtRows : kNnCols) * c.batch;
-  const int64_t rounds = hk::ceil_div(c.K, kRowUnroll * (c.tb ? kNtStep : kNnRows));
-  return groups < 512 && rounds > 4;
+// One CU reads some 20 bytes a nanosecond, so what counts is that all of them get equal parts of B, and what
+// a second launch costs, some 2 us of a graph and 2.6 of the host's time (bias and GELU, B from
+// memory, in a graph, us).
+// B [K, N]: enough columns for a workgroup of 64 on nearly every CU are left whole (K 2560, N 16000: 17.6
+// with 16 waves, 26.8 with 8, four shares 20.3; N 50304, K 1280: 34.3, 31.2 and 29.1). A short k, too:
+// 32 columns and one trip of the loop (N 5120, K 1280: 8.65 in one launch, 8.05 in two, 5.6 against
+// 7.4 for K 512 to 768). Everything else is cut to some 640 workgroups of 64 columns, two or three a CU, of
+// at least 160 rows (N 5120, K 2048: 11.8 whole, 9.3 cut; K 5120: 24.6 and 14.6; K 10240: 45.8 and 22.8).
+// B [N, K]: a workgroup takes 16 whole rows of B unless they are few and long (N 5120, K 5120: 13.6
+// whole, 11.9 cut; N 1280: 11.0 and 7.2; N 8192: 14.9 and 16.5; N 2560, K 2560: 7.6 and 6.9, and
+// 8.0 and 10.6 outside a graph, where the host is the slower one).
+RowForm row_form(const Call& c, const hk::GemvPlan& gemv) {
+  if (c.tb) {
+    const bool cut = hk::ceil_div(c.N, kNtRows) * c.batch < 512 && c.K > 2560;
+    return {cut ? gemv.nsplit : 1, 0};
+  }
+  const int64_t groups = hk::ceil_div(c.N, 64) * c.batch;
+  if (groups >= 224) return {1, groups >= 512 ? 2 : 1};
+  if (c.K <= 1536) return {1, 0};
+  return {static_cast<int>(std::min<int64_t>(640 / groups, c.K / 160)), 2};
 }
+int row_share(const Call& c, const RowForm& f) { return static_cast<int>(hk::ceil_div(c.K, f.splits)); }
 
 // may_split false: k splits only where the product needs them (one row).
 Plan make_plan(const Call& c, bool may_split) {
@@ -355,11 +389,10 @@ Plan make_plan(const Call& c, bool may_split) {
   const bool sums = c.ep.backward && c.dbias;
   if (c.M == 1 && c.K > 0) {
     p.kind = Plan::kRow;
-    p.split_row = split_row(c);
-    if (p.split_row) {
-      p.gemv = hk::bgemv_plan(c.tb, c.N, c.K, c.batch);
-      p.part_bytes = static_cast<size_t>(c.batch) * p.gemv.nsplit * c.N * sizeof(float);
-    }
+    if (c.tb) p.gemv = hk::bgemv_plan(c.tb, c.N, c.K, c.batch);
+    p.row = row_form(c, p.gemv);
+    if (p.row.splits > 1)
+      p.part_bytes = static_cast<size_t>(c.batch) * p.row.splits * c.N * sizeof(float);
     p.sum_rows = sums && c.batch > 1 && c.sD == 0 ? 1 : 0;
   } else {
     using hk::aligned16;
@@ -437,18 +470,26 @@ hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t str
     // C[0][n] = sum_k op(A)[0][k] op(B)[k][n]
     const int64_t incx = c.ta ? c.lda : 1;
     const RowOut out{ep, c.C, c.sC, ep.sums ? nullptr : c.dbias, c.sD, c.accumulate ? 1 : 0};
-    if (p.split_row) {
+    const bool split = p.row.splits > 1;
+    if (c.tb && split) {
       HK_RETURN_IF_ERROR(hk::bgemv_partials(c.tb, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, c.batch,
                                             p.gemv, part, stream));
-      hipLaunchKernelGGL(act_row_sum, dim3((c.N + 255) / 256, 1, c.batch), dim3(256), 0, stream, part,
-                         p.gemv.nsplit, c.N, out);
     } else if (c.tb) {
       hipLaunchKernelGGL(act_row_nt, dim3((c.N + kNtRows - 1) / kNtRows, 1, c.batch), dim3(256), 0,
                          stream, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, out);
     } else {
-      hipLaunchKernelGGL(act_row_nn, dim3((c.N + kNnCols - 1) / kNnCols, 1, c.batch),
-                         dim3(kNnWaves * HK_WAVE), 0, stream, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx,
-                         c.sA, out);
+      const int cols = p.row.nn == 0 ? 32 : 64, waves = p.row.nn == 2 ? 8 : 16;
+      const auto kernel = p.row.nn == 0   ? act_row_nn<32, 16>
+                          : p.row.nn == 1 ? act_row_nn<64, 16>
+                                          : act_row_nn<64, 8>;
+      hipLaunchKernelGGL(kernel, dim3((c.N + cols - 1) / cols, p.row.splits, c.batch),
+                         dim3(waves * HK_WAVE), 0, stream, c.N, c.K, row_share(c, p.row), c.B, c.ldb,
+                         c.sB, c.A, incx, c.sA, split ? part : nullptr, out);
+    }
+    if (split) {
+      HK_RETURN_IF_ERROR(hk::launch_status());
+      hipLaunchKernelGGL(act_row_sum, dim3((c.N + 255) / 256, 1, c.batch), dim3(256), 0, stream, part,
+                         p.row.splits, c.N, out);
     }
     HK_RETURN_IF_ERROR(hk::launch_status());
     return ep.sums ? column_sums(c, ep.sums, 1, stream) : hipSuccess;
@@ -497,12 +538,13 @@ float bf16_value(hk_bf16 h) {
 
 // The arguments that both entry points share.
 hipError_t check(int transA, int transB, int M, int N, int K, const void* A, int lda, const void* B,
-                 int ldb, int activation, const void* C, int ldc, int batchCount) {
+                 int ldb, int activation, const void* C, int ldc, long long strideC, int batchCount) {
   HK_CHECK_ARG(transA >= 0 && transA <= 2 && transB >= 0 && transB <= 2);
   HK_CHECK_ARG(M >= 0 && N >= 0 && K >= 0 && batchCount >= 0 && batchCount <= kMaxGridZ);
+  HK_CHECK_ARG(M <= kMaxSide && N <= kMaxSide && K <= kMaxSide);
   HK_CHECK_ARG(activation >= HK_ACT_NONE && activation <= HK_ACT_SILU);
   if (M == 0 || N == 0 || batchCount == 0) return hipSuccess;
-  HK_CHECK_ARG(C != nullptr && ldc >= N);
+  HK_CHECK_ARG(C != nullptr && ldc >= N && (batchCount == 1 || strideC != 0));
   HK_CHECK_ARG(K == 0 || (A != nullptr && B != nullptr));
   HK_CHECK_ARG(lda >= (transA ? M : K) && ldb >= (transB ? K : N));
   return hipSuccess;
@@ -533,9 +575,10 @@ extern "C" hipError_t hk_bgemm_act(int transA, int transB, int M, int N, int K, 
                                    long long strideZ, hk_bf16* C, int ldc, long long strideC,
                                    int batchCount, void* workspace, int64_t workspace_bytes,
                                    hipStream_t stream) {
-  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, batchCount));
+  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, strideC,
+                           batchCount));
   HK_CHECK_ARG(!residual || ldr >= N);
-  HK_CHECK_ARG(!preact || ldz >= N);
+  HK_CHECK_ARG(!preact || (ldz >= N && (batchCount <= 1 || strideZ != 0)));
   return run(forward_call(transA, transB, M, N, K, alpha, A, lda, strideA, B, ldb, strideB, bias,
                           strideBias, activation, residual, ldr, strideR, preact, ldz, strideZ, C, ldc,
                           strideC, batchCount),
@@ -550,10 +593,12 @@ extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N
                                             long long strideC, float* dbias, long long strideDbias,
                                             int accumulate, int batchCount, void* workspace,
                                             int64_t workspace_bytes, hipStream_t stream) {
-  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, batchCount));
+  HK_RETURN_IF_ERROR(check(transA, transB, M, N, K, A, lda, B, ldb, activation, C, ldc, strideC,
+                           batchCount));
   const bool empty = M == 0 || N == 0 || batchCount == 0;
   HK_CHECK_ARG(activation == HK_ACT_NONE || empty || (preact != nullptr && ldz >= N));
   HK_CHECK_ARG((reinterpret_cast<uintptr_t>(dbias) & 3u) == 0);
+  HK_CHECK_ARG(batchCount <= 1 || strideDbias == 0 || strideDbias >= N || strideDbias <= -N);
   ActEpi ep{};
   ep.alpha = bf16_value(alpha);
   ep.act = hk::make_activation(activation);
@@ -568,7 +613,7 @@ extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N
 extern "C" int64_t hk_bgemm_act_workspace(int transA, int transB, int M, int N, int K, int batchCount,
                                           int dbias) {
   if (transA < 0 || transA > 2 || transB < 0 || transB > 2 || M < 0 || N < 0 || K < 0 ||
-      batchCount < 0 || batchCount > kMaxGridZ)
+      batchCount < 0 || batchCount > kMaxGridZ || M > kMaxSide || N > kMaxSide || K > kMaxSide)
     return -1;
   if (M == 0 || N == 0 || batchCount == 0) return 0;
   // the most of what the rows' alignments make of the call

@@ -232,6 +232,22 @@ def test_batches(hk, batch, M, N, K, ta, tb, pad, own_bias):
     d.untouched()
 
 
+@pytest.mark.parametrize("N,K,tb,batch", [(300, 1536, 0, None), (300, 1537, 0, None), (64, 20481, 0, None),
+                                          (4001, 3001, 0, None), (14400, 1700, 0, None),
+                                          (33001, 300, 0, None), (1500, 2000, 0, 3), (77, 12000, 0, 5),
+                                          (1280, 2049, 1, None), (9001, 2100, 1, None), (700, 6000, 1, 3)])
+def test_every_form_of_one_row(hk, N, K, tb, batch):
+    """Whole columns on each workgroup, and k cut into shares."""
+    say("act row", N, K, tb, batch)
+    d = Data(1, N, K, 0, tb, 900 + N, batch=batch, bias_batch=batch is not None)
+    d.check_forward(hk, "gelu")
+    d.check_forward(hk, "silu", inplace=True, alpha=0.5)
+    d.check_backward(hk, "gelu", shared=batch is None)
+    if batch:
+        d.check_backward(hk, "gelu")
+    d.untouched()
+
+
 def test_leading_dimensions_past_the_tiles(hk):
     """Leading dimensions from 2^22 on run on the plain kernel."""
     M, N, K, ld = 70, 40, 24, (1 << 22) + 8

@@ -179,6 +179,23 @@ def test_bgemm_act_refuses(L, backward):
     assert L.hk_bgemm_act_workspace(0, 0, 4, 8, 16, 1, 1) > 0
 
 
+def test_bgemm_act_refuses_overlapping_outputs_and_huge_sides(L):
+    def fwd(M=4, N=8, K=16, sZ=32, sC=32, batch=2):
+        return L.hk_bgemm_act(0, 0, M, N, K, 0x3F80, 64, K, 0, 64, N, 0, 64, 0, 2, 64, N, 0, 64, N, sZ,
+                              64, N, sC, batch, NULL, 0, NULL)
+
+    def bwd(N=8, sC=32, sD=8, batch=2):
+        return L.hk_bgemm_act_backward(0, 0, 4, N, 16, 0x3F80, 64, 16, 0, 64, N, 0, 2, 64, N, 0, 64, N,
+                                       sC, 64, sD, 0, batch, NULL, 0, NULL)
+
+    huge = 2 ** 31 - 2 ** 16 + 1
+    for status in (fwd(sC=0), fwd(sZ=0), fwd(M=huge), fwd(N=huge), fwd(K=huge), bwd(sC=0), bwd(sD=7),
+                   bwd(sD=-7), bwd(N=huge)):
+        assert status == INVALID
+    for n in ((huge, 8, 16), (4, huge, 16), (4, 8, huge)):
+        assert L.hk_bgemm_act_workspace(0, 0, *n, 1, 0) == -1
+
+
 def test_bgemm_act_front_end_refuses():
     from hyperkernels_amd import kernels as hk
 
