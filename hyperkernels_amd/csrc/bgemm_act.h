@@ -28,10 +28,11 @@ struct ActEpi {
   static constexpr int kWideStage = 2;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
-// Eight bf16 of a row, n of them inside it. The whole vectors of rows that are not ragged are aligned.
+// Eight bf16 of a row, n of them inside it. The whole vectors of rows that are not ragged are aligned, and
+// read once: non-temporal (8192 x 1280 -> 5120: residual and GELU' 1 us less).
 template <bool RAGGED>
 __device__ __forceinline__ uint4 load_row8(const uint16_t* p, int n) {
-  if (!RAGGED) return *reinterpret_cast<const uint4*>(p);
+  if (!RAGGED) return ld_nt(reinterpret_cast<const uint4*>(p));
   uint32_t w[4];
   if (n == 8) {
     __builtin_memcpy(w, p, 16);
@@ -43,7 +44,8 @@ __device__ __forceinline__ uint4 load_row8(const uint16_t* p, int n) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Stores are non-temporal like those of the plain product: nothing here is read again by this one.
+// Stores are non-temporal like those of the plain product: nothing here is read again by this one (GELU with
+// its preact: 117.7 us; both outputs stored through the caches 131.4, preact alone 121.6).
 template <bool RAGGED>
 __device__ __forceinline__ void store_row8(uint16_t* p, int n, const float (&f)[8]) {
   const uint4 v = BF16::pack(f);
