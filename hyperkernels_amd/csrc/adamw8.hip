@@ -26,6 +26,8 @@
 // moments from then on: 8 bits cannot hold it in its element alone.
 #include <math.h>
 
+#include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "hk_device.h"
@@ -375,6 +377,22 @@ extern "C" hipError_t hk_adam8_plan_create(int num_tensors, float* const* params
   }
   HK_CHECK_ARG(blocks == 0 || (m_codes && v_codes && m_scales && v_scales));
   HK_CHECK_ARG(aligned4(m_codes) && aligned4(v_codes) && aligned4(m_scales) && aligned4(v_scales));
+  // what a step writes, each memory once: blocks of one step run in any order
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  auto writes = [&](const void* q, int64_t bytes) {
+    const auto a = reinterpret_cast<uintptr_t>(q);
+    if (q && bytes > 0) written.emplace_back(a, a + bytes);
+  };
+  for (int t = 0; t < num_tensors; ++t) {
+    writes(params[t], 4 * sizes[t]);
+    if (copies) writes(copies[t], 2 * sizes[t]);
+  }
+  writes(m_codes, kBlock * blocks);
+  writes(v_codes, kBlock * blocks);
+  writes(m_scales, 4 * blocks);
+  writes(v_scales, 4 * blocks);
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i) HK_CHECK_ARG(written[i - 1].second <= written[i].first);
   tensor_of.reserve(blocks);
   for (int t = 0; t < num_tensors; ++t)
     tensor_of.insert(tensor_of.end(), hk::ceil_div(sizes[t], kBlock), t);

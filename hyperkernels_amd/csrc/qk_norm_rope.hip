@@ -380,6 +380,23 @@ hipError_t check(const hk_qk_norm_rope_params* p, int type, bool backward) {
   return hipSuccess;
 }
 
+// Whether no two rows that a call writes are the same memory.
+bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
+  const int64_t stride[2][3] = {
+      {backward ? p->dq_strideB : p->qo_strideB, backward ? p->dq_strideM : p->qo_strideM,
+       backward ? p->dq_strideH : p->qo_strideH},
+      {backward ? p->dk_strideB : p->ko_strideB, backward ? p->dk_strideM : p->ko_strideM,
+       backward ? p->dk_strideH : p->ko_strideH}};
+  const int heads[2] = {p->q_heads, p->k_heads};
+  for (int i = 0; i < 2; ++i)
+    if (heads[i] > 0 && ((p->B > 1 && stride[i][0] == 0) || (p->T > 1 && stride[i][1] == 0) ||
+                         (heads[i] > 1 && stride[i][2] == 0)))
+      return false;
+  if (!backward || !p->dq_weight || !p->dk_weight || heads[0] == 0 || heads[1] == 0) return true;
+  const auto a = reinterpret_cast<uintptr_t>(p->dq_weight), b = reinterpret_cast<uintptr_t>(p->dk_weight);
+  return (a > b ? a - b : b - a) >= p->head_dim * sizeof(float);
+}
+
 // Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it. 8 (16-byte
 // vectors of 16-bit elements) where a row is only read and written in 16 bits; 4 where outputs are fp32
 // (forward, 8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: 17.5 -> 16.2 us; bf16 -> bf16 the
@@ -474,6 +491,7 @@ extern "C" hipError_t hk_qk_norm_rope_forward(const hk_qk_norm_rope_params* p, i
   const int v = unit_pairs(type, p->head_dim, p->rotary_dim, !p->f32_io);
   const Args g = make_args(p, v, false);
   if (g.side[0].rows + g.side[1].rows == 0) return hipSuccess;
+  HK_CHECK_ARG(rows_apart(p, false));
   return by_type(g, type, p->f32_io, v, false, stream);
 }
 
@@ -488,6 +506,7 @@ extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, 
                                                void* workspace, int64_t workspace_bytes,
                                                hipStream_t stream) {
   HK_RETURN_IF_ERROR(check(p, type, true));
+  HK_CHECK_ARG(rows_apart(p, true));
   const int v = unit_pairs(type, p->head_dim, p->rotary_dim, false);
   Args g = make_args(p, v, true);
   Weights w{{nullptr, nullptr},

@@ -241,7 +241,8 @@ HK_API int64_t hk_adam_plan_num_chunks(const hk_adam_plan* plan);
  *   tensor t has ceil(sizes[t] / HK_ADAM8_BLOCK) blocks behind those of the tensors before it.
  *   m_codes and v_codes hold HK_ADAM8_BLOCK bytes a block, m_scales and v_scales one float a block
  *   (hk_adam8_plan_num_blocks gives the count); codes behind a tensor's end are written as 0.
- *   Parameters and gradients may have any alignment of their element type, the codes need 4 bytes.
+ *   Parameters and gradients may have any alignment of their element type, the codes need 4 bytes. No two
+ *   of the arrays that a step writes (parameters, copies, states) may overlap.
  * hk_adam8_plan_step: on the device that was current at creation; steps of plans that share memory
  *   have to be ordered. It takes no workspace and can be captured into a graph.
  * A gradient that is not finite, or a moment past fp32, leaves the block's scales NaN, and with them
@@ -648,10 +649,11 @@ HK_API hipError_t hk_attn_backward_set(const hk_attn_bwd_params* params, int hea
  * hk_qk_norm_rope_backward reads q, k and the gradients dq_out, dk_out (strides qo_*, ko_*, like the
  *   outputs') and writes dq, dk, which may be q, k or, with f32_io unset, dq_out and dk_out themselves.
  *   dq_weight and dk_weight (fp32, NULL: not wanted) are written, or added to where accumulate is
- *   set, summed over tokens and heads in a fixed order. The partial sums take
+ *   set, summed over tokens and heads in a fixed order; they may not overlap. The partial sums take
  *   hk_qk_norm_rope_workspace bytes (0 where neither is wanted, -1 for invalid arguments): at
  *   `workspace`, or in the stream's workspace where that is NULL. A call that needs some and is captured
  *   into a graph brings its own, as for hk_bgemm_act.
+ * No two rows of one output may be the same memory (no stride of 0 over more than one).
  * ---------------------------------------------------------------------------------------- */
 typedef struct hk_qk_norm_rope_params {
   const void* q;

@@ -28,8 +28,8 @@ def test_adam8_plan_refuses(L):
     plan = ctypes.c_void_p(1)
     sizes = (ctypes.c_int64 * 1)(300)
 
-    def create(n=1, params=_arr(64), grads=_arr(64), kind=0, copies=NULL, sz=sizes,
-               states=(64, 64, 64, 64)):
+    def create(n=1, params=_arr(1 << 20), grads=_arr(1 << 21), kind=0, copies=NULL, sz=sizes,
+               states=(1 << 12, 1 << 13, 1 << 14, 1 << 15)):
         return L.hk_adam8_plan_create(n, params, grads, kind, copies, sz, *states,
                                       ctypes.byref(plan))
 
@@ -37,9 +37,17 @@ def test_adam8_plan_refuses(L):
                 dict(sz=NULL), dict(params=_arr(0)), dict(grads=_arr(0)), dict(params=_arr(66)),
                 dict(grads=_arr(66)), dict(grads=_arr(65), kind=1), dict(copies=_arr(65)),
                 dict(sz=(ctypes.c_int64 * 1)(-1)), dict(sz=(ctypes.c_int64 * 1)(1 << 60)),
-                dict(states=(0, 64, 64, 64)), dict(states=(64, 0, 64, 64)),
-                dict(states=(64, 64, 0, 64)), dict(states=(64, 64, 64, 0)),
-                dict(states=(66, 64, 64, 64)), dict(states=(64, 66, 64, 64))):
+                dict(states=(0, 1 << 13, 1 << 14, 1 << 15)), dict(states=(1 << 12, 0, 1 << 14, 1 << 15)),
+                dict(states=(1 << 12, 1 << 13, 0, 1 << 15)), dict(states=(1 << 12, 1 << 13, 1 << 14, 0)),
+                dict(states=(4098, 1 << 13, 1 << 14, 1 << 15)),
+                dict(states=(1 << 12, 8194, 1 << 14, 1 << 15)),
+                # memory that two parts of a step would write
+                dict(n=2, params=_arr(1 << 20, (1 << 20) + 1196), grads=_arr(1 << 21, 1 << 22),
+                     sz=(ctypes.c_int64 * 2)(300, 300)),
+                dict(copies=_arr((1 << 20) + 1198)), dict(copies=_arr((1 << 20) - 598)),
+                dict(states=(1 << 12, (1 << 12) + 508, 1 << 14, 1 << 15)),
+                dict(states=(1 << 12, 1 << 13, 1 << 14, (1 << 14) + 4)),
+                dict(states=(1 << 20, 1 << 13, 1 << 14, 1 << 15))):
         assert create(**bad) == INVALID, bad
         assert plan.value is None  # no plan is handed out
     assert L.hk_adam8_plan_create(0, NULL, NULL, 0, NULL, NULL, *([NULL] * 4), NULL) == INVALID
@@ -86,7 +94,8 @@ def _qk(**kw):
 
     base = dict(q=64, k=64, cos=64, sin=64, q_out=64, k_out=64, dq_out=64, dk_out=64, dq=64, dk=64,
                 B=1, T=4, q_heads=2, k_heads=1, head_dim=64, rotary_dim=64, eps=1e-6, table_rows=4,
-                table_stride=32)
+                table_stride=32, qo_strideM=128, qo_strideH=64, ko_strideM=64, dq_strideM=128,
+                dq_strideH=64, dk_strideM=64)
     return QkNormRopeParams(**{**base, **kw})
 
 
@@ -122,6 +131,20 @@ def test_qk_norm_rope_refuses(L, backward):
     else:
         assert L.hk_qk_norm_rope_forward(NULL, 0, NULL) == INVALID
         assert L.hk_qk_norm_rope_forward(ctypes.byref(_qk(B=0, q=0, k=0)), 0, NULL) == 0
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_qk_refuses_rows_written_twice(L, backward):
+    q, k = ("dq", "dk") if backward else ("qo", "ko")
+    bad = [{f"{q}_strideM": 0}, {f"{q}_strideH": 0}, {f"{k}_strideM": 0}, dict(B=2),
+           {"B": 2, f"{q}_strideB": 512}, {"k_heads": 2}]
+    if backward:
+        bad += [dict(dq_weight=4096, dk_weight=4096), dict(dq_weight=4096, dk_weight=4096 + 252)]
+    for kw in bad:
+        p = ctypes.byref(_qk(**kw))
+        status = L.hk_qk_norm_rope_backward(p, 0, NULL, 0, NULL) if backward else (
+            L.hk_qk_norm_rope_forward(p, 0, NULL))
+        assert status == INVALID, kw
 
 
 def test_qk_front_end_refuses_host_tensors():
