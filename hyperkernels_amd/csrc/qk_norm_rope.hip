@@ -389,8 +389,9 @@ bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
        backward ? p->dk_strideH : p->ko_strideH}};
   const int heads[2] = {p->q_heads, p->k_heads};
   for (int i = 0; i < 2; ++i)
-    if (heads[i] > 0 && ((p->B > 1 && stride[i][0] == 0) || (p->T > 1 && stride[i][1] == 0) ||
-                         (heads[i] > 1 && stride[i][2] == 0)))
+    if (heads[i] > 0 && p->B > 0 && p->T > 0 &&
+        ((p->B > 1 && stride[i][0] == 0) || (p->T > 1 && stride[i][1] == 0) ||
+         (heads[i] > 1 && stride[i][2] == 0)))
       return false;
   if (!backward || !p->dq_weight || !p->dk_weight || heads[0] == 0 || heads[1] == 0) return true;
   const auto a = reinterpret_cast<uintptr_t>(p->dq_weight), b = reinterpret_cast<uintptr_t>(p->dk_weight);
