@@ -15,7 +15,9 @@
 // lanes is the sum of squares (and of g w n), a register butterfly over the row's lanes. Vectors are
 // 16 bytes where head_dim and rotary_dim allow (multiples of 2 V elements), at any element alignment.
 // Rows go to lane groups token by token, heads innermost, so that the groups of a wave read the same
-// table rows. Elements behind rotary_dim are units of two neighbouring vectors with an angle of zero.
+// table rows. Elements behind rotary_dim are units of two neighbouring vectors with an angle of zero. Stores
+// are non-temporal (8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: forward 16.3 -> 14.7 us,
+// backward with dw 23.9 -> 22.5), loads are not (18.8 and 25.7: heads share their cache lines).
 //
 // The gradients of the two weight vectors are summed in registers over the rows of a lane group, over
 // a workgroup through LDS, and over the workgroups by a second kernel, all in a fixed order.
@@ -34,9 +36,18 @@ template <typename S, int V>
 __device__ __forceinline__ void load_vec(const S* p, S (&f)[V]) {
   __builtin_memcpy(f, p, V * sizeof(S));
 }
-template <typename S, int V>
+// ONCE: device memory that this call does not read again.
+template <bool ONCE, typename S, int V>
 __device__ __forceinline__ void store_vec(S* p, const S (&f)[V]) {
-  __builtin_memcpy(p, f, V * sizeof(S));
+  if constexpr (ONCE && V > 1) {
+    typedef S vec_t __attribute__((ext_vector_type(V), aligned(sizeof(S))));
+    vec_t v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = f[e];
+    __builtin_nontemporal_store(v, reinterpret_cast<vec_t*>(p));
+  } else {
+    __builtin_memcpy(p, f, V * sizeof(S));
+  }
 }
 template <class F, int V>
 __device__ __forceinline__ void load_f32(const typename F::storage* p, float (&f)[V]) {
@@ -45,12 +56,12 @@ __device__ __forceinline__ void load_f32(const typename F::storage* p, float (&f
 #pragma unroll
   for (int e = 0; e < V; ++e) f[e] = F::load(s, e);
 }
-template <class F, int V>
+template <class F, int V, bool ONCE>
 __device__ __forceinline__ void store_f32(typename F::storage* p, const float (&f)[V]) {
   typename F::storage s[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) F::store(s, e, f[e]);
-  store_vec(p, s);
+  store_vec<ONCE>(p, s);
 }
 
 struct Shape {
@@ -98,7 +109,7 @@ __device__ __forceinline__ void load_unit(const typename F::storage* row, const 
     for (int e = 0; e < V; ++e) a[e] = t[2 * e], b[e] = t[2 * e + 1];
   }
 }
-template <class F, int V>
+template <class F, int V, bool ONCE = true>
 __device__ __forceinline__ void store_unit(typename F::storage* row, const Unit<V>& u, int d,
                                            const float (&a)[V], const float (&b)[V]) {
   if (V > 1 && u.pairs) {
@@ -107,11 +118,11 @@ __device__ __forceinline__ void store_unit(typename F::storage* row, const Unit<
     for (int e = 0; e < V; ++e) t[2 * e] = a[e], t[2 * e + 1] = b[e];
 #pragma unroll
     for (int e = 0; e < V; ++e) lo[e] = t[e], hi[e] = t[V + e];
-    store_f32<F, V>(row + u.a, lo);
-    store_f32<F, V>(row + u.b, hi);
+    store_f32<F, V, ONCE>(row + u.a, lo);
+    store_f32<F, V, ONCE>(row + u.b, hi);
   } else {
-    store_f32<F, V>(row + u.a, a);
-    if (V > 1 || u.b < d) store_f32<F, V>(row + u.b, b);
+    store_f32<F, V, ONCE>(row + u.a, a);
+    if (V > 1 || u.b < d) store_f32<F, V, ONCE>(row + u.b, b);
   }
 }
 
@@ -305,7 +316,7 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
       }
     }
     if (u.on && (threadIdx.x & 63) < g.s.lanes) {
-      store_unit<hk::F32, V>(lds[threadIdx.x / HK_WAVE], u, g.s.d, da[k], db[k]);
+      store_unit<hk::F32, V, false>(lds[threadIdx.x / HK_WAVE], u, g.s.d, da[k], db[k]);
     }
   }
   __syncthreads();
@@ -400,10 +411,10 @@ bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
 
 // Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it. 8 (16-byte
 // vectors of 16-bit elements) where a row is only read and written in 16 bits; 4 where outputs are fp32
-// (forward, 8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: 17.5 -> 16.2 us; bf16 -> bf16 the
-// other way: 11.7 and 12.6), and in the backward pass, which holds weights and their gradients beside
-// the row (110 registers a lane with 8: 25.4 us with dw, with 4 and three workgroups a CU 23.9;
-// 16 + 4 heads of 128, fp16: 46.3 and 36.8).
+// (stores through the caches, forward, 8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: 17.5 and
+// 16.2 us; bf16 -> bf16 the other way: 11.7 and 12.6), and in the backward pass, which holds weights and
+// their gradients beside the row (110 registers a lane with 8: 25.4 us with dw, with 4 and three
+// workgroups a CU 23.9; 16 + 4 heads of 128, fp16: 46.3 and 36.8).
 int unit_pairs(int type, int d, int rot, bool wide) {
   for (int v = type != HK_TYPE_F32 && wide ? 8 : 4; v > 1; v -= 4)
     if (d % (2 * v) == 0 && rot % (2 * v) == 0) return v;
