@@ -342,8 +342,15 @@ __global__ __launch_bounds__(1024) void qk_weight_sums(Weights a, int d, int acc
   if (!a.dw[which]) return;
   float v = 0.f;
   if (col < d) {
-#pragma unroll 4
-    for (int i = grp; i < a.n[which]; i += 64) v += a.part[which][static_cast<int64_t>(i) * d + col];
+    const float* p = a.part[which] + col;
+    const int n = a.n[which];
+    for (int i0 = grp; i0 < n; i0 += 512) {  // eight loads in flight
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] = i0 + 64 * u < n ? p[static_cast<int64_t>(i0 + 64 * u) * d] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += f[u];
+    }
   }
   v += __shfl_xor(v, 16);
   v += __shfl_xor(v, 32);
