@@ -13,7 +13,9 @@
 // token and come from the caches). A row is held by 2^k lanes, each with a unit of V pairs: the two
 // vectors of V elements that its rotation combines sit in one lane, so the only exchange between
 // lanes is the sum of squares (and of g w n), a register butterfly over the row's lanes. Vectors are
-// 16 bytes where head_dim and rotary_dim allow (multiples of 2 V elements), at any element alignment.
+// 16 bytes of 16-bit elements where both parts of a row, the rotated one and the rest, are whole units of
+// them; else 4 elements, at any element alignment, and a part that is not whole units ends with one that
+// overlaps the unit before it.
 // Rows go to lane groups token by token, heads innermost, so that the groups of a wave read the same
 // table rows. Elements behind rotary_dim are units of two neighbouring vectors with an angle of zero. Stores
 // are non-temporal (8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: forward 16.3 -> 14.7 us,
@@ -65,34 +67,51 @@ __device__ __forceinline__ void store_f32(typename F::storage* p, const float (&
 }
 
 struct Shape {
-  int d, rot, half, units, lanes;  // half: rot / 2; lanes: of a row, a power of two
+  int d, rot, half;           // half: rot / 2
+  int rotated, units, lanes;  // rotated: units that are; lanes: of a row, a power of two
   bool interleaved;
 };
 
 // Where the two vectors of unit u lie in a row, and whether the second exists (a head of odd size,
-// V == 1).
-template <int V>
+// V == 1). OVERLAP: the last unit of the rotated part and that of the rest are moved back to whole
+// vectors; their first elements are the unit's before them too, and only its (old).
+template <int V, bool OVERLAP>
 struct Unit {
-  int a, b, angle;  // angle: first pair of the table row, -1: not rotated
-  bool on, pairs;   // pairs: neighbouring elements are rotated together
+  int a, b, angle;   // angle: first pair of the table row, -1: not rotated
+  int old_a, old_b;  // elements of the two vectors that are another unit's
+  bool on, pairs;    // pairs: neighbouring elements are rotated together
   __device__ Unit(const Shape& s, int u) {
-    const int rotated = s.half / V;
     on = u < s.units;
-    pairs = u < rotated && s.interleaved;
-    angle = u < rotated ? u * V : -1;
-    if (u < rotated) {
-      a = s.interleaved ? 2 * u * V : u * V;
-      b = s.interleaved ? a + V : s.half + u * V;
+    pairs = u < s.rotated && s.interleaved;
+    angle = -1;
+    old_a = old_b = 0;
+    if (u < s.rotated) {
+      angle = u * V;
+      if (OVERLAP && angle + V > s.half) {
+        old_a = old_b = angle + V - s.half;
+        angle = s.half - V;
+      }
+      a = s.interleaved ? 2 * angle : angle;
+      b = s.interleaved ? a + V : s.half + angle;
     } else {
-      a = 2 * u * V;  // rot is 2 V rotated
+      a = s.rot + 2 * (u - s.rotated) * V;
+      if (OVERLAP && a + 2 * V > s.d) {
+        const int old = a + 2 * V - s.d;
+        old_a = min(V, old);
+        old_b = old - old_a;
+        a = s.d - 2 * V;
+      }
       b = a + V;
     }
   }
+  // v where element e of the first (second) vector is the unit's own, else 0
+  __device__ float own_a(int e, float v) const { return OVERLAP && e < old_a ? 0.f : v; }
+  __device__ float own_b(int e, float v) const { return OVERLAP && e < old_b ? 0.f : v; }
 };
 
 // x as the pairs (a[j], b[j]) of a unit.
-template <class F, int V>
-__device__ __forceinline__ void load_unit(const typename F::storage* row, const Unit<V>& u, int d,
+template <class F, int V, bool O>
+__device__ __forceinline__ void load_unit(const typename F::storage* row, const Unit<V, O>& u, int d,
                                           float (&a)[V], float (&b)[V]) {
   load_f32<F, V>(row + u.a, a);
   if (V > 1 || u.b < d) {
@@ -109,8 +128,8 @@ __device__ __forceinline__ void load_unit(const typename F::storage* row, const 
     for (int e = 0; e < V; ++e) a[e] = t[2 * e], b[e] = t[2 * e + 1];
   }
 }
-template <class F, int V, bool ONCE = true>
-__device__ __forceinline__ void store_unit(typename F::storage* row, const Unit<V>& u, int d,
+template <class F, int V, bool ONCE = true, bool O>
+__device__ __forceinline__ void store_unit(typename F::storage* row, const Unit<V, O>& u, int d,
                                            const float (&a)[V], const float (&b)[V]) {
   if (V > 1 && u.pairs) {
     float t[2 * V], lo[V], hi[V];
@@ -170,8 +189,8 @@ __device__ __forceinline__ int64_t position(const Args& g, int b, int t) {
   return g.positions ? g.positions[b * g.pos_stride + t] : t;
 }
 // The cosines and sines of a unit at a position; NaN where the table has no such one.
-template <int V>
-__device__ __forceinline__ void angles(const Args& g, const Unit<V>& u, int64_t pos, float (&c)[V],
+template <int V, bool O>
+__device__ __forceinline__ void angles(const Args& g, const Unit<V, O>& u, int64_t pos, float (&c)[V],
                                        float (&s)[V]) {
   if (pos < 0 || pos >= g.table_rows) {
 #pragma unroll
@@ -185,8 +204,8 @@ __device__ __forceinline__ void angles(const Args& g, const Unit<V>& u, int64_t 
   }
 }
 
-template <class F, int V>
-__device__ __forceinline__ void weights(const void* w, const Unit<V>& u, int d, float (&a)[V],
+template <class F, int V, bool O>
+__device__ __forceinline__ void weights(const void* w, const Unit<V, O>& u, int d, float (&a)[V],
                                         float (&b)[V]) {
   if (w && u.on) {
     load_unit<F, V>(static_cast<const typename F::storage*>(w), u, d, a, b);
@@ -196,8 +215,8 @@ __device__ __forceinline__ void weights(const void* w, const Unit<V>& u, int d, 
   }
 }
 
-// U: units a lane holds (more than one only where a row needs more than 64 of them, V == 1).
-template <class FI, class FO, int V, int U>
+// U: units a lane holds (more than one only where a row needs more than 64 of them, V == 1). O: OVERLAP.
+template <class FI, class FO, int V, int U, bool O>
 __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
   const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
   const Side& sd = g.side[which];
@@ -213,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
   float xa[U][V], xb[U][V], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const Unit<V> u(g.s, j + k * HK_WAVE);
+    const Unit<V, O> u(g.s, j + k * HK_WAVE);
     if (!u.on) {
 #pragma unroll
       for (int e = 0; e < V; ++e) xa[k][e] = xb[k][e] = 0.f;
@@ -221,16 +240,17 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
     }
     load_unit<FI, V>(x, u, g.s.d, xa[k], xb[k]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum += xa[k][e] * xa[k][e] + xb[k][e] * xb[k][e];
+    for (int e = 0; e < V; ++e)
+      sum += u.own_a(e, xa[k][e] * xa[k][e]) + u.own_b(e, xb[k][e] * xb[k][e]);
   }
   const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const Unit<V> u(g.s, j + k * HK_WAVE);
+    const Unit<V, O> u(g.s, j + k * HK_WAVE);
     if (!u.on) continue;
     float wa[V], wb[V], c[V], s[V], ya[V], yb[V];
     weights<FI, V>(sd.w, u, g.s.d, wa, wb);
-    angles<V>(g, u, position(g, b, t), c, s);
+    angles(g, u, position(g, b, t), c, s);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float a = xa[k][e] * r * wa[e], bb = xb[k][e] * r * wb[e];
@@ -241,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
   }
 }
 
-template <class FI, class FO, int V, int U>
+template <class FI, class FO, int V, int U, bool O>
 __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
   __shared__ float lds[kBackWaves][kMaxDim];
   const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
@@ -252,7 +272,7 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
   float wa[U][V], wb[U][V], da[U][V], db[U][V];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    weights<FI, V>(sd.w, Unit<V>(g.s, j + k * HK_WAVE), g.s.d, wa[k], wb[k]);
+    weights<FI, V>(sd.w, Unit<V, O>(g.s, j + k * HK_WAVE), g.s.d, wa[k], wb[k]);
 #pragma unroll
     for (int e = 0; e < V; ++e) da[k][e] = db[k][e] = 0.f;
   }
@@ -267,7 +287,7 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
     float xa[U][V], xb[U][V], ga[U][V], gb[U][V], sum = 0.f, dot = 0.f;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const Unit<V> u(g.s, j + k * HK_WAVE);
+      const Unit<V, O> u(g.s, j + k * HK_WAVE);
       if (!u.on) {
 #pragma unroll
         for (int e = 0; e < V; ++e) xa[k][e] = xb[k][e] = ga[k][e] = gb[k][e] = 0.f;
@@ -276,13 +296,13 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
       float c[V], s[V], ya[V], yb[V];
       load_unit<FI, V>(x, u, g.s.d, xa[k], xb[k]);
       load_unit<FO, V>(dy, u, g.s.d, ya, yb);
-      angles<V>(g, u, pos, c, s);
+      angles(g, u, pos, c, s);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         ga[k][e] = ya[e] * c[e] + yb[e] * s[e];
         gb[k][e] = yb[e] * c[e] - ya[e] * s[e];
-        sum += xa[k][e] * xa[k][e] + xb[k][e] * xb[k][e];
-        dot += ga[k][e] * wa[k][e] * xa[k][e] + gb[k][e] * wb[k][e] * xb[k][e];
+        sum += u.own_a(e, xa[k][e] * xa[k][e]) + u.own_b(e, xb[k][e] * xb[k][e]);
+        dot += u.own_a(e, ga[k][e] * wa[k][e] * xa[k][e]) + u.own_b(e, gb[k][e] * wb[k][e] * xb[k][e]);
       }
     }
     const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
@@ -290,7 +310,7 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
     const float m = lanes_sum(dot, g.s.lanes) * g.inv_d * r;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const Unit<V> u(g.s, j + k * HK_WAVE);
+      const Unit<V, O> u(g.s, j + k * HK_WAVE);
       float oa[V], ob[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -307,7 +327,7 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
   // the row groups of a wave, then the waves of the workgroup, in a fixed order
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const Unit<V> u(g.s, j + k * HK_WAVE);
+    const Unit<V, O> u(g.s, j + k * HK_WAVE);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       for (int step = g.s.lanes; step < HK_WAVE; step *= 2) {
@@ -422,16 +442,24 @@ bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
 // 16.2 us; bf16 -> bf16 the other way: 11.7 and 12.6), and in the backward pass, which holds weights and
 // their gradients beside the row (110 registers a lane with 8: 25.4 us with dw, with 4 and three
 // workgroups a CU 23.9; 16 + 4 heads of 128, fp16: 46.3 and 36.8).
+// Parts that are no whole vectors of 4 keep them where they are long enough for the last unit to be moved
+// back (8 x 1024 tokens, forward: 12 + 12 bf16 heads of 64 with 20 rotated 31.7 us one by one, 21.3 so; 8 + 8 of
+// 90, all rotated, 41.2 and 16.5; fp16 of 96 with 50 rotated 43.6 and 17.4; backward 36.5, 49.1 and 51.5
+// against 27.0, 21.3 and 22.9; an element-wise tail on each unit instead: 44.4, 31.5, 34.3 forward).
+int units_of(int d, int rot, int v) { return (rot / 2 + v - 1) / v + (d - rot + 2 * v - 1) / (2 * v); }
+bool whole_units(int d, int rot, int v) { return d % (2 * v) == 0 && rot % (2 * v) == 0; }
 int unit_pairs(int type, int d, int rot, bool wide) {
-  for (int v = type != HK_TYPE_F32 && wide ? 8 : 4; v > 1; v -= 4)
-    if (d % (2 * v) == 0 && rot % (2 * v) == 0) return v;
+  if (type != HK_TYPE_F32 && wide && whole_units(d, rot, 8)) return 8;
+  for (int v = 4; v > 1; v /= 2)
+    if ((rot == 0 || rot >= 2 * v) && (d == rot || d - rot >= 2 * v) && units_of(d, rot, v) <= HK_WAVE)
+      return v;
   return 1;
 }
 
 Args make_args(const hk_qk_norm_rope_params* p, int v, bool backward) {
   Args g{};
-  g.s = Shape{p->head_dim, p->rotary_dim, p->rotary_dim / 2, (p->head_dim + 2 * v - 1) / (2 * v), 1,
-              p->interleaved};
+  const int d = p->head_dim, rot = p->rotary_dim;
+  g.s = Shape{d, rot, rot / 2, (rot / 2 + v - 1) / v, units_of(d, rot, v), 1, p->interleaved};
   while (g.s.lanes < g.s.units && g.s.lanes < HK_WAVE) g.s.lanes *= 2;
   g.cos = p->cos, g.sin = p->sin;
   g.table_stride = p->table_stride;
@@ -469,26 +497,29 @@ Args make_args(const hk_qk_norm_rope_params* p, int v, bool backward) {
   return g;
 }
 
-template <class FI, class FO, int V, int U>
+template <class FI, class FO, int V, int U, bool O>
 hipError_t launch(const Args& g, bool backward, hipStream_t stream) {
   const unsigned blocks = g.side[0].blocks + g.side[1].blocks;
   if constexpr (V == 8) {
     if (backward) return hipErrorInvalidValue;  // unit_pairs
-    hipLaunchKernelGGL((qk_forward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+    hipLaunchKernelGGL((qk_forward<FI, FO, V, U, O>), dim3(blocks), dim3(kThreads), 0, stream, g);
   } else if (backward) {
-    hipLaunchKernelGGL((qk_backward<FI, FO, V, U>), dim3(blocks), dim3(kBackThreads), 0, stream, g);
+    hipLaunchKernelGGL((qk_backward<FI, FO, V, U, O>), dim3(blocks), dim3(kBackThreads), 0, stream, g);
   } else {
-    hipLaunchKernelGGL((qk_forward<FI, FO, V, U>), dim3(blocks), dim3(kThreads), 0, stream, g);
+    hipLaunchKernelGGL((qk_forward<FI, FO, V, U, O>), dim3(blocks), dim3(kThreads), 0, stream, g);
   }
   return hk::launch_status();
 }
 template <class FI, class FO>
 hipError_t by_unit(const Args& g, int v, bool backward, hipStream_t stream) {
   if constexpr (FI::kPerVec == 8 && FO::kPerVec == 8)
-    if (v == 8) return launch<FI, FO, 8, 1>(g, backward, stream);
-  if (v == 4) return launch<FI, FO, 4, 1>(g, backward, stream);
-  return g.s.units > HK_WAVE ? launch<FI, FO, 1, 2>(g, backward, stream)
-                             : launch<FI, FO, 1, 1>(g, backward, stream);
+    if (v == 8) return launch<FI, FO, 8, 1, false>(g, backward, stream);
+  if (v == 4)
+    return whole_units(g.s.d, g.s.rot, 4) ? launch<FI, FO, 4, 1, false>(g, backward, stream)
+                                          : launch<FI, FO, 4, 1, true>(g, backward, stream);
+  if (v == 2) return launch<FI, FO, 2, 1, true>(g, backward, stream);
+  return g.s.units > HK_WAVE ? launch<FI, FO, 1, 2, false>(g, backward, stream)
+                             : launch<FI, FO, 1, 1, false>(g, backward, stream);
 }
 hipError_t by_type(const Args& g, int type, bool f32_io, int v, bool backward, hipStream_t stream) {
   using namespace hk;

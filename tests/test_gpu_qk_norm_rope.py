@@ -208,6 +208,44 @@ def test_in_place_and_one_side_alone(hk, side, dt):
     assert torch.equal(x2, y)
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16-f32"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rot", [(64, 20), (64, 6), (70, 64), (66, 50), (90, 90), (17, 8), (22, 14),
+                                   (256, 6), (250, 8), (10, 0), (9, 4), (127, 118)])
+def test_parts_that_are_no_whole_vectors(hk, d, rot, inter, io):
+    """Rotated parts and rests of every remainder; into a wider buffer, and in place."""
+    say("qk parts", d, rot, inter, io)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(d * 300 + rot)
+    dt, out = TYPES[io.split("-")[0]], TYPES[io.split("-")[-1]]
+    B, H, T = 2, 3, 21
+    q, dy = _heads(gen, B, H, T, d, dt, "wide"), _heads(gen, B, H, T, d, out, "token")
+    w = torch.randn(d, generator=gen, device=DEV).to(dt)
+    cos, sin = _table(T, rot, pad=1) if rot else (None, None)
+    kw = dict(cos=cos, sin=sin, q_weight=w, interleaved=inter)
+    buf = torch.full((B, T, H + 2, d + 7), 9.0, device=DEV, dtype=out)
+    y = buf[:, :, 1:H + 1, 3:d + 3].transpose(1, 2)
+    hk.qk_norm_rope_forward(q, None, q_out=y, **kw)
+    gw = torch.zeros(d, device=DEV)
+    dq, _ = hk.qk_norm_rope_backward(dy, None, q, None, grad_q_weight=gw, **kw)
+    ry, ty, rx, tx, rw, tw = _reference(q, w, cos, sin, None, rot, inter, 1e-6, dy)
+    _close(y, ry, ty, "y")
+    _close(dq, rx, tx, "dq")
+    _close(gw, rw, tw, "dw")
+    if dt == out:
+        q2 = q.clone()
+        hk.qk_norm_rope_forward(q2, None, q_out=q2, **kw)
+        assert torch.equal(q2, y)
+        q2.copy_(q)
+        hk.qk_norm_rope_backward(dy, None, q2, None, dq=q2, **kw)
+        assert torch.equal(q2, dq)
+        d2 = dy.clone()
+        hk.qk_norm_rope_backward(d2, None, q, None, dq=d2, **kw)
+        assert torch.equal(d2, dq)
+    y.fill_(9.0)
+    assert bool((buf == 9.0).all())
+
+
 def test_positions_outside_the_table_give_nan_for_their_tokens(hk):
     gen = torch.Generator(device=DEV)
     gen.manual_seed(7)
