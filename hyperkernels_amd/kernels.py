@@ -63,16 +63,6 @@ def _device(fn: str, t: torch.Tensor) -> int:
     return d
 
 
-def _here(fn: str, *ts: torch.Tensor | None) -> None:
-    """Device tensors of the current device."""
-    cur = None
-    for t in ts:
-        if t is not None and t.get_device() != cur:
-            if cur is not None:
-                raise ValueError(f"{fn}: tensors of the current device only")
-            cur = _device(fn, t)
-
-
 # ----------------------------------------------------------------------------------------------
 # GELU: gelu_forward_sm89_kernel<T> (kernels/gelu/gelu_forward_sm89_kernel.cu:35-37),
 #       gelu_backward_sm89_kernel<T> (kernels/gelu/gelu_backward_sm89_kernel.cu:44-47)
@@ -591,7 +581,7 @@ def bgemm_act(a, b, bias=None, activation: str = "none", residual=None, preact=N
               trans_a: bool = False, trans_b: bool = False, alpha: float = 1.0):
     """act(alpha op(a) op(b) + bias) + residual for bf16 matrices [rows, cols] or batches of them; what
     goes into the activation ("none", "relu", "gelu" or "silu") is stored in `preact` where that is
-    passed. bias is [N], or [batch, N]; residual may be `out` itself."""
+    passed. bias is [N], or [batch, N]; residual may be `out` itself; alpha is rounded to bf16."""
     fn = "bgemm_act"
     batch, M, N, K, act, dev = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
@@ -615,7 +605,7 @@ def bgemm_act_backward(a, b, preact=None, activation: str = "none", dbias=None, 
     """d = alpha op(a) op(b) * act'(preact) in bf16: the gradient of a layer's pre-activation, from the
     gradient behind the next layer and that layer's weights. dbias (fp32 [N], or [batch, N]; None: not
     wanted) is added to, or written where accumulate is False: the sums of d over rows (and, [N],
-    batches) before it is rounded."""
+    batches) before it is rounded. alpha is rounded to bf16."""
     fn = "bgemm_act_backward"
     batch, M, N, K, act, dev = _product(fn, a, b, trans_a, trans_b, activation)
     if out is None:
