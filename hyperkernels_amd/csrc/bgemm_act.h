@@ -25,6 +25,7 @@ struct ActEpi {
   float* sums;
   int sum_rows, pitch;
   static constexpr int kWideAhead = 4;  // passes whose inputs are in flight there
+  static constexpr bool kShareRows = true;
   static constexpr int kWideStage = 2;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
@@ -260,6 +261,71 @@ __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN /
                                            const ActAhead<kWaveN, DEPTH>& ahead) {
   if (ep.ragged) act_rows<kWaveN, kBlkM, true, kStage, DEPTH>(acc, lane, ep, w, ahead);
   else act_rows<kWaveN, kBlkM, false, kStage, DEPTH>(acc, lane, ep, w, ahead);
+}
+
+// Tiles of several k groups T::KG: every wave stages its sums, and those of a group, wave `wave` of T::kGroupWaves,
+// then take T::kShareM of the rows that its tile part has in all groups, add the sums in group order and work
+// on them. With one group at work and the others at their end it took longer (2048 x 2048 -> 2048 with bias,
+// GELU and residual 25.9 us, now 24.4; 1024 x 4096 -> 1024 18.2 and 16.6; 512 x 768 -> 768 7.2 and 6.9 in a
+// graph). w: the rows of the share; the inputs of all of its passes are ahead.
+template <class T, bool RAGGED>
+__device__ __forceinline__ void act_shared(const unsigned char HK_LDS* lds, int group, int wave, int lane,
+                                           const ActEpi& ep, const WaveRows& w,
+                                           const ActAhead<T::kWaveN, T::kSharePasses>& ahead) {
+  constexpr int LPR = T::kWaveN / 8, RPP = 64 / LPR, NP = T::kSharePasses;
+  constexpr int kAtOnce = NP > 1 ? 2 : 1;
+  ActLane<RAGGED> out(ep, w, (lane % LPR) * 8, ahead.bias);
+  uint4 next[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) next[p] = ahead.first[p];
+#pragma unroll 1
+  for (int s = 0; s < T::kShareM; s += kAtOnce * RPP) {
+    f32x4_t a[kAtOnce], b[kAtOnce];
+    uint4 extra[kAtOnce];
+    const int row = s + lane / LPR;
+#pragma unroll
+    for (int p = 0; p < kAtOnce; ++p) {
+      const unsigned char HK_LDS* at = lds + wave * T::kRowsArea +
+                                       (group * T::kShareM + row + p * RPP) * T::kRowsPitch +
+                                       (lane % LPR) * 32;
+      a[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at);
+      b[p] = *reinterpret_cast<const f32x4_t HK_LDS*>(at + 16);
+#pragma unroll
+      for (int grp = 1; grp < T::KG; ++grp) {
+        at += T::kGroupWaves * T::kRowsArea;
+        a[p] += *reinterpret_cast<const f32x4_t HK_LDS*>(at);
+        b[p] += *reinterpret_cast<const f32x4_t HK_LDS*>(at + 16);
+      }
+      extra[p] = next[p];
+    }
+#pragma unroll
+    for (int p = 0; p + kAtOnce < NP; ++p) next[p] = next[p + kAtOnce];
+#pragma unroll
+    for (int p = 0; p < kAtOnce; ++p) out.row(w.wrow0 + row + p * RPP, extra[p], a[p], b[p]);
+  }
+  if (ep.backward) out.template store_sums<LPR>(lane);
+}
+template <class T>
+__device__ __forceinline__ void store_shared(const f32x16_t (&acc)[T::kBlkM][T::kBlkN],
+                                             unsigned char HK_LDS* lds, int group, int wave, int lane,
+                                             const ActEpi& ep, const WaveRows& w,
+                                             const ActAhead<T::kWaveN, T::kSharePasses>& ahead) {
+  const int r = lane & 31, h = lane >> 5;
+  unsigned char HK_LDS* area = lds + (group * T::kGroupWaves + wave) * T::kRowsArea;
+#pragma unroll
+  for (int i = 0; i < T::kBlkM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::kBlkN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4_t HK_LDS*>(area + (32 * i + r) * T::kRowsPitch +
+                                          (32 * j + 8 * q + 4 * h) * 4) =
+            f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                    acc[i][j][4 * q + 3]};
+  __syncthreads();
+  if (group >= T::kShares) return;
+  if (ep.ragged) act_shared<T, true>(lds, group, wave, lane, ep, w, ahead);
+  else act_shared<T, false>(lds, group, wave, lane, ep, w, ahead);
 }
 
 // The same where the caller hands out the rows itself: the inputs of four passes are in flight.

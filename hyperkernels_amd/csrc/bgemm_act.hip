@@ -412,7 +412,7 @@ Plan make_plan(const Call& c, bool may_split) {
       if (p.gemm.used > 1) {
         p.part_bytes = hk::bgemm_partial_bytes(p.gemm.used, c.M, c.N, c.batch);
       } else if (p.gemm.flex) {
-        block = hk::bgemm_flex_tile_rows(p.gemm.flex) / 2;  // two rows of waves
+        block = act_flex_wave_rows(p.gemm.flex);
       } else {
         block = w160_plan(c.ta, c.tb, c.M, c.N, c.K, c.batch, 1) ? w160::kWaveM
                                                                  : row_tile(c.ta, c.M, c.N, c.batch, 1) / 2;

@@ -15,8 +15,17 @@ const ActFlexRun kShapes[] = {
     HK_FLEX_SHAPES(HK_SHAPE)
 #undef HK_SHAPE
 };
+const int kWaveRows[] = {
+#define HK_SHAPE(bm, bn, ragged, alone, shared, per_cu, fixed, tile) tile::kShareM,
+    HK_FLEX_SHAPES(HK_SHAPE)
+#undef HK_SHAPE
+};
 constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
 }  // namespace
+
+int act_flex_wave_rows(int tile) {
+  return tile >= 1 && tile <= kNumShapes ? kWaveRows[tile - 1] : 0;
+}
 
 hipError_t act_flex_run(int tile, bool ta, bool tb, const FlexArgs<ActEpi>& g, int batch,
                         hipStream_t stream) {

@@ -11,6 +11,8 @@ namespace gemm {
 // The small and any-alignment tiles: tile shape `tile` of bgemm_flex_plan.
 hipError_t act_flex_run(int tile, bool ta, bool tb, const FlexArgs<ActEpi>& g, int batch,
                         hipStream_t stream);
+// The rows of C that a wave of such a tile writes: as many share a row of column sums.
+int act_flex_wave_rows(int tile);
 typedef hipError_t (*ActFlexRun)(bool, bool, const FlexArgs<ActEpi>&, int, hipStream_t);
 ActFlexRun act_ragged(int tile);  // the shapes for rows of any alignment, NULL for another
 

@@ -45,9 +45,17 @@ struct Tile {
   static constexpr int kCopies = kCopiesA + kCopiesB;
   static constexpr int kStaging = 32 * (kWaveN * 4 + 16);  // epilogue area of one wave
   static constexpr int kSums = BMT * BNT * 4;              // one k group's accumulators
-  static constexpr size_t lds(bool ragged) {
+  // Where the groups share out the rows: kShares of them take part, with kShareM rows of a wave's in
+  // kSharePasses passes. Every wave of every group stages all of its rows.
+  static constexpr int kPassRows = 64 / (kWaveN / 8);
+  static constexpr int kShares = KG == 1 ? 1 : KG < kWaveM / kPassRows ? KG : kWaveM / kPassRows;
+  static constexpr int kShareM = kWaveM / kShares, kSharePasses = kShareM / kPassRows;
+  static constexpr int kRowsPitch = kWaveN * 4 + 16, kRowsArea = kWaveM * kRowsPitch;
+  static constexpr size_t lds(bool ragged, bool share_rows) {
     const size_t ring = static_cast<size_t>(KG) * (ragged ? 2 : S) * kStage;
-    const size_t end = static_cast<size_t>(kGroupWaves) * kStaging + (KG - 1) * kSums;
+    const size_t end = share_rows && KG > 1
+                           ? static_cast<size_t>(KG) * kGroupWaves * kRowsArea
+                           : static_cast<size_t>(kGroupWaves) * kStaging + (KG - 1) * kSums;
     return ring > end ? ring : end;
   }
   static_assert(kCopiesA * kGroupWaves * 1024 == kStageA, "whole copies per wave");
@@ -199,10 +207,15 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
   // The wave's rows of C, staged for the stores at the start of the LDS. What the epilogue reads ahead is
   // issued before the copies, so that the waits below, which count those, cover it.
   const int wrow0 = m0 + wm * T::kWaveM, wcol0 = n0 + wn * T::kWaveN;
-  const WaveRows rows{g.C, g.ldc, g.sC, batch, M, N, wrow0, wcol0, tm * T::WM + wm,
+  constexpr bool kShared = E::kShareRows && T::KG > 1;
+  // the rows that the wave writes: with shared rows those of its group's share, none where that has none
+  const WaveRows rows{g.C, g.ldc, g.sC, batch, M, N,
+                      !kShared ? wrow0 : group < T::kShares ? wrow0 + group * T::kShareM : M, wcol0,
+                      kShared ? (tm * T::WM + wm) * T::kShares + group : tm * T::WM + wm,
                       lds + wave * T::kStaging};
   // up to four passes of the wave over its rows
-  const auto ahead = rows_ahead<T::kWaveN, T::kWaveM * T::kWaveN >= 2048 ? 4 : 2>(g.ep, rows, lane);
+  constexpr int kAheadPasses = kShared ? T::kSharePasses : T::kWaveM * T::kWaveN >= 2048 ? 4 : 2;
+  const auto ahead = rows_ahead<T::kWaveN, kAheadPasses>(g.ep, rows, lane);
 
   if constexpr (RAGGED) {
     if (ktiles > 0) {
@@ -299,7 +312,10 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
 
   // Epilogue. The ring is free after this barrier; the k groups' sums are added in group order.
   __syncthreads();
-  if constexpr (T::KG > 1) {
+  if constexpr (kShared) {
+    store_shared<T>(acc, lds, group, wave, lane, g.ep, rows, ahead);
+    return;
+  } else if constexpr (T::KG > 1) {
     if (merge_groups<T>(acc, lds, group, wave, lane)) return;
   }
   if (g.fo.C) {
@@ -318,7 +334,7 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads >= 512 ? 1 : 2) void bgemm
 
 template <class T, bool AK, bool BKM, bool RAGGED, class E>
 hipError_t flex_launch(const FlexArgs<E>& g, int batch, hipStream_t stream) {
-  constexpr size_t kLds = T::lds(RAGGED);
+  constexpr size_t kLds = T::lds(RAGGED, E::kShareRows);
   static_assert(kLds <= 160 * 1024, "fits gfx950's 160 KiB of LDS");
   static std::once_flag once;
   static hipError_t attr_status = hipSuccess;

@@ -162,6 +162,7 @@ struct Epi {
   int64_t brow, bcol;
   bool ragged;  // rows of C that are no whole number of aligned 16-byte vectors
   static constexpr int kWideAhead = 0;
+  static constexpr bool kShareRows = false;  // whether the k groups share out the rows of C behind the k loop
   static constexpr int kWideStage = 1;  // block rows that a wave of the 256-wide tiles stages at a time
 };
 
