@@ -329,19 +329,21 @@ __device__ __forceinline__ void store_shared(const f32x16_t (&acc)[T::kBlkM][T::
 }
 
 // The same where the caller hands out the rows itself: the inputs of four passes are in flight.
-template <int LPR, int BLOCK, bool RAGGED>
+template <int LPR, int BLOCK, int PASSES, bool RAGGED>
 struct ActPasses {
   static constexpr int RPP = HK_WAVE / LPR, kPerBlock = (BLOCK + RPP - 1) / RPP;
   ActLane<RAGGED> lane_out;
-  int row0;  // of the lane in a pass
+  int row0;  // of the lane in a pass, in a block
   uint4 extra, next[4];
   __device__ ActPasses(const ActEpi& ep, const WaveRows& w, int lane)
-      : lane_out(ep, w, (lane % LPR) * 8), row0(w.wrow0 + lane / LPR) {
+      : lane_out(ep, w, (lane % LPR) * 8), row0(lane / LPR) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) next[n] = fetch(n);
   }
   __device__ uint4 fetch(int n) const {
-    return lane_out.fetch(row0 + BLOCK * (n / kPerBlock) + RPP * (n % kPerBlock));
+    const int row = row0 + RPP * (n % kPerBlock);  // not those behind the block's and the wave's last ones
+    return n < PASSES && row < BLOCK ? lane_out.fetch(lane_out.w.wrow0 + BLOCK * (n / kPerBlock) + row)
+                                     : make_uint4(0, 0, 0, 0);
   }
   __device__ void pass(int n) {
     extra = next[n % 4];
@@ -351,17 +353,17 @@ struct ActPasses {
     lane_out.row(lane_out.w.wrow0 + rr, extra, a, b);
   }
 };
-template <int LPR, int BLOCK, bool RAGGED, class Emit>
+template <int LPR, int BLOCK, int PASSES, bool RAGGED, class Emit>
 __device__ __forceinline__ void emit_act(const ActEpi& ep, const WaveRows& w, int lane, Emit&& emit) {
-  ActPasses<LPR, BLOCK, RAGGED> out(ep, w, lane);
+  ActPasses<LPR, BLOCK, PASSES, RAGGED> out(ep, w, lane);
   emit(out);
   if (ep.backward) out.lane_out.template store_sums<LPR>(lane);
 }
-template <int LPR, int BLOCK, class Emit>
+template <int LPR, int BLOCK, int PASSES, class Emit>
 __device__ __forceinline__ void emit_rows(const ActEpi& ep, const WaveRows& w, int lane,
                                           Emit&& emit) {
-  if (ep.ragged) emit_act<LPR, BLOCK, true>(ep, w, lane, emit);
-  else emit_act<LPR, BLOCK, false>(ep, w, lane, emit);
+  if (ep.ragged) emit_act<LPR, BLOCK, PASSES, true>(ep, w, lane, emit);
+  else emit_act<LPR, BLOCK, PASSES, false>(ep, w, lane, emit);
 }
 
 }  // namespace gemm

@@ -308,8 +308,8 @@ struct WaveRows {
   unsigned char HK_LDS* area;
 };
 // Writes a wave's rows to C through the form the call needs: emit(out) hands every group of 8 columns to out,
-// behind out.pass(n) of the wave's n-th pass. LPR lanes hold a row, BLOCK rows are a block of passes.
-template <int LPR, int BLOCK, class Emit>
+// behind out.pass(n) of the wave's n-th pass of PASSES. LPR lanes hold a row, BLOCK rows are a block of passes.
+template <int LPR, int BLOCK, int PASSES, class Emit>
 __device__ __forceinline__ void emit_rows(const Epi& ep, const WaveRows& w, int, Emit&& emit) {
   uint16_t* Cb = w.C + static_cast<int64_t>(w.batch) * w.sC;
   if (ep.ragged) {
@@ -332,7 +332,7 @@ __device__ __forceinline__ NothingAhead rows_ahead(const Epi&, const WaveRows&, 
 template <int kWaveN, int kBlkM, int kStage>
 __device__ __forceinline__ void store_bf16(const f32x16_t (&acc)[kBlkM][kWaveN / 32], int lane,
                                            const Epi& ep, const WaveRows& w, const NothingAhead&) {
-  emit_rows<kWaveN / 8, 32>(ep, w, lane, [&](auto&& out) {
+  emit_rows<kWaveN / 8, 32, kBlkM * kWaveN / 16>(ep, w, lane, [&](auto&& out) {
     staged_rows<kWaveN, kBlkM>(acc, w.area, lane, out);
   });
 }

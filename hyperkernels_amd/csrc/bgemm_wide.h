@@ -518,8 +518,8 @@ __global__ __launch_bounds__(kThreads, 1) void bgemm_nt_w160(
       }
     }
   };
-  emit_rows<kWaveN / 8, 16>(ep, WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 4 * tm + wm, area},
-                            lane, emit);
+  emit_rows<kWaveN / 8, 16, 3 * kBlkM>(
+      ep, WaveRows{C, ldc, sC, batch, M, N, wrow0, wcol0, 4 * tm + wm, area}, lane, emit);
 }
 
 // BNT 256 or 128: one column region (bgemm_tiled); BNT 0: both regions (bgemm_mixed), with
