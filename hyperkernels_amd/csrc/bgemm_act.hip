@@ -551,6 +551,7 @@ hipError_t check(int transA, int transB, int M, int N, int K, const void* A, int
   if (M == 0 || N == 0 || batchCount == 0) return hipSuccess;
   HK_CHECK_ARG(C != nullptr && ldc >= N && (batchCount == 1 || strideC != 0));
   HK_CHECK_ARG(K == 0 || (A != nullptr && B != nullptr));
+  HK_CHECK_ARG(K == 0 || (C != A && C != B));  // operands are read while C is written
   HK_CHECK_ARG(lda >= (transA ? M : K) && ldb >= (transB ? K : N));
   return hipSuccess;
 }
@@ -584,6 +585,7 @@ extern "C" hipError_t hk_bgemm_act(int transA, int transB, int M, int N, int K, 
                            batchCount));
   HK_CHECK_ARG(!residual || ldr >= N);
   HK_CHECK_ARG(!preact || (ldz >= N && (batchCount <= 1 || strideZ != 0)));
+  HK_CHECK_ARG(!preact || (preact != C && preact != residual && (K == 0 || (preact != A && preact != B))));
   return run(forward_call(transA, transB, M, N, K, alpha, A, lda, strideA, B, ldb, strideB, bias,
                           strideBias, activation, residual, ldr, strideR, preact, ldz, strideZ, C, ldc,
                           strideC, batchCount),

@@ -418,7 +418,7 @@ hipError_t check(const hk_qk_norm_rope_params* p, int type, bool backward) {
   return hipSuccess;
 }
 
-// Whether no two rows that a call writes are the same memory.
+// Whether no two rows that a call writes are the same memory, nor one that the other side still reads.
 bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
   const int64_t stride[2][3] = {
       {backward ? p->dq_strideB : p->qo_strideB, backward ? p->dq_strideM : p->qo_strideM,
@@ -431,6 +431,12 @@ bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
         ((p->B > 1 && stride[i][0] == 0) || (p->T > 1 && stride[i][1] == 0) ||
          (heads[i] > 1 && stride[i][2] == 0)))
       return false;
+  if (heads[0] > 0 && heads[1] > 0 && p->B > 0 && p->T > 0) {
+    const void* oq = backward ? p->dq : p->q_out;
+    const void* ok = backward ? p->dk : p->k_out;
+    if (oq == ok || oq == p->k || ok == p->q) return false;
+    if (backward && (oq == p->dk_out || ok == p->dq_out)) return false;
+  }
   if (!backward || !p->dq_weight || !p->dk_weight || heads[0] == 0 || heads[1] == 0) return true;
   const auto a = reinterpret_cast<uintptr_t>(p->dq_weight), b = reinterpret_cast<uintptr_t>(p->dk_weight);
   return (a > b ? a - b : b - a) >= p->head_dim * sizeof(float);

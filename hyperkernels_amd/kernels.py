@@ -603,7 +603,7 @@ def bgemm_act_backward(a, b, preact=None, activation: str = "none", dbias=None, 
                        trans_a: bool = False, trans_b: bool = False, alpha: float = 1.0,
                        accumulate: bool = True):
     """d = alpha op(a) op(b) * act'(preact) in bf16: the gradient of a layer's pre-activation, from the
-    gradient behind the next layer and that layer's weights. dbias (fp32 [N], or [batch, N]; None: not
+    gradient behind the next layer and that layer's weights; out may be `preact` itself. dbias (fp32 [N], or [batch, N]; None: not
     wanted) is added to, or written where accumulate is False: the sums of d over rows (and, [N],
     batches) before it is rounded. alpha is rounded to bf16."""
     fn = "bgemm_act_backward"

@@ -462,7 +462,8 @@ HK_API hipError_t hk_bgemm_core_bias(int layout, int splitK, int M, int N, int K
  * M, N and K at most 2^31 - 2^16; batches of C and of a preact that is written lie apart); bf16 everywhere but dbias (fp32). Everything is fp32 until C and preact are rounded, once each: the
  * activation takes z and dbias takes d before that. bias (N elements a batch, strideBias apart, 0: one
  * for all), residual and preact (M x N like C, leading dimensions ldr and ldz) may be NULL; preact is
- * needed by hk_bgemm_act_backward unless the activation is HK_ACT_NONE. residual may be C itself.
+ * needed by hk_bgemm_act_backward unless the activation is HK_ACT_NONE. residual may be C itself, as may
+ * the preact of hk_bgemm_act_backward; A and B may not overlap C, nor anything a preact that is written.
  * dbias may be NULL; strideDbias 0 sums over the batches too, else it is N at least. GELU is the tanh form, as in
  * hk_gelu_forward. Sums are in a fixed order.
  * The k splits of some products and the bias gradient take device memory, hk_bgemm_act_workspace bytes
@@ -653,7 +654,8 @@ HK_API hipError_t hk_attn_backward_set(const hk_attn_bwd_params* params, int hea
  *   hk_qk_norm_rope_workspace bytes (0 where neither is wanted, -1 for invalid arguments): at
  *   `workspace`, or in the stream's workspace where that is NULL. A call that needs some and is captured
  *   into a graph brings its own, as for hk_bgemm_act.
- * No two rows of one output may be the same memory (no stride of 0 over more than one).
+ * No two rows that are written may be the same memory (no stride of 0 over more than one), nor may one
+ * side's outputs lie on the other's inputs.
  * ---------------------------------------------------------------------------------------- */
 typedef struct hk_qk_norm_rope_params {
   const void* q;

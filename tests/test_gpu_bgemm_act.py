@@ -248,6 +248,25 @@ def test_every_form_of_one_row(hk, N, K, tb, batch):
     d.untouched()
 
 
+@pytest.mark.parametrize("M,N,K,tb", [(512, 768, 2304, 1), (512, 2304, 768, 0), (300, 304, 4096, 0),
+                                      (301, 303, 1001, 1), (8192, 1280, 448, 1), (8192, 5120, 128, 0),
+                                      (1, 1000, 1024, 0), (1, 1000, 5000, 0), (1, 1000, 5000, 1)])
+def test_in_place(hk, M, N, K, tb):
+    """The residual and the backward pass's preact as the output, on every kind of plan."""
+    say("act in place", M, N, K, tb)
+    d = Data(M, N, K, 0, tb, 77 + M)
+    kw = dict(trans_b=bool(tb), activation="gelu")
+    want = hk.bgemm_act(d.a, d.b, bias=d.bias, residual=d.r, preact=d.z, **kw)
+    got = d.r.clone()
+    hk.bgemm_act(d.a, d.b, bias=d.bias, residual=got, out=got, **kw)
+    assert torch.equal(got, want)
+    db = torch.zeros(2, N, device=DEV)
+    want = hk.bgemm_act_backward(d.a, d.b, preact=d.z, dbias=db[0], **kw)
+    got = d.z.clone()
+    hk.bgemm_act_backward(d.a, d.b, preact=got, out=got, dbias=db[1], **kw)
+    assert torch.equal(got, want) and torch.equal(db[0], db[1])
+
+
 def test_leading_dimensions_past_the_tiles(hk):
     """Leading dimensions from 2^22 on run on the plain kernel."""
     M, N, K, ld = 70, 40, 24, (1 << 22) + 8

@@ -92,7 +92,7 @@ def test_adam8_front_end_refuses_host_tensors():
 def _qk(**kw):
     from hyperkernels_amd.kernels import QkNormRopeParams
 
-    base = dict(q=64, k=64, cos=64, sin=64, q_out=64, k_out=64, dq_out=64, dk_out=64, dq=64, dk=64,
+    base = dict(q=64, k=128, cos=192, sin=256, q_out=320, k_out=384, dq_out=448, dk_out=512, dq=576, dk=640,
                 B=1, T=4, q_heads=2, k_heads=1, head_dim=64, rotary_dim=64, eps=1e-6, table_rows=4,
                 table_stride=32, qo_strideM=128, qo_strideH=64, ko_strideM=64, dq_strideM=128,
                 dq_strideH=64, dk_strideM=64)
@@ -139,7 +139,10 @@ def test_qk_refuses_rows_written_twice(L, backward):
     bad = [{f"{q}_strideM": 0}, {f"{q}_strideH": 0}, {f"{k}_strideM": 0}, dict(B=2),
            {"B": 2, f"{q}_strideB": 512}, {"k_heads": 2}]
     if backward:
-        bad += [dict(dq_weight=4096, dk_weight=4096), dict(dq_weight=4096, dk_weight=4096 + 252)]
+        bad += [dict(dq_weight=4096, dk_weight=4096), dict(dq_weight=4096, dk_weight=4096 + 252),
+                dict(dq=640), dict(dq=128), dict(dk=64), dict(dq=512), dict(dk=448)]
+    else:
+        bad += [dict(q_out=384), dict(q_out=128), dict(k_out=64)]
     for kw in bad:
         p = ctypes.byref(_qk(**kw))
         status = L.hk_qk_norm_rope_backward(p, 0, NULL, 0, NULL) if backward else (
@@ -178,8 +181,8 @@ def test_qk_parameter_block_matches_the_header(tmp_path):
 
 @pytest.mark.parametrize("backward", [False, True])
 def test_bgemm_act_refuses(L, backward):
-    def go(ta=0, tb=0, M=4, N=8, K=16, A=64, lda=16, B=64, ldb=8, act=2, res=64, ldr=8, Z=64, ldz=8,
-           C=64, ldc=8, dbias=64, batch=1, ws=0, ws_bytes=0):
+    def go(ta=0, tb=0, M=4, N=8, K=16, A=64, lda=16, B=1024, ldb=8, act=2, res=2048, ldr=8, Z=4096,
+           ldz=8, C=8192, ldc=8, dbias=64, batch=1, ws=0, ws_bytes=0):
         if backward:
             return L.hk_bgemm_act_backward(ta, tb, M, N, K, 0x3F80, A, lda, 0, B, ldb, 0, act, Z, ldz,
                                            0, C, ldc, 0, dbias, 0, 0, batch, ws, ws_bytes, NULL)
@@ -189,7 +192,9 @@ def test_bgemm_act_refuses(L, backward):
     bad = [dict(ta=3), dict(ta=-1), dict(tb=3), dict(M=-1), dict(N=-1), dict(K=-1), dict(A=0),
            dict(B=0), dict(C=0), dict(lda=15), dict(ldb=7), dict(ldc=7), dict(act=4), dict(act=-1),
            dict(batch=-1), dict(batch=65536), dict(ldz=7), dict(ta=1, lda=3), dict(tb=1, ldb=15)]
-    bad += [dict(Z=0), dict(dbias=66)] if backward else [dict(ldr=7)]
+    bad += [dict(C=64), dict(C=1024)]
+    bad += [dict(Z=0), dict(dbias=66)] if backward else [dict(ldr=7), dict(Z=64), dict(Z=1024),
+                                                         dict(Z=2048), dict(Z=8192)]
     for kw in bad:
         assert go(**kw) == INVALID, kw
     if not backward:
@@ -204,11 +209,11 @@ def test_bgemm_act_refuses(L, backward):
 
 def test_bgemm_act_refuses_overlapping_outputs_and_huge_sides(L):
     def fwd(M=4, N=8, K=16, sZ=32, sC=32, batch=2):
-        return L.hk_bgemm_act(0, 0, M, N, K, 0x3F80, 64, K, 0, 64, N, 0, 64, 0, 2, 64, N, 0, 64, N, sZ,
-                              64, N, sC, batch, NULL, 0, NULL)
+        return L.hk_bgemm_act(0, 0, M, N, K, 0x3F80, 64, K, 0, 1024, N, 0, 64, 0, 2, 2048, N, 0, 4096, N, sZ,
+                              8192, N, sC, batch, NULL, 0, NULL)
 
     def bwd(N=8, sC=32, sD=8, batch=2):
-        return L.hk_bgemm_act_backward(0, 0, 4, N, 16, 0x3F80, 64, 16, 0, 64, N, 0, 2, 64, N, 0, 64, N,
+        return L.hk_bgemm_act_backward(0, 0, 4, N, 16, 0x3F80, 64, 16, 0, 1024, N, 0, 2, 4096, N, 0, 8192, N,
                                        sC, 64, sD, 0, batch, NULL, 0, NULL)
 
     huge = 2 ** 31 - 2 ** 16 + 1
