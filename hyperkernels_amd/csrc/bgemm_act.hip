@@ -25,24 +25,39 @@ using namespace hk::gemm;
 constexpr int kMaxGridZ = 65535;
 constexpr int kMaxSide = INT32_MAX - 0xFFFF;  // extents to which whole tiles can be added
 
-// One element's epilogue, for the kernels that hold one at a time: returns d in the backward pass.
+// One element's epilogue, for the kernels that hold one at a time, and what it reads beside the sum: bias and
+// residual, or z in the backward pass.
+struct ActElement {
+  uint16_t bias, other;  // as stored: a conversion would wait for the load
+};
+__device__ __forceinline__ ActElement act_inputs(const ActEpi& ep, int b, int64_t row, int col) {
+  ActElement in{0, 0};
+  if (ep.backward) {
+    if (ep.act.kind != HK_ACT_NONE) in.other = ep.z[b * ep.sZ + row * ep.ldz + col];
+  } else {
+    if (ep.bias) in.bias = ep.bias[b * ep.sBias + col];
+    if (ep.residual) in.other = ep.residual[b * ep.sR + row * ep.ldr + col];
+  }
+  return in;
+}
+// Returns d in the backward pass.
 __device__ __forceinline__ float act_element(const ActEpi& ep, uint16_t* C, int64_t ldc, int64_t sC,
-                                             int b, int64_t row, int col, float acc) {
-  uint16_t* cp = C + b * sC + row * ldc + col;
+                                             int b, int64_t row, int col, float acc,
+                                             const ActElement& in) {
   float v[1];
   if (ep.backward) {
     v[0] = ep.alpha * acc;
     if (ep.act.kind != HK_ACT_NONE) {
-      const float z[1] = {hk::bf16_to_f32(ep.z[b * ep.sZ + row * ep.ldz + col])};
+      const float z[1] = {hk::bf16_to_f32(in.other)};
       hk::scale_by_grad(ep.act, z, v);
     }
   } else {
-    v[0] = __builtin_fmaf(ep.alpha, acc, ep.bias ? hk::bf16_to_f32(ep.bias[b * ep.sBias + col]) : 0.f);
+    v[0] = __builtin_fmaf(ep.alpha, acc, hk::bf16_to_f32(in.bias));
     if (ep.z) ep.z[b * ep.sZ + row * ep.ldz + col] = hk::f32_to_bf16(v[0]);
     hk::activate(ep.act, v);
-    if (ep.residual) v[0] += hk::bf16_to_f32(ep.residual[b * ep.sR + row * ep.ldr + col]);
+    if (ep.residual) v[0] += hk::bf16_to_f32(in.other);
   }
-  *cp = hk::f32_to_bf16(v[0]);
+  C[b * sC + row * ldc + col] = hk::f32_to_bf16(v[0]);
   return v[0];
 }
 
@@ -124,7 +139,7 @@ __global__ __launch_bounds__(256) void act_simple(int ta, int tb, int col_blocks
                                          : Bb[static_cast<int64_t>(k) * ldb + col]);
       acc += a * v;
     }
-    sum += act_element(ep, C, ldc, sC, b, row, col, acc);
+    sum += act_element(ep, C, ldc, sC, b, row, col, acc, act_inputs(ep, b, row, col));
   }
   if (!ep.backward || !ep.sums) return;
   lds[ty][tx] = sum;
@@ -155,8 +170,9 @@ struct RowOut {
   float* dbias;  // the bias gradient where that is this row alone (else ep.sums takes the row)
   int64_t sD;
   int accumulate;
-  __device__ void operator()(int b, int col, float sum) const {
-    const float d = act_element(ep, C, 0, sC, b, 0, col, sum);
+  __device__ ActElement inputs(int b, int col) const { return act_inputs(ep, b, 0, col); }
+  __device__ void operator()(int b, int col, float sum, const ActElement& in) const {
+    const float d = act_element(ep, C, 0, sC, b, 0, col, sum, in);
     if (!ep.backward) return;
     if (dbias) {
       float* dst = dbias + b * sD + col;
@@ -224,40 +240,45 @@ __global__ __launch_bounds__(WAVES * HK_WAVE) void act_row_nn(int N, int K, int 
     for (int e = 0; e < 8; ++e) lds[wave][c + e] = acc[e];
   }
   __syncthreads();
-  const int i = threadIdx.x;
-  if (i < COLS && block * COLS + i < N) {
+  const int i = threadIdx.x, own = block * COLS + i;
+  if (i < COLS && own < N) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) s += lds[w][i];
-    if (part) part[(static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * N + block * COLS + i] = s;
-    else out(b, block * COLS + i, s);
+    if (part) part[(static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * N + own] = s;
+    else out(b, own, s, out.inputs(b, own));
   }
 }
 
-// B [N, K]: 16 lanes take a row of B, 16 rows a workgroup.
-constexpr int kNtRows = 16, kNtStep = 16 * 8;
-__global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* __restrict__ B,
-                                                  int64_t ldb, int64_t sB,
-                                                  const uint16_t* __restrict__ x, int64_t incx,
-                                                  int64_t sx, RowOut out) {
-  const int b = blockIdx.z, j = threadIdx.x & 15;
-  const int col = blockIdx.x * kNtRows + (threadIdx.x >> 4);
+// B [N, K]: a wave takes a row of B, 4 rows a workgroup, and eight waves share a SIMD, so that rows begin while
+// others end (bias and GELU, in a graph: 1 x 1280 -> 5120 5.2 us, 6.8 with 16 lanes a row and two waves a
+// SIMD; 2560 -> 2560 5.4 and 7.6, 1280 -> 50304 23.5 and 35.0).
+constexpr int kNtRows = 4, kNtUnroll = 4, kNtStep = HK_WAVE * 8;
+template <bool UNIT>  // incx == 1
+__global__ __launch_bounds__(kNtRows * HK_WAVE, UNIT ? 8 : 4) void act_row_nt(
+    int N, int K, const uint16_t* __restrict__ B, int64_t ldb, int64_t sB,
+    const uint16_t* __restrict__ x, int64_t incx, int64_t sx, RowOut out) {
+  const int b = blockIdx.z, j = threadIdx.x & 63;
+  const int col = blockIdx.x * kNtRows + (threadIdx.x >> 6);
   const uint16_t* xb = x + b * sx;
   const uint16_t* row = B + b * sB + static_cast<int64_t>(min(col, N - 1)) * ldb;
   auto x8 = [&](unsigned k) {
-    if (incx == 1) return load_row8<true>(xb + k, 8);
+    if (UNIT) return load_row8<true>(xb + k, 8);
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       w[e] = xb[(k + 2 * e) * incx] | static_cast<uint32_t>(xb[(k + 2 * e + 1) * incx]) << 16;
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
+  // read ahead of the loop, whose latency hides theirs
+  ActElement in{};
+  if (j == 0 && col < N) in = out.inputs(b, col);
   float acc = 0.f;
   const unsigned kvec = K & ~7;
-  for (unsigned k0 = 8 * j; k0 < kvec; k0 += kRowUnroll * kNtStep) {
-    uint4 m[kRowUnroll], v[kRowUnroll];
+  for (unsigned k0 = 8 * j; k0 < kvec; k0 += kNtUnroll * kNtStep) {
+    uint4 m[kNtUnroll], v[kNtUnroll];
 #pragma unroll
-    for (int u = 0; u < kRowUnroll; ++u) {
+    for (int u = 0; u < kNtUnroll; ++u) {
       const unsigned k = k0 + u * kNtStep;
       m[u] = v[u] = make_uint4(0, 0, 0, 0);
       if (k < kvec) {
@@ -266,7 +287,7 @@ __global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* 
       }
     }
 #pragma unroll
-    for (int u = 0; u < kRowUnroll; ++u) {
+    for (int u = 0; u < kNtUnroll; ++u) {
       float fa[8], fb[8];
       hk::BF16::unpack(m[u], fa);
       hk::BF16::unpack(v[u], fb);
@@ -277,8 +298,8 @@ __global__ __launch_bounds__(256) void act_row_nt(int N, int K, const uint16_t* 
     }
   }
   if (kvec + j < static_cast<unsigned>(K)) acc += hk::bf16_to_f32(row[kvec + j]) * hk::bf16_to_f32(xb[(kvec + j) * incx]);
-  acc = hk::row16_sum(acc);
-  if (j == 0 && col < N) out(b, col, acc);
+  acc = hk::wave_sum(acc);
+  if (j == 0 && col < N) out(b, col, acc, in);
 }
 
 // The epilogue on the partials [batch][nsplit][N] of a product that is split over k.
@@ -287,6 +308,7 @@ __global__ __launch_bounds__(256) void act_row_sum(const float* __restrict__ par
   const int col = blockIdx.x * 256 + threadIdx.x, b = blockIdx.z;
   if (col >= N) return;
   const float* p = part + static_cast<int64_t>(b) * nsplit * N + col;
+  const ActElement in = out.inputs(b, col);
   float s = 0.f;
   // eight loads in flight, added in split order
   for (int k = 0; k < nsplit; k += 8) {
@@ -296,7 +318,7 @@ __global__ __launch_bounds__(256) void act_row_sum(const float* __restrict__ par
 #pragma unroll
     for (int u = 0; u < 8; ++u) s += v[u];
   }
-  out(b, col, s);
+  out(b, col, s, in);
 }
 
 // dst[y * stride + col] (+)= the sum of `rows` rows of sums[y][rows][pitch]: 32 columns a workgroup, each
@@ -373,12 +395,11 @@ struct Plan {
 // 32 columns and one trip of the loop (N 5120, K 1280: 8.65 in one launch, 8.05 in two, 5.6 against
 // 7.4 for K 512 to 768). Everything else is cut to some 640 workgroups of 64 columns, two or three a CU, of
 // at least 160 rows (N 5120, K 2048: 11.8 whole, 9.3 cut; K 5120: 24.6 and 14.6; K 10240: 45.8 and 22.8).
-// B [N, K]: a workgroup takes 16 whole rows of B unless they are few and long (N 5120, K 5120: 13.6
-// whole, 11.9 cut; N 1280: 11.0 and 7.2; N 8192: 14.9 and 16.5; N 2560, K 2560: 7.6 and 6.9, and
-// 8.0 and 10.6 outside a graph, where the host is the slower one).
+// B [N, K]: rows are left whole unless they are few and very long (N 256, K 10240: 6.7 whole, 6.0 cut, K 5120:
+// 4.8 and 5.1; N 1280, K 10240: 8.0 and 9.5, K 50304: 31 and 24; N 5120, K 5120: 11.1 and 12.2).
 RowForm row_form(const Call& c, const hk::GemvPlan& gemv) {
   if (c.tb) {
-    const bool cut = hk::ceil_div(c.N, kNtRows) * c.batch < 512 && c.K > 2560;
+    const bool cut = c.K > 8192 && int64_t{16} * c.N * c.batch <= c.K;
     return {cut ? gemv.nsplit : 1, 0};
   }
   const int64_t groups = hk::ceil_div(c.N, 64) * c.batch;
@@ -480,8 +501,10 @@ hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t str
       HK_RETURN_IF_ERROR(hk::bgemv_partials(c.tb, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, c.batch,
                                             p.gemv, part, stream));
     } else if (c.tb) {
-      hipLaunchKernelGGL(act_row_nt, dim3((c.N + kNtRows - 1) / kNtRows, 1, c.batch), dim3(256), 0,
-                         stream, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, out);
+      hipLaunchKernelGGL(incx == 1 ? act_row_nt<true> : act_row_nt<false>,
+                         dim3((c.N + kNtRows - 1) / kNtRows, 1, c.batch),
+                         dim3(kNtRows * HK_WAVE), 0, stream, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx,
+                         c.sA, out);
     } else {
       const int cols = p.row.nn == 0 ? 32 : 64, waves = p.row.nn == 2 ? 8 : 16;
       const auto kernel = p.row.nn == 0   ? act_row_nn<32, 16>

@@ -235,7 +235,8 @@ def test_batches(hk, batch, M, N, K, ta, tb, pad, own_bias):
 @pytest.mark.parametrize("N,K,tb,batch", [(300, 1536, 0, None), (300, 1537, 0, None), (64, 20481, 0, None),
                                           (4001, 3001, 0, None), (14400, 1700, 0, None),
                                           (33001, 300, 0, None), (1500, 2000, 0, 3), (77, 12000, 0, 5),
-                                          (1280, 2049, 1, None), (9001, 2100, 1, None), (700, 6000, 1, 3)])
+                                          (1280, 2049, 1, None), (9001, 2100, 1, None), (700, 6000, 1, 3),
+                                          (100, 9000, 1, None), (33, 30001, 1, 3)])
 def test_every_form_of_one_row(hk, N, K, tb, batch):
     """Whole columns on each workgroup, and k cut into shares."""
     say("act row", N, K, tb, batch)
