@@ -8,8 +8,8 @@
 // gradient 3, the bias gradient 1) are part of the product's stores.
 //
 // The products are those of bgemm.hip and bgemm_flex.hip, on the same tiles by the same choice, with the
-// epilogue of bgemm_act.h in the tiles' place of the plain one; a product of one row runs on the kernels
-// of bgemv.hip. Where K is split, a second kernel adds the fp32 partials in split order and applies the
+// epilogue of bgemm_act.h in the tiles' place of the plain one; a product of one row has kernels of its own
+// (below). Where K is split, a second kernel adds the fp32 partials in split order and applies the
 // epilogue. The bias gradient is summed in fp32 from the values before their rounding: over the rows of
 // a wave in registers, over the waves of the grid by a further kernel, in a fixed order.
 #include <algorithm>
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void act_simple(int ta, int tb, int col_blocks
 
 // ---- one row: a matrix that is read once, each of its elements for one product ---------------------
 // A workgroup takes some columns of B over all of k and finishes them itself, in the one launch that a short
-// decoding step wants, or over a share of k, and a second kernel adds the shares (split_row says when).
+// decoding step wants, or over a share of k, and a second kernel adds the shares (row_form says when).
 // Loads are 16 bytes at any alignment, eight in flight a lane.
 typedef uint32_t u32x4a2_t __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint4 load8_anywhere(const uint16_t* p) {
