@@ -182,8 +182,9 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
     cm[e] = __builtin_floorf(tm);
     cv[e] = __builtin_floorf(tv);
   }
-  // scales whose reciprocals or whose elements fp32 does not hold go the long way, too
-  if (__ballot(far < kNear) != 0 || sm < 1e-25f || sv < 1e-25f) {
+  // Scales whose elements or whose reciprocals fp32 does not hold go the long way, too: from 2^126 = 8.5e37 on
+  // the reciprocal is subnormal, and the instruction gives 0.
+  if (__ballot(far < kNear) != 0 || sm < 1e-25f || sv < 1e-25f || sm > 1e37f || sv > 1e37f) {
     const double um = sm > 0.f ? sm * (1.0 / kUnitM) : 1.0, uv = sv > 0.f ? sv * (1.0 / kUnitV) : 1.0;
     const double jm = __builtin_amdgcn_rcp(um), jv = __builtin_amdgcn_rcp(uv);
 #pragma unroll
