@@ -170,7 +170,7 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
   // rounding to fp32 keeps the order: the largest of the rounded is the largest, rounded
   sm = block_max(mf);
   sv = block_max(vf);
-  if (!(sm + sv < INFINITY)) sm = sv = NAN;
+  if (!(sm < INFINITY && sv < INFINITY)) sm = sv = NAN;
   // estimates; a scale of 0 has no element over 0
   const float im = sm > 0.f ? __builtin_amdgcn_rcpf(sm) * static_cast<float>(kUnitM) : 0.f;
   const float iv = sv > 0.f ? __builtin_amdgcn_rcpf(sv) * static_cast<float>(kUnitV) : 0.f;

@@ -1,5 +1,5 @@
 """8-bit AdamW at the ends of fp32's range, against the definition in 64 bits: blocks with scales whose reciprocal
-fp32 does not hold.
+fp32 does not hold, or whose sum.
 
 The codes and scales have to be the definition's own; the parameters' tolerance is test_gpu_adam8.py's."""
 from __future__ import annotations
@@ -37,6 +37,18 @@ def test_codes_of_large_scales(hk, m_scale, v_scale):
     wm, wv = _decode(*want)
     assert np.allclose(mo.cpu().numpy().reshape(m.shape), wm, rtol=2.0 ** -23, atol=1e-44)
     assert np.allclose(vo.cpu().numpy().reshape(m.shape), wv, rtol=2.0 ** -23, atol=1e-44)
+
+
+def test_finite_scales_whose_sum_is_not(hk):
+    rng = np.random.default_rng(3)
+    m = (rng.uniform(-1, 1, (2, BLOCK)) * 3e38).astype(np.float32)
+    v = (rng.uniform(0, 1, (2, BLOCK)) * 3e38).astype(np.float32)
+    m[1, 5] = np.inf  # this block only
+    _, got = _quantized(hk, m, v)
+    want = _encode(m[:1].astype(np.float64), v[:1].astype(np.float64))
+    for a, b in zip(got, want):
+        assert np.array_equal(a[:1], b)
+    assert np.isnan(got[2][1]) and np.isnan(got[3][1])
 
 
 @pytest.mark.parametrize("size", [5e19, 5.5e19])
