@@ -17,7 +17,8 @@
 //   um (c^2 - c + 1/2)    and    uv ((c - 1)^4 + c^4) / 2 = uv (h^4 + 3/2 h^2 + 1/16), h = c - 1/2.
 // The parameter itself is updated in fp32 from the moments
 // before they are rounded to codes, with the hardware's square root and reciprocal (1 ulp each, of a
-// step that is lr times smaller than the parameter's own scale).
+// step that is lr times smaller than the parameter's own scale); in fp64 where v is no normal fp32 number and
+// eps does not hide it.
 //
 // Bound: HBM, 16 bytes a parameter with fp32 gradients (28 with states in 32 bits: 573 us for the same
 // step). One wave takes a block: 4 consecutive elements a lane, 16-byte accesses of p and g at any
@@ -223,7 +224,12 @@ struct Hyper {
   double beta1, beta2, rest1, rest2;  // rest: 1 - beta
   float root_ibc2, eps;               // sqrt(1 / bias correction 2)
   float lr1, decay;                   // lr / bias correction 1, lr * weight decay
+  int small_eps;                      // eps < kSmallEps
 };
+// The hardware's square root takes a subnormal v for 0, and a v under those is 0 in fp32. Both roots are under
+// 1.1e-19 (divided by bias correction 2's root, under 1e-17): nothing beside an eps from here on, but all of the
+// denominator where eps is 0.
+constexpr float kSmallEps = 1e-9f, kLeastNormal = 1.1754944e-38f;
 
 // One block of tensor t: its elements from `start` on, block `blk` of the states.
 template <class G, bool FULL>
@@ -256,8 +262,10 @@ __device__ __forceinline__ void step_block(const TensorEntry& t, const States& s
     vf[e] = static_cast<float>(v[e]);
     // p - lr wd p - lr (m / bc1) / (sqrt(v / bc2) + eps)
     const float denom = __builtin_fmaf(__builtin_amdgcn_sqrtf(vf[e]), h.root_ibc2, h.eps);
-    p[e] = __builtin_fmaf(-h.lr1 * mf[e], __builtin_amdgcn_rcpf(denom),
-                          __builtin_fmaf(-h.decay, p[e], p[e]));
+    const float rest = __builtin_fmaf(-h.decay, p[e], p[e]);
+    p[e] = __builtin_fmaf(-h.lr1 * mf[e], __builtin_amdgcn_rcpf(denom), rest);
+    if (h.small_eps && vf[e] < kLeastNormal && v[e] > 0.0)
+      p[e] = static_cast<float>(rest - h.lr1 * m[e] / (sqrt(v[e]) * h.root_ibc2 + h.eps));
   }
   uint32_t mw, vw;
   float sm1, sv1;
@@ -435,7 +443,7 @@ extern "C" hipError_t hk_adam8_plan_step(const hk_adam8_plan* plan, float lr, fl
   const Hyper h{beta1, beta2, 1.0 - beta1, 1.0 - beta2,
                 static_cast<float>(1.0 / sqrt(static_cast<double>(bias_correction2))), eps,
                 static_cast<float>(static_cast<double>(lr) / bias_correction1),
-                static_cast<float>(static_cast<double>(lr) * weight_decay)};
+                static_cast<float>(static_cast<double>(lr) * weight_decay), eps < kSmallEps};
   auto* k = plan->grad_type == HK_TYPE_F32    ? adam8_step<GradF32>
             : plan->grad_type == HK_TYPE_BF16 ? adam8_step<Grad16<hk::bf16_to_f32>>
                                               : adam8_step<Grad16<hk::f16_to_f32>>;

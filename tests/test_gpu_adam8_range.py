@@ -1,5 +1,5 @@
 """8-bit AdamW at the ends of fp32's range, against the definition in 64 bits: blocks with scales whose reciprocal
-fp32 does not hold, or whose sum.
+fp32 does not hold, or whose sum, and squares of gradients that fp32 does not hold.
 
 The codes and scales have to be the definition's own; the parameters' tolerance is test_gpu_adam8.py's."""
 from __future__ import annotations
@@ -71,6 +71,33 @@ def test_steps_of_large_gradients(hk, size):
                   1 - HYPER["beta1"] ** step, 1 - HYPER["beta2"] ** step)
         want, s, tol = _step(before, x, old, step)
         assert np.isfinite(want).all() and np.isfinite(s[3]).all() and (step > 1 or s[3].max() > 2.0 ** 126)
+        for a, b in zip(_split(state, [n])[0], s):
+            assert np.array_equal(a, b), step
+        assert (np.abs(dev.cpu().numpy() - want) <= tol).all(), step
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-20, 1e-12])
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_steps_of_gradients_whose_squares_fp32_does_not_hold(hk, eps, grad):
+    """Subnormal v, and v that fp32 rounds to 0, under an eps that does not hide them."""
+    h = dict(HYPER, eps=eps)
+    rng = np.random.default_rng(9)
+    n = 3 * BLOCK + 5
+    p = rng.normal(0, 0.02, n).astype(np.float32)
+    g = torch.zeros(n, device=DEV, dtype=torch.float32 if grad == "f32" else torch.bfloat16)
+    dev = torch.from_numpy(p).to(DEV)
+    state = hk.adam8_states([n], DEV)
+    plan = hk.Adam8Plan([dev], [g], *state)
+    for step in (1, 2):
+        sign = np.where(rng.random(n) < 0.5, -1.0, 1.0)
+        # squares of 1e-60 .. 1e-36; fp32 holds 1e-45, whole digits from 1e-38 on
+        x = sign * 10.0 ** rng.uniform(-30, -18, n)
+        g.copy_(torch.from_numpy(x.astype(np.float32)))
+        before, old = dev.cpu().numpy(), _split(state, [n])[0]
+        plan.step(h["lr"], h["beta1"], h["beta2"], eps, h["weight_decay"], 1 - h["beta1"] ** step,
+                  1 - h["beta2"] ** step)
+        want, s, tol = _step(before, g.float().cpu().numpy(), old, step, h)
+        assert np.isfinite(want).all()
         for a, b in zip(_split(state, [n])[0], s):
             assert np.array_equal(a, b), step
         assert (np.abs(dev.cpu().numpy() - want) <= tol).all(), step
