@@ -280,13 +280,13 @@ __device__ __forceinline__ void step_block(const TensorEntry& t, const States& s
   }
 }
 
-// tensor_of: the tensor of each block. One block a workgroup of one wave: 124.4 M parameters, fp32 gradients,
-// 300 us, 315 with two blocks, 329 with four.
+// tensor_of: the tensor of each block, from block `first` on. One block a workgroup of one wave: 124.4 M parameters,
+// fp32 gradients, 300 us, 315 with two blocks, 329 with four.
 template <class G>
 __global__ __launch_bounds__(HK_WAVE) void adam8_step(const TensorEntry* __restrict__ tensors,
                                                       const int32_t* __restrict__ tensor_of,
-                                                      States st, Hyper h) {
-  const int64_t blk = blockIdx.x;
+                                                      States st, Hyper h, uint32_t first) {
+  const int64_t blk = first + blockIdx.x;
   const TensorEntry t = tensors[tensor_of[blk]];
   const int64_t start = (blk - t.block0) * kBlock;
   if (start + kBlock <= t.numel) step_block<G, true>(t, st, h, start, blk, threadIdx.x);
@@ -346,6 +346,10 @@ __global__ __launch_bounds__(256) void adam8_dequantize(const uint32_t* __restri
   store4<false>(m, i, numel, mf);
   store4<false>(v, i, numel, vf);
 }
+
+// Blocks of one launch: a dimension of a grid has under 2^32 threads, and more of them run as their number
+// modulo 2^32, with no error.
+constexpr int64_t kLaunchBlocks = int64_t{1} << 25;
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -447,9 +451,13 @@ extern "C" hipError_t hk_adam8_plan_step(const hk_adam8_plan* plan, float lr, fl
   auto* k = plan->grad_type == HK_TYPE_F32    ? adam8_step<GradF32>
             : plan->grad_type == HK_TYPE_BF16 ? adam8_step<Grad16<hk::bf16_to_f32>>
                                               : adam8_step<Grad16<hk::f16_to_f32>>;
-  hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(plan->num_blocks)), dim3(HK_WAVE), 0, stream,
-                     plan->d_tensors, plan->d_tensor_of, plan->st, h);
-  return hk::launch_status();
+  for (int64_t first = 0; first < plan->num_blocks; first += kLaunchBlocks) {
+    const int64_t n = std::min(kLaunchBlocks, plan->num_blocks - first);
+    hipLaunchKernelGGL(k, dim3(static_cast<unsigned>(n)), dim3(HK_WAVE), 0, stream, plan->d_tensors,
+                       plan->d_tensor_of, plan->st, h, static_cast<uint32_t>(first));
+    HK_RETURN_IF_ERROR(hk::launch_status());
+  }
+  return hipSuccess;
 }
 
 extern "C" hipError_t hk_adam8_plan_destroy(hk_adam8_plan* plan) {
@@ -469,42 +477,51 @@ extern "C" int64_t hk_adam8_plan_num_blocks(const hk_adam8_plan* plan) {
 }
 
 namespace {
-// Workgroups of four blocks, or -1 where the arguments do not hold.
-int64_t conversion_grid(const void* m_codes, const void* v_codes, const float* m_scales,
-                        const float* v_scales, int64_t numel, const float* m, const float* v) {
-  if (numel < 0) return -1;
-  if (numel == 0) return 0;
-  if (!m_codes || !v_codes || !m_scales || !v_scales || !m || !v) return -1;
+// What a conversion works on; the checks that both have in common.
+bool conversion_holds(const void* m_codes, const void* v_codes, const float* m_scales,
+                      const float* v_scales, int64_t numel, const float* m, const float* v) {
+  if (numel < 0 || numel > int64_t{INT32_MAX} * kBlock) return false;
+  if (numel == 0) return true;
   for (const void* p : {m_codes, v_codes, static_cast<const void*>(m_scales),
                         static_cast<const void*>(v_scales), static_cast<const void*>(m),
                         static_cast<const void*>(v)})
-    if (!aligned4(p)) return -1;
-  const int64_t grid = hk::ceil_div(hk::ceil_div(numel, kBlock), 4);
-  return grid <= INT32_MAX ? grid : -1;
+    if (!p || !aligned4(p)) return false;
+  return true;
+}
+// Calls launch(first block, elements from there on, workgroups of four blocks) for each launch's blocks.
+template <class Launch>
+hipError_t by_launch(int64_t numel, Launch&& launch) {
+  constexpr int64_t kElements = kLaunchBlocks * kBlock;
+  for (int64_t at = 0; at < numel; at += kElements) {
+    const int64_t n = std::min(kElements, numel - at);
+    launch(at / kBlock, n, dim3(static_cast<unsigned>(hk::ceil_div(n, 4 * kBlock))));
+    HK_RETURN_IF_ERROR(hk::launch_status());
+  }
+  return hipSuccess;
 }
 }  // namespace
 
 extern "C" hipError_t hk_adam8_quantize(const float* m, const float* v, int64_t numel,
                                         int8_t* m_codes, uint8_t* v_codes, float* m_scales,
                                         float* v_scales, hipStream_t stream) {
-  const int64_t grid = conversion_grid(m_codes, v_codes, m_scales, v_scales, numel, m, v);
-  HK_CHECK_ARG(grid >= 0);
-  if (grid == 0) return hipSuccess;
-  const States st{reinterpret_cast<uint32_t*>(m_codes), reinterpret_cast<uint32_t*>(v_codes),
-                  m_scales, v_scales};
-  hipLaunchKernelGGL(adam8_quantize, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream, m, v,
-                     numel, st);
-  return hk::launch_status();
+  HK_CHECK_ARG(conversion_holds(m_codes, v_codes, m_scales, v_scales, numel, m, v));
+  return by_launch(numel, [&](int64_t block, int64_t n, dim3 grid) {
+    const int64_t i = block * kBlock;
+    const States st{reinterpret_cast<uint32_t*>(m_codes + i), reinterpret_cast<uint32_t*>(v_codes + i),
+                    m_scales + block, v_scales + block};
+    hipLaunchKernelGGL(adam8_quantize, grid, dim3(256), 0, stream, m + i, v + i, n, st);
+  });
 }
 
 extern "C" hipError_t hk_adam8_dequantize(const int8_t* m_codes, const uint8_t* v_codes,
                                           const float* m_scales, const float* v_scales,
                                           int64_t numel, float* m, float* v, hipStream_t stream) {
-  const int64_t grid = conversion_grid(m_codes, v_codes, m_scales, v_scales, numel, m, v);
-  HK_CHECK_ARG(grid >= 0);
-  if (grid == 0) return hipSuccess;
-  hipLaunchKernelGGL(adam8_dequantize, dim3(static_cast<unsigned>(grid)), dim3(256), 0, stream,
-                     reinterpret_cast<const uint32_t*>(m_codes),
-                     reinterpret_cast<const uint32_t*>(v_codes), m_scales, v_scales, numel, m, v);
-  return hk::launch_status();
+  HK_CHECK_ARG(conversion_holds(m_codes, v_codes, m_scales, v_scales, numel, m, v));
+  return by_launch(numel, [&](int64_t block, int64_t n, dim3 grid) {
+    const int64_t i = block * kBlock;
+    hipLaunchKernelGGL(adam8_dequantize, grid, dim3(256), 0, stream,
+                       reinterpret_cast<const uint32_t*>(m_codes + i),
+                       reinterpret_cast<const uint32_t*>(v_codes + i), m_scales + block,
+                       v_scales + block, n, m + i, v + i);
+  });
 }
