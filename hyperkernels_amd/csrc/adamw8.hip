@@ -378,7 +378,7 @@ extern "C" hipError_t hk_adam8_plan_create(int num_tensors, float* const* params
   int64_t blocks = 0;
   const unsigned grad_align = grad_type == HK_TYPE_F32 ? 3u : 1u;
   for (int t = 0; t < num_tensors; ++t) {
-    HK_CHECK_ARG(sizes[t] >= 0);
+    HK_CHECK_ARG(sizes[t] >= 0 && sizes[t] <= int64_t{INT32_MAX} * kBlock);
     uint16_t* copy = copies ? copies[t] : nullptr;
     HK_CHECK_ARG(sizes[t] == 0 || (params[t] && grads[t]));
     HK_CHECK_ARG(aligned4(params[t]) && (reinterpret_cast<uintptr_t>(grads[t]) & grad_align) == 0 &&
