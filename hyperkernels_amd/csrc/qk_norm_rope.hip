@@ -23,6 +23,8 @@
 //
 // The gradients of the two weight vectors are summed in registers over the rows of a lane group, over
 // a workgroup through LDS, and over the workgroups by a second kernel, all in a fixed order.
+#include <algorithm>
+
 #include "hk_device.h"
 #include "hk_host.h"
 
@@ -182,6 +184,7 @@ struct Args {
   const int64_t* positions;  // NULL: the token's index
   int64_t pos_stride;
   int T;
+  int first;  // forward: the launch's first workgroup
   float eps, inv_d;
 };
 
@@ -218,9 +221,9 @@ __device__ __forceinline__ void weights(const void* w, const Unit<V, O>& u, int 
 // U: units a lane holds (more than one only where a row needs more than 64 of them, V == 1). O: OVERLAP.
 template <class FI, class FO, int V, int U, bool O>
 __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
-  const int which = static_cast<int>(blockIdx.x) >= g.side[0].blocks ? 1 : 0;
+  const int group = blockIdx.x + g.first, which = group >= g.side[0].blocks ? 1 : 0;
   const Side& sd = g.side[which];
-  const int block = blockIdx.x - (which ? g.side[0].blocks : 0);
+  const int block = group - (which ? g.side[0].blocks : 0);
   const int per_block = kThreads / g.s.lanes;
   const int row = block * per_block + threadIdx.x / g.s.lanes;
   const int j = threadIdx.x & (g.s.lanes - 1);
@@ -504,17 +507,22 @@ Args make_args(const hk_qk_norm_rope_params* p, int v, bool backward) {
 }
 
 template <class FI, class FO, int V, int U, bool O>
-hipError_t launch(const Args& g, bool backward, hipStream_t stream) {
-  const unsigned blocks = g.side[0].blocks + g.side[1].blocks;
-  if constexpr (V == 8) {
-    if (backward) return hipErrorInvalidValue;  // unit_pairs
-    hipLaunchKernelGGL((qk_forward<FI, FO, V, U, O>), dim3(blocks), dim3(kThreads), 0, stream, g);
-  } else if (backward) {
-    hipLaunchKernelGGL((qk_backward<FI, FO, V, U, O>), dim3(blocks), dim3(kBackThreads), 0, stream, g);
-  } else {
-    hipLaunchKernelGGL((qk_forward<FI, FO, V, U, O>), dim3(blocks), dim3(kThreads), 0, stream, g);
+hipError_t launch(const Args& args, bool backward, hipStream_t stream) {
+  Args g = args;
+  const int blocks = g.side[0].blocks + g.side[1].blocks;
+  if (backward) {
+    if constexpr (V == 8) return hipErrorInvalidValue;  // unit_pairs
+    else hipLaunchKernelGGL((qk_backward<FI, FO, V, U, O>), dim3(blocks), dim3(kBackThreads), 0, stream, g);
+    return hk::launch_status();
   }
-  return hk::launch_status();
+  // a dimension of a grid has under 2^32 threads, and more of them run as their number modulo 2^32
+  constexpr int kMost = 1 << 23;
+  for (; g.first < blocks; g.first += kMost) {
+    hipLaunchKernelGGL((qk_forward<FI, FO, V, U, O>), dim3(std::min(kMost, blocks - g.first)), dim3(kThreads),
+                       0, stream, g);
+    HK_RETURN_IF_ERROR(hk::launch_status());
+  }
+  return hipSuccess;
 }
 template <class FI, class FO>
 hipError_t by_unit(const Args& g, int v, bool backward, hipStream_t stream) {

@@ -7,6 +7,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 DEV, BF = "cuda", torch.bfloat16
+ULP, HALF_STEP = 2.0 ** -24, 2.0 ** -8
 FIRST = 2 ** 20  # elements at the start of a tensor that are compared
 
 
@@ -32,6 +33,26 @@ def _gen(seed):
     gen = torch.Generator(device=DEV)
     gen.manual_seed(seed)
     return gen
+
+
+def test_query_norms_of_64_lanes_a_row(hk):
+    """Two rotated elements of 128: a row takes 64 lanes, so 2^26 of them are 2^32."""
+    B, H, T, d = 1, 64, 2 ** 20 + 3, 128
+    _room(20)
+    q = _normal(_gen(4), B, T, H, d).transpose(1, 2)
+    ang = torch.randn(T, 1, generator=_gen(5), device=DEV)
+    cos, sin = ang.cos(), ang.sin()
+    parts = [slice(0, 5), slice(T // 2, T // 2 + 5), slice(T - 5, T)]
+    x = [q[:, :, s].double() for s in parts]
+    hk.qk_norm_rope_forward(q, None, cos, sin, q_out=q)
+    for s, t in zip(parts, x):
+        n = t * (t.square().mean(-1, keepdim=True) + 1e-6) ** -0.5
+        c, sn = cos[s, 0].double(), sin[s, 0].double()
+        want, spread = n.clone(), n.abs()
+        want[..., 0], want[..., 1] = n[..., 0] * c - n[..., 1] * sn, n[..., 1] * c + n[..., 0] * sn
+        spread[..., :2] = n[..., :2].abs().sum(-1, keepdim=True)
+        tol = 24 * ULP * spread + HALF_STEP * want.abs()
+        assert bool(((q[:, :, s].double() - want).abs() <= tol).all()), s
 
 
 def test_8_bit_adamw(hk):
