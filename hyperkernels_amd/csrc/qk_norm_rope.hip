@@ -165,6 +165,15 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
+// Rows whose mean of squares (eps added) fp32 does not hold well are taken times a power of two: n does not change
+// when x, and eps with its square, do. Under 2^-80 squares begin to lose digits (elements are under 2^-36 then,
+// times 2^88 their squares lie between 2^-122 and 2^104); where the sum passes fp32, elements of up to 2^128
+// times 2^-70 have sums up to 2^124. The branch that asks is the wave's; all other rows get 1 in it.
+__device__ __forceinline__ bool in_range(float mean) { return mean >= 0x1p-80f && mean < INFINITY; }
+__device__ __forceinline__ float row_scale(float mean) {
+  return in_range(mean) ? 1.0f : mean < 1.0f ? 0x1p88f : 0x1p-70f;
+}
+
 // Queries or keys: a strided [B, heads, T, d] tensor and what belongs to it.
 struct Side {
   const void* x;
@@ -246,7 +255,22 @@ __global__ __launch_bounds__(kThreads) void qk_forward(Args g) {
     for (int e = 0; e < V; ++e)
       sum += u.own_a(e, xa[k][e] * xa[k][e]) + u.own_b(e, xb[k][e] * xb[k][e]);
   }
-  const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
+  float mean = lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps;
+  if (__ballot(!in_range(mean)) != 0) {
+    const float by = row_scale(mean);
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const Unit<V, O> u(g.s, j + k * HK_WAVE);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xa[k][e] *= by, xb[k][e] *= by;
+        sum += u.own_a(e, xa[k][e] * xa[k][e]) + u.own_b(e, xb[k][e] * xb[k][e]);
+      }
+    }
+    mean = lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps * by * by;
+  }
+  const float r = __builtin_amdgcn_rsqf(mean);
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const Unit<V, O> u(g.s, j + k * HK_WAVE);
@@ -308,7 +332,23 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
         dot += u.own_a(e, ga[k][e] * wa[k][e] * xa[k][e]) + u.own_b(e, gb[k][e] * wb[k][e] * xb[k][e]);
       }
     }
-    const float r = __builtin_amdgcn_rsqf(lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps);
+    float mean = lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps, by = 1.f;
+    if (__ballot(!in_range(mean)) != 0) {
+      by = row_scale(mean);
+      sum = dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const Unit<V, O> u(g.s, j + k * HK_WAVE);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          xa[k][e] *= by, xb[k][e] *= by;
+          sum += u.own_a(e, xa[k][e] * xa[k][e]) + u.own_b(e, xb[k][e] * xb[k][e]);
+          dot += u.own_a(e, ga[k][e] * wa[k][e] * xa[k][e]) + u.own_b(e, gb[k][e] * wb[k][e] * xb[k][e]);
+        }
+      }
+      mean = lanes_sum(sum, g.s.lanes) * g.inv_d + g.eps * by * by;
+    }
+    const float r = __builtin_amdgcn_rsqf(mean), rx = r * by;  // of x as it is held, and of x
     // mean(g w n) = r mean(g w x)
     const float m = lanes_sum(dot, g.s.lanes) * g.inv_d * r;
 #pragma unroll
@@ -320,8 +360,8 @@ __global__ __launch_bounds__(kBackThreads, 6) void qk_backward(Args g) {
         const float na = xa[k][e] * r, nb = xb[k][e] * r;
         da[k][e] += ga[k][e] * na;
         db[k][e] += gb[k][e] * nb;
-        oa[e] = r * (ga[k][e] * wa[k][e] - na * m);
-        ob[e] = r * (gb[k][e] * wb[k][e] - nb * m);
+        oa[e] = rx * (ga[k][e] * wa[k][e] - na * m);
+        ob[e] = rx * (gb[k][e] * wb[k][e] - nb * m);
       }
       if (u.on) store_unit<FI, V>(dx, u, g.s.d, oa, ob);
     }
