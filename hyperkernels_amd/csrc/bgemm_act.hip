@@ -122,7 +122,9 @@ __global__ __launch_bounds__(256) void act_simple(int ta, int tb, int col_blocks
                                                   int64_t sB, uint16_t* __restrict__ C, int64_t ldc,
                                                   int64_t sC) {
   __shared__ float lds[16][17];
-  const int rb = blockIdx.x / col_blocks, cb = blockIdx.x - rb * col_blocks;
+  const int block = blockIdx.y * gridDim.x + blockIdx.x;
+  const int rb = block / col_blocks, cb = block - rb * col_blocks;
+  if (rb * kSimpleRows >= M) return;  // the last of blockIdx.y
   const int b = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int col = cb * 16 + tx;
   const uint16_t* Ab = A + b * sA;
@@ -462,7 +464,7 @@ hipError_t column_sums(const Call& c, const float* sums, int64_t rows, hipStream
   return hk::launch_status();
 }
 
-hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+hipError_t run_piece(Call c, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   if (c.N == 0) return hipSuccess;
   if (c.M == 0 || c.batch == 0)  // no rows: a bias gradient of zero
     return c.ep.backward && c.dbias && (c.batch > 0 || c.sD == 0)
@@ -526,14 +528,17 @@ hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t str
     const int cols = (c.N + 15) / 16;
     const int64_t blocks = hk::ceil_div(c.M, kSimpleRows) * cols;
     HK_CHECK_ARG(blocks <= INT32_MAX);
-    hipLaunchKernelGGL(act_simple, dim3(static_cast<unsigned>(blocks), 1, c.batch), dim3(256), 0,
-                       stream, c.ta ? 1 : 0, c.tb ? 1 : 0, cols, c.M, c.N, c.K, ep, c.A, c.lda, c.sA,
-                       c.B, c.ldb, c.sB, c.C, c.ldc, c.sC);
+    // under 2^32 threads in x
+    const auto gx = static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 23));
+    const auto gy = static_cast<unsigned>(hk::ceil_div(blocks, gx));
+    hipLaunchKernelGGL(act_simple, dim3(gx, gy, c.batch), dim3(256), 0, stream, c.ta ? 1 : 0,
+                       c.tb ? 1 : 0, cols, c.M, c.N, c.K, ep, c.A, c.lda, c.sA, c.B, c.ldb, c.sB, c.C,
+                       c.ldc, c.sC);
     HK_RETURN_IF_ERROR(hk::launch_status());
   } else if (p.gemm.used > 1) {
     const int cols = (c.N + 127) / 128;
     const int64_t blocks = hk::ceil_div(c.M, kFinalRows) * cols;
-    HK_CHECK_ARG(blocks <= INT32_MAX);
+    HK_CHECK_ARG(blocks < 1 << 24);  // 2^32 threads
     HK_RETURN_IF_ERROR(hk::bgemm_write_partials(c.ta, c.tb, c.M, c.N, c.K, c.A, c.lda, c.sA, c.B, c.ldb,
                                                 c.sB, c.batch, p.gemm, part, stream));
     hipLaunchKernelGGL(act_finalize, dim3(static_cast<unsigned>(blocks), 1, c.batch), dim3(256), 0,
@@ -555,6 +560,34 @@ hipError_t run(Call c, void* workspace, int64_t workspace_bytes, hipStream_t str
                                     c.B, c.ldb, c.sB, c.C, c.ldc, c.sC));
   }
   return ep.sums ? column_sums(c, ep.sums, p.sum_rows, stream) : hipSuccess;
+}
+
+// A dimension of a grid has under 2^32 threads, and more of them run as their number modulo 2^32, with no error.
+// One row takes up to 64 threads a column, the smallest tiles of many rows 16 a row, so products of more than
+// kPieceSide rows or columns run as several; whole tiles and vectors.
+constexpr int kPieceSide = 1 << 25;
+
+hipError_t run(const Call& c, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  if (c.M <= kPieceSide && c.N <= kPieceSide) return run_piece(c, workspace, workspace_bytes, stream);
+  for (int64_t n0 = 0; n0 < c.N; n0 += kPieceSide) {
+    for (int64_t m0 = 0; m0 == 0 || m0 < c.M; m0 += kPieceSide) {  // no rows: a bias gradient of zero
+      Call p = c;
+      p.M = static_cast<int>(std::min<int64_t>(kPieceSide, c.M - m0));
+      p.N = static_cast<int>(std::min<int64_t>(kPieceSide, c.N - n0));
+      if (c.K > 0) {
+        p.A += c.ta ? m0 : m0 * c.lda;
+        p.B += c.tb ? n0 * c.ldb : n0;
+      }
+      p.C += m0 * c.ldc + n0;
+      if (c.ep.bias) p.ep.bias += n0;
+      if (c.ep.residual) p.ep.residual += m0 * c.ep.ldr + n0;
+      if (c.ep.z) p.ep.z += m0 * c.ep.ldz + n0;
+      if (c.dbias) p.dbias += n0;
+      p.accumulate = c.accumulate || m0 > 0;  // the bias gradients of the rows before are there
+      HK_RETURN_IF_ERROR(run_piece(p, workspace, workspace_bytes, stream));
+    }
+  }
+  return hipSuccess;
 }
 
 float bf16_value(hk_bf16 h) {
@@ -646,21 +679,25 @@ extern "C" int64_t hk_bgemm_act_workspace(int transA, int transB, int M, int N, 
       batchCount < 0 || batchCount > kMaxGridZ || M > kMaxSide || N > kMaxSide || K > kMaxSide)
     return -1;
   if (M == 0 || N == 0 || batchCount == 0) return 0;
-  // the most of what the rows' alignments make of the call
+  // the most of what the rows' alignments make of the call, and of its whole and last pieces
   Call c{};
   c.ta = transA != 0, c.tb = transB != 0;
-  c.M = M, c.N = N, c.K = K, c.batch = batchCount;
+  c.K = K, c.batch = batchCount;
   c.ep.backward = dbias != 0;
   float none;
   c.dbias = dbias ? &none : nullptr;  // compared with NULL only
   size_t most = 0;
-  for (int odd = 0; odd < 4; ++odd) {
-    // aligned, unaligned C, unaligned A and B, and the fallback's leading dimensions
-    c.lda = (odd == 3 ? int64_t{1} << 22 : hk::ceil_div(c.ta ? M : K, 8) * 8) + (odd == 2 ? 1 : 0);
-    c.ldb = hk::ceil_div(c.tb ? K : N, 8) * 8;
-    c.ldc = hk::ceil_div(N, 8) * 8 + (odd == 1 ? 1 : 0);
-    const size_t bytes = make_plan(c, true).bytes();
-    if (bytes > most) most = bytes;
+  for (int piece = 0; piece < 4; ++piece) {
+    if ((piece & 1 && M <= kPieceSide) || (piece & 2 && N <= kPieceSide)) continue;
+    c.M = piece & 1 ? (M - 1) % kPieceSide + 1 : std::min(M, kPieceSide);
+    c.N = piece & 2 ? (N - 1) % kPieceSide + 1 : std::min(N, kPieceSide);
+    for (int odd = 0; odd < 4; ++odd) {
+      // aligned, unaligned C, unaligned A and B, and the fallback's leading dimensions
+      c.lda = (odd == 3 ? int64_t{1} << 22 : hk::ceil_div(c.ta ? M : K, 8) * 8) + (odd == 2 ? 1 : 0);
+      c.ldb = hk::ceil_div(c.tb ? K : N, 8) * 8;
+      c.ldc = hk::ceil_div(N, 8) * 8 + (odd == 1 ? 1 : 0);
+      most = std::max(most, make_plan(c, true).bytes());
+    }
   }
   return static_cast<int64_t>(most);
 }

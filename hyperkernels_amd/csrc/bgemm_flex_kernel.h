@@ -345,7 +345,8 @@ hipError_t flex_launch(const FlexArgs<E>& g, int batch, hipStream_t stream) {
   });
   HK_RETURN_IF_ERROR(attr_status);
   const int64_t tiles = hk::ceil_div(g.M, T::BMT) * hk::ceil_div(g.N, T::BNT);
-  HK_CHECK_ARG(tiles <= INT32_MAX && static_cast<int64_t>(batch) * g.split_k <= 65535);
+  // a dimension of a grid has under 2^32 threads
+  HK_CHECK_ARG(tiles * T::kThreads <= UINT32_MAX && static_cast<int64_t>(batch) * g.split_k <= 65535);
   FlexArgs<E> a = g;
   a.by_matrix = batch > 1 && tiles * batch * g.split_k <= INT32_MAX;
   hipLaunchKernelGGL((bgemm_flex<T, AK, BKM, RAGGED, E>),

@@ -35,6 +35,103 @@ def _gen(seed):
     return gen
 
 
+def _spans(n, *at):
+    """Short ranges at the ends and around the given places."""
+    return [slice(0, 70), slice(n - 90, n)] + [slice(a - 70, a + 70) for a in at]
+
+
+@pytest.mark.parametrize("tb,N,K", [(1, 2 ** 26 + 44, 8), (0, 2 ** 29 + 72, 2)])
+def test_one_row(hk, tb, N, K):
+    _room(12)
+    gen = _gen(1)
+    x, w, b = _normal(gen, 1, K), _normal(gen, *((N, K) if tb else (K, N))), _normal(gen, N)
+    r, z = _normal(gen, 1, N), torch.empty(1, N, device=DEV, dtype=BF)
+    y = hk.bgemm_act(x, w, bias=b, activation="relu", residual=r, preact=z, trans_b=bool(tb))
+    print("forward", flush=True)
+    db = torch.full((N,), 0.5, device=DEV)
+    d = hk.bgemm_act_backward(x, w, preact=z, activation="relu", dbias=db, trans_b=bool(tb))
+    print("backward", flush=True)
+    for s in _spans(N, N // 2, 2 ** 25, 2 ** 26 - 30, N - N // 3):
+        ws = (w[s].t() if tb else w[:, s]).double().contiguous()
+        prod, mag = x.double() @ ws, x.double().abs() @ ws.abs()
+        want = prod + b[s].double()
+        tol = (K + 4) * ULP * (mag + b[s].double().abs())
+        assert bool(((z[:, s].double() - want).abs() <= tol + HALF_STEP * want.abs()).all())
+        want = want.clamp_min(0) + r[:, s].double()
+        assert bool(((y[:, s].double() - want).abs() <= tol + (ULP + HALF_STEP) * want.abs() + 1e-37).all())
+        want = prod * (z[:, s] > 0)
+        assert bool(((d[:, s].double() - want).abs() <= tol + HALF_STEP * want.abs()).all())
+        assert bool(((db[s].double() - want[0] - 0.5).abs() <= tol[0] + ULP * (want[0].abs() + 1)).all())
+
+
+def test_products_without_k(hk):
+    """The plain kernel: 16 GiB of outputs."""
+    M, N = 2 ** 17 + 40, 2 ** 16 + 8
+    _room(36)
+    gen = _gen(2)
+    x, w = torch.empty(M, 0, device=DEV, dtype=BF), torch.empty(0, N, device=DEV, dtype=BF)
+    b = _normal(gen, N)
+    y = torch.full((M, N), 7.0, device=DEV, dtype=BF)
+    hk.bgemm_act(x, w, bias=b, activation="relu", out=y)
+    for at in range(0, M, 2 ** 13):
+        assert bool((y[at:at + 2 ** 13] == b.clamp_min(0)).all()), at
+    print("forward", flush=True)
+    db = torch.full((N,), 3.0, device=DEV)
+    hk.bgemm_act_backward(x, w, preact=y, activation="relu", dbias=db, out=y, accumulate=False)
+    for at in range(0, M, 2 ** 13):
+        assert bool((y[at:at + 2 ** 13] == 0).all()), at
+    assert bool((db == 0).all())
+
+
+def test_no_rows(hk):
+    """A bias gradient of zero in more columns than one launch has."""
+    N, K = 2 ** 29 + 72, 2
+    _room(6)
+    empty, w = torch.empty(0, K, device=DEV, dtype=BF), torch.empty(K, N, device=DEV, dtype=BF)
+    db = torch.full((N,), 2.0, device=DEV)
+    hk.bgemm_act_backward(empty, w, dbias=db)
+    assert bool((db == 2).all())
+    hk.bgemm_act_backward(empty, w, dbias=db, accumulate=False)
+    assert bool((db == 0).all())
+
+
+@pytest.mark.parametrize("K", [8, 9])
+def test_rows_past_the_tiles(hk, K):
+    """Small tiles over more than 2^30 rows; of 9 elements, unaligned."""
+    M, N = 2 ** 30 + 72, 8
+    _room(68)
+    gen = _gen(3)
+    x, w, b = _normal(gen, M, K), _normal(gen, K, N), _normal(gen, N)
+    z = torch.empty(M, N, device=DEV, dtype=BF)
+    y = hk.bgemm_act(x, w, bias=b, activation="relu", preact=z)
+    print("forward, tile", hk.lib().hk_bgemm_small_tile(0, 0, M, N, K, 1, 0), flush=True)
+    wd = w.double()
+    for s in _spans(M, 2 ** 25, M // 2, 2 ** 30):
+        xd = x[s].double()
+        want = xd @ wd + b.double()
+        tol = (K + 4) * ULP * (xd.abs() @ wd.abs() + b.double().abs())
+        assert bool(((z[s].double() - want).abs() <= tol + HALF_STEP * want.abs()).all())
+        want = want.clamp_min(0)
+        assert bool(((y[s].double() - want).abs() <= tol + HALF_STEP * want.abs()).all())
+    del y
+    db = torch.full((N,), 5.0, device=DEV)
+    d = hk.bgemm_act_backward(x, w, preact=z, activation="relu", dbias=db, accumulate=False)
+    print("backward", flush=True)
+    total, size, tol = (torch.zeros(N, device=DEV, dtype=torch.float64) for _ in range(3))
+    for at in range(0, M, 2 ** 24):
+        s = slice(at, min(M, at + 2 ** 24))
+        xd = x[s].double()
+        want = xd @ wd * (z[s] > 0)
+        t = (K + 4) * ULP * (xd.abs() @ wd.abs())
+        assert bool(((d[s].double() - want).abs() <= t + HALF_STEP * want.abs()).all()), at
+        total += want.sum(0)
+        size += want.abs().sum(0)
+        tol += t.sum(0)
+    # a chain of at most 48 + M / 128 additions of values of either sign, and one for each call that adds to it
+    tol += (48 + M / 128) * ULP * size
+    assert bool(((db.double() - total).abs() <= tol).all())
+
+
 def test_query_norms_of_64_lanes_a_row(hk):
     """Two rotated elements of 128: a row takes 64 lanes, so 2^26 of them are 2^32."""
     B, H, T, d = 1, 64, 2 ** 20 + 3, 128
