@@ -17,6 +17,7 @@
 #include "bgemm_act_tiles.h"
 #include "bgemm_plan.h"
 #include "bgemm_wide.h"
+#include "hk_overlap.h"
 
 namespace {
 
@@ -607,9 +608,25 @@ hipError_t check(int transA, int transB, int M, int N, int K, const void* A, int
   if (M == 0 || N == 0 || batchCount == 0) return hipSuccess;
   HK_CHECK_ARG(C != nullptr && ldc >= N && (batchCount == 1 || strideC != 0));
   HK_CHECK_ARG(K == 0 || (A != nullptr && B != nullptr));
-  HK_CHECK_ARG(K == 0 || (C != A && C != B));  // operands are read while C is written
   HK_CHECK_ARG(lda >= (transA ? M : K) && ldb >= (transB ? K : N));
   return hipSuccess;
+}
+
+// A matrix, or a batch of them, as memory.
+hk::Rows memory(const void* p, int rows, int cols, int64_t ld, int64_t stride, int batch) {
+  return hk::Rows(p, 2, cols).along(batch, 2 * stride).along(rows, 2 * ld);
+}
+// Whether C lies apart from the other output and from all inputs, but for `same` (the residual, or a preact that is
+// read), which may be C itself.
+bool outputs_apart(const Call& c, const hk::Rows& out, const hk::Rows& same) {
+  const hk::Rows C = memory(c.C, c.M, c.N, c.ldc, c.sC, c.batch);
+  const hk::Rows bias = hk::Rows(c.ep.bias, 2, c.N).along(c.batch, 2 * c.ep.sBias);
+  if (hk::overlaps_itself(C) || hk::overlap_unless_same(C, same) || hk::overlap(out, same)) return false;
+  if (hk::overlap(C, out) || hk::overlap(C, bias) || hk::overlap(out, bias)) return false;
+  if (c.K == 0) return true;
+  const hk::Rows A = memory(c.A, c.ta ? c.K : c.M, c.ta ? c.M : c.K, c.lda, c.sA, c.batch);
+  const hk::Rows B = memory(c.B, c.tb ? c.N : c.K, c.tb ? c.K : c.N, c.ldb, c.sB, c.batch);
+  return !hk::overlap(C, A) && !hk::overlap(C, B) && !hk::overlap(out, A) && !hk::overlap(out, B);
 }
 
 Call forward_call(int transA, int transB, int M, int N, int K, hk_bf16 alpha, const hk_bf16* A, int lda,
@@ -641,11 +658,13 @@ extern "C" hipError_t hk_bgemm_act(int transA, int transB, int M, int N, int K, 
                            batchCount));
   HK_CHECK_ARG(!residual || ldr >= N);
   HK_CHECK_ARG(!preact || (ldz >= N && (batchCount <= 1 || strideZ != 0)));
-  HK_CHECK_ARG(!preact || (preact != C && preact != residual && (K == 0 || (preact != A && preact != B))));
-  return run(forward_call(transA, transB, M, N, K, alpha, A, lda, strideA, B, ldb, strideB, bias,
-                          strideBias, activation, residual, ldr, strideR, preact, ldz, strideZ, C, ldc,
-                          strideC, batchCount),
-             workspace, workspace_bytes, stream);
+  const Call c = forward_call(transA, transB, M, N, K, alpha, A, lda, strideA, B, ldb, strideB, bias,
+                              strideBias, activation, residual, ldr, strideR, preact, ldz, strideZ, C, ldc,
+                              strideC, batchCount);
+  const hk::Rows z = memory(preact, M, N, ldz, strideZ, batchCount);
+  HK_CHECK_ARG(!hk::overlaps_itself(z) &&
+               outputs_apart(c, z, memory(residual, M, N, ldr, strideR, batchCount)));
+  return run(c, workspace, workspace_bytes, stream);
 }
 
 extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N, int K, hk_bf16 alpha,
@@ -668,9 +687,12 @@ extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N
   ep.backward = true;
   ep.z = activation == HK_ACT_NONE ? nullptr : const_cast<hk_bf16*>(preact);
   ep.ldz = ldz, ep.sZ = strideZ;
-  return run(Call{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
-                  ep, C, ldc, strideC, dbias, strideDbias, accumulate != 0},
-             workspace, workspace_bytes, stream);
+  const Call c{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
+               ep, C, ldc, strideC, dbias, strideDbias, accumulate != 0};
+  HK_CHECK_ARG(outputs_apart(
+      c, hk::Rows(dbias, 4, N).along(strideDbias != 0 ? batchCount : 1, 4 * int64_t{strideDbias}),
+      memory(ep.z, M, N, ldz, strideZ, batchCount)));
+  return run(c, workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t hk_bgemm_act_workspace(int transA, int transB, int M, int N, int K, int batchCount,

@@ -459,13 +459,15 @@ HK_API hipError_t hk_bgemm_core_bias(int layout, int splitK, int M, int N, int K
  * A hidden layer h = act(x W + b) is the first with A = x, B = W; the gradient of its pre-activation the
  * second with A the gradient behind the next layer and B that layer's weights, transposed as needed.
  * Layouts, extents, leading dimensions, strides and alignment as for hk_bgemm (at most 65,535 batches,
- * M, N and K at most 2^31 - 2^16; batches of C and of a preact that is written lie apart); bf16 everywhere but dbias (fp32). Everything is fp32 until C and preact are rounded, once each: the
- * activation takes z and dbias takes d before that. bias (N elements a batch, strideBias apart, 0: one
- * for all), residual and preact (M x N like C, leading dimensions ldr and ldz) may be NULL; preact is
- * needed by hk_bgemm_act_backward unless the activation is HK_ACT_NONE. residual may be C itself, as may
- * the preact of hk_bgemm_act_backward; A and B may not overlap C, nor anything a preact that is written.
- * dbias may be NULL; strideDbias 0 sums over the batches too, else it is N at least. GELU is the tanh form, as in
- * hk_gelu_forward. Sums are in a fixed order.
+ * M, N and K at most 2^31 - 2^16); bf16 everywhere but dbias (fp32). Everything is fp32 until C and preact
+ * are rounded, once each: the activation takes z and dbias takes d before that. bias (N elements a batch,
+ * strideBias apart, 0: one for all), residual and preact (M x N like C, leading dimensions ldr and ldz) may
+ * be NULL; preact is needed by hk_bgemm_act_backward unless the activation is HK_ACT_NONE. residual may be C
+ * itself, with the same leading dimension and stride, as may the preact of hk_bgemm_act_backward. Nothing
+ * else may share memory with what a call writes (C, a preact of hk_bgemm_act, dbias), nor any two rows of
+ * that with each other: hipErrorInvalidValue.
+ * dbias may be NULL; strideDbias 0 sums over the batches too, else it is N at least. GELU is the tanh form,
+ * as in hk_gelu_forward. Sums are in a fixed order.
  * The k splits of some products and the bias gradient take device memory, hk_bgemm_act_workspace bytes
  * at most (whatever the alignment of the rows; dbias: whether one is wanted; -1 for an invalid
  * argument): at `workspace` (16-byte aligned), or, where that is NULL, in the stream's workspace. A
