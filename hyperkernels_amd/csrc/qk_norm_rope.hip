@@ -27,6 +27,7 @@
 
 #include "hk_device.h"
 #include "hk_host.h"
+#include "hk_overlap.h"
 
 namespace {
 
@@ -461,28 +462,44 @@ hipError_t check(const hk_qk_norm_rope_params* p, int type, bool backward) {
   return hipSuccess;
 }
 
-// Whether no two rows that a call writes are the same memory, nor one that the other side still reads.
-bool rows_apart(const hk_qk_norm_rope_params* p, bool backward) {
-  const int64_t stride[2][3] = {
-      {backward ? p->dq_strideB : p->qo_strideB, backward ? p->dq_strideM : p->qo_strideM,
-       backward ? p->dq_strideH : p->qo_strideH},
-      {backward ? p->dk_strideB : p->ko_strideB, backward ? p->dk_strideM : p->ko_strideM,
-       backward ? p->dk_strideH : p->ko_strideH}};
-  const int heads[2] = {p->q_heads, p->k_heads};
-  for (int i = 0; i < 2; ++i)
-    if (heads[i] > 0 && p->B > 0 && p->T > 0 &&
-        ((p->B > 1 && stride[i][0] == 0) || (p->T > 1 && stride[i][1] == 0) ||
-         (heads[i] > 1 && stride[i][2] == 0)))
-      return false;
-  if (heads[0] > 0 && heads[1] > 0 && p->B > 0 && p->T > 0) {
-    const void* oq = backward ? p->dq : p->q_out;
-    const void* ok = backward ? p->dk : p->k_out;
-    if (oq == ok || oq == p->k || ok == p->q) return false;
-    if (backward && (oq == p->dk_out || ok == p->dq_out)) return false;
+// Whether what a call writes lies apart: no two rows of it, nor one and what the call reads, share memory, but for
+// an output that is its own side's input (in the backward pass, or the gradient of its output) row by row.
+bool outputs_apart(const hk_qk_norm_rope_params* p, int type, bool backward) {
+  const int64_t ei = elem_size(type), eo = p->f32_io ? 4 : ei, d = p->head_dim;
+  auto tensor = [&](const void* t, int heads, int64_t elem, int64_t sB, int64_t sM, int64_t sH) {
+    return hk::Rows(t, elem, d).along(p->B, elem * sB).along(heads, elem * sH).along(p->T, elem * sM);
+  };
+  const hk::Rows x[2] = {tensor(p->q, p->q_heads, ei, p->q_strideB, p->q_strideM, p->q_strideH),
+                         tensor(p->k, p->k_heads, ei, p->k_strideB, p->k_strideM, p->k_strideH)};
+  const hk::Rows y[2] = {  // the outputs, or their gradients
+      tensor(backward ? p->dq_out : p->q_out, p->q_heads, eo, p->qo_strideB, p->qo_strideM, p->qo_strideH),
+      tensor(backward ? p->dk_out : p->k_out, p->k_heads, eo, p->ko_strideB, p->ko_strideM, p->ko_strideH)};
+  hk::Rows out[4] = {y[0], y[1], hk::Rows(nullptr, 4, d), hk::Rows(nullptr, 4, d)};
+  if (backward) {
+    out[0] = tensor(p->dq, p->q_heads, ei, p->dq_strideB, p->dq_strideM, p->dq_strideH);
+    out[1] = tensor(p->dk, p->k_heads, ei, p->dk_strideB, p->dk_strideM, p->dk_strideH);
+    if (p->q_heads > 0) out[2] = hk::Rows(p->dq_weight, 4, d);
+    if (p->k_heads > 0) out[3] = hk::Rows(p->dk_weight, 4, d);
   }
-  if (!backward || !p->dq_weight || !p->dk_weight || heads[0] == 0 || heads[1] == 0) return true;
-  const auto a = reinterpret_cast<uintptr_t>(p->dq_weight), b = reinterpret_cast<uintptr_t>(p->dk_weight);
-  return (a > b ? a - b : b - a) >= p->head_dim * sizeof(float);
+  const int64_t half = p->rotary_dim / 2;
+  const hk::Rows shared[5] = {
+      hk::Rows(p->q_heads > 0 ? p->q_weight : nullptr, ei, d),
+      hk::Rows(p->k_heads > 0 ? p->k_weight : nullptr, ei, d),
+      hk::Rows(half > 0 ? p->cos : nullptr, 4, half).along(p->table_rows, 4 * p->table_stride),
+      hk::Rows(half > 0 ? p->sin : nullptr, 4, half).along(p->table_rows, 4 * p->table_stride),
+      hk::Rows(half > 0 ? p->positions : nullptr, 8, p->T).along(p->B, 8 * p->pos_strideB)};
+  for (int i = 0; i < 4; ++i) {
+    if (i < 2 && hk::overlaps_itself(out[i])) return false;
+    for (int j = 0; j < i; ++j)
+      if (hk::overlap(out[i], out[j])) return false;
+    for (int j = 0; j < 2; ++j) {
+      if (i == j ? hk::overlap_unless_same(out[i], x[j]) : hk::overlap(out[i], x[j])) return false;
+      if (backward && (i == j ? hk::overlap_unless_same(out[i], y[j]) : hk::overlap(out[i], y[j]))) return false;
+    }
+    for (const hk::Rows& s : shared)
+      if (hk::overlap(out[i], s)) return false;
+  }
+  return true;
 }
 
 // Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it. 8 (16-byte
@@ -595,7 +612,7 @@ extern "C" hipError_t hk_qk_norm_rope_forward(const hk_qk_norm_rope_params* p, i
   const int v = unit_pairs(type, p->head_dim, p->rotary_dim, !p->f32_io);
   const Args g = make_args(p, v, false);
   if (g.side[0].rows + g.side[1].rows == 0) return hipSuccess;
-  HK_CHECK_ARG(rows_apart(p, false));
+  HK_CHECK_ARG(outputs_apart(p, type, false));
   return by_type(g, type, p->f32_io, v, false, stream);
 }
 
@@ -610,7 +627,7 @@ extern "C" hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* p, 
                                                void* workspace, int64_t workspace_bytes,
                                                hipStream_t stream) {
   HK_RETURN_IF_ERROR(check(p, type, true));
-  HK_CHECK_ARG(rows_apart(p, true));
+  HK_CHECK_ARG(outputs_apart(p, type, true));
   const int v = unit_pairs(type, p->head_dim, p->rotary_dim, false);
   Args g = make_args(p, v, true);
   Weights w{{nullptr, nullptr},

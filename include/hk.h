@@ -648,16 +648,18 @@ HK_API hipError_t hk_attn_backward_set(const hk_attn_bwd_params* params, int hea
  * (what the attention takes and returns). Tensors are [B, heads, T, head_dim] with any batch / row /
  * head strides (elements; last-dim stride 1) and any alignment of their element type. q and k may have
  * different numbers of heads; one of them with 0 is left out.
- * hk_qk_norm_rope_forward reads q, k and writes q_out, k_out, which may be q and k themselves.
+ * hk_qk_norm_rope_forward reads q, k and writes q_out, k_out, which may be q and k themselves (with their
+ *   strides, where the outputs are of the call's type).
  * hk_qk_norm_rope_backward reads q, k and the gradients dq_out, dk_out (strides qo_*, ko_*, like the
- *   outputs') and writes dq, dk, which may be q, k or, with f32_io unset, dq_out and dk_out themselves.
+ *   outputs') and writes dq, dk, which may be q, k or, where those are of the call's type, dq_out and dk_out
+ *   themselves (with their strides).
  *   dq_weight and dk_weight (fp32, NULL: not wanted) are written, or added to where accumulate is
- *   set, summed over tokens and heads in a fixed order; they may not overlap. The partial sums take
+ *   set, summed over tokens and heads in a fixed order. The partial sums take
  *   hk_qk_norm_rope_workspace bytes (0 where neither is wanted, -1 for invalid arguments): at
  *   `workspace`, or in the stream's workspace where that is NULL. A call that needs some and is captured
  *   into a graph brings its own, as for hk_bgemm_act.
- * No two rows that are written may be the same memory (no stride of 0 over more than one), nor may one
- * side's outputs lie on the other's inputs.
+ * Otherwise no two rows that are written may share memory, nor one with anything that the call reads (the other
+ * side, weights, tables and positions among it): hipErrorInvalidValue.
  * ---------------------------------------------------------------------------------------- */
 typedef struct hk_qk_norm_rope_params {
   const void* q;

@@ -50,3 +50,40 @@ def test_gemm_in_one_buffer(hk, M, N, K, batch):
     for a in (0, 2 * N):
         assert torch.equal(buf[:, :, a:a + N if a == 0 else a + K], before[:, :, a:a + N if a == 0 else a + K])
     assert torch.equal(buf[:, :, 3 * N + K:], before[:, :, 3 * N + K:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("H,K,d,rot", [(4, 4, 64, 64), (6, 2, 70, 50), (4, 1, 33, 32)])
+def test_queries_and_keys_of_one_projection(hk, dtype, H, K, d, rot):
+    """q, k and v as the projection has them: turned in place, and gradients into a buffer like it or in place."""
+    B, T, gen = 2, 37, _gen(2)
+    heads = (slice(0, H), slice(H, H + K), slice(H + K, H + 2 * K))
+
+    def packed():
+        buf = torch.randn(B, T, H + 2 * K, d, generator=gen, device=DEV).to(dtype)
+        return buf, *(buf[:, :, h].transpose(1, 2) for h in heads)
+
+    ang = torch.randn(T, rot // 2, generator=gen, device=DEV)
+    cs = (ang.cos(), ang.sin())
+    w = (torch.rand(2, d, generator=gen, device=DEV) + 0.5).to(dtype)
+    kw = dict(q_weight=w[0], k_weight=w[1])
+    buf, q, k, v = packed()
+    grad, gq, gk, _ = packed()
+    keep = [t.clone() for t in (q, k, v, gq, gk)]
+    want = hk.qk_norm_rope_forward(q, k, *cs, **kw)
+    dw = torch.zeros(4, d, device=DEV)
+    dwant = hk.qk_norm_rope_backward(gq, gk, q, k, *cs, grad_q_weight=dw[0], grad_k_weight=dw[1], **kw)
+    # into the parts of another projection's gradient, and over the gradients and the inputs themselves
+    dbuf, dq, dk, dv = packed()
+    held = dv.clone()
+    hk.qk_norm_rope_backward(gq, gk, q, k, *cs, grad_q_weight=dw[2], grad_k_weight=dw[3], dq=dq, dk=dk, **kw)
+    assert torch.equal(dq, dwant[0]) and torch.equal(dk, dwant[1]) and torch.equal(dv, held)
+    assert torch.equal(dw[:2], dw[2:])
+    hk.qk_norm_rope_backward(gq, gk, q, k, *cs, dq=gq, dk=gk, **kw)
+    assert torch.equal(gq, dwant[0]) and torch.equal(gk, dwant[1])
+    gq.copy_(keep[3]), gk.copy_(keep[4])
+    hk.qk_norm_rope_forward(q, k, *cs, q_out=q, k_out=k, **kw)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, keep[2])
+    q.copy_(keep[0]), k.copy_(keep[1])
+    hk.qk_norm_rope_backward(gq, gk, q, k, *cs, dq=q, dk=k, **kw)
+    assert torch.equal(q, dwant[0]) and torch.equal(k, dwant[1]) and torch.equal(v, keep[2])

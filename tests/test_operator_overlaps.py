@@ -59,3 +59,53 @@ def test_gemm_with_an_epilogue(L, bad):
     dict(sC=32), dict(batch=1, db=C + 4), dict(batch=1, db=C - 124), dict(db=C - 4 * 63, sD=32), dict(db=C - 124, sD=0)])
 def test_gradient_with_an_epilogue(L, bad):
     assert _backward(L, **bad) == INVALID
+
+
+def _qk(L, backward, kind=1, **kw):
+    """16-bit q [2, 4, 8, 64] and k [2, 2, 8, 64] by token, each tensor in memory of its own."""
+    from hyperkernels_amd.kernels import QkNormRopeParams
+
+    B, T, H, K, d = 2, 8, 4, 2, 64
+    a = dict(q=AT, k=2 * AT, q_weight=3 * AT, k_weight=4 * AT, cos=5 * AT, sin=6 * AT, positions=7 * AT, q_out=8 * AT,
+             k_out=9 * AT, dq_out=10 * AT, dk_out=11 * AT, dq=12 * AT, dk=13 * AT, dq_weight=14 * AT, dk_weight=15 * AT,
+             B=B, T=T, q_heads=H, k_heads=K, head_dim=d, rotary_dim=32, eps=1e-6, table_rows=20, table_stride=16,
+             pos_strideB=T)
+    for n, h in (("q", H), ("k", K), ("qo", H), ("ko", K), ("dq", H), ("dk", K)):
+        a |= {f"{n}_strideB": T * h * d, f"{n}_strideM": h * d, f"{n}_strideH": d}
+    p = ctypes.byref(QkNormRopeParams(**a | kw))
+    if backward:
+        return L.hk_qk_norm_rope_backward(p, kind, NULL, 0, NULL)
+    return L.hk_qk_norm_rope_forward(p, kind, NULL)
+
+
+Q, K, QO, KO, DQ, DK = AT, 2 * AT, 8 * AT, 9 * AT, 12 * AT, 13 * AT
+Q_LAST, K_LAST = 2 * (2 * 4 * 8 * 64 - 1), 2 * (2 * 2 * 8 * 64 - 1)
+DENSE = {"strideM": 64, "strideH": 8 * 64}  # [B, heads, T, d] in order
+
+
+def _as(name, strides):
+    return {f"{name}_{s}": v for s, v in strides.items()}
+
+
+@pytest.mark.parametrize("bad", [
+    # in place with other strides, or with elements of another size
+    dict(q_out=Q, **_as("qo", DENSE)), dict(k_out=K, ko_strideM=144, ko_strideB=8 * 144), dict(q_out=Q, f32_io=True),
+    dict(k_out=K, f32_io=True), dict(q_out=Q, T=4, q_heads=4, qo_strideM=64, qo_strideH=256),
+    # shifted
+    dict(q_out=Q + 2), dict(q_out=Q - 128), dict(q_out=Q + Q_LAST), dict(k_out=K + 64), dict(k_out=K - K_LAST),
+    # on the other side, on what both sides read, and on itself
+    dict(q_out=K + 4), dict(k_out=Q + Q_LAST), dict(k_out=Q), dict(k_out=QO + 64), dict(q_out=3 * AT), dict(k_out=4 * AT + 64),
+    dict(q_out=5 * AT + 1200), dict(q_out=6 * AT + 64), dict(k_out=7 * AT + 64), dict(qo_strideM=63, qo_strideH=512),
+    dict(qo_strideH=32), dict(ko_strideB=1000), dict(qo_strideM=0), dict(ko_strideH=-8)])
+def test_query_and_key_norms(L, bad):
+    assert _qk(L, False, **bad) == INVALID
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dq=Q, **_as("dq", DENSE)), dict(dq=10 * AT, **_as("dq", DENSE)), dict(dk=11 * AT, f32_io=True),
+    dict(dq=10 * AT, f32_io=True), dict(dq=Q + 2), dict(dk=11 * AT - 128), dict(dq=10 * AT + Q_LAST), dict(dq=K),
+    dict(dk=10 * AT + 64), dict(dq=11 * AT), dict(dk=DQ + 640), dict(dq_strideM=32), dict(dk_strideB=4),
+    dict(dq_weight=15 * AT - 252), dict(dq_weight=DQ + 64), dict(dk_weight=DQ + 64), dict(dk_weight=Q + 64),
+    dict(dq_weight=11 * AT + 64), dict(dq_weight=3 * AT), dict(dk_weight=5 * AT + 64), dict(dq=3 * AT), dict(dk=6 * AT)])
+def test_gradients_of_query_and_key_norms(L, bad):
+    assert _qk(L, True, **bad) == INVALID
