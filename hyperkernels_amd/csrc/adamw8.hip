@@ -28,11 +28,13 @@
 #include <math.h>
 
 #include <algorithm>
+#include <iterator>
 #include <utility>
 #include <vector>
 
 #include "hk_device.h"
 #include "hk_host.h"
+#include "hk_overlap.h"
 
 namespace {
 
@@ -406,6 +408,14 @@ extern "C" hipError_t hk_adam8_plan_create(int num_tensors, float* const* params
   writes(v_scales, 4 * blocks);
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i) HK_CHECK_ARG(written[i - 1].second <= written[i].first);
+  // nor a gradient on any of it, but on its own parameter element by element
+  const int64_t grad_bytes = grad_type == HK_TYPE_F32 ? 4 : 2;
+  for (int t = 0; t < num_tensors; ++t) {
+    if (sizes[t] == 0 || (grad_bytes == 4 && grads[t] == params[t])) continue;
+    const auto a = reinterpret_cast<uintptr_t>(grads[t]), end = a + grad_bytes * sizes[t];
+    const auto next = std::lower_bound(written.begin(), written.end(), std::make_pair(end, uintptr_t{0}));
+    HK_CHECK_ARG(next == written.begin() || std::prev(next)->second <= a);
+  }
   tensor_of.reserve(blocks);
   for (int t = 0; t < num_tensors; ++t)
     tensor_of.insert(tensor_of.end(), hk::ceil_div(sizes[t], kBlock), t);
@@ -486,6 +496,14 @@ bool conversion_holds(const void* m_codes, const void* v_codes, const float* m_s
                         static_cast<const void*>(v_scales), static_cast<const void*>(m),
                         static_cast<const void*>(v)})
     if (!p || !aligned4(p)) return false;
+  // blocks are converted in any order: all six apart
+  const int64_t blocks = hk::ceil_div(numel, kBlock);
+  const hk::Rows part[6] = {hk::Rows(m_codes, kBlock, blocks), hk::Rows(v_codes, kBlock, blocks),
+                            hk::Rows(m_scales, 4, blocks),     hk::Rows(v_scales, 4, blocks),
+                            hk::Rows(m, 4, numel),             hk::Rows(v, 4, numel)};
+  for (int i = 1; i < 6; ++i)
+    for (int j = 0; j < i; ++j)
+      if (hk::overlap(part[i], part[j])) return false;
   return true;
 }
 // Calls launch(first block, elements from there on, workgroups of four blocks) for each launch's blocks.

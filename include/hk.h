@@ -242,14 +242,15 @@ HK_API int64_t hk_adam_plan_num_chunks(const hk_adam_plan* plan);
  *   m_codes and v_codes hold HK_ADAM8_BLOCK bytes a block, m_scales and v_scales one float a block
  *   (hk_adam8_plan_num_blocks gives the count); codes behind a tensor's end are written as 0.
  *   Parameters and gradients may have any alignment of their element type, the codes need 4 bytes. No two
- *   of the arrays that a step writes (parameters, copies, states) may overlap.
+ *   of the arrays that a step writes (parameters, copies, states) may overlap, nor a gradient any of them
+ *   (but an fp32 one its own parameter, element by element).
  * hk_adam8_plan_step: on the device that was current at creation; steps of plans that share memory
  *   have to be ordered. It takes no workspace and can be captured into a graph.
  * A gradient that is not finite, or a moment past fp32, leaves the block's scales NaN, and with them
  *   all its moments from then on (the step's parameters: those of the elements themselves).
  * hk_adam8_quantize / hk_adam8_dequantize convert between fp32 moments and these states (a 32-bit run
  *   that goes on in 8 bits, a checkpoint): numel elements of whole blocks, but for the last one. v is
- *   taken as 0 where it is negative.
+ *   taken as 0 where it is negative. No two of the six arrays may overlap.
  * ---------------------------------------------------------------------------------------- */
 #define HK_ADAM8_BLOCK 256
 typedef struct hk_adam8_plan hk_adam8_plan;

@@ -109,3 +109,37 @@ def test_query_and_key_norms(L, bad):
     dict(dq_weight=11 * AT + 64), dict(dq_weight=3 * AT), dict(dk_weight=5 * AT + 64), dict(dq=3 * AT), dict(dk=6 * AT)])
 def test_gradients_of_query_and_key_norms(L, bad):
     assert _qk(L, True, **bad) == INVALID
+
+
+def _arr(*xs):
+    return (ctypes.c_void_p * len(xs))(*xs)
+
+
+@pytest.mark.parametrize("kind,grads,ok", [
+    (0, (AT + 4, 4 * AT), False), (0, (AT - 4 * 299, 4 * AT), False), (0, (3 * AT, AT + 1196), False),
+    (0, (2 * AT, 4 * AT), False), (1, (AT, 4 * AT), False), (1, (3 * AT, 4 * AT + 2), True), (0, (AT, 4 * AT), True),
+    (1, (3 * AT, 5 * AT + 600), True),  # behind the copy's 600 bytes
+    (1, (3 * AT, 5 * AT + 598), False), (1, (5 * AT - 2 * 299, 4 * AT), False), (0, (6 * AT + 508, 4 * AT), False),
+    (0, (7 * AT, 4 * AT), False), (0, (3 * AT, 8 * AT + 12), False), (2, (3 * AT, 9 * AT), False)])
+def test_gradients_on_what_a_step_writes(L, kind, grads, ok):
+    """Two tensors of 300 elements with a copy of the second; states of four blocks."""
+    plan = ctypes.c_void_p(1)
+    status = L.hk_adam8_plan_create(2, _arr(AT, 2 * AT), _arr(*grads), kind, _arr(0, 5 * AT),
+                                    (ctypes.c_int64 * 2)(300, 300), 6 * AT, 7 * AT, 8 * AT, 9 * AT,
+                                    ctypes.byref(plan))
+    assert (status != INVALID) == ok
+    if status == 0:
+        L.hk_adam8_plan_destroy(plan)
+
+
+@pytest.mark.parametrize("name", ["hk_adam8_quantize", "hk_adam8_dequantize"])
+@pytest.mark.parametrize("at", [(1, 1, 3, 4, 5, 6), (1, 2, 1, 4, 5, 6), (1, 2, 3, 2, 5, 6), (1, 2, 3, 4, 1, 6),
+                                (1, 2, 3, 4, 5, 5), (1, 2, 3, 3, 5, 6), (1, 2, 3, 4, 3, 6)])
+@pytest.mark.parametrize("shift", [0, 4])
+def test_conversions(L, name, at, shift):
+    """300 elements: fp32 moments of 1,200 bytes, codes of 512, scales of 8."""
+    m, v, a, b, c, d = (AT * x + shift * at[:i].count(x) for i, x in enumerate(at))
+    if name == "hk_adam8_quantize":
+        assert L.hk_adam8_quantize(m, v, 300, a, b, c, d, NULL) == INVALID
+    else:
+        assert L.hk_adam8_dequantize(a, b, c, d, 300, m, v, NULL) == INVALID
