@@ -510,6 +510,7 @@ def attn_backward(q, k, v, do, lse, D, causal: bool, scale: float | None = None,
 # counterpart in the reference)
 # ----------------------------------------------------------------------------------------------
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}  # HK_ACT_*
+_INT_MAX = 2 ** 31 - 1  # ctypes cuts a larger one to its low 32 bits
 
 
 def _matrix(fn: str, t: torch.Tensor, dev: int, batch: int, rows: int,
@@ -526,8 +527,10 @@ def _matrix(fn: str, t: torch.Tensor, dev: int, batch: int, rows: int,
     if t.dtype is not _BF16 or t.get_device() != dev or (st[-1] != 1 and cols > 1):
         raise ValueError(f"{fn}: bf16 matrices of one device with a unit last-dim stride")
     ld = st[-2]
-    if rows == 1 and ld < cols:
+    if rows == 1 and not cols <= ld <= _INT_MAX:
         ld = cols
+    if ld > _INT_MAX:
+        raise ValueError(f"{fn}: leading dimensions below 2^31 only")
     return t.data_ptr(), ld, step
 
 
@@ -553,8 +556,10 @@ def _product(fn: str, a, b, trans_a: bool, trans_b: bool, activation: str):
         K, M = ash[-2], ash[-1]
     else:
         M, K = ash[-2], ash[-1]
-    return (ash[0] if len(ash) == 3 else 1, M, bsh[-2] if trans_b else bsh[-1], K, act,
-            _device(fn, a))
+    batch, N = ash[0] if len(ash) == 3 else 1, bsh[-2] if trans_b else bsh[-1]
+    if max(M, N, K, batch) > _INT_MAX:
+        raise ValueError(f"{fn}: extents below 2^31 only")
+    return batch, M, N, K, act, _device(fn, a)
 
 
 def _call_captured(name: str, need, *args) -> None:

@@ -25,3 +25,24 @@ def test_adam8_sizes_past_the_blocks(L, size):
     assert plan.value is None
     assert L.hk_adam8_quantize(64, 64, size, 64, 64, 64, 64, NULL) == INVALID
     assert L.hk_adam8_dequantize(64, 64, 64, 64, size, 64, 64, NULL) == INVALID
+
+
+def test_front_end_sizes_past_int():
+    """Extents and leading dimensions that the C entry's int does not hold are not cut to one that it does."""
+    import torch
+    from hyperkernels_amd import kernels as hk
+
+    meta = lambda *s: torch.empty(*s, device="meta", dtype=torch.bfloat16)  # noqa: E731
+    big = 2 ** 32 + 8
+    for a, b, ta, tb in ((meta(big, 8), meta(8, 16), False, False), (meta(4, 8), meta(8, big), False, False),
+                         (meta(4, big), meta(big, 8), False, False), (meta(8, big), meta(8, 16), True, False),
+                         (meta(4, 8), meta(big, 8), False, True),
+                         (meta(big, 1, 8), meta(big, 8, 16), False, False)):
+        for f in (hk.bgemm_act, hk.bgemm_act_backward):
+            with pytest.raises(ValueError, match="2\\^31"):
+                f(a, b, trans_a=ta, trans_b=tb)
+    for t in (meta(4, big)[:, :16], meta(2, 4, big)[:, :, :16]):
+        with pytest.raises(ValueError, match="2\\^31"):
+            hk._matrix("f", t, -1, 1 if t.dim() == 2 else 2, 4, 16)
+    assert hk._matrix("f", meta(4, 2 ** 31 - 1)[:, :16], -1, 1, 4, 16)[1] == 2 ** 31 - 1
+    assert hk._matrix("f", meta(1, big)[:, :16], -1, 1, 1, 16)[1] == 16  # one row: any leading dimension
