@@ -149,13 +149,6 @@ __global__ __launch_bounds__(256) void bgemm_simple(int ta, int tb, int M, int N
   *dst = hk::f32_to_bf16(f);
 }
 
-float bf16_bits_to_float(hk_bf16 h) {
-  const uint32_t u = static_cast<uint32_t>(h) << 16;
-  float f;
-  __builtin_memcpy(&f, &u, 4);
-  return f;
-}
-
 // Split-K chosen by the library when the caller gives none, at most `most`: the split with the least modelled
 // time (us), summed over the rounds of 256 x 256 work items on the CUs:
 //   - a round costs (k-tiles per split) x t(busy) plus a fixed prologue / epilogue (8 us with
@@ -312,7 +305,7 @@ hipError_t bgemm_run(int transA, int transB, int M, int N, int K, hk_bf16 alpha_
     return hk::bgemv_run(!ta, M, K, alpha_bits, beta_bits, A, lda, strideA, B, tb ? 1 : ldb,
                          strideB, C, ldc, strideC, batchCount, stream);
   }
-  Epi ep{bf16_bits_to_float(alpha_bits), bf16_bits_to_float(beta_bits), bias, 0, 0, false};
+  Epi ep{hk::bf16_bits_to_float(alpha_bits), hk::bf16_bits_to_float(beta_bits), bias, 0, 0, false};
   if (bias) {
     if (bias_numel == N) ep.bcol = 1;
     else if (bias_numel == M) ep.brow = 1;

@@ -358,7 +358,6 @@ __global__ __launch_bounds__(256) void act_column_sums(const float* __restrict__
 struct Call {
   bool ta, tb;
   int M, N, K, batch;
-  hk_bf16 alpha;
   const hk_bf16* A;
   int64_t lda, sA;
   const hk_bf16* B;
@@ -418,7 +417,7 @@ Plan make_plan(const Call& c, bool may_split) {
   const bool sums = c.ep.backward && c.dbias;
   if (c.M == 1 && c.K > 0) {
     p.kind = Plan::kRow;
-    if (c.tb) p.gemv = hk::bgemv_plan(c.tb, c.N, c.K, c.batch);
+    if (c.tb) p.gemv = hk::bgemv_plan(true, c.N, c.K, c.batch);
     p.row = row_form(c, p.gemv);
     if (p.row.splits > 1)
       p.part_bytes = static_cast<size_t>(c.batch) * p.row.splits * c.N * sizeof(float);
@@ -501,7 +500,7 @@ hipError_t run_piece(Call c, void* workspace, int64_t workspace_bytes, hipStream
     const RowOut out{ep, c.C, c.sC, ep.sums ? nullptr : c.dbias, c.sD, c.accumulate ? 1 : 0};
     const bool split = p.row.splits > 1;
     if (c.tb && split) {
-      HK_RETURN_IF_ERROR(hk::bgemv_partials(c.tb, c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, c.batch,
+      HK_RETURN_IF_ERROR(hk::bgemv_partials(c.N, c.K, c.B, c.ldb, c.sB, c.A, incx, c.sA, c.batch,
                                             p.gemv, part, stream));
     } else if (c.tb) {
       hipLaunchKernelGGL(incx == 1 ? act_row_nt<true> : act_row_nt<false>,
@@ -591,13 +590,6 @@ hipError_t run(const Call& c, void* workspace, int64_t workspace_bytes, hipStrea
   return hipSuccess;
 }
 
-float bf16_value(hk_bf16 h) {
-  const uint32_t u = static_cast<uint32_t>(h) << 16;
-  float f;
-  __builtin_memcpy(&f, &u, 4);
-  return f;
-}
-
 // The arguments that both entry points share.
 hipError_t check(int transA, int transB, int M, int N, int K, const void* A, int lda, const void* B,
                  int ldb, int activation, const void* C, int ldc, long long strideC, int batchCount) {
@@ -635,12 +627,12 @@ Call forward_call(int transA, int transB, int M, int N, int K, hk_bf16 alpha, co
                   const hk_bf16* residual, int ldr, long long strideR, hk_bf16* preact, int ldz,
                   long long strideZ, hk_bf16* C, int ldc, long long strideC, int batchCount) {
   ActEpi ep{};
-  ep.alpha = bf16_value(alpha);
+  ep.alpha = hk::bf16_bits_to_float(alpha);
   ep.act = hk::make_activation(activation);
   ep.bias = bias, ep.sBias = strideBias;
   ep.residual = residual, ep.ldr = ldr, ep.sR = strideR;
   ep.z = preact, ep.ldz = ldz, ep.sZ = strideZ;
-  return Call{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
+  return Call{transA != 0, transB != 0, M, N, K, batchCount, A, lda, strideA, B, ldb, strideB,
               ep, C, ldc, strideC, nullptr, 0, false};
 }
 
@@ -682,12 +674,12 @@ extern "C" hipError_t hk_bgemm_act_backward(int transA, int transB, int M, int N
   HK_CHECK_ARG((reinterpret_cast<uintptr_t>(dbias) & 3u) == 0);
   HK_CHECK_ARG(batchCount <= 1 || strideDbias == 0 || strideDbias >= N || strideDbias <= -N);
   ActEpi ep{};
-  ep.alpha = bf16_value(alpha);
+  ep.alpha = hk::bf16_bits_to_float(alpha);
   ep.act = hk::make_activation(activation);
   ep.backward = true;
   ep.z = activation == HK_ACT_NONE ? nullptr : const_cast<hk_bf16*>(preact);
   ep.ldz = ldz, ep.sZ = strideZ;
-  const Call c{transA != 0, transB != 0, M, N, K, batchCount, alpha, A, lda, strideA, B, ldb, strideB,
+  const Call c{transA != 0, transB != 0, M, N, K, batchCount, A, lda, strideA, B, ldb, strideB,
                ep, C, ldc, strideC, dbias, strideDbias, accumulate != 0};
   HK_CHECK_ARG(outputs_apart(
       c, hk::Rows(dbias, 4, N).along(strideDbias != 0 ? batchCount : 1, 4 * int64_t{strideDbias}),

@@ -296,13 +296,6 @@ __global__ __launch_bounds__(kThreads) void gemv_finalize(int R, int batch, Out 
   emit(o, b, 0, R, r, s);
 }
 
-float bf16_bits_to_float(hk_bf16 h) {
-  const uint32_t u = static_cast<uint32_t>(h) << 16;
-  float f;
-  __builtin_memcpy(&f, &u, 4);
-  return f;
-}
-
 // k split so that (groups per split) x nsplit reaches `target`, keeping at least
 // min_k k per split; the chunk is a multiple of `align`.
 void pick_split(int64_t groups, int64_t target, int K, int min_k, int align, int* nsplit,
@@ -376,12 +369,12 @@ GemvPlan bgemv_plan(bool dot_form, int R, int K, int batch) {
   return p;
 }
 
-hipError_t bgemv_partials(bool dot_form, int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
+hipError_t bgemv_partials(int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
                           const hk_bf16* x, int64_t incx, int64_t sx, int batch,
                           const GemvPlan& plan, float* part, hipStream_t stream) {
   HK_CHECK_ARG(R > 0 && K >= 0 && batch > 0 && batch <= 65535 && part != nullptr);
   HK_CHECK_ARG(plan.nsplit >= 1 && plan.nsplit <= 65535);
-  return launch(dot_form, R, K, mtx, ld, sm, x, incx, sx, batch, plan,
+  return launch(true, R, K, mtx, ld, sm, x, incx, sx, batch, plan,
                 Out{1.0f, 0.0f, nullptr, 1, 0, part, plan.nsplit}, stream);
 }
 

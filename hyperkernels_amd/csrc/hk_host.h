@@ -48,13 +48,13 @@ hipError_t bgemv_run(bool dot_form, int R, int K, hk_bf16 alpha, hk_bf16 beta,
                      int64_t sx, hk_bf16* y, int64_t incy, int64_t sy, int batch,
                      hipStream_t stream);
 
-// The same product without its epilogue, for one of the caller's own: the sums of plan.nsplit k ranges as
-// fp32 partials part[batch][nsplit][R], to be added in split order.
+// The dot form without its epilogue, for one of the caller's own: the sums of plan.nsplit k ranges (of
+// bgemv_plan(true, ..)) as fp32 partials part[batch][nsplit][R], to be added in split order.
 struct GemvPlan {
   int nsplit, kchunk;
 };
 GemvPlan bgemv_plan(bool dot_form, int R, int K, int batch);
-hipError_t bgemv_partials(bool dot_form, int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
+hipError_t bgemv_partials(int R, int K, const hk_bf16* mtx, int64_t ld, int64_t sm,
                           const hk_bf16* x, int64_t incx, int64_t sx, int batch,
                           const GemvPlan& plan, float* part, hipStream_t stream);
 
@@ -91,6 +91,13 @@ hipError_t bgemm_partials(bool ta, bool tb, int M, int N, int K, const hk_bf16* 
                           int64_t sA, const hk_bf16* B, int64_t ldb, int64_t sB, int batch,
                           const GemmPlan& plan, float* part, const F32Out* out,
                           hipStream_t stream);
+
+inline float bf16_bits_to_float(hk_bf16 h) {
+  const uint32_t u = static_cast<uint32_t>(h) << 16;
+  float f;
+  __builtin_memcpy(&f, &u, 4);
+  return f;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
