@@ -123,7 +123,7 @@ __device__ __forceinline__ void root_units_v(uint32_t w, float (&f)[4]) {
 //   c <= t = 1/2 + sqrt(x - 1/4), and h^4 + 3/2 h^2 + 1/16 <= x when c <= t = 1/2 + sqrt(sqrt(x + 1/2) - 3/4),
 // so that the code is the whole part of t. x is off by a few parts in 10^7, t, at most 255, by less than
 // 10^-4: nearer than that to a whole number, the border itself decides, in fp64. About one block in
-// fifteen has such an element; deciding all of them that way took VALU time that the loads did not
+// eleven has such an element; deciding all of them that way took VALU time that the loads did not
 // hide (124.4 M parameters, fp32 and bf16 gradients: 375 and 366 us; so, and with 60 instructions fewer a
 // block elsewhere, 298 and 277, 6.7 and 6.3 TB/s).
 constexpr float kNear = 1e-4f;

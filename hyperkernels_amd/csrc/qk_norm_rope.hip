@@ -510,9 +510,9 @@ bool outputs_apart(const hk_qk_norm_rope_params* p, int type, bool backward) {
 // Pairs a unit holds: whole vectors of both halves of the rotated part and of what lies behind it. 8 (16-byte
 // vectors of 16-bit elements) where a row is only read and written in 16 bits; 4 where outputs are fp32
 // (stores through the caches, forward, 8 x 1024 tokens of 12 + 12 heads of 64, bf16 -> fp32: 17.5 and
-// 16.2 us; bf16 -> bf16 the other way: 11.7 and 12.6), and in the backward pass, which holds weights and
-// their gradients beside the row (110 registers a lane with 8: 25.4 us with dw, with 4 and three
-// workgroups a CU 23.9; 16 + 4 heads of 128, fp16: 46.3 and 36.8).
+// 16.2 us; bf16 -> bf16 the other way: 11.7 and 12.6; stored past them, as here, fp32 13.2 with 4, bf16 11.2 with
+// 8), and in the backward pass, which holds weights and their gradients beside the row (110 registers a lane
+// with 8: 25.4 us with dw, with 4 and three workgroups a CU 23.9; 16 + 4 heads of 128, fp16: 46.3 and 36.8).
 // Parts that are no whole vectors of 4 keep them where they are long enough for the last unit to be moved
 // back (8 x 1024 tokens, forward: 12 + 12 bf16 heads of 64 with 20 rotated 31.7 us one by one, 21.3 so; 8 + 8 of
 // 90, all rotated, 41.2 and 16.5; fp16 of 96 with 50 rotated 43.6 and 17.4; backward 36.5, 49.1 and 51.5

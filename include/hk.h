@@ -238,7 +238,8 @@ HK_API int64_t hk_adam_plan_num_chunks(const hk_adam_plan* plan);
  *   grad_type HK_TYPE_* is the gradients' element type. copies may be NULL, and so may each of its
  *   elements: otherwise the updated parameter is stored there in bf16 too (rounded to nearest even).
  *   The states of all tensors lie one behind the other, each tensor from a block's first element on:
- *   tensor t has ceil(sizes[t] / HK_ADAM8_BLOCK) blocks behind those of the tensors before it.
+ *   tensor t has ceil(sizes[t] / HK_ADAM8_BLOCK) blocks behind those of the tensors before it (2^31 - 1 in
+ *   all at most, as in a conversion).
  *   m_codes and v_codes hold HK_ADAM8_BLOCK bytes a block, m_scales and v_scales one float a block
  *   (hk_adam8_plan_num_blocks gives the count); codes behind a tensor's end are written as 0.
  *   Parameters and gradients may have any alignment of their element type, the codes need 4 bytes. No two
