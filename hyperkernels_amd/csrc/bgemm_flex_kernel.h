@@ -338,6 +338,9 @@ template <class T, bool AK, bool BKM, bool RAGGED, class E>
 hipError_t flex_launch(const FlexArgs<E>& g, int batch, hipStream_t stream) {
   constexpr size_t kLds = T::lds(RAGGED, E::kShareRows);
   static_assert(kLds <= 160 * 1024, "fits gfx950's 160 KiB of LDS");
+  const int64_t tiles = hk::ceil_div(g.M, T::BMT) * hk::ceil_div(g.N, T::BNT);
+  // a dimension of a grid has under 2^32 threads
+  HK_CHECK_ARG(tiles * T::kThreads <= UINT32_MAX && static_cast<int64_t>(batch) * g.split_k <= 65535);
   static std::once_flag once;
   static hipError_t attr_status = hipSuccess;
   std::call_once(once, [] {
@@ -346,9 +349,6 @@ hipError_t flex_launch(const FlexArgs<E>& g, int batch, hipStream_t stream) {
                                       static_cast<int>(kLds));
   });
   HK_RETURN_IF_ERROR(attr_status);
-  const int64_t tiles = hk::ceil_div(g.M, T::BMT) * hk::ceil_div(g.N, T::BNT);
-  // a dimension of a grid has under 2^32 threads
-  HK_CHECK_ARG(tiles * T::kThreads <= UINT32_MAX && static_cast<int64_t>(batch) * g.split_k <= 65535);
   FlexArgs<E> a = g;
   a.by_matrix = batch > 1 && tiles * batch * g.split_k <= INT32_MAX;
   hipLaunchKernelGGL((bgemm_flex<T, AK, BKM, RAGGED, E>),

@@ -46,3 +46,12 @@ def test_front_end_sizes_past_int():
             hk._matrix("f", t, -1, 1 if t.dim() == 2 else 2, 4, 16)
     assert hk._matrix("f", meta(4, 2 ** 31 - 1)[:, :16], -1, 1, 4, 16)[1] == 2 ** 31 - 1
     assert hk._matrix("f", meta(1, big)[:, :16], -1, 1, 1, 16)[1] == 16  # one row: any leading dimension
+
+
+@pytest.mark.parametrize("M,N,tb", [(2 ** 30 + 72, 8, 0), (8, 2 ** 30 + 72, 1)])
+def test_plain_products_of_tiles_past_one_launch(L, M, N, tb):
+    """Rows of 9 elements take the tiles for any alignment: 2^24 of them and two more, of 256 threads."""
+    K = 9
+    assert L.hk_bgemm_small_tile(0, tb, M, N, K, 1, 0) == 64
+    assert L.hk_bgemm(0, tb, M, N, K, 0x3F80, 64, K, 0, 1 << 40, K if tb else N, 0, 0, 1 << 41, N, 0, 1,
+                      NULL) == INVALID
