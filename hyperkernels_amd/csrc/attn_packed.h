@@ -1,0 +1,368 @@
+// attn_packed.h - device pieces shared by the packed 16-bit attention kernels (attn_packed_fwd.hip,
+// attn_packed_bwd.hip): which rows a workgroup owns, the LDS layout of a tile and the matrix products.
+//
+// Sequence s has queries cu_q[s] .. cu_q[s + 1] and keys cu_k[s] .. cu_k[s + 1]. The `group` query heads that share
+// one key head are taken together: row r of (sequence, key head) is query r / group of head r % group, so a tile
+// of rows reads each key once whatever the group is, and a single token of a large group still fills a tile.
+#pragma once
+
+#include <math.h>
+
+#include <atomic>
+
+#include "hk_device.h"
+#include "hk_host.h"
+#include "hk_overlap.h"
+
+namespace hk {
+namespace packed {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+#define HK_LDS __attribute__((address_space(3)))
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// The element types: the product of 32 x 16 and 16 x 32 (lane l of A holds row l % 32 and k = 8 (l / 32) .. + 7, of B
+// column l % 32 and the same k; element i of C is row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32), and the
+// rounding of two fp32 values (to nearest even).
+struct TypeBF16 {
+  using format = BF16;
+  static __device__ __forceinline__ f32x16_t mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x, y}, bf16x2_t));
+  }
+  static __device__ __forceinline__ f32x2_t unpack(uint32_t w) {
+    return f32x2_t{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+  }
+};
+struct TypeF16 {
+  using format = F16;
+  static __device__ __forceinline__ f32x16_t mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x, y}, f16x2_t));
+  }
+  static __device__ __forceinline__ f32x2_t unpack(uint32_t w) {
+    return __builtin_convertvector(__builtin_bit_cast(f16x2_t, w), f32x2_t);
+  }
+};
+
+// A tensor [tokens, heads, head_dim]: strides in bytes.
+struct Tensor {
+  char* p;
+  int64_t m, h;
+};
+
+struct Args {
+  Tensor q, k, v, o, dout, dq, dk, dv;
+  float* lse;
+  int64_t lse_stride;  // elements between heads
+  const int32_t *cu_q, *cu_k;
+  int64_t q_tokens, k_tokens;
+  int n, group, k_heads, d;  // sequences, query heads a key head, key heads, elements a head
+  int causal;
+  float scale;
+  int tiles;   // slots of row (or key) tiles, all sequences
+  int splits;  // shares of a tile's loop, each with partial results of its own
+  float* part;   // partial results
+  float2* stat;  // forward: (max, sum) of them
+  float* delta;  // backward: rowsum(dout * o), [q head][token]
+};
+
+__host__ __device__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
+  return x < lo ? lo : x > hi ? hi : x;
+}
+
+// Tiles of B rows, `group` rows a token: slot floor(cu[s] group / B) + s is the first of sequence s, which leaves
+// every sequence the tiles it needs (and at most one more) without a table of lengths: the grid goes by the number of
+// tokens and sequences alone, so nothing about the lengths has to be known on the host.
+__host__ __device__ inline int64_t slots(int64_t tokens, int n, int group, int B) {
+  return tokens * group / B + n;
+}
+
+struct Seq {
+  int64_t q0, k0;  // first query and key
+  int mq, mk;      // how many of them
+  int tile;        // the workgroup's tile of this sequence
+};
+
+// The sequence of slot x: the last one that begins at it or before, 64 candidates a step. Starts outside 0 .. tokens
+// count as the nearer of both and lengths under 0 as 0, so whatever cu holds the rows are some of the tensor.
+__device__ __forceinline__ bool find_tile(const int32_t* cu, int64_t tokens, const Args& a, int group, int B,
+                                          int x, Seq& s) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = a.n;
+  do {
+    const int step = (hi - lo + 63) >> 6;
+    const int i = lo + lane * step;
+    const bool before = i < hi && clamp64(cu[i < hi ? i : lo], 0, tokens) * group / B + i <= x;
+    const int count = __popcll(__ballot(before));
+    if (count == 0) return false;
+    lo += (count - 1) * step;
+    hi = min(hi, lo + step);
+  } while (hi - lo > 1);
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int64_t q0 = clamp64(a.cu_q[lo], 0, a.q_tokens), q1 = clamp64(a.cu_q[lo + 1], q0, a.q_tokens);
+  const int64_t k0 = clamp64(a.cu_k[lo], 0, a.k_tokens), k1 = clamp64(a.cu_k[lo + 1], k0, a.k_tokens);
+  s.q0 = q0, s.mq = static_cast<int>(q1 - q0);
+  s.k0 = k0, s.mk = static_cast<int>(k1 - k0);
+  const int64_t first = cu == a.cu_q ? q0 : k0;
+  s.tile = x - static_cast<int>(first * group / B + lo);
+  return s.tile >= 0;
+}
+
+// LDS tile: rows of D elements (2 D bytes) as they lie in memory, the 16-byte chunk c of row r at chunk c ^ swz(r).
+// gfx950's LDS serves 256 bytes a cycle over 64 banks: 16 lanes of a 16-byte read, which here take 16 consecutive
+// rows at one chunk, and 32 lanes of a transposing read, which take 4 consecutive rows by 4 consecutive chunks; both
+// cover the banks once, so one copy of a tile serves the products over its columns and those over its rows.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+template <int D>
+__device__ __forceinline__ int at_chunk(int r, int c) {
+  return r * (2 * D) + ((c ^ swz<D>(r)) << 4);
+}
+
+// 16 bytes a lane from memory into LDS (1 KiB a wave at lds_addr + 16 lane), past the registers. In asm, so that the
+// compiler does not wait for every copy before each LDS read: the kernel waits (vmcnt) before the barrier that
+// publishes a tile. m0 is an input operand; an SGPR base just written by a VALU needs 5 wait states, which the
+// compiler's own checks do not add inside asm.
+__device__ __forceinline__ void copy16_to_lds(const void* sbase, int voff, unsigned lds_addr) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_addr));
+}
+__device__ __forceinline__ void copy16_to_lds(const void* addr, unsigned lds_addr) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "{m0}"(lds_addr));
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Copies of N consecutive tokens of one head by 4 waves. Rows behind the sequence's last and chunks behind the
+// head's last element read the last one: they stay inside the sequence, and what they meet is masked (rows) or
+// zero on the other side of the product (columns of queries) or not stored (columns of values).
+template <int D, int N>
+struct KeyCopy {
+  static constexpr int kChunks = D / 8, kRows = 64 / kChunks;  // rows a wave and instruction
+  static constexpr int kCopies = N / (4 * kRows);              // instructions a wave
+  int row, chunk16[kCopies];
+  __device__ KeyCopy(int wave, int lane, int d) {
+    row = wave * kRows + lane / kChunks;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      chunk16[i] = 16 * min((lane % kChunks) ^ swz<D>(row + 4 * kRows * i), d / 8 - 1);
+  }
+  // base: token 0 of the tile; last: the sequence's last token as the tile counts
+  __device__ void operator()(const char* base, int stride, int last, int wave, unsigned lds) const {
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      copy16_to_lds(base, min(row + 4 * kRows * i, last) * stride + chunk16[i],
+                    lds + 1024 * (wave + 4 * i));
+  }
+};
+
+// Lane offsets of a tile's reads. rows(): 16 bytes of row r at 8 (2 s + lane / 32) elements, the operand of a product
+// over columns. cols(): the operand of a product over rows, elements 0 .. 3 of rows R + 4 h + {0 .. 3} and 4 .. 7 of
+// rows R + 8 + 4 h + {0 .. 3} (h = lane / 32) at column 32 b + lane % 32: the order in which a C block's column holds
+// its rows, so that block's values are the other operand as they are.
+template <int D>
+struct Reads {
+  int row[D / 16];
+  int col[2][D / 32];
+  __device__ explicit Reads(int lane) {
+    const int c = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) row[s] = at_chunk<D>(c, 2 * s + h);
+    // within each 16 lanes, lane j reads 4 elements of row j / 4 at columns 4 (j % 4)
+    const int j = lane & 15, x = 16 * ((lane >> 4) & 1) + 4 * (j & 3);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+        col[e][b] = at_chunk<D>(8 * e + 4 * h + (j >> 2), 4 * b + (x >> 3)) + 2 * (x & 7);
+  }
+  __device__ __forceinline__ s16x8_t rows(const char HK_LDS* tile, int first, int s) const {
+    return *reinterpret_cast<const s16x8_t HK_LDS*>(tile + first * (2 * D) + row[s]);
+  }
+  __device__ __forceinline__ s16x8_t cols(const char HK_LDS* tile, int first, int b) const {
+    const char HK_LDS* p = tile + first * (2 * D);
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t HK_LDS*)(p + col[0][b]));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4_t HK_LDS*)(p + col[1][b]));
+    return s16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+};
+
+// A row's operand of a product over columns from memory: element s is columns 16 s + 8 h .. + 7, zero behind d.
+template <int D>
+__device__ __forceinline__ void load_row(const char* p, int h, int d, s16x8_t (&x)[D / 16]) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    const int c = 16 * s + 8 * h;
+    x[s] = c < d ? *reinterpret_cast<const s16x8_t*>(p + 2 * c) : s16x8_t{};
+  }
+}
+
+// P of two 16-row halves of a C block as operands.
+template <class T>
+__device__ __forceinline__ void pack_block(const f32x16_t& p, s16x8_t (&x)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = T::pack(p[8 * s + 2 * i], p[8 * s + 2 * i + 1]);
+    x[s] = __builtin_bit_cast(s16x8_t, w);
+  }
+}
+
+// Stores a lane's column of a C block set (32 b + 8 (i / 4) + 4 h + i % 4 of row r, elements < d) times f.
+template <class T, int D>
+__device__ __forceinline__ void store_row(char* p, int h, int d, const f32x16_t (&o)[D / 32], float f) {
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * b + 8 * g + 4 * h;
+      if (c < d)
+        *reinterpret_cast<u32x2_t*>(p + 2 * c) = u32x2_t{T::pack(o[b][4 * g] * f, o[b][4 * g + 1] * f),
+                                                         T::pack(o[b][4 * g + 2] * f, o[b][4 * g + 3] * f)};
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+// Shapes, strides and pointers of a call. Keys' strides are bounded so that a tile's offsets fit 32 bits.
+inline hipError_t check(const hk_attn_packed_params* p, int type, bool backward) {
+  HK_CHECK_ARG(p != nullptr && (type == HK_TYPE_BF16 || type == HK_TYPE_F16));
+  HK_CHECK_ARG(p->num_seqs >= 0 && p->q_tokens >= 0 && p->k_tokens >= 0);
+  HK_CHECK_ARG(p->k_heads >= 1 && p->q_heads >= 1 && p->q_heads % p->k_heads == 0);
+  HK_CHECK_ARG(p->head_dim >= 8 && p->head_dim <= 128 && p->head_dim % 8 == 0);
+  HK_CHECK_ARG(p->scale > 0.f && p->scale < INFINITY);
+  constexpr int64_t kMost = INT32_MAX / 2;  // rows and keys are counted in 32 bits, a tile's worth behind the last
+  HK_CHECK_ARG(p->q_tokens <= kMost / p->q_heads && p->k_tokens <= kMost);
+  // workgroups of one launch: 2^32 threads are more than it takes
+  constexpr int64_t kGrid = int64_t(1) << 23;
+  HK_CHECK_ARG((slots(p->q_tokens, p->num_seqs, p->q_heads / p->k_heads, 32)) <= kGrid / p->k_heads);
+  HK_CHECK_ARG(slots(p->k_tokens, p->num_seqs, 1, 128) <= kGrid / p->k_heads);
+  if (p->num_seqs == 0) return hipSuccess;
+  HK_CHECK_ARG(p->cu_q && p->cu_k && (reinterpret_cast<uintptr_t>(p->cu_q) & 3) == 0 &&
+               (reinterpret_cast<uintptr_t>(p->cu_k) & 3) == 0);
+  auto tensor = [](const void* t, int64_t m, int64_t h) {
+    constexpr int64_t kStride = int64_t(1) << 40;
+    return t && aligned16(t) && m >= 0 && h >= 0 && m % 8 == 0 && h % 8 == 0 && m < kStride && h < kStride;
+  };
+  auto keys = [&](const void* t, int64_t m, int64_t h) { return tensor(t, m, h) && m <= (int64_t(1) << 23); };
+  if (p->q_tokens > 0) {
+    HK_CHECK_ARG(tensor(p->q, p->q_strideM, p->q_strideH) && tensor(p->o, p->o_strideM, p->o_strideH));
+    HK_CHECK_ARG((reinterpret_cast<uintptr_t>(p->lse) & 3) == 0 && (!backward || p->lse));
+    HK_CHECK_ARG(!p->lse || p->lse_strideH >= 0);
+    HK_CHECK_ARG(!backward || (tensor(p->dout, p->do_strideM, p->do_strideH) &&
+                               tensor(p->dq, p->dq_strideM, p->dq_strideH)));
+  }
+  if (p->k_tokens > 0) {
+    HK_CHECK_ARG(keys(p->k, p->k_strideM, p->k_strideH) && keys(p->v, p->v_strideM, p->v_strideH));
+    HK_CHECK_ARG(!backward || (tensor(p->dk, p->dk_strideM, p->dk_strideH) &&
+                               tensor(p->dv, p->dv_strideM, p->dv_strideH)));
+  }
+  return hipSuccess;
+}
+
+// Whether what a call writes shares no memory with anything else of it.
+inline bool outputs_apart(const hk_attn_packed_params* p, bool backward) {
+  auto rows = [&](const void* t, int64_t tokens, int heads, int64_t m, int64_t h) {
+    return Rows(tokens > 0 ? t : nullptr, 2, p->head_dim).along(heads, 2 * h).along(tokens, 2 * m);
+  };
+  const int64_t tq = p->q_tokens, tk = p->k_tokens;
+  const Rows lse = Rows(p->lse, 4, tq).along(p->q_heads, 4 * p->lse_strideH);
+  const Rows o = rows(p->o, tq, p->q_heads, p->o_strideM, p->o_strideH);
+  const Rows in[7] = {rows(p->q, tq, p->q_heads, p->q_strideM, p->q_strideH),
+                      rows(p->k, tk, p->k_heads, p->k_strideM, p->k_strideH),
+                      rows(p->v, tk, p->k_heads, p->v_strideM, p->v_strideH),
+                      Rows(p->cu_q, 4, p->num_seqs + 1),
+                      Rows(p->cu_k, 4, p->num_seqs + 1),
+                      backward ? rows(p->dout, tq, p->q_heads, p->do_strideM, p->do_strideH) : Rows(nullptr, 2, 1),
+                      backward ? lse : Rows(nullptr, 4, 1)};
+  const Rows out[3] = {backward ? rows(p->dq, tq, p->q_heads, p->dq_strideM, p->dq_strideH) : o,
+                       backward ? rows(p->dk, tk, p->k_heads, p->dk_strideM, p->dk_strideH) : lse,
+                       backward ? rows(p->dv, tk, p->k_heads, p->dv_strideM, p->dv_strideH) : Rows(nullptr, 2, 1)};
+  for (int i = 0; i < 3; ++i) {
+    if (overlaps_itself(out[i]) || (backward && overlap(out[i], o))) return false;
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return false;
+    for (const Rows& x : in)
+      if (overlap(out[i], x)) return false;
+  }
+  return true;
+}
+
+inline Args make_args(const hk_attn_packed_params* p) {
+  Args a{};
+  auto t = [](const void* x, int64_t m, int64_t h) {
+    return Tensor{static_cast<char*>(const_cast<void*>(x)), 2 * m, 2 * h};
+  };
+  a.q = t(p->q, p->q_strideM, p->q_strideH), a.k = t(p->k, p->k_strideM, p->k_strideH);
+  a.v = t(p->v, p->v_strideM, p->v_strideH), a.o = t(p->o, p->o_strideM, p->o_strideH);
+  a.dout = t(p->dout, p->do_strideM, p->do_strideH), a.dq = t(p->dq, p->dq_strideM, p->dq_strideH);
+  a.dk = t(p->dk, p->dk_strideM, p->dk_strideH), a.dv = t(p->dv, p->dv_strideM, p->dv_strideH);
+  a.lse = p->lse, a.lse_stride = p->lse_strideH;
+  a.cu_q = p->cu_q, a.cu_k = p->cu_k;
+  a.q_tokens = p->q_tokens, a.k_tokens = p->k_tokens;
+  a.n = p->num_seqs, a.group = p->q_heads / p->k_heads, a.k_heads = p->k_heads, a.d = p->head_dim;
+  a.causal = p->is_causal ? 1 : 0;
+  a.scale = p->scale;
+  return a;
+}
+
+int64_t forward_workspace(const hk_attn_packed_params* p);
+
+// The workspace of a call: the caller's, or the stream's.
+inline hipError_t workspace(int64_t need, void* given, int64_t given_bytes, hipStream_t stream, void** out) {
+  *out = given;
+  if (need == 0) return hipSuccess;
+  if (given) {
+    HK_CHECK_ARG(given_bytes >= need && aligned16(given));
+    return hipSuccess;
+  }
+  // a graph would keep the stream's workspace, which other graphs and eager calls write too
+  if (stream_capturing(stream)) return hipErrorStreamCaptureUnsupported;
+  return device_workspace(static_cast<size_t>(need), stream, out);
+}
+
+// Launches one kernel, whose LDS is past the 64 KiB that need no asking.
+template <auto Kernel, int kLds>
+hipError_t launch(dim3 grid, const Args& a, hipStream_t stream) {
+  if constexpr (kLds > 0) {
+    static std::atomic<uint64_t> asked;  // a bit a device
+    int dev = 0;
+    HK_RETURN_IF_ERROR(hipGetDevice(&dev));
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev > 63 || !(asked.load(std::memory_order_relaxed) & bit)) {
+      HK_RETURN_IF_ERROR(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+      asked.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  hipLaunchKernelGGL(Kernel, grid, dim3(256), kLds, stream, a);
+  return launch_status();
+}
+
+}  // namespace packed
+}  // namespace hk

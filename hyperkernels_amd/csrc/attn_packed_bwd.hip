@@ -1,0 +1,396 @@
+// attn_packed_bwd.hip - the gradients of packed 16-bit attention (attn_packed_fwd.hip): with p = exp(s - lse),
+// dp = dout v^T, delta = rowsum(dout * o) and ds = p (dp - delta),
+//   dv = p^T dout,  dq = scale ds k,  dk = scale ds^T q.
+//
+// Two kernels, each of which owns what it writes, so nothing is added atomically and every sum has a fixed order; that
+// forms s and dp twice (seven products instead of five). attn_packed_dq goes by rows like the forward (S^T = K Q^T and
+// dP^T = V dO^T with a row a lane, dS^T the operand of dQ^T += K^T dS^T as it lies) and leaves delta and lse for
+// attn_packed_dkv, which goes by keys: S = Q K^T and dP = dO V^T with a key a lane, P and dS the operands of
+// dV^T += dO^T P and dK^T += Q^T dS as they lie. The rows of a group's heads are one loop there, which sums them.
+// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32.
+#include "attn_packed.h"
+
+namespace hk {
+namespace packed {
+
+template <int D, int KG>
+struct DqShape {
+  static constexpr int kRows = 128 / KG;
+  static constexpr int kKeys = KG == 1 ? 64 : 128;
+  static constexpr int kBlocks = kKeys / KG / 32;
+  static constexpr int kTile = kKeys * D * 2;
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kPitch = D + 4;
+  static constexpr int kExchange = KG == 1 ? 0 : 4 * 32 * kPitch * 4;
+  static constexpr int kLds = 2 * kStage > kExchange ? 2 * kStage : kExchange;
+};
+
+template <class T, int D, int KG>
+__global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_dq(Args a) {
+  using S = DqShape<D, KG>;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  char HK_LDS* const lds = (char HK_LDS*)lds_raw;
+
+  const int item = blockIdx.x / a.k_heads, kh = blockIdx.x - item * a.k_heads;
+  Seq q;
+  if (!find_tile(a.cu_q, a.q_tokens, a, a.group, S::kRows, a.tiles - 1 - item, q)) return;
+  const int rows = q.mq * a.group, r0 = q.tile * S::kRows;
+  if (r0 >= rows) return;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 31, h = lane >> 5;
+  const int kg = KG == 1 ? 0 : wave, w0 = KG == 1 ? r0 + 32 * wave : r0;
+  const int row = w0 + c, rr = min(row, rows - 1);
+  const int tok = rr / a.group, qh = kh * a.group + rr - tok * a.group;
+  const int ahead = q.mk - q.mq;
+  const int lim = a.causal ? tok + ahead : q.mk - 1;
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lim);
+  const int lim_hi = __builtin_amdgcn_readlane(lim, 31);
+  const int last_tok = min(r0 + S::kRows, rows) - 1;
+  const int end = a.causal ? min(q.mk, last_tok / a.group + ahead + 1) : q.mk;
+  const int t1 = end > 0 ? (end + S::kKeys - 1) / S::kKeys : 0;
+
+  const char* kb = a.k.p + q.k0 * a.k.m + kh * a.k.h;
+  const char* vb = a.v.p + q.k0 * a.v.m + kh * a.v.h;
+  const KeyCopy<D, S::kKeys> copy(wave, lane, a.d);
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds));
+  auto fetch = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * S::kStage;
+    const int64_t at = static_cast<int64_t>(t) * S::kKeys;
+    const int last = q.mk - 1 - t * S::kKeys;
+    copy(kb + at * a.k.m, static_cast<int>(a.k.m), last, wave, to);
+    copy(vb + at * a.v.m, static_cast<int>(a.v.m), last, wave, to + S::kTile);
+  };
+  if (t1 > 0) fetch(0);
+
+  s16x8_t qx[D / 16], gx[D / 16];
+  float delta = 0.f, lse2;
+  {
+    const int64_t at = q.q0 + tok;
+    load_row<D>(a.q.p + at * a.q.m + qh * a.q.h, h, a.d, qx);
+    load_row<D>(a.dout.p + at * a.dout.m + qh * a.dout.h, h, a.d, gx);
+    const float lse = a.lse[qh * a.lse_stride + at];
+    // a row that sees nothing has exponentials of 0
+    lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    s16x8_t ox[D / 16];
+    load_row<D>(a.o.p + at * a.o.m + qh * a.o.h, h, a.d, ox);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const u32x4_t x = __builtin_bit_cast(u32x4_t, ox[s]), y = __builtin_bit_cast(u32x4_t, gx[s]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2_t u = T::unpack(x[i]), w = T::unpack(y[i]);
+        delta += u[0] * w[0] + u[1] * w[1];
+      }
+    }
+    delta = half32_reduce(delta, AddOp{});
+    if (kg == 0 && h == 0 && row < rows) {
+      float* st = a.delta + qh * a.q_tokens + at;
+      st[0] = delta;
+      st[static_cast<int64_t>(a.k_heads) * a.group * a.q_tokens] = lse2;
+    }
+  }
+
+  const Reads<D> rd(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16_t dq[D / 32];
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b) dq[b] = f32x16_t{};
+
+  for (int t = 0; t < t1; ++t) {
+    wait_copies();
+    barrier();
+    if (t + 1 < t1) fetch(t + 1);
+    const int key0 = t * S::kKeys + 32 * S::kBlocks * kg;
+    const char HK_LDS* kt = lds + (t & 1) * S::kStage + 32 * S::kBlocks * kg * (2 * D);
+    const char HK_LDS* vt = kt + S::kTile;
+#pragma unroll
+    for (int n = 0; n < S::kBlocks; ++n) {
+      if (key0 + 32 * n > lim_hi) break;
+      f32x16_t s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s = T::mfma(rd.rows(kt, 32 * n, i), qx[i], s);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dp = T::mfma(rd.rows(vt, 32 * n, i), gx[i], dp);
+      if (key0 + 32 * n + 31 > lim_lo) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3) > lim) s[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, -lse2)) * (dp[i] - delta);
+      s16x8_t ds[2];
+      pack_block<T>(s, ds);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) dq[b] = T::mfma(rd.cols(kt, 32 * n + 16 * e, b), ds[e], dq[b]);
+    }
+  }
+
+  if constexpr (KG > 1) {
+    float HK_LDS* ex = (float HK_LDS*)lds;
+    wait_copies();
+    barrier();
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t HK_LDS*>(ex + (32 * wave + c) * S::kPitch + 32 * b + 8 * g + 4 * h) =
+            f32x4_t{dq[b][4 * g], dq[b][4 * g + 1], dq[b][4 * g + 2], dq[b][4 * g + 3]};
+    __syncthreads();
+    const int er = 8 * wave + (lane >> 3), e0 = lane & 7;
+    if (r0 + er >= rows) return;
+    const int et = (r0 + er) / a.group, eh = kh * a.group + (r0 + er) - et * a.group;
+    char* op = a.dq.p + (q.q0 + et) * a.dq.m + eh * a.dq.h;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      const int col = 32 * u + 4 * e0;
+      f32x4_t x = {};
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        x += *reinterpret_cast<const f32x4_t HK_LDS*>(ex + (32 * g + er) * S::kPitch + col);
+      x *= a.scale;
+      if (col < a.d)
+        *reinterpret_cast<u32x2_t*>(op + 2 * col) = u32x2_t{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+    }
+    return;
+  }
+  if (row >= rows) return;
+  store_row<T, D>(a.dq.p + (q.q0 + tok) * a.dq.m + qh * a.dq.h, h, a.d, dq, a.scale);
+}
+
+template <int D>
+struct DkvShape {
+  static constexpr int kKeys = 128;
+  static constexpr int kRows = 64;  // rows a tile
+  static constexpr int kTile = kRows * D * 2;
+  static constexpr int kStage = 2 * kTile + 2 * kRows * 4;  // Q, dO, lse, delta
+  static constexpr int kLds = 2 * kStage;
+};
+
+__device__ __forceinline__ void copy4_to_lds(const void* addr, unsigned lds_addr) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(addr), "{m0}"(lds_addr));
+}
+
+template <class T, int D, bool SPLIT>
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_packed_dkv(Args a) {
+  using S = DkvShape<D>;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  char HK_LDS* const lds = (char HK_LDS*)lds_raw;
+
+  // under the causal mask the first keys meet the most rows: they go first
+  const int item = blockIdx.x / a.k_heads, kh = blockIdx.x - item * a.k_heads;
+  Seq q;
+  if (!find_tile(a.cu_k, a.k_tokens, a, 1, S::kKeys, item, q)) return;
+  const int k0 = q.tile * S::kKeys;
+  if (k0 >= q.mk) return;
+  const int rows = q.mq * a.group, ahead = q.mk - q.mq;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 31, h = lane >> 5;
+  const int kw = k0 + 32 * wave, key = kw + c, kk = min(key, q.mk - 1);
+  // key j is seen by queries from j - ahead on: rows from group times that on
+  auto first_row = [&](int j) { return a.causal ? min(max(j - ahead, 0) * a.group, rows) : 0; };
+  const int from = first_row(kk);
+  const int from_lo = __builtin_amdgcn_readfirstlane(from), from_hi = __builtin_amdgcn_readlane(from, 31);
+
+  int t0 = first_row(k0) / S::kRows, t1 = (rows + S::kRows - 1) / S::kRows;
+  if (SPLIT) {
+    const int per = (t1 - t0 + a.splits - 1) / a.splits;
+    t0 += blockIdx.y * per;
+    t1 = min(t1, t0 + per);
+  }
+
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds));
+  constexpr int kChunks = D / 8, kCopyRows = 64 / kChunks, kCopies = S::kRows / (4 * kCopyRows);
+  const int64_t heads = static_cast<int64_t>(a.k_heads) * a.group;
+  auto fetch = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * S::kStage;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int lr = (wave + 4 * i) * kCopyRows + lane / kChunks;
+      const int r = min(t * S::kRows + lr, rows - 1);
+      const int tok = r / a.group, qh = kh * a.group + r - tok * a.group;
+      const int ch = 16 * min((lane % kChunks) ^ swz<D>(lr), a.d / 8 - 1);
+      copy16_to_lds(a.q.p + (q.q0 + tok) * a.q.m + qh * a.q.h + ch, to + 1024 * (wave + 4 * i));
+      copy16_to_lds(a.dout.p + (q.q0 + tok) * a.dout.m + qh * a.dout.h + ch,
+                    to + S::kTile + 1024 * (wave + 4 * i));
+    }
+    if (wave < 2) {
+      const int r = min(t * S::kRows + lane, rows - 1);
+      const int tok = r / a.group, qh = kh * a.group + r - tok * a.group;
+      copy4_to_lds(a.delta + (wave * heads + qh) * a.q_tokens + q.q0 + tok, to + 2 * S::kTile + 256 * wave);
+    }
+  };
+  if (t0 < t1) fetch(t0);
+
+  s16x8_t kx[D / 16], vx[D / 16];
+  load_row<D>(a.k.p + (q.k0 + kk) * a.k.m + kh * a.k.h, h, a.d, kx);
+  load_row<D>(a.v.p + (q.k0 + kk) * a.v.m + kh * a.v.h, h, a.d, vx);
+  const Reads<D> rd(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16_t dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b) dk[b] = dv[b] = f32x16_t{};
+
+  for (int t = t0; t < t1; ++t) {
+    wait_copies();
+    barrier();
+    if (t + 1 < t1) fetch(t + 1);
+    const char HK_LDS* qt = lds + (t & 1) * S::kStage;
+    const char HK_LDS* gt = qt + S::kTile;
+    const float HK_LDS* dl = (const float HK_LDS*)(gt + S::kTile);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r0 = t * S::kRows + 32 * n;
+      if (r0 + 31 < from_lo) continue;  // none of these rows sees the wave's keys
+      f32x16_t s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s = T::mfma(rd.rows(qt, 32 * n, i), kx[i], s);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dp = T::mfma(rd.rows(gt, 32 * n, i), vx[i], dp);
+      if (r0 < from_hi || r0 + 32 > rows) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
+          if (r < from || r >= rows) s[i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t de = *reinterpret_cast<const f32x4_t HK_LDS*>(dl + 32 * n + 8 * g + 4 * h);
+        const f32x4_t ls = *reinterpret_cast<const f32x4_t HK_LDS*>(dl + 64 + 32 * n + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], sc, -ls[e]));
+          dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - de[e]);
+        }
+      }
+      s16x8_t p[2], ds[2];
+      pack_block<T>(s, p);
+      pack_block<T>(dp, ds);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) dv[b] = T::mfma(rd.cols(gt, 32 * n + 16 * e, b), p[e], dv[b]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) dk[b] = T::mfma(rd.cols(qt, 32 * n + 16 * e, b), ds[e], dk[b]);
+    }
+  }
+  if (key >= q.mk) return;
+  if constexpr (SPLIT) {
+    float* p = a.part + ((static_cast<int64_t>(blockIdx.y) * a.k_heads + kh) * a.k_tokens + q.k0 + key) * (2 * D);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = 32 * b + 8 * g + 4 * h;
+        *reinterpret_cast<f32x4_t*>(p + at) =
+            f32x4_t{dk[b][4 * g], dk[b][4 * g + 1], dk[b][4 * g + 2], dk[b][4 * g + 3]};
+        *reinterpret_cast<f32x4_t*>(p + D + at) =
+            f32x4_t{dv[b][4 * g], dv[b][4 * g + 1], dv[b][4 * g + 2], dv[b][4 * g + 3]};
+      }
+    return;
+  }
+  store_row<T, D>(a.dk.p + (q.k0 + key) * a.dk.m + kh * a.dk.h, h, a.d, dk, a.scale);
+  store_row<T, D>(a.dv.p + (q.k0 + key) * a.dv.m + kh * a.dv.h, h, a.d, dv, 1.f);
+}
+
+// Sums the shares of dk and dv in order: D / 2 lanes a key and key head, four elements of both a lane.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_packed_dkv_join(Args a) {
+  constexpr int kLanes = D / 2;
+  const int64_t keys = a.k_tokens * a.k_heads;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (i >= keys) return;
+  const int kh = static_cast<int>(i / a.k_tokens);
+  const int64_t tok = i - kh * a.k_tokens;
+  if (tok < a.cu_k[0] || tok >= a.cu_k[a.n]) return;
+  const int col = 4 * (threadIdx.x % kLanes);  // dk, then dv
+  f32x4_t x = {};
+  for (int s = 0; s < a.splits; ++s)
+    x += *reinterpret_cast<const f32x4_t*>(a.part + (s * keys + i) * (2 * D) + col);
+  const bool is_dk = col < D;
+  const int at = is_dk ? col : col - D;
+  if (at >= a.d) return;
+  if (is_dk) x *= a.scale;
+  const Tensor& t = is_dk ? a.dk : a.dv;
+  *reinterpret_cast<u32x2_t*>(t.p + tok * t.m + kh * t.h + 2 * at) =
+      u32x2_t{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+namespace {
+
+struct Plan {
+  int kg, row_tiles, key_tiles, splits;
+  int64_t part, stat;  // bytes
+};
+Plan plan(const hk_attn_packed_params* p) {
+  const int group = p->q_heads / p->k_heads, cus = device_cu_count();
+  const int64_t rows = p->q_tokens * group, wide = slots(p->q_tokens, p->num_seqs, group, 128) * p->k_heads;
+  Plan r{};
+  r.kg = rows >= int64_t(96) * p->num_seqs && wide >= cus ? 1 : 4;
+  r.row_tiles = static_cast<int>(slots(p->q_tokens, p->num_seqs, group, 128 / r.kg));
+  r.key_tiles = static_cast<int>(slots(p->k_tokens, p->num_seqs, 1, 128));
+  // Key tiles that leave CUs idle share their rows between workgroups, 256 rows each at least.
+  const int64_t wgs = static_cast<int64_t>(r.key_tiles) * p->k_heads;
+  const int64_t want = wgs < 2 * cus ? ceil_div(3 * cus, wgs) : 1;
+  r.splits = static_cast<int>(clamp64(want, 1, clamp64(rows / p->num_seqs / 256, 1, 64)));
+  if (r.splits > 1) r.part = r.splits * p->k_tokens * p->k_heads * (p->head_dim <= 64 ? 64 : 128) * 8;
+  r.stat = ceil_div(8 * p->q_tokens * p->q_heads, 16) * 16;
+  return r;
+}
+
+template <class T, int D>
+hipError_t run(Args a, const Plan& r, hipStream_t stream) {
+  if (a.q_tokens > 0) {
+    a.tiles = r.row_tiles;
+    const dim3 grid(static_cast<unsigned>(a.tiles) * a.k_heads);
+    HK_RETURN_IF_ERROR(r.kg == 1 ? (launch<&attn_packed_dq<T, D, 1>, DqShape<D, 1>::kLds>(grid, a, stream))
+                                 : (launch<&attn_packed_dq<T, D, 4>, DqShape<D, 4>::kLds>(grid, a, stream)));
+  }
+  if (a.k_tokens == 0) return hipSuccess;
+  a.tiles = r.key_tiles;
+  const unsigned x = static_cast<unsigned>(a.tiles) * a.k_heads;
+  if (r.splits == 1) return launch<&attn_packed_dkv<T, D, false>, DkvShape<D>::kLds>(dim3(x), a, stream);
+  HK_RETURN_IF_ERROR((launch<&attn_packed_dkv<T, D, true>, DkvShape<D>::kLds>(dim3(x, r.splits), a, stream)));
+  const int64_t keys = a.k_tokens * a.k_heads;
+  return launch<&attn_packed_dkv_join<T, D>, 0>(dim3(static_cast<unsigned>(ceil_div(keys, 512 / D))), a, stream);
+}
+template <class T>
+hipError_t by_width(const Args& a, const Plan& r, hipStream_t stream) {
+  return a.d <= 64 ? run<T, 64>(a, r, stream) : run<T, 128>(a, r, stream);
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace hk
+
+using namespace hk::packed;
+
+extern "C" int64_t hk_attn_packed_workspace(const hk_attn_packed_params* p, int type, int backward) {
+  if (check(p, type, backward != 0) != hipSuccess) return -1;
+  if (!backward) return forward_workspace(p);
+  if (p->num_seqs == 0 || p->q_tokens + p->k_tokens == 0) return 0;
+  const Plan r = plan(p);
+  return r.part + r.stat;
+}
+
+extern "C" hipError_t hk_attn_packed_backward(const hk_attn_packed_params* p, int type, void* ws,
+                                              int64_t workspace_bytes, hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(p, type, true));
+  if (p->num_seqs == 0 || p->q_tokens + p->k_tokens == 0) return hipSuccess;
+  HK_CHECK_ARG(outputs_apart(p, true));
+  const Plan r = plan(p);
+  HK_RETURN_IF_ERROR(workspace(r.part + r.stat, ws, workspace_bytes, stream, &ws));
+  Args a = make_args(p);
+  a.splits = r.splits;
+  a.part = static_cast<float*>(ws);
+  a.delta = reinterpret_cast<float*>(static_cast<char*>(ws) + r.part);
+  return type == HK_TYPE_BF16 ? by_width<TypeBF16>(a, r, stream) : by_width<TypeF16>(a, r, stream);
+}

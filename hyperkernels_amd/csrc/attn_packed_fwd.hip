@@ -1,0 +1,305 @@
+// attn_packed_fwd.hip - attention over packed sequences, bf16 or fp16, causal or not, query heads in groups that
+// share a key head: o = softmax(scale q k^T) v and the log-sum-exp of each row.
+//
+// A workgroup of 4 waves owns 128 rows (32 a wave) or, where there are few, 32 rows, whose keys its waves share
+// (KG = 4). The scores are formed transposed, S^T = K Q^T: a lane holds one row's scores, so the running maximum is a
+// reduction in registers and one exchange with lane + 32, and the exponentials are, as they lie, the operand of
+// O^T += V^T P^T. P is rounded to 16 bits for that product (half a step of the type, as the inputs are; the sum that
+// divides it is of the fp32 values); scores, maximum, sum and O are fp32.
+// Tiles of keys and values go from memory to LDS past the registers, the next one while this one is used.
+#include "attn_packed.h"
+
+namespace hk {
+namespace packed {
+
+constexpr float kLazy = 8.f;
+
+template <int D, int KG>
+struct FwdShape {
+  static constexpr int kRows = 128 / KG;
+  static constexpr int kKeys = KG == 1 ? 64 : 128;  // keys a tile
+  static constexpr int kBlocks = kKeys / KG / 32;   // blocks of 32 keys a wave
+  static constexpr int kTile = kKeys * D * 2;       // bytes
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kPitch = D + 4;  // floats a row of the exchange
+  static constexpr int kExchange = KG == 1 ? 0 : 4 * 32 * kPitch * 4 + 4 * 32 * 8;
+  static constexpr int kLds = 2 * kStage > kExchange ? 2 * kStage : kExchange;
+};
+
+template <class T, int D, int KG, bool SPLIT>
+__global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) {
+  using S = FwdShape<D, KG>;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  char HK_LDS* const lds = (char HK_LDS*)lds_raw;
+
+  // the last tile of a sequence has the most keys: it goes first; key heads of one tile side by side
+  const int item = blockIdx.x / a.k_heads, kh = blockIdx.x - item * a.k_heads;
+  Seq q;
+  if (!find_tile(a.cu_q, a.q_tokens, a, a.group, S::kRows, a.tiles - 1 - item, q)) return;
+  const int rows = q.mq * a.group, r0 = q.tile * S::kRows;
+  if (r0 >= rows) return;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 31, h = lane >> 5;
+  const int kg = KG == 1 ? 0 : wave, w0 = KG == 1 ? r0 + 32 * wave : r0;
+  const int row = w0 + c, rr = min(row, rows - 1);
+  const int tok = rr / a.group, qh = kh * a.group + rr - tok * a.group;
+  const int ahead = q.mk - q.mq;  // row of query i sees keys 0 .. i + ahead
+  const int lim = a.causal ? tok + ahead : q.mk - 1;
+  const int lim_lo = __builtin_amdgcn_readfirstlane(lim);  // rows rise, and with them the limits
+  const int lim_hi = __builtin_amdgcn_readlane(lim, 31);
+
+  const int last_tok = min(r0 + S::kRows, rows) - 1;
+  const int end = a.causal ? min(q.mk, last_tok / a.group + ahead + 1) : q.mk;
+  int t0 = 0, t1 = end > 0 ? (end + S::kKeys - 1) / S::kKeys : 0;
+  if (SPLIT) {
+    const int per = (t1 + a.splits - 1) / a.splits;
+    t0 = blockIdx.y * per;
+    t1 = min(t1, t0 + per);
+  }
+
+  s16x8_t qx[D / 16];
+  load_row<D>(a.q.p + (q.q0 + tok) * a.q.m + qh * a.q.h, h, a.d, qx);
+
+  const char* kb = a.k.p + q.k0 * a.k.m + kh * a.k.h;
+  const char* vb = a.v.p + q.k0 * a.v.m + kh * a.v.h;
+  const KeyCopy<D, S::kKeys> copy(wave, lane, a.d);
+  const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds));
+  auto fetch = [&](int t) {
+    const unsigned to = lds0 + (t & 1) * S::kStage;
+    const int64_t at = static_cast<int64_t>(t) * S::kKeys;
+    const int last = q.mk - 1 - t * S::kKeys;
+    copy(kb + at * a.k.m, static_cast<int>(a.k.m), last, wave, to);
+    copy(vb + at * a.v.m, static_cast<int>(a.v.m), last, wave, to + S::kTile);
+  };
+  if (t0 < t1) fetch(t0);
+
+  const Reads<D> rd(lane);
+  const float sc = a.scale * kLog2e;
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b) o[b] = f32x16_t{};
+  float m = -INFINITY, l = 0.f;  // in units of log 2
+
+  for (int t = t0; t < t1; ++t) {
+    wait_copies();
+    barrier();  // this tile has landed, and every wave is done with the one before it
+    if (t + 1 < t1) fetch(t + 1);
+    const int key0 = t * S::kKeys + 32 * S::kBlocks * kg;
+    if (key0 > lim_hi) continue;  // the wave's rows see none of these
+    const char HK_LDS* kt = lds + (t & 1) * S::kStage + 32 * S::kBlocks * kg * (2 * D);
+    const char HK_LDS* vt = kt + S::kTile;
+
+    f32x16_t s[S::kBlocks];
+#pragma unroll
+    for (int n = 0; n < S::kBlocks; ++n) {
+      s[n] = f32x16_t{};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s[n] = T::mfma(rd.rows(kt, 32 * n, i), qx[i], s[n]);
+    }
+    if (key0 + 32 * S::kBlocks - 1 > lim_lo) {
+#pragma unroll
+      for (int n = 0; n < S::kBlocks; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3) > lim) s[n][i] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < S::kBlocks; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+    top = half32_reduce(top, MaxOp{}) * sc;
+    // The reference moves only where a score passes it by 2^8 or a row meets its first key: exponentials stay under
+    // 2^8 and most tiles leave O alone.
+    const bool move = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+    if (__any(move)) {
+      const float mn = move ? top : m;
+      const float f = move ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= f;
+      m = mn;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < S::kBlocks; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], sc, -base));
+        part[i & 3] += s[n][i];
+      }
+      s16x8_t p[2];
+      pack_block<T>(s[n], p);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) o[b] = T::mfma(rd.cols(vt, 32 * n + 16 * e, b), p[e], o[b]);
+    }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  l = half32_reduce(l, AddOp{});
+
+  if constexpr (KG > 1) {
+    // the four waves' parts of the same rows
+    float HK_LDS* ex = (float HK_LDS*)lds;
+    float HK_LDS* st = ex + 4 * 32 * S::kPitch;
+    wait_copies();
+    barrier();
+    if (h == 0) st[64 * wave + 2 * c] = m, st[64 * wave + 2 * c + 1] = l;
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4_t HK_LDS*>(ex + (32 * wave + c) * S::kPitch + 32 * b + 8 * g + 4 * h) =
+            f32x4_t{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
+    __syncthreads();
+    // wave w, rows 8 w .. + 7: 8 lanes a row, D / 8 elements a lane
+    const int er = 8 * wave + (lane >> 3), e0 = lane & 7;
+    float em[4], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) em[g] = st[64 * g + 2 * er], mx = fmaxf(mx, em[g]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      em[g] = __builtin_amdgcn_exp2f(em[g] - ref);
+      sum += em[g] * st[64 * g + 2 * er + 1];
+    }
+    if (r0 + er >= rows) return;
+    const int et = (r0 + er) / a.group, eh = kh * a.group + (r0 + er) - et * a.group;
+    const int64_t at = static_cast<int64_t>(blockIdx.y * a.k_heads + kh) * a.q_tokens * a.group +
+                       q.q0 * a.group + r0 + er;
+    const float f = SPLIT ? 1.f : sum > 0.f ? 1.f / sum : sum;  // a NaN stays one
+    char* op = a.o.p + (q.q0 + et) * a.o.m + eh * a.o.h;
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      const int col = 32 * u + 4 * e0;
+      f32x4_t x = {};
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        x += em[g] * *reinterpret_cast<const f32x4_t HK_LDS*>(ex + (32 * g + er) * S::kPitch + col);
+      if (SPLIT) *reinterpret_cast<f32x4_t*>(a.part + at * D + col) = x;
+      else if (col < a.d)
+        *reinterpret_cast<u32x2_t*>(op + 2 * col) = u32x2_t{T::pack(x[0] * f, x[1] * f), T::pack(x[2] * f, x[3] * f)};
+    }
+    if (e0 == 0) {
+      if (SPLIT) a.stat[at] = make_float2(mx, sum);
+      else if (a.lse) a.lse[eh * a.lse_stride + q.q0 + et] = (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+    return;
+  }
+  if (row >= rows) return;
+  store_row<T, D>(a.o.p + (q.q0 + tok) * a.o.m + qh * a.o.h, h, a.d, o, l > 0.f ? 1.f / l : l);
+  if (h == 0 && a.lse) a.lse[qh * a.lse_stride + q.q0 + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Joins the shares of each row's keys, one wave a row of one query head.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_packed_join(Args a) {
+  const int64_t rows = a.q_tokens * a.group;  // of one key head
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (i >= rows * a.k_heads) return;
+  const int kh = static_cast<int>(i / rows);
+  const int64_t r = i - kh * rows, tok = r / a.group;
+  if (tok < a.cu_q[0] || tok >= a.cu_q[a.n]) return;  // of no sequence
+  const int qh = kh * a.group + static_cast<int>(r - tok * a.group);
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stat[s * rows * a.k_heads + i].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = s * rows * a.k_heads + i;
+    const float2 st = a.stat[at];
+    const float w = __builtin_amdgcn_exp2f(st.x - ref);
+    l += w * st.y;
+    if (D == 128) {
+      const float2 p = reinterpret_cast<const float2*>(a.part + at * D)[lane];
+      x0 += w * p.x, x1 += w * p.y;
+    } else {
+      x0 += w * a.part[at * D + lane];
+    }
+  }
+  const float f = l > 0.f ? 1.f / l : l;
+  char* op = a.o.p + tok * a.o.m + qh * a.o.h;
+  if (D == 128) {
+    if (2 * lane < a.d) reinterpret_cast<uint32_t*>(op)[lane] = T::pack(x0 * f, x1 * f);
+  } else if (lane < a.d) {
+    T::format::store(reinterpret_cast<uint16_t*>(op), lane, x0 * f);
+  }
+  if (lane == 0 && a.lse) a.lse[qh * a.lse_stride + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+namespace {
+
+struct Plan {
+  int kg, tiles, splits;
+  int64_t part, stat;  // bytes
+};
+// 128 rows a workgroup where a sequence fills them and the card gets a round of workgroups so; else 32, and where even
+// those leave CUs idle each row's keys are cut into shares.
+Plan plan(const hk_attn_packed_params* p) {
+  const int group = p->q_heads / p->k_heads, cus = device_cu_count();
+  const int64_t rows = p->q_tokens * group, wide = slots(p->q_tokens, p->num_seqs, group, 128) * p->k_heads;
+  Plan r{};
+  r.splits = 1;
+  if (rows >= int64_t(96) * p->num_seqs && wide >= cus) {
+    r.kg = 1;
+    r.tiles = static_cast<int>(wide / p->k_heads);
+    return r;
+  }
+  r.kg = 4;
+  r.tiles = static_cast<int>(slots(p->q_tokens, p->num_seqs, group, 32));
+  const int64_t wgs = static_cast<int64_t>(r.tiles) * p->k_heads, keys = p->k_tokens / p->num_seqs;
+  const int64_t want = wgs < cus ? ceil_div(2 * cus, wgs) : 1;
+  r.splits = static_cast<int>(clamp64(want, 1, clamp64(keys / 256, 1, 64)));
+  if (r.splits > 1) {
+    const int64_t n = r.splits * p->q_tokens * p->q_heads, D = p->head_dim <= 64 ? 64 : 128;
+    r.part = n * D * 4, r.stat = n * 8;
+  }
+  return r;
+}
+
+template <class T, int D>
+hipError_t run(Args a, const Plan& r, hipStream_t stream) {
+  const unsigned x = static_cast<unsigned>(a.tiles) * a.k_heads;
+  if (r.kg == 1) return launch<&attn_packed_fwd<T, D, 1, false>, FwdShape<D, 1>::kLds>(dim3(x), a, stream);
+  if (r.splits == 1) return launch<&attn_packed_fwd<T, D, 4, false>, FwdShape<D, 4>::kLds>(dim3(x), a, stream);
+  HK_RETURN_IF_ERROR((launch<&attn_packed_fwd<T, D, 4, true>, FwdShape<D, 4>::kLds>(dim3(x, r.splits), a, stream)));
+  const int64_t rows = a.q_tokens * a.group * a.k_heads;
+  return launch<&attn_packed_join<T, D>, 0>(dim3(static_cast<unsigned>(ceil_div(rows, 4))), a, stream);
+}
+template <class T>
+hipError_t by_width(const Args& a, const Plan& r, hipStream_t stream) {
+  return a.d <= 64 ? run<T, 64>(a, r, stream) : run<T, 128>(a, r, stream);
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace hk
+
+using namespace hk::packed;
+
+int64_t hk::packed::forward_workspace(const hk_attn_packed_params* p) {
+  if (p->num_seqs == 0 || p->q_tokens == 0) return 0;
+  const Plan r = plan(p);
+  return r.part + r.stat;
+}
+
+extern "C" hipError_t hk_attn_packed_forward(const hk_attn_packed_params* p, int type, void* ws,
+                                             int64_t workspace_bytes, hipStream_t stream) {
+  HK_RETURN_IF_ERROR(check(p, type, false));
+  if (p->num_seqs == 0 || p->q_tokens == 0) return hipSuccess;
+  HK_CHECK_ARG(outputs_apart(p, false));
+  const Plan r = plan(p);
+  HK_RETURN_IF_ERROR(workspace(r.part + r.stat, ws, workspace_bytes, stream, &ws));
+  Args a = make_args(p);
+  a.tiles = r.tiles, a.splits = r.splits;
+  a.part = static_cast<float*>(ws);
+  a.stat = reinterpret_cast<float2*>(static_cast<char*>(ws) + r.part);
+  return type == HK_TYPE_BF16 ? by_width<TypeBF16>(a, r, stream) : by_width<TypeF16>(a, r, stream);
+}

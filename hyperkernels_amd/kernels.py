@@ -21,7 +21,7 @@ __all__ = [
     "ln_backward_gamma_beta", "layer_norm_backward", "sparse_ce_forward", "sparse_ce_backward",
     "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "Adam8Plan", "ADAM8_BLOCK",
     "adam8_states", "adam8_quantize", "adam8_dequantize", "qk_norm_rope_forward",
-    "qk_norm_rope_backward", "ReductionLayout",
+    "qk_norm_rope_backward", "attn_packed_forward", "attn_packed_backward", "ReductionLayout",
     "unified_reduce_sum", "reduce_generic", "REDUCE_INNER", "REDUCE_OUTER", "REDUCE_GENERIC",
 ]
 
@@ -774,6 +774,97 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, cos=None, sin=None, positions=No
     _call_captured("hk_qk_norm_rope_backward", lambda: lib().hk_qk_norm_rope_workspace(p, kind), p,
                    kind)
     return dq, dk
+
+
+# ----------------------------------------------------------------------------------------------
+# 16-bit attention over packed sequences (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+class AttnPackedParams(ctypes.Structure):
+    """hk_attn_packed_params (hk.h), field for field."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv", "lse", "cu_q",
+                                               "cu_k")] + [
+        (n, ctypes.c_int) for n in ("num_seqs", "q_heads", "k_heads", "head_dim")] + [
+        ("scale", ctypes.c_float), ("is_causal", ctypes.c_bool), ("q_tokens", _I64), ("k_tokens", _I64)] + [
+        (f"{t}_stride{s}", _I64) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("M", "H")] + [
+        ("lse_strideH", _I64)]
+
+
+_PACKED_PACK = struct.Struct("@11P4if?19q").pack
+
+
+def _heads(fn: str, t: torch.Tensor, tokens: int, heads: int, d: int, dt, dev: int) -> tuple[int, int, int]:
+    """(address, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    if t.shape != (tokens, heads, d) or t.dtype is not dt or t.get_device() != dev:
+        raise ValueError(f"{fn}: {dt} [{tokens}, {heads}, {d}] of one device expected, "
+                         f"{t.dtype} {tuple(t.shape)} given")
+    m, h, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{fn}: tensors are [tokens, heads, head_dim] with a unit last-dim stride")
+    # the stride of a single token or head is never used, whatever it is
+    return t.data_ptr(), m if tokens > 1 else 0, h if heads > 1 else 0
+
+
+def _packed_params(fn, q, k, v, cu_q, cu_k, causal, scale, o, lse, do=None, dq=None, dk=None, dv=None):
+    if q.dim() != 3 or k.dim() != 3 or (q.dtype is not _BF16 and q.dtype is not torch.float16):
+        raise ValueError(f"{fn}: bf16 or fp16 tensors [tokens, heads, head_dim]")
+    dev, dt = _device(fn, q), q.dtype
+    (tq, hq, d), (tk, hk, _) = q.shape, k.shape
+    cu_k = cu_q if cu_k is None else cu_k
+    n = cu_q.numel() - 1
+    for cu in (cu_q, cu_k):
+        if cu.dtype is not torch.int32 or cu.dim() != 1 or cu.numel() != n + 1 or n < 0 or (
+                cu.get_device() != dev or (n > 0 and cu.stride(0) != 1)):
+            raise ValueError(f"{fn}: cu_q and cu_k are int32 [sequences + 1], contiguous, on the device")
+    if hk == 0 or hq == 0 or hq % hk or d % 8 or not 8 <= d <= 128:
+        raise ValueError(f"{fn}: key heads divide the query heads; head_dim is a multiple of 8, at most 128")
+    Q = _heads(fn, q, tq, hq, d, dt, dev)
+    K, V = _heads(fn, k, tk, hk, d, dt, dev), _heads(fn, v, tk, hk, d, dt, dev)
+    O = _heads(fn, o, tq, hq, d, dt, dev)  # noqa: E741
+    lp = ls = 0
+    if lse is not None:
+        if lse.dtype is not _F32 or lse.shape != (hq, tq) or lse.get_device() != dev or (
+                lse.stride(1) != 1 and tq > 1):
+            raise ValueError(f"{fn}: lse is fp32 [heads, tokens] with a unit last-dim stride")
+        lp, ls = lse.data_ptr(), lse.stride(0) if hq > 1 else 0
+    if do is None:
+        G = DQ = DK = DV = (0, 0, 0)
+    else:
+        G, DQ = _heads(fn, do, tq, hq, d, dt, dev), _heads(fn, dq, tq, hq, d, dt, dev)
+        DK, DV = _heads(fn, dk, tk, hk, d, dt, dev), _heads(fn, dv, tk, hk, d, dt, dev)
+    return _PACKED_PACK(Q[0], K[0], V[0], O[0], G[0], DQ[0], DK[0], DV[0], lp, cu_q.data_ptr(), cu_k.data_ptr(),
+                        n, hq, hk, d, d ** -0.5 if scale is None else scale, causal, tq, tk, Q[1], Q[2], K[1],
+                        K[2], V[1], V[2], O[1], O[2], G[1], G[2], DQ[1], DQ[2], DK[1], DK[2], DV[1], DV[2], ls)
+
+
+def attn_packed_forward(q, k, v, cu_q, cu_k=None, causal: bool = True, scale: float | None = None, o=None,
+                        lse=None):
+    """Attention over packed sequences: q [tokens, q_heads, head_dim], k and v [key tokens, k_heads, head_dim],
+    bf16 or fp16; sequence s has the queries cu_q[s] .. cu_q[s + 1] - 1 and the keys cu_k[s] .. (int32 on the device;
+    None: as cu_q), and query i of m sees key j of n where j <= i + n - m, or all keys. Query head h goes with key
+    head h // (q_heads / k_heads). Returns (o, lse): o like q, lse fp32 [q_heads, tokens], 0 and -inf where a
+    query sees no key; rows of no sequence are not written."""
+    o = q.new_empty(q.shape) if o is None else o
+    lse = q.new_empty((q.shape[1], q.shape[0]), dtype=_F32) if lse is None and q.dim() == 3 else lse
+    p = _packed_params("attn_packed_forward", q, k, v, cu_q, cu_k, causal, scale, o, lse)
+    kind = _TYPE[q.dtype]
+    _call_captured("hk_attn_packed_forward", lambda: lib().hk_attn_packed_workspace(p, kind, 0), p, kind)
+    return o, lse
+
+
+def attn_packed_backward(do, q, k, v, o, lse, cu_q, cu_k=None, causal: bool = True, scale: float | None = None,
+                         dq=None, dk=None, dv=None):
+    """Gradients (dq, dk, dv) of attn_packed_forward's inputs from that of its output, all of q's type. Written, not
+    added to; those of rows of no sequence are not written."""
+    dq = q.new_empty(q.shape) if dq is None else dq
+    dk = k.new_empty(k.shape) if dk is None else dk
+    dv = v.new_empty(v.shape) if dv is None else dv
+    if lse is None:
+        raise ValueError("attn_packed_backward: the forward's lse is needed")
+    p = _packed_params("attn_packed_backward", q, k, v, cu_q, cu_k, causal, scale, o, lse, do, dq, dk, dv)
+    kind = _TYPE[q.dtype]
+    _call_captured("hk_attn_packed_backward", lambda: lib().hk_attn_packed_workspace(p, kind, 1), p, kind)
+    return dq, dk, dv
 
 
 # ----------------------------------------------------------------------------------------------

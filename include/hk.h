@@ -701,6 +701,66 @@ HK_API hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* params,
                                            hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention in 16 bits over sequences of different lengths that lie one behind the other, query heads in groups
+ * that share a key head, with its backward pass. No counterpart in the reference.
+ * Sequence s (of num_seqs) has the queries cu_q[s] .. cu_q[s + 1] - 1 and the keys and values cu_k[s] ..
+ * cu_k[s + 1] - 1 (int32 in device memory, num_seqs + 1 each, rising; cu_q itself may be cu_k). Query i of m sees
+ * key j of n where is_causal is not set or j <= i + n - m: the last query is level with the last key, so a prompt is
+ * m == n, a chunk of one or a new token over a cache m < n, and the first m - n queries see nothing where m > n.
+ * Query head h reads key head h / (q_heads / k_heads).
+ *   forward   o = softmax(scale q k^T) v,  lse = the log of the sum of exp(scale q k^T)  (0 and -inf without a key)
+ *   backward  from dout, the gradient of o, and the forward's o and lse: dq, dk, dv (written)
+ * q, o, dout, dq are [q_tokens, q_heads, head_dim], k, v, dk, dv [k_tokens, k_heads, head_dim], all of the call's type
+ * (HK_TYPE_BF16 or HK_TYPE_F16): any strides of tokens (M) and heads (H) that are multiples of 8 elements, unit
+ * last-dim stride, 16-byte aligned; those of tokens of k and v at most 2^23. head_dim is a multiple of 8, 128 at
+ * most. lse is fp32 [q_heads, q_tokens], heads lse_strideH elements apart; NULL in the forward pass: not wanted.
+ * scale is positive and finite. At most 2^30 rows (q_tokens * q_heads) and 2^23 tiles of 32 rows or 128 keys.
+ * Rows before cu[0] and from cu[num_seqs] on are not written. Starts past the tensors count as their ends and a
+ * sequence that would end before it begins as empty: nothing outside the tensors is read or written whatever cu holds.
+ * Scores, softmax and sums are fp32; P, and in the backward pass P and dS, are rounded to the call's type for the
+ * products over keys or rows. Sums are in a fixed order (no atomics). Elements that are not finite make outputs of
+ * their own sequence NaN, also those of queries that a mask keeps from them, but of no other sequence.
+ * No output may share memory with anything else of the call, nor two of its rows with each other.
+ * Workspace: hk_attn_packed_workspace bytes (0: none is needed, -1: invalid arguments), as for
+ * hk_qk_norm_rope_backward: at `workspace` (16-byte aligned) or, where that is NULL, the stream's; a call that needs
+ * some and is captured into a graph brings its own (hipErrorStreamCaptureUnsupported otherwise).
+ * ---------------------------------------------------------------------------------------- */
+typedef struct hk_attn_packed_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o; /* backward: read */
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* lse; /* backward: read */
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int num_seqs;
+  int q_heads, k_heads;
+  int head_dim;
+  float scale;
+  bool is_causal;
+  int64_t q_tokens, k_tokens;
+  int64_t q_strideM, q_strideH;
+  int64_t k_strideM, k_strideH;
+  int64_t v_strideM, v_strideH;
+  int64_t o_strideM, o_strideH;
+  int64_t do_strideM, do_strideH;
+  int64_t dq_strideM, dq_strideH;
+  int64_t dk_strideM, dk_strideH;
+  int64_t dv_strideM, dv_strideH;
+  int64_t lse_strideH;
+} hk_attn_packed_params;
+
+HK_API int64_t hk_attn_packed_workspace(const hk_attn_packed_params* params, int type, int backward);
+HK_API hipError_t hk_attn_packed_forward(const hk_attn_packed_params* params, int type, void* workspace,
+                                         int64_t workspace_bytes, hipStream_t stream);
+HK_API hipError_t hk_attn_packed_backward(const hk_attn_packed_params* params, int type, void* workspace,
+                                          int64_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement
  * ---------------------------------------------------------------------------------------- */
 /* HBM stream with a given read/write mix. No counterpart in the reference: a measurement aid for
