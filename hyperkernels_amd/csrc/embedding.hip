@@ -1,0 +1,614 @@
+// embedding.hip - embedding lookup, out[i] = scale table[token_i] + residual[i], and the table's gradient,
+// grad_table[v] (+)= scale sum of grad[i] over the i with token_i = v. fp32, bf16 and fp16, any d, strides, alignment.
+//
+// Both are bound by memory. The gradient has to be the same whatever the order in which workgroups run, and texts repeat a
+// few words very often, so rows are neither added atomically nor owned by one workgroup each:
+//   embedding_sort     a workgroup per range of table rows reads all tokens (from L2), counts those below its range, which
+//                      is where its part of the sorted order begins, and places its own by row, in the tokens' order. It
+//                      also writes the rows without a token, most of a large table, while it has little else to do.
+//   embedding_sum      the sorted order in equal chunks, a wave each and 64 units of columns: rows that lie inside a chunk
+//                      are written, the parts of those that go on across its ends are left as partial sums,
+//   embedding_combine  which are added in order where such a row begins.
+// Few tokens take one launch: each workgroup finds its rows' tokens and sums them itself.
+#include <initializer_list>
+
+#include "hk_device.h"
+#include "hk_host.h"
+#include "hk_overlap.h"
+
+namespace hk {
+namespace {
+
+__device__ __forceinline__ int64_t token_of(const void* tokens, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(tokens)[i] : static_cast<const int32_t*>(tokens)[i];
+}
+
+// E elements of a row as fp32: whole vectors where E > 1.
+template <class F, int E>
+__device__ __forceinline__ void load(const void* p, int64_t at, float* f) {
+  using S = typename F::storage;
+  const S* x = static_cast<const S*>(p) + at;
+  if constexpr (E == 1) {
+    f[0] = F::load(x, 0);
+  } else if constexpr (E * sizeof(S) == 8) {
+    const uint2 w = *reinterpret_cast<const uint2*>(x);
+    float t[8];
+    F::unpack(make_uint4(w.x, w.y, 0, 0), t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i += F::kPerVec) F::unpack(*reinterpret_cast<const uint4*>(x + i), f + i);
+  }
+}
+template <class F, int E>
+__device__ __forceinline__ void store(void* p, int64_t at, const float* f) {
+  using S = typename F::storage;
+  S* x = static_cast<S*>(p) + at;
+  if constexpr (E == 1) {
+    F::store(x, 0, f[0]);
+  } else if constexpr (E * sizeof(S) == 8) {
+    *reinterpret_cast<uint2*>(x) = make_uint2(F::pack2(f[0], f[1]), F::pack2(f[2], f[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i += F::kPerVec) st_nt(reinterpret_cast<uint4*>(x + i), F::pack(f + i));
+  }
+}
+
+// ---- lookup ------------------------------------------------------------------------------------------------
+struct Lookup {
+  const void *table, *tokens, *residual;
+  void* out;
+  int wide_tokens;
+  int64_t vocab, table_stride, residual_stride, out_stride;
+  float scale;
+  int units;       // a row, of E elements
+  int64_t first;   // row of this launch's first unit
+  uint32_t total;  // units of this launch
+};
+
+template <class FT, class FO, int E>
+__global__ __launch_bounds__(256) void embedding_lookup(Lookup a) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= a.total) return;
+  const uint32_t r = i / a.units;
+  const int64_t row = a.first + r;
+  const int col = static_cast<int>(i - r * a.units) * E;
+  const int64_t t = token_of(a.tokens, a.wide_tokens, row);
+  float f[E], g[E];
+  if (static_cast<uint64_t>(t) < static_cast<uint64_t>(a.vocab)) {
+    load<FT, E>(a.table, t * a.table_stride + col, f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] *= a.scale;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = __uint_as_float(0x7fc00000u);
+  }
+  if (a.residual) {
+    load<FO, E>(a.residual, row * a.residual_stride + col, g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] += g[e];
+  }
+  store<FO, E>(a.out, row * a.out_stride + col, f);
+}
+
+// ---- gradient ----------------------------------------------------------------------------------------------
+struct Grad {
+  const void *grad, *tokens;
+  void* table;
+  int wide_tokens;
+  int64_t n, vocab, grad_stride, table_stride;
+  int d;
+  float scale;
+  int accumulate;
+  int range;        // table rows a workgroup (sort, few)
+  int table_elem;   // bytes
+  int chunk;        // positions a chunk
+  int col_blocks;   // waves a chunk
+  uint2* sorted;    // (token's place, its table row) in order of the rows; row ~0 behind the last
+  float* part;      // [chunk][2][d]: of the row that goes on from before, of the one that goes on behind
+};
+
+// Zeros one row of the table: all lanes of a group of `lanes`.
+__device__ __forceinline__ void zero_row(const Grad& a, int64_t row, int lane, int lanes) {
+  char* p = static_cast<char*>(a.table) + row * a.table_stride * a.table_elem;
+  const int bytes = a.d * a.table_elem;
+  const uintptr_t both = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(bytes);
+  if ((both & 15) == 0) {
+    for (int i = lane * 16; i < bytes; i += lanes * 16) st_nt(reinterpret_cast<uint4*>(p + i), make_uint4(0, 0, 0, 0));
+  } else if ((both & 3) == 0) {
+    for (int i = lane * 4; i < bytes; i += lanes * 4) *reinterpret_cast<uint32_t*>(p + i) = 0;
+  } else {
+    for (int i = lane * 2; i < bytes; i += lanes * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
+  }
+}
+
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kRounds = 8;                             // tokens a lane and tile
+constexpr int kTileTokens = kSortThreads * kRounds;    // 4096
+constexpr int kMaxRange = 1024;
+
+__global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
+  __shared__ int count[kMaxRange];             // of each row, then where its next token goes
+  __shared__ int wave_at[kSortWaves][kMaxRange];
+  __shared__ uint2 list[kTileTokens];
+  __shared__ int sums[kSortWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
+  const int rows = static_cast<int>(min(static_cast<uint64_t>(a.range), static_cast<uint64_t>(a.vocab) - lo));
+
+  for (int i = tid; i < rows; i += kSortThreads) count[i] = 0;
+  __syncthreads();
+  int below = 0;
+  for (int64_t i = tid; i < a.n; i += kSortThreads * 4) {
+    uint64_t t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = i + u * kSortThreads;
+      t[u] = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) : ~uint64_t(0);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      below += t[u] < lo;
+      if (t[u] - lo < static_cast<uint64_t>(rows)) atomicAdd(&count[static_cast<int>(t[u] - lo)], 1);
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) below += __shfl_xor(below, s);
+  if (lane == 0) sums[wave] = below;
+  __syncthreads();
+  below = 0;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) below += sums[w];
+  __syncthreads();
+
+  if (!a.accumulate)
+    for (int r = wave; r < rows; r += kSortWaves)
+      if (count[r] == 0) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
+  __syncthreads();
+  // count[r]: the first place of row r in the sorted order
+  {
+    constexpr int kPer = kMaxRange / kSortThreads;
+    int mine[kPer], sum = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int r = tid * kPer + u;
+      mine[u] = r < rows ? count[r] : 0;
+      sum += mine[u];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int up = __shfl_up(incl, s);
+      if (lane >= s) incl += up;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int at = below + incl - sum;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int r = tid * kPer + u;
+      if (r < rows) count[r] = at;
+      at += mine[u];
+    }
+    // the last workgroup knows where the valid tokens end
+    int total = below;
+    for (int w = 0; w < kSortWaves; ++w) total += sums[w];
+    if (lo + rows == static_cast<uint64_t>(a.vocab))
+      for (int64_t i = total + tid; i < a.n; i += kSortThreads) a.sorted[i] = make_uint2(0, ~0u);
+    if (total == below) return;  // none of these rows
+  }
+
+  int bits = 1;
+  while ((1 << bits) < rows) ++bits;
+  for (int64_t base = 0; base < a.n; base += kTileTokens) {
+    // this range's tokens of the tile in order: each wave looks through 64 x kRounds of them
+    uint64_t row[kRounds], mask[kRounds];
+    int found = 0;
+    const int64_t w0 = base + wave * (64 * kRounds) + lane;
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+      const int64_t at = w0 + 64 * u;
+      row[u] = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) - lo : ~uint64_t(0);
+    }
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+      mask[u] = __ballot(row[u] < static_cast<uint64_t>(rows));
+      found += __popcll(mask[u]);
+    }
+    __syncthreads();  // the tile before is done with list and sums
+    if (lane == 0) sums[wave] = found;
+    for (int i = tid; i < kSortWaves * rows; i += kSortThreads) wave_at[i / rows][i % rows] = 0;
+    __syncthreads();
+    int at = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      if (w < wave) at += sums[w];
+      total += sums[w];
+    }
+    if (total == 0) continue;
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+      const int before = __popcll(mask[u] & ((uint64_t(1) << lane) - 1));
+      if (row[u] < static_cast<uint64_t>(rows))
+        list[at + before] = make_uint2(static_cast<uint32_t>(w0 + 64 * u), static_cast<uint32_t>(row[u]));
+      at += __popcll(mask[u]);
+    }
+    __syncthreads();
+    // each wave takes an equal part of the list: how many of each row it has, where they go, and there
+    const int per = ((total + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
+    const int from = wave * per, to = min(from + per, total);
+    for (int i = from + lane; i < to; i += 64) atomicAdd(&wave_at[wave][list[i].y], 1);
+    __syncthreads();
+    for (int r = tid; r < rows; r += kSortThreads) {
+      int next = count[r];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) {
+        const int c = wave_at[w][r];
+        wave_at[w][r] = next;
+        next += c;
+      }
+      count[r] = next;
+    }
+    __syncthreads();
+    for (int i0 = from; i0 < to; i0 += 64) {
+      const int i = i0 + lane;
+      const bool some = i < to;
+      const uint2 e = some ? list[i] : make_uint2(0, 0);
+      uint64_t same = __ballot(some);
+      for (int b = 0; b < bits; ++b) {
+        const bool bit = (e.y >> b) & 1;
+        const uint64_t with = __ballot(some && bit);
+        same &= bit ? with : ~with;
+      }
+      const int before = __popcll(same & ((uint64_t(1) << lane) - 1));
+      int place = 0;
+      if (some) place = wave_at[wave][e.y] + before;
+      if (some && (same >> lane) == 1) wave_at[wave][e.y] = place + 1;  // the last of them
+      if (some) a.sorted[place] = make_uint2(e.x, static_cast<uint32_t>(lo) + e.y);
+    }
+  }
+}
+
+template <class FT, int E>
+__device__ __forceinline__ void put_row(const Grad& a, uint32_t row, int col, float* f) {
+  const int64_t at = static_cast<int64_t>(row) * a.table_stride + col;
+#pragma unroll
+  for (int e = 0; e < E; ++e) f[e] *= a.scale;
+  if (a.accumulate) {
+    float g[E];
+    load<FT, E>(a.table, at, g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] += g[e];
+  }
+  store<FT, E>(a.table, at, f);
+}
+
+constexpr int kAhead = 8;  // rows in flight
+
+template <class FG, class FT, int E>
+__global__ __launch_bounds__(256) void embedding_sum(Grad a) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t chunk = item / a.col_blocks;
+  const int lane = threadIdx.x & 63, col = (static_cast<int>(item - chunk * a.col_blocks) * 64 + lane) * E;
+  const int64_t from = chunk * a.chunk;
+  if (from >= a.n) return;
+  const int64_t to = min(from + a.chunk, a.n);
+  const uint32_t before = from > 0 ? a.sorted[from - 1].y : ~0u, behind = to < a.n ? a.sorted[to].y : ~0u;
+  const bool mine = col < a.d;
+  float acc[E] = {};
+  uint32_t row = a.sorted[from].y;
+  if (row == ~0u) return;
+  auto flush = [&](bool last) {
+    if (!mine) return;
+    if (row == before || (last && row == behind)) {
+      float* p = a.part + (chunk * 2 + (row == before ? 0 : 1)) * a.d + col;
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = acc[e];
+    } else {
+      put_row<FT, E>(a, row, col, acc);
+    }
+  };
+  for (int64_t p0 = from; p0 < to; p0 += kAhead) {
+    uint2 s[kAhead];
+    float x[kAhead][E];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) s[u] = p0 + u < to ? a.sorted[p0 + u] : make_uint2(0, ~0u);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (s[u].y != ~0u && mine) load<FG, E>(a.grad, static_cast<int64_t>(s[u].x) * a.grad_stride + col, x[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s[u].y == ~0u) continue;
+      if (s[u].y != row) {
+        flush(false);
+        row = s[u].y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      }
+      if (mine)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x[u][e];
+    }
+  }
+  flush(true);
+}
+
+// The row that begins in a chunk and goes on behind it: its part of this chunk, and of the chunks that it goes on into.
+template <class FT, int E>
+__global__ __launch_bounds__(256) void embedding_combine(Grad a) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t chunk = item / a.col_blocks;
+  const int lane = threadIdx.x & 63, col = (static_cast<int>(item - chunk * a.col_blocks) * 64 + lane) * E;
+  const int64_t from = chunk * a.chunk, to = from + a.chunk;
+  if (to >= a.n) return;
+  const uint32_t row = a.sorted[to].y;
+  if (row == ~0u || a.sorted[to - 1].y != row || (from > 0 && a.sorted[from - 1].y == row)) return;
+  const bool mine = col < a.d;
+  float acc[E] = {};
+  if (mine)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = a.part[(chunk * 2 + 1) * a.d + col + e];
+  for (int64_t c = chunk + 1;; c += 64) {
+    // how many of the next chunks begin with it
+    const int64_t first = (c + lane) * a.chunk;
+    const uint64_t on = __ballot(first < a.n && a.sorted[first < a.n ? first : to].y == row);
+    const int more = ~on ? __ffsll(static_cast<unsigned long long>(~on)) - 1 : 64;
+    if (mine)
+      for (int i = 0; i < more; i += 4) {
+        float x[4][E];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = i + u < more ? a.part[(c + i + u) * 2 * a.d + col + e] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += x[u][e];
+      }
+    if (more < 64) break;
+  }
+  if (mine) put_row<FT, E>(a, row, col, acc);
+}
+
+// Few tokens: a workgroup finds those of its rows and sums them in order.
+constexpr int kFew = 512;
+template <class FG, class FT, int E>
+__global__ __launch_bounds__(256) void embedding_few(Grad a) {
+  __shared__ uint2 list[kFew];
+  __shared__ int sums[4];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
+  const int rows = static_cast<int>(min(static_cast<uint64_t>(a.range), static_cast<uint64_t>(a.vocab) - lo));
+  constexpr int kTokens = kFew / 4, kU = kTokens / 64;  // a wave, a lane
+  uint64_t row[kU], mask[kU];
+  int found = 0;
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int at = wave * kTokens + 64 * u + lane;
+    row[u] = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) - lo : ~uint64_t(0);
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    mask[u] = __ballot(row[u] < static_cast<uint64_t>(rows));
+    found += __popcll(mask[u]);
+  }
+  if (lane == 0) sums[wave] = found;
+  __syncthreads();
+  int at = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) at += sums[w];
+    total += sums[w];
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    if (row[u] < static_cast<uint64_t>(rows))
+      list[at + __popcll(mask[u] & ((uint64_t(1) << lane) - 1))] =
+          make_uint2(wave * kTokens + 64 * u + lane, static_cast<uint32_t>(row[u]));
+    at += __popcll(mask[u]);
+  }
+  __syncthreads();
+  for (int r = wave; r < rows; r += 4) {
+    bool any = false;
+    for (int i = 0; i < total; i += 64) any |= __any(i + lane < total && list[min(i + lane, total - 1)].y == r);
+    if (!any) {
+      if (!a.accumulate) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
+      continue;
+    }
+    for (int c0 = 0; c0 < a.d; c0 += 64 * E) {
+      const int col = c0 + lane * E;
+      const bool mine = col < a.d;
+      float acc[E] = {};
+      for (int i = 0; i < total; i += 64) {
+        uint64_t of = __ballot(i + lane < total && list[min(i + lane, total - 1)].y == r);
+        while (of) {
+          float x[kAhead][E];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+            if (of) {
+              const int k = __ffsll(static_cast<unsigned long long>(of)) - 1;
+              of &= of - 1;
+              if (mine) load<FG, E>(a.grad, static_cast<int64_t>(list[i + k].x) * a.grad_stride + col, x[u]);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] += x[u][e];
+        }
+      }
+      if (mine) put_row<FT, E>(a, static_cast<uint32_t>(lo) + r, col, acc);
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+int64_t elem(int type) { return type == HK_TYPE_F32 ? 4 : 2; }
+bool type_ok(int type) { return type >= HK_TYPE_F32 && type <= HK_TYPE_F16; }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Elements a lane takes at once: 8 where all tensors have them as 16-byte vectors (fp32: two), 4, or 1.
+struct Matrix {
+  const void* p;
+  int64_t stride, elem;
+  int64_t rows;
+};
+int unit(int64_t d, std::initializer_list<Matrix> ts) {
+  for (int e = 8; e >= 4; e /= 2) {
+    bool all = d % e == 0;
+    for (const Matrix& t : ts) {
+      const int64_t bytes = e * t.elem < 16 ? e * t.elem : 16;
+      all = all && (!t.p || (aligned(t.p, bytes) && (t.rows <= 1 || t.stride * t.elem % bytes == 0)));
+    }
+    if (all) return e;
+  }
+  return 1;
+}
+
+template <class FT, class FO>
+hipError_t lookup(Lookup a, int64_t n, int64_t d, int e, hipStream_t stream) {
+  a.units = static_cast<int>(d / e);
+  const int64_t step = std::max<int64_t>(1, (int64_t(1) << 30) / a.units);
+  for (a.first = 0; a.first < n; a.first += step) {
+    a.total = static_cast<uint32_t>(std::min(step, n - a.first) * a.units);
+    const dim3 grid((a.total + 255) / 256);
+    if (e == 8) hipLaunchKernelGGL((embedding_lookup<FT, FO, 8>), grid, dim3(256), 0, stream, a);
+    else if (e == 4) hipLaunchKernelGGL((embedding_lookup<FT, FO, 4>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((embedding_lookup<FT, FO, 1>), grid, dim3(256), 0, stream, a);
+    HK_RETURN_IF_ERROR(launch_status());
+  }
+  return hipSuccess;
+}
+template <class FT>
+hipError_t lookup_to(const Lookup& a, int64_t n, int64_t d, int e, int out_type, hipStream_t stream) {
+  return out_type == HK_TYPE_F32    ? lookup<FT, F32>(a, n, d, e, stream)
+         : out_type == HK_TYPE_BF16 ? lookup<FT, BF16>(a, n, d, e, stream)
+                                    : lookup<FT, F16>(a, n, d, e, stream);
+}
+
+// Positions a chunk: a wave's serial work, and the partial sums of a frequent row, both grow as the root of n.
+int chunk_of(int64_t n) {
+  int c = 32;
+  while (int64_t(c) * c * 16 < n && c < 4096) c *= 2;
+  return c;
+}
+int64_t chunks_of(int64_t n) { return ceil_div(n, chunk_of(n)); }
+int64_t gradient_workspace(int64_t n, int64_t d) {
+  return n <= kFew ? 0 : ceil_div(8 * n, 16) * 16 + chunks_of(n) * 2 * d * 4;
+}
+
+template <class FG, class FT, int E>
+hipError_t gradient(Grad a, hipStream_t stream) {
+  if (a.n <= kFew) {
+    // a wave a row, and workgroups for all CUs
+    a.range = static_cast<int>(std::max<int64_t>(4, ceil_div(a.vocab, 2048)));
+    hipLaunchKernelGGL((embedding_few<FG, FT, E>), dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range))), dim3(256), 0,
+                       stream, a);
+    return launch_status();
+  }
+  a.range = 64;
+  while (a.range < kMaxRange && ceil_div(a.vocab, a.range) > 1024) a.range *= 2;
+  hipLaunchKernelGGL(embedding_sort, dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range))), dim3(kSortThreads), 0,
+                     stream, a);
+  HK_RETURN_IF_ERROR(launch_status());
+  a.chunk = chunk_of(a.n);
+  a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
+  const int64_t waves = chunks_of(a.n) * a.col_blocks;
+  const dim3 grid(static_cast<unsigned>(ceil_div(waves, 4)));
+  hipLaunchKernelGGL((embedding_sum<FG, FT, E>), grid, dim3(256), 0, stream, a);
+  HK_RETURN_IF_ERROR(launch_status());
+  hipLaunchKernelGGL((embedding_combine<FT, E>), grid, dim3(256), 0, stream, a);
+  return launch_status();
+}
+template <class FG, class FT>
+hipError_t gradient_by(const Grad& a, int e, hipStream_t stream) {
+  return e == 8 ? gradient<FG, FT, 8>(a, stream) : e == 4 ? gradient<FG, FT, 4>(a, stream)
+                                                          : gradient<FG, FT, 1>(a, stream);
+}
+template <class FG>
+hipError_t gradient_to(const Grad& a, int e, int table_type, hipStream_t stream) {
+  return table_type == HK_TYPE_F32    ? gradient_by<FG, F32>(a, e, stream)
+         : table_type == HK_TYPE_BF16 ? gradient_by<FG, BF16>(a, e, stream)
+                                      : gradient_by<FG, F16>(a, e, stream);
+}
+
+constexpr int64_t kMost = int64_t(1) << 31, kStride = int64_t(1) << 40;
+bool sizes_ok(int64_t n, int64_t vocab, int64_t d) {
+  return n >= 0 && n < kMost && vocab >= 1 && vocab < kMost && d >= 1 && d < kMost;
+}
+bool gradient_ok(int64_t n, int64_t vocab, int64_t d) {
+  if (!sizes_ok(n, vocab, d) || n >= kMost / 2) return false;
+  return chunks_of(n) * ceil_div(d, 64) < (int64_t(1) << 25);  // waves of a launch
+}
+
+}  // namespace
+}  // namespace hk
+
+extern "C" hipError_t hk_embedding_forward(const void* table, int type, int64_t vocab, int64_t d, int64_t table_stride,
+                                           const void* tokens, int wide_tokens, int64_t n, float scale,
+                                           const void* residual, int64_t residual_stride, void* out, int out_type,
+                                           int64_t out_stride, hipStream_t stream) {
+  using namespace hk;
+  HK_CHECK_ARG(type_ok(type) && type_ok(out_type) && sizes_ok(n, vocab, d));
+  for (int64_t s : {table_stride, residual_stride, out_stride}) HK_CHECK_ARG(s >= 0 && s < kStride);
+  if (n == 0) return hipSuccess;
+  const int64_t et = elem(type), eo = elem(out_type), ei = wide_tokens ? 8 : 4;
+  HK_CHECK_ARG(table && tokens && out && aligned(table, et) && aligned(tokens, ei) && aligned(out, eo) &&
+               aligned(residual, eo));
+  const Rows o = Rows(out, eo, d).along(n, eo * out_stride);
+  HK_CHECK_ARG(!overlaps_itself(o) && !overlap(o, Rows(table, et, d).along(vocab, et * table_stride)) &&
+               !overlap(o, Rows(tokens, ei, n)) &&
+               !overlap_unless_same(o, Rows(residual, eo, d).along(n, eo * residual_stride)));
+  Lookup a{};
+  a.table = table, a.tokens = tokens, a.residual = residual, a.out = out, a.wide_tokens = wide_tokens;
+  a.vocab = vocab, a.table_stride = table_stride, a.residual_stride = residual_stride, a.out_stride = out_stride;
+  a.scale = scale;
+  const int e = unit(d, {{table, table_stride, et, vocab}, {residual, residual_stride, eo, n}, {out, out_stride, eo, n}});
+  return type == HK_TYPE_F32    ? lookup_to<F32>(a, n, d, e, out_type, stream)
+         : type == HK_TYPE_BF16 ? lookup_to<BF16>(a, n, d, e, out_type, stream)
+                                : lookup_to<F16>(a, n, d, e, out_type, stream);
+}
+
+extern "C" int64_t hk_embedding_workspace(int64_t n, int64_t vocab, int64_t d) {
+  return hk::gradient_ok(n, vocab, d) ? hk::gradient_workspace(n, d) : -1;
+}
+
+extern "C" hipError_t hk_embedding_backward(const void* grad, int type, int64_t n, int64_t d, int64_t grad_stride,
+                                            const void* tokens, int wide_tokens, float scale, void* grad_table,
+                                            int table_type, int64_t vocab, int64_t table_stride, int accumulate,
+                                            void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  using namespace hk;
+  HK_CHECK_ARG(type_ok(type) && type_ok(table_type) && gradient_ok(n, vocab, d));
+  HK_CHECK_ARG(grad_stride >= 0 && grad_stride < kStride && table_stride >= 0 && table_stride < kStride);
+  if (n == 0 && accumulate) return hipSuccess;
+  const int64_t eg = elem(type), et = elem(table_type), ei = wide_tokens ? 8 : 4;
+  HK_CHECK_ARG(grad_table && aligned(grad_table, et));
+  HK_CHECK_ARG(n == 0 || (grad && tokens && aligned(grad, eg) && aligned(tokens, ei)));
+  const Rows o = Rows(grad_table, et, d).along(vocab, et * table_stride);
+  HK_CHECK_ARG(!overlaps_itself(o) && !overlap(o, Rows(grad, eg, d).along(n, eg * grad_stride)) &&
+               !overlap(o, Rows(tokens, ei, n)));
+  const int64_t need = gradient_workspace(n, d);
+  if (need > 0) {
+    if (workspace) {
+      HK_CHECK_ARG(workspace_bytes >= need && aligned16(workspace));
+    } else {
+      // a graph would keep the stream's workspace, which other graphs and eager calls write too
+      if (stream_capturing(stream)) return hipErrorStreamCaptureUnsupported;
+      HK_RETURN_IF_ERROR(device_workspace(static_cast<size_t>(need), stream, &workspace));
+    }
+  }
+  Grad a{};
+  a.grad = grad, a.tokens = tokens, a.table = grad_table, a.wide_tokens = wide_tokens;
+  a.n = n, a.vocab = vocab, a.grad_stride = grad_stride, a.table_stride = table_stride, a.d = static_cast<int>(d);
+  a.scale = scale, a.accumulate = accumulate, a.table_elem = static_cast<int>(et);
+  a.sorted = static_cast<uint2*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ceil_div(8 * n, 16) * 16);
+  const int e = unit(d, {{grad, grad_stride, eg, n}, {grad_table, table_stride, et, vocab}});
+  return type == HK_TYPE_F32    ? gradient_to<F32>(a, e, table_type, stream)
+         : type == HK_TYPE_BF16 ? gradient_to<BF16>(a, e, table_type, stream)
+                                : gradient_to<F16>(a, e, table_type, stream);
+}

@@ -1,0 +1,522 @@
+// token_logprobs.hip - log probabilities of given tokens over rows of logits, with the log-sum-exp, the entropy and the
+// likeliest alternatives, and the gradient of the first and third. fp32, bf16 or fp16 logits, any row stride and
+// alignment.
+//
+//   lse = log sum_j exp(x_j),  logp = x_token - lse,  H = -sum p log p = log s - u / s
+//   with m = max x, s = sum exp(x - m), u = sum (x - m) exp(x - m);
+//   dx_j = g ([j = token] - p_j) - h p_j (x_j - lse + H).
+//
+// Forward: a workgroup holds a row (or a piece of one) in registers, so it is read once whatever follows: the maximum, then
+// both sums against it without any rescaling, then the selection. Rows that are longer than the registers, or too
+// few to fill the card, are cut into pieces that a second kernel joins. 16-byte loads from the row's first
+// 16-byte boundary on; the up to 2 x 7 elements beside them go one to a lane.
+//
+// The `top` largest: with W waves, the ceil(top / W)-th largest of each wave's 64 lane maxima is reached by that many
+// elements of the wave, so the least of those over the waves is a bound that `top` elements reach and few others do (some
+// 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, where all lanes look them through and
+// collect (value, index) keys, which are ranked by counting the larger ones. Where more pass than these lists take
+// (equal values, or a mask that leaves few), `top` passes over the row find the next largest.
+#include "hk_device.h"
+#include "hk_host.h"
+#include "hk_overlap.h"
+
+namespace hk {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTop = 64;
+constexpr int kMaxPieces = 64;
+constexpr int kList = 1024;  // candidates in LDS
+constexpr int kLanes = 128;  // lanes whose vectors LDS holds
+
+struct Row {
+  const void* x;
+  int64_t stride;  // elements
+  const void* tokens;
+  int wide_tokens;  // int64
+  int64_t vocab;
+  int64_t rows;
+  float *logp, *lse, *entropy, *top_logp;
+  int64_t* top_index;
+  int top;
+  int pieces, piece;  // pieces a row, elements a piece
+  // of each piece: (max, s, u, unused), and `top` keys
+  float4* part;
+  uint64_t* keys;
+  int64_t first;  // row of this launch's first workgroup
+};
+
+__device__ __forceinline__ int64_t token_of(const void* tokens, int wide, int64_t row) {
+  return wide ? static_cast<const int64_t*>(tokens)[row] : static_cast<const int32_t*>(tokens)[row];
+}
+
+// (value, index) as a number that is larger for larger values, and for the lower index of equal ones; NaN is under
+// all values, and 0 stands for nothing.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  uint32_t b = __float_as_uint(v + 0.f);  // -0 is 0
+  b = v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return (static_cast<uint64_t>(b) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t b = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float(b == 0 ? 0x7fc00000u : (b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ int64_t key_index(uint64_t key) {
+  return 0xffffffffu - static_cast<uint32_t>(key);
+}
+
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t k) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(k), d);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+// Ranks the n keys of `list` (all different) and hands (rank, key) of the first `top` to put. All threads.
+template <int THREADS, class Put>
+__device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int top, Put put) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+    if (rank < top) put(rank, mine);
+  }
+}
+
+template <class F, int THREADS, int V, bool ENT, bool TOP>
+__global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 4) void logprobs_kernel(Row a) {
+  constexpr int kE = F::kPerVec, W = THREADS / 64;
+  using S = typename F::storage;
+  __shared__ float red[3][W];
+  __shared__ uint64_t list[TOP ? kList : 1];
+  __shared__ uint4 stash[TOP ? kLanes * V : 1];
+  __shared__ uint16_t owner[TOP ? kLanes : 1];
+  __shared__ int count, lanes;
+
+  const int64_t item = blockIdx.x + a.first * a.pieces, row = a.pieces == 1 ? item : item / a.pieces;
+  const int pc = static_cast<int>(item - row * a.pieces);
+  const int base = pc * a.piece;  // first element of the piece
+  const int n = static_cast<int>(min(a.vocab - base, static_cast<int64_t>(a.piece)));
+  const S* x = static_cast<const S*>(a.x) + row * a.stride + base;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S));
+  const int head = min(off ? kE - off : 0, n), vecs = (n - head) / kE, tail0 = head + vecs * kE;
+  uint4 d[V];
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    d[v] = make_uint4(0, 0, 0, 0);
+    if (v * THREADS + tid < vecs) d[v] = ld_nt(xv + v * THREADS + tid);
+  }
+  // one of the elements beside the vectors
+  const int odd = tid < head ? tid : tid >= 32 && tid - 32 < n - tail0 ? tail0 + tid - 32 : -1;
+  const float x0 = odd >= 0 ? F::load(x, odd) : -INFINITY;
+
+  // calls f(value, index in the piece) for each of the lane's elements
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int at = v * THREADS + tid;
+      if (at < vecs) {
+        float e[kE];
+        F::unpack(d[v], e);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) f(e[i], head + at * kE + i);
+      }
+    }
+  };
+  float mx = x0;
+  each([&](float e, int) { mx = fmaxf(mx, e); });
+
+  float m = wave_max(mx);
+  if (TOP && tid == 0) count = lanes = 0;
+  if (W > 1) {
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = red[0][lane & (W - 1)];
+    m = row16_reduce(m, MaxOp{});  // W <= 16, and every lane of the row has one of the values
+  }
+  const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: the sums are 0
+  const float r2 = ref * kLog2e;
+  float s = 0.f, u = 0.f;
+  // as far as the compiler can see these are new: else it keeps the first pass's fp32 values of 16-bit rows
+#pragma unroll
+  for (int v = 0; v < V; ++v) asm("" : "+v"(d[v].x), "+v"(d[v].y), "+v"(d[v].z), "+v"(d[v].w));
+  auto add = [&](float e) {
+    const float t = __builtin_fmaf(e, kLog2e, -r2);  // log2 of the term
+    const float p = __builtin_amdgcn_exp2f(t);
+    s += p;
+    // -inf has p = 0 and counts for nothing; a NaN is in s
+    if (ENT) u = __builtin_fmaf(fmaxf(t, -1000.f), p, u);
+  };
+  if (odd >= 0) add(x0);
+  each([&](float e, int) { add(e); });
+  s = wave_sum(s);
+  if (ENT) u = wave_sum(u);
+  if (W > 1) {
+    if (lane == 0) red[1][wave] = s, red[2][wave] = u;
+    __syncthreads();
+    s = u = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += red[1][w], u += red[2][w];
+  }
+  u *= kLn2;
+  const float lse = ref + __logf(s);
+  if (tid == 0) {
+    if (a.pieces > 1) {
+      a.part[item] = make_float4(m, s, u, 0.f);
+    } else {
+      if (a.lse) a.lse[row] = lse;
+      if (ENT) a.entropy[row] = __logf(s) - u / s;
+      const int64_t t = token_of(a.tokens, a.wide_tokens, row);
+      a.logp[row] = t >= 0 && t < n ? F::load(x, t) - lse : __uint_as_float(0x7fc00000u);
+    }
+  }
+  if constexpr (TOP) {
+    auto put = [&](int rank, uint64_t key) {
+      if (a.pieces > 1) {
+        a.keys[item * a.top + rank] = key;
+      } else {
+        a.top_logp[row * a.top + rank] = key_value(key) - lse;
+        a.top_index[row * a.top + rank] = key_index(key);
+      }
+    };
+    // the bound
+    float left = mx, bound = -INFINITY;
+    for (int r = (a.top + W - 1) / W; r > 0; --r) {
+      bound = wave_max(left);
+      const uint64_t who = __ballot(left == bound);
+      if (who == 0 || lane == __ffsll(static_cast<unsigned long long>(who)) - 1) left = -INFINITY;
+    }
+    if (W > 1) {
+      if (lane == 0) red[0][wave] = bound;
+      __syncthreads();
+      bound = row16_reduce(red[0][lane & (W - 1)], [](float p, float q) { return fminf(p, q); });
+    }
+    auto collect = [&](float e, int i) {
+      if (!(e < bound)) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kList) list[at] = key_of(e, base + i);
+      }
+    };
+    if (!(mx < bound)) {
+      const int slot = atomicAdd(&lanes, 1);
+      if (slot < kLanes) {
+        owner[slot] = static_cast<uint16_t>(tid);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v * THREADS + tid < vecs) stash[slot * V + v] = d[v];
+      }
+      if (odd >= 0) collect(x0, odd);
+    }
+    __syncthreads();
+    const int held = lanes;
+    if (held <= kLanes) {
+      for (int i = tid; i < held * V; i += THREADS) {
+        const int at = (i % V) * THREADS + owner[i / V];
+        if (at < vecs) {
+          float e[kE];
+          F::unpack(stash[i], e);
+#pragma unroll
+          for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
+        }
+      }
+    }
+    __syncthreads();
+    const int found = count;
+    if (held <= kLanes && found <= kList) {
+      rank_keys<THREADS>(list, found, a.top, put);
+      // a piece of fewer elements
+      for (int i = found + tid; i < a.top; i += THREADS) put(i, 0);
+    } else {
+      uint64_t last = ~uint64_t(0);
+      for (int r = 0; r < a.top; ++r) {
+        uint64_t best = 0;
+        for (int i = tid; i < n; i += THREADS) {
+          const uint64_t k = key_of(F::load(x, i), base + i);
+          if (k < last && k > best) best = k;
+        }
+        best = wave_max_u64(best);
+        if (W > 1) {
+          __syncthreads();  // the round before is done with the list
+          if (lane == 0) list[wave] = best;
+          __syncthreads();
+          best = list[0];
+#pragma unroll
+          for (int w = 1; w < W; ++w) best = list[w] > best ? list[w] : best;
+        }
+        last = best;
+        if (tid == 0) put(r, best);
+      }
+    }
+  }
+}
+
+// Joins the pieces of a row.
+template <class F>
+__global__ __launch_bounds__(256) void logprobs_join(Row a) {
+  extern __shared__ uint64_t list[];
+  __shared__ int count;
+  const int64_t row = a.first + blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const bool some = lane < a.pieces;
+  const float4 p = some ? a.part[row * a.pieces + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  const float m = wave_max(p.x), ref = m == -INFINITY ? 0.f : m;
+  // a piece of nothing above -inf has sums of 0 against 0
+  const float shift = fmaxf(p.x - ref, -1000.f);  // of the piece's reference
+  const float f = p.x == -INFINITY ? 0.f : __expf(p.x - ref);
+  const float s = wave_sum(p.x == -INFINITY ? p.y : f * p.y);
+  const float u = wave_sum(p.x == -INFINITY ? 0.f : f * __builtin_fmaf(shift, p.y, p.z));
+  const float lse = ref + __logf(s);
+  if (tid == 0) {
+    if (a.lse) a.lse[row] = lse;
+    if (a.entropy) a.entropy[row] = __logf(s) - u / s;
+    using S = typename F::storage;
+    const int64_t t = token_of(a.tokens, a.wide_tokens, row);
+    a.logp[row] = t >= 0 && t < a.vocab ? F::load(static_cast<const S*>(a.x) + row * a.stride, t) - lse
+                                        : __uint_as_float(0x7fc00000u);
+    count = 0;
+  }
+  if (a.top == 0) return;
+  __syncthreads();
+  // each piece's keys fall: its ceil(top / pieces)-th bounds what can be among the first, as the waves' do above
+  const uint64_t* keys = a.keys + row * a.pieces * a.top;
+  const int r = (a.top + a.pieces - 1) / a.pieces;
+  uint64_t bound = some ? keys[lane * a.top + r - 1] : ~uint64_t(0);
+  bound = ~wave_max_u64(~bound);
+  for (int i = tid; i < a.pieces * a.top; i += 256) {
+    const uint64_t k = keys[i];
+    if (k >= bound && k != 0) list[atomicAdd(&count, 1)] = k;
+  }
+  __syncthreads();
+  rank_keys<256>(list, count, a.top, [&](int rank, uint64_t key) {
+    a.top_logp[row * a.top + rank] = key_value(key) - lse;
+    a.top_index[row * a.top + rank] = key_index(key);
+  });
+}
+
+struct Grad {
+  const void* x;
+  void* dx;
+  int64_t stride, dstride;  // elements
+  const void* tokens;
+  int wide_tokens;
+  int vocab;
+  const float *lse, *entropy, *g, *h;
+  int segments;  // workgroups a row
+  int64_t first;
+};
+
+constexpr int kGradVecs = 2;  // 16-byte vectors a lane
+
+// VEC: rows of x and dx have the same place within 16 bytes, so the vectors of one are vectors of the other.
+template <class F, bool VEC>
+__global__ __launch_bounds__(256) void logprobs_grad(Grad a) {
+  constexpr int kE = F::kPerVec;
+  using S = typename F::storage;
+  const int64_t item = blockIdx.x + a.first, row = item / a.segments;
+  const int seg = static_cast<int>(item - row * a.segments), tid = threadIdx.x;
+  const S* x = static_cast<const S*>(a.x) + row * a.stride;
+  S* dx = static_cast<S*>(a.dx) + row * a.dstride;
+  const float lse = a.lse[row];
+  const int64_t token = token_of(a.tokens, a.wide_tokens, row);
+  float g = a.g ? a.g[row] : 0.f;
+  const float h = a.h ? a.h[row] : 0.f, ent = a.h ? a.entropy[row] : 0.f;
+  // a row without a softmax has no gradient either: what the terms below leave out would hide it
+  const float all = lse - lse == 0.f ? g : __uint_as_float(0x7fc00000u);
+  auto one = [&](float e, int i) {
+    const float d = fmaxf(e - lse, -200.f);  // exp of less is 0, and -inf has to be no factor
+    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    const float t = p * __builtin_fmaf(h, d + ent, all);
+    return (i == token ? g : 0.f) - t;
+  };
+  if (VEC) {
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S));
+    const int head = min(off ? kE - off : 0, a.vocab), vecs = (a.vocab - head) / kE, tail0 = head + vecs * kE;
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    uint4* ov = reinterpret_cast<uint4*>(dx + head);
+    uint4 d[kGradVecs];
+    const int v0 = seg * (256 * kGradVecs) + tid;
+#pragma unroll
+    for (int v = 0; v < kGradVecs; ++v)
+      if (v0 + 256 * v < vecs) d[v] = ld_nt(xv + v0 + 256 * v);
+    if (seg == 0) {
+      const int odd = tid < head ? tid : tid >= 32 && tid - 32 < a.vocab - tail0 ? tail0 + tid - 32 : -1;
+      if (odd >= 0) F::store(dx, odd, one(F::load(x, odd), odd));
+    }
+#pragma unroll
+    for (int v = 0; v < kGradVecs; ++v) {
+      const int at = v0 + 256 * v;
+      if (at < vecs) {
+        float e[kE];
+        F::unpack(d[v], e);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) e[i] = one(e[i], head + at * kE + i);
+        st_nt(ov + at, F::pack(e));
+      }
+    }
+  } else {
+    const int per = 256 * kGradVecs * kE, from = seg * per;
+    for (int i = from + tid; i < min(from + per, a.vocab); i += 256) F::store(dx, i, one(F::load(x, i), i));
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+size_t elem(int type) { return type == HK_TYPE_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+constexpr int64_t kMaxVocab = int64_t(1) << 21;
+constexpr int64_t kGrid = int64_t(1) << 22;  // workgroups a launch
+
+bool shape_ok(int type, int64_t rows, int64_t vocab, int64_t stride) {
+  return type >= HK_TYPE_F32 && type <= HK_TYPE_F16 && rows >= 0 && rows < (int64_t(1) << 31) && vocab >= 1 &&
+         vocab <= kMaxVocab && stride >= 0 && stride < (int64_t(1) << 40);
+}
+
+struct Plan {
+  int threads, vecs, pieces, piece;
+};
+// One wave a row where it holds it and there are rows for all, else 512 lanes. Rows are cut where they pass 16 vectors a
+// lane, and where they leave CUs idle, into pieces of 2048 elements at least.
+Plan plan(int type, int64_t rows, int64_t vocab) {
+  const int e = 16 / static_cast<int>(elem(type)), cus = device_cu_count();
+  Plan p{512, 4, 1, static_cast<int>(vocab)};
+  // a piece may begin anywhere within 16 bytes: its vectors are no more than those of its elements
+  if (vocab <= 64 * 4 * e && (rows >= 2 * cus || vocab <= 256)) {
+    p.threads = 64;
+    return p;
+  }
+  int64_t pieces = ceil_div(vocab, int64_t(512) * 16 * e);
+  if (rows < cus) {
+    const int64_t fill = ceil_div(cus, rows > 0 ? rows : 1), most = vocab / 2048;
+    pieces = pieces > (fill < most ? fill : most) ? pieces : (fill < most ? fill : most);
+  }
+  if (pieces > kMaxPieces) pieces = kMaxPieces;
+  p.pieces = static_cast<int>(pieces < 1 ? 1 : pieces);
+  p.piece = static_cast<int>(ceil_div(ceil_div(vocab, p.pieces), e) * e);
+  p.pieces = static_cast<int>(ceil_div(vocab, p.piece));
+  p.vecs = p.piece <= 512 * 4 * e ? 4 : 16;
+  return p;
+}
+int64_t workspace_bytes_of(const Plan& p, int64_t rows, int top) {
+  return p.pieces > 1 ? rows * p.pieces * (16 + 8 * int64_t(top)) : 0;
+}
+
+template <class F, int THREADS, int V>
+hipError_t launch(const Row& a, int64_t blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(blocks)), block(THREADS);
+  if (a.top > 0) {
+    if (a.entropy) hipLaunchKernelGGL((logprobs_kernel<F, THREADS, V, true, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((logprobs_kernel<F, THREADS, V, false, true>), grid, block, 0, stream, a);
+  } else {
+    if (a.entropy) hipLaunchKernelGGL((logprobs_kernel<F, THREADS, V, true, false>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((logprobs_kernel<F, THREADS, V, false, false>), grid, block, 0, stream, a);
+  }
+  return launch_status();
+}
+template <class F>
+hipError_t run(Row a, const Plan& p, hipStream_t stream) {
+  const int64_t step = kGrid / p.pieces;
+  for (a.first = 0; a.first < a.rows; a.first += step) {
+    const int64_t rows = a.rows - a.first < step ? a.rows - a.first : step, blocks = rows * p.pieces;
+    HK_RETURN_IF_ERROR(p.threads == 64 ? (launch<F, 64, 4>(a, blocks, stream))
+                       : p.vecs == 4   ? (launch<F, 512, 4>(a, blocks, stream))
+                                       : (launch<F, 512, 16>(a, blocks, stream)));
+    if (p.pieces > 1) {
+      hipLaunchKernelGGL(logprobs_join<F>, dim3(static_cast<unsigned>(rows)), dim3(256),
+                         static_cast<size_t>(8) * p.pieces * a.top, stream, a);
+      HK_RETURN_IF_ERROR(launch_status());
+    }
+  }
+  return hipSuccess;
+}
+
+template <class F>
+hipError_t run_grad(Grad a, int64_t rows, bool vec, hipStream_t stream) {
+  const int64_t items = rows * a.segments;
+  for (a.first = 0; a.first < items; a.first += kGrid) {
+    const dim3 grid(static_cast<unsigned>(items - a.first < kGrid ? items - a.first : kGrid));
+    if (vec) hipLaunchKernelGGL((logprobs_grad<F, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((logprobs_grad<F, false>), grid, dim3(256), 0, stream, a);
+    HK_RETURN_IF_ERROR(launch_status());
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+}  // namespace hk
+
+extern "C" int64_t hk_token_logprobs_workspace(int type, int64_t rows, int64_t vocab, int top) {
+  if (!hk::shape_ok(type, rows, vocab, vocab) || top < 0 || top > hk::kMaxTop || top > vocab) return -1;
+  return hk::workspace_bytes_of(hk::plan(type, rows, vocab), rows, top);
+}
+
+extern "C" hipError_t hk_token_logprobs(const void* logits, int type, int64_t rows, int64_t vocab, int64_t row_stride,
+                                        const void* tokens, int wide_tokens, float* logp, float* lse, float* entropy,
+                                        int top, float* top_logp, int64_t* top_index, void* workspace,
+                                        int64_t workspace_bytes, hipStream_t stream) {
+  HK_CHECK_ARG(hk::shape_ok(type, rows, vocab, row_stride) && top >= 0 && top <= hk::kMaxTop && top <= vocab);
+  if (rows == 0) return hipSuccess;
+  const int64_t es = static_cast<int64_t>(hk::elem(type)), et = wide_tokens ? 8 : 4;
+  HK_CHECK_ARG(logits && tokens && logp && hk::aligned(logits, es) && hk::aligned(tokens, et) && hk::aligned(logp, 4) &&
+               hk::aligned(lse, 4) && hk::aligned(entropy, 4));
+  HK_CHECK_ARG(top == 0 || (top_logp && top_index && hk::aligned(top_logp, 4) && hk::aligned(top_index, 8)));
+  const hk::Rows in[2] = {hk::Rows(logits, es, vocab).along(rows, es * row_stride), hk::Rows(tokens, et, rows)};
+  const hk::Rows out[5] = {hk::Rows(logp, 4, rows), hk::Rows(lse, 4, rows), hk::Rows(entropy, 4, rows),
+                           hk::Rows(top ? top_logp : nullptr, 4, rows * top),
+                           hk::Rows(top ? top_index : nullptr, 8, rows * top)};
+  for (int i = 0; i < 5; ++i) {
+    HK_CHECK_ARG(!hk::overlap(out[i], in[0]) && !hk::overlap(out[i], in[1]));
+    for (int j = 0; j < i; ++j) HK_CHECK_ARG(!hk::overlap(out[i], out[j]));
+  }
+  const hk::Plan p = hk::plan(type, rows, vocab);
+  hk::Row a{};
+  a.x = logits, a.stride = row_stride, a.tokens = tokens, a.wide_tokens = wide_tokens;
+  a.vocab = vocab, a.rows = rows, a.logp = logp, a.lse = lse, a.entropy = entropy;
+  a.top_logp = top_logp, a.top_index = top_index, a.top = top, a.pieces = p.pieces, a.piece = p.piece;
+  if (const int64_t need = hk::workspace_bytes_of(p, rows, top)) {
+    if (workspace) {
+      HK_CHECK_ARG(workspace_bytes >= need && hk::aligned16(workspace));
+    } else {
+      // a graph would keep the stream's workspace, which other graphs and eager calls write too
+      if (hk::stream_capturing(stream)) return hipErrorStreamCaptureUnsupported;
+      HK_RETURN_IF_ERROR(hk::device_workspace(static_cast<size_t>(need), stream, &workspace));
+    }
+    a.part = static_cast<float4*>(workspace);
+    a.keys = reinterpret_cast<uint64_t*>(a.part + rows * p.pieces);
+  }
+  return type == HK_TYPE_F32    ? hk::run<hk::F32>(a, p, stream)
+         : type == HK_TYPE_BF16 ? hk::run<hk::BF16>(a, p, stream)
+                                : hk::run<hk::F16>(a, p, stream);
+}
+
+extern "C" hipError_t hk_token_logprobs_backward(const void* logits, int type, int64_t rows, int64_t vocab,
+                                                 int64_t row_stride, const void* tokens, int wide_tokens,
+                                                 const float* lse, const float* entropy, const float* grad_logp,
+                                                 const float* grad_entropy, void* grad, int64_t grad_stride,
+                                                 hipStream_t stream) {
+  HK_CHECK_ARG(hk::shape_ok(type, rows, vocab, row_stride) && hk::shape_ok(type, rows, vocab, grad_stride));
+  if (rows == 0) return hipSuccess;
+  const int64_t es = static_cast<int64_t>(hk::elem(type)), et = wide_tokens ? 8 : 4;
+  HK_CHECK_ARG(logits && tokens && lse && grad && hk::aligned(logits, es) && hk::aligned(grad, es) &&
+               hk::aligned(tokens, et) && hk::aligned(lse, 4) && hk::aligned(entropy, 4) && hk::aligned(grad_logp, 4) &&
+               hk::aligned(grad_entropy, 4) && (!grad_entropy || entropy));
+  const hk::Rows x = hk::Rows(logits, es, vocab).along(rows, es * row_stride);
+  const hk::Rows dx = hk::Rows(grad, es, vocab).along(rows, es * grad_stride);
+  HK_CHECK_ARG(!hk::overlaps_itself(dx) && !hk::overlap_unless_same(dx, x) &&
+               !hk::overlap(dx, hk::Rows(tokens, et, rows)));
+  for (const float* p : {lse, entropy, grad_logp, grad_entropy}) HK_CHECK_ARG(!hk::overlap(dx, hk::Rows(p, 4, rows)));
+  hk::Grad a{};
+  a.x = logits, a.dx = grad, a.stride = row_stride, a.dstride = grad_stride;
+  a.tokens = tokens, a.wide_tokens = wide_tokens, a.vocab = static_cast<int>(vocab);
+  a.lse = lse, a.entropy = entropy, a.g = grad_logp, a.h = grad_entropy;
+  a.segments = static_cast<int>(hk::ceil_div(vocab, 256 * hk::kGradVecs * (16 / es)));
+  const uintptr_t apart = reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad);
+  const bool vec = (apart & 15) == 0 && (rows == 1 || (es * (row_stride - grad_stride)) % 16 == 0);
+  return type == HK_TYPE_F32    ? hk::run_grad<hk::F32>(a, rows, vec, stream)
+         : type == HK_TYPE_BF16 ? hk::run_grad<hk::BF16>(a, rows, vec, stream)
+                                : hk::run_grad<hk::F16>(a, rows, vec, stream);
+}

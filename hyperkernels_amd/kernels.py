@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import torch
 
@@ -21,7 +21,9 @@ __all__ = [
     "ln_backward_gamma_beta", "layer_norm_backward", "sparse_ce_forward", "sparse_ce_backward",
     "AdamLaunchMetadata", "multi_tensor_adam", "AdamPlan", "Adam8Plan", "ADAM8_BLOCK",
     "adam8_states", "adam8_quantize", "adam8_dequantize", "qk_norm_rope_forward",
-    "qk_norm_rope_backward", "attn_packed_forward", "attn_packed_backward", "ReductionLayout",
+    "qk_norm_rope_backward", "attn_packed_forward", "attn_packed_backward",
+    "TokenLogprobs", "token_logprobs", "token_logprobs_backward", "embedding_forward", "embedding_backward",
+    "ReductionLayout",
     "unified_reduce_sum", "reduce_generic", "REDUCE_INNER", "REDUCE_OUTER", "REDUCE_GENERIC",
 ]
 
@@ -865,6 +867,142 @@ def attn_packed_backward(do, q, k, v, o, lse, cu_q, cu_k=None, causal: bool = Tr
     kind = _TYPE[q.dtype]
     _call_captured("hk_attn_packed_backward", lambda: lib().hk_attn_packed_workspace(p, kind, 1), p, kind)
     return dq, dk, dv
+
+
+# ----------------------------------------------------------------------------------------------
+# Log probabilities of given tokens (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns; None for what was not asked for."""
+
+    logp: torch.Tensor
+    lse: torch.Tensor
+    entropy: torch.Tensor | None
+    top_logp: torch.Tensor | None
+    top_index: torch.Tensor | None
+
+
+_WIDE = {torch.int32: 0, torch.int64: 1}
+
+
+def _logits(fn: str, x: torch.Tensor, tokens: torch.Tensor) -> tuple[int, int, int, int]:
+    """(device, rows, vocabulary, row stride) of logits [rows, vocabulary] and their tokens."""
+    if x.dim() != 2 or x.dtype not in _TYPE or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{fn}: fp32, bf16 or fp16 logits [rows, vocabulary] with a unit last-dim stride")
+    dev, (rows, vocab) = _device(fn, x), x.shape
+    if vocab == 0:
+        raise ValueError(f"{fn}: a vocabulary of one word at least")
+    _tokens(fn, tokens, dev, rows)
+    return dev, rows, vocab, x.stride(0) if rows > 1 else vocab
+
+
+def _tokens(fn: str, t: torch.Tensor, dev: int, n: int) -> None:
+    if t.dtype not in _WIDE or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{fn}: tokens are int32 or int64 [{n}], contiguous, on the device")
+
+
+def _row_values(fn: str, name: str, t: torch.Tensor | None, dev: int, shape, dtype=_F32) -> int | None:
+    """The address of one value (or `top` of them) a row."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{fn}: {name} is {dtype} {list(shape)}, contiguous, on the device")
+    return t.data_ptr()
+
+
+def token_logprobs(logits, tokens, entropy=False, top: int = 0, logp=None, lse=None, top_logp=None,
+                   top_index=None) -> TokenLogprobs:
+    """Per row of logits (fp32, bf16 or fp16 [rows, vocabulary], any row stride): the log probability of the row's
+    token, the log-sum-exp, and where asked for the entropy (True, or an output) and the `top` largest log
+    probabilities with their indices, falling, of equal ones the lowest index first. All fp32, indices int64."""
+    fn = "token_logprobs"
+    dev, rows, vocab, stride = _logits(fn, logits, tokens)
+    if not 0 <= top <= min(64, vocab):
+        raise ValueError(f"{fn}: top is 64 at most, and the vocabulary")
+    new = lambda dt, *shape: torch.empty(shape, device=logits.device, dtype=dt)  # noqa: E731
+    logp = new(_F32, rows) if logp is None else logp
+    lse = new(_F32, rows) if lse is None else lse
+    ent = new(_F32, rows) if entropy is True else None if entropy is False else entropy
+    if top:
+        top_logp = new(_F32, rows, top) if top_logp is None else top_logp
+        top_index = new(torch.int64, rows, top) if top_index is None else top_index
+    elif top_logp is not None or top_index is not None:
+        raise ValueError(f"{fn}: outputs of alternatives that are not asked for")
+    kind = _TYPE[logits.dtype]
+    _call_captured("hk_token_logprobs", lambda: lib().hk_token_logprobs_workspace(kind, rows, vocab, top),
+                   logits.data_ptr(), kind, rows, vocab, stride, tokens.data_ptr(), _WIDE[tokens.dtype],
+                   _row_values(fn, "logp", logp, dev, (rows,)), _row_values(fn, "lse", lse, dev, (rows,)),
+                   _row_values(fn, "entropy", ent, dev, (rows,)), top,
+                   _row_values(fn, "top_logp", top_logp, dev, (rows, top)),
+                   _row_values(fn, "top_index", top_index, dev, (rows, top), torch.int64))
+    return TokenLogprobs(logp, lse, ent, top_logp, top_index)
+
+
+def token_logprobs_backward(logits, tokens, lse, grad_logp=None, entropy=None, grad_entropy=None, grad=None):
+    """The gradient of the logits, of their type, from those of logp and of the entropy (fp32 [rows]; None: zero) and
+    token_logprobs' lse and entropy. grad may be the logits themselves."""
+    fn = "token_logprobs_backward"
+    dev, rows, vocab, stride = _logits(fn, logits, tokens)
+    grad = torch.empty((rows, vocab), device=logits.device, dtype=logits.dtype) if grad is None else grad
+    if grad.dtype is not logits.dtype or grad.shape != logits.shape or grad.get_device() != dev or (
+            vocab > 1 and grad.stride(1) != 1):
+        raise ValueError(f"{fn}: grad has the logits' type and shape, with a unit last-dim stride")
+    if lse is None or (grad_entropy is not None and entropy is None):
+        raise ValueError(f"{fn}: lse, and for its gradient the entropy, are needed")
+    call("hk_token_logprobs_backward", logits.data_ptr(), _TYPE[logits.dtype], rows, vocab, stride,
+         tokens.data_ptr(), _WIDE[tokens.dtype], _row_values(fn, "lse", lse, dev, (rows,)),
+         _row_values(fn, "entropy", entropy, dev, (rows,)), _row_values(fn, "grad_logp", grad_logp, dev, (rows,)),
+         _row_values(fn, "grad_entropy", grad_entropy, dev, (rows,)), grad.data_ptr(),
+         grad.stride(0) if rows > 1 else vocab, _stream())
+    return grad
+
+
+# ----------------------------------------------------------------------------------------------
+# Embedding lookup and the table's gradient (no counterpart in the reference)
+# ----------------------------------------------------------------------------------------------
+def _rows_of(fn: str, name: str, t: torch.Tensor, dev: int, shape) -> tuple[int, int, int]:
+    """(address, type, row stride) of a matrix."""
+    if t.dtype not in _TYPE or t.shape != shape or t.get_device() != dev or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{fn}: {name} is fp32, bf16 or fp16 {list(shape)} with a unit last-dim stride, on the device")
+    return t.data_ptr(), _TYPE[t.dtype], t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def embedding_forward(table, tokens, scale: float = 1.0, residual=None, out=None, out_dtype=None):
+    """scale * table[tokens] + residual: table [vocabulary, d], tokens [n], residual and out [n, d]; each of fp32, bf16
+    or fp16, residual of out's type (it may be out). out_dtype: of an out that is not passed (None: the table's). A
+    token outside the table gives a row of NaN."""
+    fn = "embedding_forward"
+    if table.dim() != 2 or tokens.dim() != 1:
+        raise ValueError(f"{fn}: a table [vocabulary, d] and tokens [n]")
+    dev, (vocab, d), n = _device(fn, table), table.shape, tokens.shape[0]
+    _tokens(fn, tokens, dev, n)
+    out = torch.empty((n, d), device=table.device, dtype=out_dtype or table.dtype) if out is None else out
+    tp, tt, ts = _rows_of(fn, "table", table, dev, (vocab, d))
+    op, ot, os_ = _rows_of(fn, "out", out, dev, (n, d))
+    rp = rs = 0
+    if residual is not None:
+        rp, rt, rs = _rows_of(fn, "residual", residual, dev, (n, d))
+        if rt != ot:
+            raise ValueError(f"{fn}: residual has out's type")
+    call("hk_embedding_forward", tp, tt, vocab, d, ts, tokens.data_ptr(), _WIDE[tokens.dtype], n, scale, rp, rs, op, ot,
+         os_, _stream())
+    return out
+
+
+def embedding_backward(grad, tokens, grad_table, scale: float = 1.0, accumulate: bool = True):
+    """The table's gradient from that of embedding_forward's output: scale times the sum of grad's rows [n, d] over the
+    tokens of each row of grad_table [vocabulary, d], added to it, or, where accumulate is False, written, zero for
+    rows without a token. Each of fp32, bf16 or fp16; sums in fp32 and a fixed order. Returns grad_table."""
+    fn = "embedding_backward"
+    if grad.dim() != 2 or grad_table.dim() != 2:
+        raise ValueError(f"{fn}: grad [n, d] and grad_table [vocabulary, d]")
+    dev, (n, d), vocab = _device(fn, grad), grad.shape, grad_table.shape[0]
+    _tokens(fn, tokens, dev, n)
+    gp, gt, gs = _rows_of(fn, "grad", grad, dev, (n, d))
+    tp, tt, ts = _rows_of(fn, "grad_table", grad_table, dev, (vocab, d))
+    _call_captured("hk_embedding_backward", lambda: lib().hk_embedding_workspace(n, vocab, d), gp, gt, n, d, gs,
+                   tokens.data_ptr(), _WIDE[tokens.dtype], scale, tp, tt, vocab, ts, accumulate)
+    return grad_table
 
 
 # ----------------------------------------------------------------------------------------------

@@ -761,6 +761,60 @@ HK_API hipError_t hk_attn_packed_backward(const hk_attn_packed_params* params, i
                                           int64_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Log probabilities of given tokens over rows of logits, with the entropy and the likeliest alternatives, and their
+ * gradient. No counterpart in the reference (its cross-entropy, above, takes fp32 logits without gaps).
+ * Row r is logits[r * row_stride .. + vocab) of HK_TYPE_* `type`; any row_stride (the padding of a row is not read)
+ * and any alignment of the type. tokens: int32, or int64 where wide_tokens is set.
+ *   lse = log sum_j exp(x_j),  logp = x[token] - lse,  entropy = -sum_j p_j log p_j  (p = exp(x - lse))
+ * and, where top > 0, the `top` largest log probabilities of the row, falling, with their indices (of equal ones the
+ * lowest index first; NaN counts as less than everything): [rows, top] each. lse and entropy may be NULL: not
+ * wanted. x = -inf has p = 0 and counts for nothing. A row that holds a NaN or +inf, or nothing above -inf, has
+ * no softmax: logp, entropy and top_logp are NaN (indices are as above). A token outside 0 .. vocab - 1 has logp NaN.
+ * The gradient of the logits, from those of logp and entropy (each may be NULL: zero; grad_entropy needs the forward's
+ * entropy) and the forward's lse:
+ *   dx_j = grad_logp ([j == token] - p_j) - grad_entropy p_j (x_j - lse + entropy),
+ * without the first term's one-hot for a token out of range, and NaN for a row without a softmax. grad is of the
+ * logits' type, rows grad_stride apart, and may be the logits themselves (with their stride). Sums are fp32; the
+ * gradient is rounded once.
+ * vocab is 1 .. 2^21, top at most 64 and vocab, rows below 2^31. No output may share memory with anything else of
+ * the call. Workspace: hk_token_logprobs_workspace bytes (rows that are cut into pieces; -1: invalid arguments), as
+ * for hk_attn_packed_forward.
+ * ---------------------------------------------------------------------------------------- */
+HK_API int64_t hk_token_logprobs_workspace(int type, int64_t rows, int64_t vocab, int top);
+HK_API hipError_t hk_token_logprobs(const void* logits, int type, int64_t rows, int64_t vocab, int64_t row_stride,
+                                    const void* tokens, int wide_tokens, float* logp, float* lse, float* entropy,
+                                    int top, float* top_logp, int64_t* top_index, void* workspace,
+                                    int64_t workspace_bytes, hipStream_t stream);
+HK_API hipError_t hk_token_logprobs_backward(const void* logits, int type, int64_t rows, int64_t vocab,
+                                             int64_t row_stride, const void* tokens, int wide_tokens,
+                                             const float* lse, const float* entropy, const float* grad_logp,
+                                             const float* grad_entropy, void* grad, int64_t grad_stride,
+                                             hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Embedding lookup and the table's gradient. No counterpart in the reference.
+ *   forward   out[i] = scale * table[tokens[i]] + residual[i]           (residual NULL: none)
+ *   backward  grad_table[v] (+)= scale * the sum of grad[i] over the i with tokens[i] == v
+ * for n tokens (int32, or int64 where wide_tokens is set) and rows of d elements of the HK_TYPE_* types given, any
+ * row stride and any alignment of the type. Arithmetic is fp32, with one rounding. residual is of out's type and
+ * may be out itself (with its stride). A token outside 0 .. vocab - 1 gives a row of NaN and has no gradient.
+ * The backward pass writes every row of grad_table (zero for those without a token), or, where accumulate is set, adds
+ * to those of the batch's tokens and touches no other. Each row's sum has a fixed order, the tokens' own but for
+ * rows of many tokens, which are summed in shares. Workspace: hk_embedding_workspace bytes (-1: invalid arguments), as for hk_attn_packed_forward.
+ * n, vocab and d are below 2^31 (n of the backward pass below 2^30). No output may otherwise share memory with
+ * anything else of the call, nor two of its rows with each other.
+ * ---------------------------------------------------------------------------------------- */
+HK_API hipError_t hk_embedding_forward(const void* table, int type, int64_t vocab, int64_t d, int64_t table_stride,
+                                       const void* tokens, int wide_tokens, int64_t n, float scale,
+                                       const void* residual, int64_t residual_stride, void* out, int out_type,
+                                       int64_t out_stride, hipStream_t stream);
+HK_API int64_t hk_embedding_workspace(int64_t n, int64_t vocab, int64_t d);
+HK_API hipError_t hk_embedding_backward(const void* grad, int type, int64_t n, int64_t d, int64_t grad_stride,
+                                        const void* tokens, int wide_tokens, float scale, void* grad_table,
+                                        int table_type, int64_t vocab, int64_t table_stride, int accumulate,
+                                        void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement
  * ---------------------------------------------------------------------------------------- */
 /* HBM stream with a given read/write mix. No counterpart in the reference: a measurement aid for
