@@ -4,12 +4,13 @@
 // Both are bound by memory. The gradient has to be the same whatever the order in which workgroups run, and texts repeat a
 // few words very often, so rows are neither added atomically nor owned by one workgroup each:
 //   embedding_sort     a workgroup per range of table rows reads all tokens (from L2), counts those below its range, which
-//                      is where its part of the sorted order begins, and places its own by row, in the tokens' order. It
-//                      also writes the rows without a token, most of a large table, while it has little else to do.
+//                      is where its part of the sorted order begins, and places its own by row, in the tokens' order.
+//                      Workgroups behind these clear the table meanwhile: the sort is latency, the clearing bandwidth.
 //   embedding_sum      the sorted order in equal chunks, a wave each and 64 units of columns: rows that lie inside a chunk
 //                      are written, the parts of those that go on across its ends are left as partial sums,
 //   embedding_combine  which are added in order where such a row begins.
 // Few tokens take one launch: each workgroup finds its rows' tokens and sums them itself.
+#include <algorithm>
 #include <initializer_list>
 
 #include "hk_device.h"
@@ -102,6 +103,8 @@ struct Grad {
   float scale;
   int accumulate;
   int range;        // table rows a workgroup (sort, few)
+  int ranges;       // workgroups that sort
+  int clear;        // table rows that each of the others clears
   int table_elem;   // bytes
   int chunk;        // positions a chunk
   int col_blocks;   // waves a chunk
@@ -134,6 +137,11 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   __shared__ uint2 list[kTileTokens];
   __shared__ int sums[kSortWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  if (static_cast<int>(blockIdx.x) >= a.ranges) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x - a.ranges) * a.clear;
+    for (int r = wave; r < a.clear && first + r < a.vocab; r += kSortWaves) zero_row(a, first + r, lane, 64);
+    return;
+  }
   const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
   const int rows = static_cast<int>(min(static_cast<uint64_t>(a.range), static_cast<uint64_t>(a.vocab) - lo));
 
@@ -162,10 +170,6 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   for (int w = 0; w < kSortWaves; ++w) below += sums[w];
   __syncthreads();
 
-  if (!a.accumulate)
-    for (int r = wave; r < rows; r += kSortWaves)
-      if (count[r] == 0) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
-  __syncthreads();
   // count[r]: the first place of row r in the sorted order
   {
     constexpr int kPer = kMaxRange / kSortThreads;
@@ -285,95 +289,121 @@ __device__ __forceinline__ void put_row(const Grad& a, uint32_t row, int col, fl
   store<FT, E>(a.table, at, f);
 }
 
-constexpr int kAhead = 8;  // rows in flight
+constexpr int kAhead = 16;   // rows in flight
+constexpr int kWindow = 32;  // positions that a wave reads at once
+
+// The wave's chunk and columns. All but the column is the same for the whole wave, and kept in scalar registers.
+struct Place {
+  int64_t chunk, from, to;
+  int col;
+  __device__ Place(const Grad& a, int unit) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+    chunk = item / a.col_blocks;
+    col = (static_cast<int>(item - chunk * a.col_blocks) * 64 + (threadIdx.x & 63)) * unit;
+    from = chunk * a.chunk, to = min(from + a.chunk, a.n);
+  }
+};
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+  return __builtin_amdgcn_readlane(v, lane);
+}
 
 template <class FG, class FT, int E>
 __global__ __launch_bounds__(256) void embedding_sum(Grad a) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t chunk = item / a.col_blocks;
-  const int lane = threadIdx.x & 63, col = (static_cast<int>(item - chunk * a.col_blocks) * 64 + lane) * E;
-  const int64_t from = chunk * a.chunk;
-  if (from >= a.n) return;
-  const int64_t to = min(from + a.chunk, a.n);
-  const uint32_t before = from > 0 ? a.sorted[from - 1].y : ~0u, behind = to < a.n ? a.sorted[to].y : ~0u;
-  const bool mine = col < a.d;
+  const Place w(a, E);
+  if (w.from >= a.n) return;
+  const int lane = threadIdx.x & 63;
+  const bool mine = w.col < a.d;
   float acc[E] = {};
-  uint32_t row = a.sorted[from].y;
-  if (row == ~0u) return;
-  auto flush = [&](bool last) {
-    if (!mine) return;
-    if (row == before || (last && row == behind)) {
-      float* p = a.part + (chunk * 2 + (row == before ? 0 : 1)) * a.d + col;
+  uint32_t before = ~0u, row = ~0u;
+  auto flush = [&](bool partial) {
+    if (row == ~0u || !mine) return;
+    if (row == before || partial) {
+      float* p = a.part + (w.chunk * 2 + (row == before ? 0 : 1)) * a.d + w.col;
 #pragma unroll
       for (int e = 0; e < E; ++e) p[e] = acc[e];
     } else {
-      put_row<FT, E>(a, row, col, acc);
+      put_row<FT, E>(a, row, w.col, acc);
     }
   };
-  for (int64_t p0 = from; p0 < to; p0 += kAhead) {
-    uint2 s[kAhead];
-    float x[kAhead][E];
+  for (int64_t p0 = w.from; p0 < w.to; p0 += kWindow) {
+    // lane l: position p0 + l - 1, from the one before the window to the one behind it
+    const int64_t at = p0 + lane - 1;
+    const uint2 s = lane <= kWindow + 1 && at >= 0 && at < a.n ? a.sorted[at] : make_uint2(0, ~0u);
+    if (p0 == w.from) before = lane_value(s.y, 0);
+    const int count = static_cast<int>(min(w.to - p0, static_cast<int64_t>(kWindow)));
+    for (int half = 0; half < kWindow / kAhead; ++half) {
+      const int q0 = half * kAhead;
+      if (q0 >= count) break;
+      float x[kAhead][E];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) s[u] = p0 + u < to ? a.sorted[p0 + u] : make_uint2(0, ~0u);
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (s[u].y != ~0u && mine) load<FG, E>(a.grad, static_cast<int64_t>(s[u].x) * a.grad_stride + col, x[u]);
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (s[u].y == ~0u) continue;
-      if (s[u].y != row) {
-        flush(false);
-        row = s[u].y;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t r = q0 + u < count ? lane_value(s.y, q0 + u + 1) : ~0u;
+        if (r != ~0u && mine)
+          load<FG, E>(a.grad, static_cast<int64_t>(lane_value(s.x, q0 + u + 1)) * a.grad_stride + w.col, x[u]);
       }
-      if (mine)
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t r = q0 + u < count ? lane_value(s.y, q0 + u + 1) : ~0u;
+        if (r == ~0u) continue;
+        if (r != row) {
+          flush(false);
+          row = r;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = 0.f;
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += x[u][e];
+      }
     }
+    if (p0 + count == w.to) flush(row == lane_value(s.y, count + 1));
   }
-  flush(true);
 }
 
 // The row that begins in a chunk and goes on behind it: its part of this chunk, and of the chunks that it goes on into.
 template <class FT, int E>
 __global__ __launch_bounds__(256) void embedding_combine(Grad a) {
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t chunk = item / a.col_blocks;
-  const int lane = threadIdx.x & 63, col = (static_cast<int>(item - chunk * a.col_blocks) * 64 + lane) * E;
-  const int64_t from = chunk * a.chunk, to = from + a.chunk;
-  if (to >= a.n) return;
-  const uint32_t row = a.sorted[to].y;
-  if (row == ~0u || a.sorted[to - 1].y != row || (from > 0 && a.sorted[from - 1].y == row)) return;
-  const bool mine = col < a.d;
+  const Place w(a, E);
+  if (w.to >= a.n) return;
+  const int lane = threadIdx.x & 63;
+  const bool mine = w.col < a.d;
+  // the rows at the ends of the chunk, and at the beginnings of the next ones
+  const int64_t end = lane == 0 ? w.to : lane == 1 ? w.to - 1 : w.from - 1;
+  const uint32_t ends = lane < 3 && end >= 0 ? a.sorted[end].y : ~0u;
+  auto begins = [&](int64_t c) {
+    const int64_t first = (c + lane) * a.chunk;
+    return first < a.n ? a.sorted[first].y : ~0u;
+  };
+  uint32_t next = begins(w.chunk + 1);
   float acc[E] = {};
   if (mine)
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = a.part[(chunk * 2 + 1) * a.d + col + e];
-  for (int64_t c = chunk + 1;; c += 64) {
+    for (int e = 0; e < E; ++e) acc[e] = a.part[(w.chunk * 2 + 1) * a.d + w.col + e];
+  const uint32_t row = lane_value(ends, 0);
+  if (row == ~0u || lane_value(ends, 1) != row || lane_value(ends, 2) == row) return;
+  for (int64_t c = w.chunk + 1;; c += 64, next = begins(c)) {
     // how many of the next chunks begin with it
-    const int64_t first = (c + lane) * a.chunk;
-    const uint64_t on = __ballot(first < a.n && a.sorted[first < a.n ? first : to].y == row);
+    const uint64_t on = __ballot(next == row);
     const int more = ~on ? __ffsll(static_cast<unsigned long long>(~on)) - 1 : 64;
     if (mine)
-      for (int i = 0; i < more; i += 4) {
-        float x[4][E];
+      for (int i = 0; i < more; i += kAhead) {
+        float x[kAhead][E];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-          for (int e = 0; e < E; ++e) x[u][e] = i + u < more ? a.part[(c + i + u) * 2 * a.d + col + e] : 0.f;
+          for (int e = 0; e < E; ++e) x[u][e] = i + u < more ? a.part[(c + i + u) * 2 * a.d + w.col + e] : 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kAhead; ++u)
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += x[u][e];
       }
     if (more < 64) break;
   }
-  if (mine) put_row<FT, E>(a, row, col, acc);
+  if (mine) put_row<FT, E>(a, row, w.col, acc);
 }
 
 // Few tokens: a workgroup finds those of its rows and sums them in order.
-constexpr int kFew = 512;
+constexpr int kFew = 1024;
 template <class FG, class FT, int E>
 __global__ __launch_bounds__(256) void embedding_few(Grad a) {
   __shared__ uint2 list[kFew];
@@ -414,11 +444,11 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
     bool any = false;
     for (int i = 0; i < total; i += 64) any |= __any(i + lane < total && list[min(i + lane, total - 1)].y == r);
     if (!any) {
-      if (!a.accumulate) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
+      if (!a.accumulate && blockIdx.y == 0) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
       continue;
     }
-    for (int c0 = 0; c0 < a.d; c0 += 64 * E) {
-      const int col = c0 + lane * E;
+    for (int c0 = blockIdx.y; c0 < a.col_blocks; c0 += gridDim.y) {
+      const int col = (c0 * 64 + lane) * E;
       const bool mine = col < a.d;
       float acc[E] = {};
       for (int i = 0; i < total; i += 64) {
@@ -457,8 +487,8 @@ struct Matrix {
   int64_t stride, elem;
   int64_t rows;
 };
-int unit(int64_t d, std::initializer_list<Matrix> ts) {
-  for (int e = 8; e >= 4; e /= 2) {
+int unit(int64_t d, int most, std::initializer_list<Matrix> ts) {
+  for (int e = most; e >= 4; e /= 2) {
     bool all = d % e == 0;
     for (const Matrix& t : ts) {
       const int64_t bytes = e * t.elem < 16 ? e * t.elem : 16;
@@ -492,8 +522,8 @@ hipError_t lookup_to(const Lookup& a, int64_t n, int64_t d, int e, int out_type,
 
 // Positions a chunk: a wave's serial work, and the partial sums of a frequent row, both grow as the root of n.
 int chunk_of(int64_t n) {
-  int c = 32;
-  while (int64_t(c) * c * 16 < n && c < 4096) c *= 2;
+  int c = kAhead;
+  while (int64_t(c) * c * 32 < n && c < 4096) c *= 2;
   return c;
 }
 int64_t chunks_of(int64_t n) { return ceil_div(n, chunk_of(n)); }
@@ -504,16 +534,26 @@ int64_t gradient_workspace(int64_t n, int64_t d) {
 template <class FG, class FT, int E>
 hipError_t gradient(Grad a, hipStream_t stream) {
   if (a.n <= kFew) {
-    // a wave a row, and workgroups for all CUs
+    // A wave a row, and workgroups for all CUs; a frequent row is a chain of loads, so its columns go to several (333
+    // tokens, 1009 x 131: 11.7 -> 6.4 us).
     a.range = static_cast<int>(std::max<int64_t>(4, ceil_div(a.vocab, 2048)));
-    hipLaunchKernelGGL((embedding_few<FG, FT, E>), dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range))), dim3(256), 0,
-                       stream, a);
+    a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
+    hipLaunchKernelGGL((embedding_few<FG, FT, E>),
+                       dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range)), std::min(a.col_blocks, 16)), dim3(256),
+                       0, stream, a);
     return launch_status();
   }
+  // as many ranges as half of the workgroups that the card holds at once
   a.range = 64;
-  while (a.range < kMaxRange && ceil_div(a.vocab, a.range) > 1024) a.range *= 2;
-  hipLaunchKernelGGL(embedding_sort, dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range))), dim3(kSortThreads), 0,
-                     stream, a);
+  while (a.range < kMaxRange && ceil_div(a.vocab, a.range) > device_cu_count()) a.range *= 2;
+  a.ranges = static_cast<int>(ceil_div(a.vocab, a.range));
+  int64_t blocks = a.ranges;
+  if (!a.accumulate) {
+    // 64 KiB a workgroup, and not more workgroups than a launch takes
+    a.clear = static_cast<int>(std::max<int64_t>({kSortWaves, 65536 / (int64_t(a.d) * a.table_elem), a.vocab >> 20}));
+    blocks += ceil_div(a.vocab, a.clear);
+  }
+  hipLaunchKernelGGL(embedding_sort, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), 0, stream, a);
   HK_RETURN_IF_ERROR(launch_status());
   a.chunk = chunk_of(a.n);
   a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
@@ -526,8 +566,7 @@ hipError_t gradient(Grad a, hipStream_t stream) {
 }
 template <class FG, class FT>
 hipError_t gradient_by(const Grad& a, int e, hipStream_t stream) {
-  return e == 8 ? gradient<FG, FT, 8>(a, stream) : e == 4 ? gradient<FG, FT, 4>(a, stream)
-                                                          : gradient<FG, FT, 1>(a, stream);
+  return e == 4 ? gradient<FG, FT, 4>(a, stream) : gradient<FG, FT, 1>(a, stream);
 }
 template <class FG>
 hipError_t gradient_to(const Grad& a, int e, int table_type, hipStream_t stream) {
@@ -567,7 +606,7 @@ extern "C" hipError_t hk_embedding_forward(const void* table, int type, int64_t 
   a.table = table, a.tokens = tokens, a.residual = residual, a.out = out, a.wide_tokens = wide_tokens;
   a.vocab = vocab, a.table_stride = table_stride, a.residual_stride = residual_stride, a.out_stride = out_stride;
   a.scale = scale;
-  const int e = unit(d, {{table, table_stride, et, vocab}, {residual, residual_stride, eo, n}, {out, out_stride, eo, n}});
+  const int e = unit(d, 8, {{table, table_stride, et, vocab}, {residual, residual_stride, eo, n}, {out, out_stride, eo, n}});
   return type == HK_TYPE_F32    ? lookup_to<F32>(a, n, d, e, out_type, stream)
          : type == HK_TYPE_BF16 ? lookup_to<BF16>(a, n, d, e, out_type, stream)
                                 : lookup_to<F16>(a, n, d, e, out_type, stream);
@@ -607,7 +646,7 @@ extern "C" hipError_t hk_embedding_backward(const void* grad, int type, int64_t 
   a.scale = scale, a.accumulate = accumulate, a.table_elem = static_cast<int>(et);
   a.sorted = static_cast<uint2*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ceil_div(8 * n, 16) * 16);
-  const int e = unit(d, {{grad, grad_stride, eg, n}, {grad_table, table_stride, et, vocab}});
+  const int e = unit(d, 4, {{grad, grad_stride, eg, n}, {grad_table, table_stride, et, vocab}});
   return type == HK_TYPE_F32    ? gradient_to<F32>(a, e, table_type, stream)
          : type == HK_TYPE_BF16 ? gradient_to<BF16>(a, e, table_type, stream)
                                 : gradient_to<F16>(a, e, table_type, stream);
