@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "hk_device.h"
 #include "hk_host.h"
@@ -81,6 +82,8 @@ struct Args {
   float scale;
   int tiles;   // slots of row (or key) tiles, all sequences
   int splits;  // shares of a tile's loop, each with partial results of its own
+  int cus;
+  int near;  // backward: groups divide 32 rows, which lie within 2^30 bytes
   float* part;   // partial results
   float2* stat;  // forward: (max, sum) of them
   float* delta;  // backward: rowsum(dout * o), [q head][token]
@@ -90,9 +93,8 @@ __host__ __device__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
   return x < lo ? lo : x > hi ? hi : x;
 }
 
-// Tiles of B rows, `group` rows a token: slot floor(cu[s] group / B) + s is the first of sequence s, which leaves
-// every sequence the tiles it needs (and at most one more) without a table of lengths: the grid goes by the number of
-// tokens and sequences alone, so nothing about the lengths has to be known on the host.
+// At most this many tiles of B rows, `group` rows a token, whatever the lengths of the n sequences are: the grid goes by
+// the numbers of tokens and sequences alone, so nothing about the lengths has to be known on the host.
 __host__ __device__ inline int64_t slots(int64_t tokens, int n, int group, int B) {
   return tokens * group / B + n;
 }
@@ -100,32 +102,94 @@ __host__ __device__ inline int64_t slots(int64_t tokens, int n, int group, int B
 struct Seq {
   int64_t q0, k0;  // first query and key
   int mq, mk;      // how many of them
-  int tile;        // the workgroup's tile of this sequence
+  int tile, tiles; // the workgroup's tile of this sequence, and how many it has
 };
+// Starts outside 0 .. tokens count as the nearer of both and lengths under 0 as 0, so whatever cu holds the rows are
+// some of the tensor.
 
-// The sequence of slot x: the last one that begins at it or before, 64 candidates a step. Starts outside 0 .. tokens
-// count as the nearer of both and lengths under 0 as 0, so whatever cu holds the rows are some of the tensor.
-__device__ __forceinline__ bool find_tile(const int32_t* cu, int64_t tokens, const Args& a, int group, int B,
-                                          int x, Seq& s) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = a.n;
-  do {
-    const int step = (hi - lo + 63) >> 6;
-    const int i = lo + lane * step;
-    const bool before = i < hi && clamp64(cu[i < hi ? i : lo], 0, tokens) * group / B + i <= x;
-    const int count = __popcll(__ballot(before));
-    if (count == 0) return false;
-    lo += (count - 1) * step;
-    hi = min(hi, lo + step);
-  } while (hi - lo > 1);
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  const int64_t q0 = clamp64(a.cu_q[lo], 0, a.q_tokens), q1 = clamp64(a.cu_q[lo + 1], q0, a.q_tokens);
-  const int64_t k0 = clamp64(a.cu_k[lo], 0, a.k_tokens), k1 = clamp64(a.cu_k[lo + 1], k0, a.k_tokens);
-  s.q0 = q0, s.mq = static_cast<int>(q1 - q0);
-  s.k0 = k0, s.mk = static_cast<int>(k1 - k0);
-  const int64_t first = cu == a.cu_q ? q0 : k0;
-  s.tile = x - static_cast<int>(first * group / B + lo);
-  return s.tile >= 0;
+__device__ __forceinline__ int wave_add(int v) {
+  auto dpp = [](int x, auto ctrl) {
+    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  v += dpp(v, std::integral_constant<int, detail::kDppXor1>{});
+  v += dpp(v, std::integral_constant<int, detail::kDppXor2>{});
+  v += dpp(v, std::integral_constant<int, detail::kDppHalfMirror>{});
+  v += dpp(v, std::integral_constant<int, detail::kDppMirror>{});
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] + r[1];
+  const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(h[0] + h[1]);
+}
+
+// Workgroup L's (tile, share, key head): the tiles of all sequences by falling number within the sequence, which under
+// the causal mask is by falling work, each with all its shares and heads side by side. Where the card holds all of them at
+// once (per_cu a CU), workgroup L and L + P (P CUs) are likely to meet on one CU, so every other P of them run backwards:
+// a CU gets heavy and light ones. (8192 tokens in 13 documents, 12 heads of 64, sequence by sequence instead: forward
+// 34.6 us against 29.8, dk and dv 59 against 48.)
+// More than 64 sequences, one a lane, are taken one after the other.
+__device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, const Args& a, int group, int B, int per_cu,
+                                          Seq& q, int& share, int& head) {
+  const int lane = threadIdx.x & 63, per_tile = a.k_heads * a.splits;
+  const bool by_q = cu == a.cu_q;
+  if (a.n > 64) {
+    // slot floor(cu[s] group / B) + s is the first of sequence s, which leaves each the tiles it needs
+    const int x = a.tiles - 1 - static_cast<int>(blockIdx.x) / per_tile, rest = blockIdx.x % per_tile;
+    int lo = 0, hi = a.n;
+    do {
+      const int step = (hi - lo + 63) >> 6;
+      const int i = lo + lane * step;
+      const bool before = i < hi && clamp64(cu[i < hi ? i : lo], 0, tokens) * group / B + i <= x;
+      const int count = __popcll(__ballot(before));
+      if (count == 0) return false;
+      lo += (count - 1) * step;
+      hi = min(hi, lo + step);
+    } while (hi - lo > 1);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int64_t q0 = clamp64(a.cu_q[lo], 0, a.q_tokens), q1 = clamp64(a.cu_q[lo + 1], q0, a.q_tokens);
+    const int64_t k0 = clamp64(a.cu_k[lo], 0, a.k_tokens), k1 = clamp64(a.cu_k[lo + 1], k0, a.k_tokens);
+    q.q0 = q0, q.mq = static_cast<int>(q1 - q0);
+    q.k0 = k0, q.mk = static_cast<int>(k1 - k0);
+    q.tile = x - static_cast<int>((by_q ? q0 : k0) * group / B + lo);
+    q.tiles = static_cast<int>(((by_q ? q.mq : q.mk) * static_cast<int64_t>(group) + B - 1) / B);
+    share = rest / a.k_heads, head = rest - share * a.k_heads;
+    return q.tile >= 0 && q.tile < q.tiles;
+  }
+  // all that is read, at once; numbers of rows and keys fit 32 bits, and so does a sequence's last tile's end
+  const int i0 = min(lane, a.n - 1), tq = static_cast<int>(a.q_tokens), tk = static_cast<int>(a.k_tokens);
+  const int cq0 = a.cu_q[i0], cq1 = a.cu_q[i0 + 1], ck0 = a.cu_k[i0], ck1 = a.cu_k[i0 + 1];
+  const int q0 = min(max(cq0, 0), tq), q1 = min(max(cq1, q0), tq);
+  const int k0 = min(max(ck0, 0), tk), k1 = min(max(ck1, k0), tk);
+  const uint32_t len = static_cast<uint32_t>(by_q ? q1 - q0 : k1 - k0) * group;
+  const int count = lane < a.n ? static_cast<int>((len + B - 1) / B) : 0;  // the sequence's tiles
+  auto over = [&](int t) { return wave_add(max(count - t, 0)); };  // tiles of number t and over
+  const int total = over(0) * per_tile;
+  int L = blockIdx.x;
+  if (L >= total) return false;
+  if (total > a.cus && total <= per_cu * a.cus) {
+    const int P = a.cus, round = L / P;
+    if (round & 1) L = round * P + min(P, total - round * P) - 1 - (L - round * P);
+  }
+  const int x = L / per_tile, rest = L - x * per_tile;
+  // the last t with more than x tiles of number t and over; counts are under 2^24, which floats hold
+  int lo = 0, above = 0, hi = __builtin_amdgcn_readfirstlane(static_cast<int>(wave_max(static_cast<float>(count))));
+  if (a.n == 1) {
+    lo = hi - 1 - x, above = x;
+  } else {
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, c = over(mid);
+      if (c > x) lo = mid;
+      else hi = mid, above = c;
+    }
+  }
+  // the (x - above)-th sequence with such a tile
+  const uint64_t with = __ballot(count > lo);
+  const bool it = count > lo && __popcll(with & ((uint64_t(1) << lane) - 1)) == x - above;
+  const int s = __ffsll(static_cast<unsigned long long>(__ballot(it))) - 1;
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+  q.q0 = of(q0), q.mq = of(q1 - q0), q.k0 = of(k0), q.mk = of(k1 - k0);
+  q.tile = lo, q.tiles = of(count);
+  share = rest / a.k_heads, head = rest - share * a.k_heads;
+  return true;
 }
 
 // LDS tile: rows of D elements (2 D bytes) as they lie in memory, the 16-byte chunk c of row r at chunk c ^ swz(r).
@@ -160,24 +224,35 @@ __device__ __forceinline__ void barrier() {
 
 // Copies of N consecutive tokens of one head by 4 waves. Rows behind the sequence's last and chunks behind the
 // head's last element read the last one: they stay inside the sequence, and what they meet is masked (rows) or
-// zero on the other side of the product (columns of queries) or not stored (columns of values).
+// zero on the other side of the product (columns of queries) or not stored (columns of values). A wave's copies are 4
+// kRows rows apart, at which the chunks lie alike: in whole tiles they differ by a scalar.
 template <int D, int N>
 struct KeyCopy {
   static constexpr int kChunks = D / 8, kRows = 64 / kChunks;  // rows a wave and instruction
   static constexpr int kCopies = N / (4 * kRows);              // instructions a wave
-  int row, chunk16[kCopies];
-  __device__ KeyCopy(int wave, int lane, int d) {
+  const char* base;  // the sequence's first token
+  int64_t step;      // of N tokens
+  int stride, row, chunk16, off;
+  __device__ KeyCopy(const Tensor& x, const Seq& q, int head, int wave, int lane, int d) {
+    base = x.p + q.k0 * x.m + head * x.h;
+    step = N * x.m;
+    stride = static_cast<int>(x.m);
     row = wave * kRows + lane / kChunks;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      chunk16[i] = 16 * min((lane % kChunks) ^ swz<D>(row + 4 * kRows * i), d / 8 - 1);
+    chunk16 = 16 * min((lane % kChunks) ^ swz<D>(row), d / 8 - 1);
+    off = row * stride + chunk16;
   }
-  // base: token 0 of the tile; last: the sequence's last token as the tile counts
-  __device__ void operator()(const char* base, int stride, int last, int wave, unsigned lds) const {
+  // tile t of a sequence of n tokens
+  __device__ __forceinline__ void operator()(int t, int n, int wave, unsigned lds) const {
+    const char* p = base + t * step;
+    const int last = n - 1 - t * N;
+    if (last >= N - 1) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      copy16_to_lds(base, min(row + 4 * kRows * i, last) * stride + chunk16[i],
-                    lds + 1024 * (wave + 4 * i));
+      for (int i = 0; i < kCopies; ++i) copy16_to_lds(p + i * (4 * kRows) * static_cast<int64_t>(stride), off, lds + 1024 * (wave + 4 * i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i)
+        copy16_to_lds(p, min(row + 4 * kRows * i, last) * stride + chunk16, lds + 1024 * (wave + 4 * i));
+    }
   }
 };
 
@@ -200,6 +275,11 @@ struct Reads {
 #pragma unroll
       for (int b = 0; b < D / 32; ++b)
         col[e][b] = at_chunk<D>(8 * e + 4 * h + (j >> 2), 4 * b + (x >> 3)) + 2 * (x & 7);
+    // kept in registers: the compiler would form them anew in every tile
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(row[s]));
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b) asm volatile("" : "+v"(col[0][b]), "+v"(col[1][b]));
   }
   __device__ __forceinline__ s16x8_t rows(const char HK_LDS* tile, int first, int s) const {
     return *reinterpret_cast<const s16x8_t HK_LDS*>(tile + first * (2 * D) + row[s]);
@@ -211,6 +291,14 @@ struct Reads {
     return s16x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
 };
+
+// A block of zeros that stays in 16 registers, for the first product of a sum: the compiler sets the sum's own registers
+// to zero instead, 16 instructions a block.
+__device__ __forceinline__ f32x16_t zero_block() {
+  f32x16_t z = {};
+  asm volatile("" : "+v"(z));
+  return z;
+}
 
 // A row's operand of a product over columns from memory: element s is columns 16 s + 8 h .. + 7, zero behind d.
 template <int D>
@@ -328,6 +416,7 @@ inline Args make_args(const hk_attn_packed_params* p) {
   a.n = p->num_seqs, a.group = p->q_heads / p->k_heads, a.k_heads = p->k_heads, a.d = p->head_dim;
   a.causal = p->is_causal ? 1 : 0;
   a.scale = p->scale;
+  a.splits = 1, a.cus = device_cu_count();
   return a;
 }
 
@@ -347,7 +436,7 @@ inline hipError_t workspace(int64_t need, void* given, int64_t given_bytes, hipS
 }
 
 // Launches one kernel, whose LDS is past the 64 KiB that need no asking.
-template <auto Kernel, int kLds>
+template <auto Kernel, int kLds, int kThreads = 256>
 hipError_t launch(dim3 grid, const Args& a, hipStream_t stream) {
   if constexpr (kLds > 0) {
     static std::atomic<uint64_t> asked;  // a bit a device
@@ -360,7 +449,7 @@ hipError_t launch(dim3 grid, const Args& a, hipStream_t stream) {
       asked.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  hipLaunchKernelGGL(Kernel, grid, dim3(256), kLds, stream, a);
+  hipLaunchKernelGGL(Kernel, grid, dim3(kThreads), kLds, stream, a);
   return launch_status();
 }
 

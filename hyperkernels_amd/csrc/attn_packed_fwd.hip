@@ -17,31 +17,30 @@ constexpr float kLazy = 8.f;
 template <int D, int KG>
 struct FwdShape {
   static constexpr int kRows = 128 / KG;
-  static constexpr int kKeys = KG == 1 ? 64 : 128;  // keys a tile
+  static constexpr int kKeys = KG == 4 ? 128 : 64;  // keys a tile
   static constexpr int kBlocks = kKeys / KG / 32;   // blocks of 32 keys a wave
   static constexpr int kTile = kKeys * D * 2;       // bytes
   static constexpr int kStage = 2 * kTile;
   static constexpr int kPitch = D + 4;  // floats a row of the exchange
-  static constexpr int kExchange = KG == 1 ? 0 : 4 * 32 * kPitch * 4 + 4 * 32 * 8;
+  static constexpr int kExchange = KG == 1 ? 0 : 4 * 32 * (kPitch * 4 + 8);
+  static constexpr int kPerCu = (KG == 4 ? 128 : 256) / D;  // workgroups that a CU holds
   static constexpr int kLds = 2 * kStage > kExchange ? 2 * kStage : kExchange;
 };
 
 template <class T, int D, int KG, bool SPLIT>
-__global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) {
+__global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) {
   using S = FwdShape<D, KG>;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   char HK_LDS* const lds = (char HK_LDS*)lds_raw;
 
-  // the last tile of a sequence has the most keys: it goes first; key heads of one tile side by side
-  const int item = blockIdx.x / a.k_heads, kh = blockIdx.x - item * a.k_heads;
   Seq q;
-  if (!find_tile(a.cu_q, a.q_tokens, a, a.group, S::kRows, a.tiles - 1 - item, q)) return;
+  int share, kh;
+  if (!find_item(a.cu_q, a.q_tokens, a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
   const int rows = q.mq * a.group, r0 = q.tile * S::kRows;
-  if (r0 >= rows) return;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 31, h = lane >> 5;
-  const int kg = KG == 1 ? 0 : wave, w0 = KG == 1 ? r0 + 32 * wave : r0;
+  const int kg = wave % KG, w0 = r0 + 32 * (wave / KG);
   const int row = w0 + c, rr = min(row, rows - 1);
   const int tok = rr / a.group, qh = kh * a.group + rr - tok * a.group;
   const int ahead = q.mk - q.mq;  // row of query i sees keys 0 .. i + ahead
@@ -54,23 +53,19 @@ __global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) 
   int t0 = 0, t1 = end > 0 ? (end + S::kKeys - 1) / S::kKeys : 0;
   if (SPLIT) {
     const int per = (t1 + a.splits - 1) / a.splits;
-    t0 = blockIdx.y * per;
+    t0 = share * per;
     t1 = min(t1, t0 + per);
   }
 
   s16x8_t qx[D / 16];
   load_row<D>(a.q.p + (q.q0 + tok) * a.q.m + qh * a.q.h, h, a.d, qx);
 
-  const char* kb = a.k.p + q.k0 * a.k.m + kh * a.k.h;
-  const char* vb = a.v.p + q.k0 * a.v.m + kh * a.v.h;
-  const KeyCopy<D, S::kKeys> copy(wave, lane, a.d);
+  const KeyCopy<D, S::kKeys> copy_k(a.k, q, kh, wave, lane, a.d), copy_v(a.v, q, kh, wave, lane, a.d);
   const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<uintptr_t>(lds));
   auto fetch = [&](int t) {
     const unsigned to = lds0 + (t & 1) * S::kStage;
-    const int64_t at = static_cast<int64_t>(t) * S::kKeys;
-    const int last = q.mk - 1 - t * S::kKeys;
-    copy(kb + at * a.k.m, static_cast<int>(a.k.m), last, wave, to);
-    copy(vb + at * a.v.m, static_cast<int>(a.v.m), last, wave, to + S::kTile);
+    copy_k(t, q.mk, wave, to);
+    copy_v(t, q.mk, wave, to + S::kTile);
   };
   if (t0 < t1) fetch(t0);
 
@@ -79,6 +74,7 @@ __global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) 
   f32x16_t o[D / 32];
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) o[b] = f32x16_t{};
+  const f32x16_t zero = zero_block();
   float m = -INFINITY, l = 0.f;  // in units of log 2
 
   for (int t = t0; t < t1; ++t) {
@@ -93,9 +89,9 @@ __global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) 
     f32x16_t s[S::kBlocks];
 #pragma unroll
     for (int n = 0; n < S::kBlocks; ++n) {
-      s[n] = f32x16_t{};
+      s[n] = T::mfma(rd.rows(kt, 32 * n, 0), qx[0], zero);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) s[n] = T::mfma(rd.rows(kt, 32 * n, i), qx[i], s[n]);
+      for (int i = 1; i < D / 16; ++i) s[n] = T::mfma(rd.rows(kt, 32 * n, i), qx[i], s[n]);
     }
     if (key0 + 32 * S::kBlocks - 1 > lim_lo) {
 #pragma unroll
@@ -144,43 +140,45 @@ __global__ __launch_bounds__(256, KG == 1 ? 2 : 1) void attn_packed_fwd(Args a) 
   l = half32_reduce(l, AddOp{});
 
   if constexpr (KG > 1) {
-    // the four waves' parts of the same rows
+    // the parts of the waves that have the same rows
+    constexpr int R = S::kRows;
     float HK_LDS* ex = (float HK_LDS*)lds;
     float HK_LDS* st = ex + 4 * 32 * S::kPitch;
+    const int mine = kg * R + w0 - r0 + c;
     wait_copies();
     barrier();
-    if (h == 0) st[64 * wave + 2 * c] = m, st[64 * wave + 2 * c + 1] = l;
+    if (h == 0) st[2 * mine] = m, st[2 * mine + 1] = l;
 #pragma unroll
     for (int b = 0; b < D / 32; ++b)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4_t HK_LDS*>(ex + (32 * wave + c) * S::kPitch + 32 * b + 8 * g + 4 * h) =
+        *reinterpret_cast<f32x4_t HK_LDS*>(ex + mine * S::kPitch + 32 * b + 8 * g + 4 * h) =
             f32x4_t{o[b][4 * g], o[b][4 * g + 1], o[b][4 * g + 2], o[b][4 * g + 3]};
     __syncthreads();
-    // wave w, rows 8 w .. + 7: 8 lanes a row, D / 8 elements a lane
-    const int er = 8 * wave + (lane >> 3), e0 = lane & 7;
-    float em[4], mx = -INFINITY, sum = 0.f;
+    // 2 KG lanes a row, four elements of it at a time
+    const int er = threadIdx.x / (2 * KG), e0 = threadIdx.x % (2 * KG);
+    float em[KG], mx = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) em[g] = st[64 * g + 2 * er], mx = fmaxf(mx, em[g]);
+    for (int g = 0; g < KG; ++g) em[g] = st[2 * (g * R + er)], mx = fmaxf(mx, em[g]);
     const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < KG; ++g) {
       em[g] = __builtin_amdgcn_exp2f(em[g] - ref);
-      sum += em[g] * st[64 * g + 2 * er + 1];
+      sum += em[g] * st[2 * (g * R + er) + 1];
     }
     if (r0 + er >= rows) return;
     const int et = (r0 + er) / a.group, eh = kh * a.group + (r0 + er) - et * a.group;
-    const int64_t at = static_cast<int64_t>(blockIdx.y * a.k_heads + kh) * a.q_tokens * a.group +
+    const int64_t at = static_cast<int64_t>(share * a.k_heads + kh) * a.q_tokens * a.group +
                        q.q0 * a.group + r0 + er;
     const float f = SPLIT ? 1.f : sum > 0.f ? 1.f / sum : sum;  // a NaN stays one
     char* op = a.o.p + (q.q0 + et) * a.o.m + eh * a.o.h;
 #pragma unroll
-    for (int u = 0; u < D / 32; ++u) {
-      const int col = 32 * u + 4 * e0;
+    for (int u = 0; u < D / (8 * KG); ++u) {
+      const int col = 8 * KG * u + 4 * e0;
       f32x4_t x = {};
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        x += em[g] * *reinterpret_cast<const f32x4_t HK_LDS*>(ex + (32 * g + er) * S::kPitch + col);
+      for (int g = 0; g < KG; ++g)
+        x += em[g] * *reinterpret_cast<const f32x4_t HK_LDS*>(ex + (g * R + er) * S::kPitch + col);
       if (SPLIT) *reinterpret_cast<f32x4_t*>(a.part + at * D + col) = x;
       else if (col < a.d)
         *reinterpret_cast<u32x2_t*>(op + 2 * col) = u32x2_t{T::pack(x[0] * f, x[1] * f), T::pack(x[2] * f, x[3] * f)};
@@ -240,16 +238,18 @@ struct Plan {
   int kg, tiles, splits;
   int64_t part, stat;  // bytes
 };
-// 128 rows a workgroup where a sequence fills them and the card gets a round of workgroups so; else 32, and where even
-// those leave CUs idle each row's keys are cut into shares.
+// 128 rows a workgroup where a sequence fills them and every CU gets two of them; 64, whose keys two waves share, where
+// it gets one (sequences of 2048, 1001 and 333, 16 heads on 4 of 128: 61.3 -> 52.2 us; with two or more 128 are as fast,
+// 13 sequences of 12 heads of 64, or faster, 8192 of 16 heads of 128: 330 against 442); else 32, and where even those
+// leave CUs idle each row's keys are cut into shares.
 Plan plan(const hk_attn_packed_params* p) {
   const int group = p->q_heads / p->k_heads, cus = device_cu_count();
   const int64_t rows = p->q_tokens * group, wide = slots(p->q_tokens, p->num_seqs, group, 128) * p->k_heads;
   Plan r{};
   r.splits = 1;
   if (rows >= int64_t(96) * p->num_seqs && wide >= cus) {
-    r.kg = 1;
-    r.tiles = static_cast<int>(wide / p->k_heads);
+    r.kg = wide < 2 * cus ? 2 : 1;
+    r.tiles = static_cast<int>(slots(p->q_tokens, p->num_seqs, group, 128 / r.kg));
     return r;
   }
   r.kg = 4;
@@ -268,8 +268,9 @@ template <class T, int D>
 hipError_t run(Args a, const Plan& r, hipStream_t stream) {
   const unsigned x = static_cast<unsigned>(a.tiles) * a.k_heads;
   if (r.kg == 1) return launch<&attn_packed_fwd<T, D, 1, false>, FwdShape<D, 1>::kLds>(dim3(x), a, stream);
+  if (r.kg == 2) return launch<&attn_packed_fwd<T, D, 2, false>, FwdShape<D, 2>::kLds>(dim3(x), a, stream);
   if (r.splits == 1) return launch<&attn_packed_fwd<T, D, 4, false>, FwdShape<D, 4>::kLds>(dim3(x), a, stream);
-  HK_RETURN_IF_ERROR((launch<&attn_packed_fwd<T, D, 4, true>, FwdShape<D, 4>::kLds>(dim3(x, r.splits), a, stream)));
+  HK_RETURN_IF_ERROR((launch<&attn_packed_fwd<T, D, 4, true>, FwdShape<D, 4>::kLds>(dim3(x * r.splits), a, stream)));
   const int64_t rows = a.q_tokens * a.group * a.k_heads;
   return launch<&attn_packed_join<T, D>, 0>(dim3(static_cast<unsigned>(ceil_div(rows, 4))), a, stream);
 }
