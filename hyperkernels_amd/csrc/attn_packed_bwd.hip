@@ -22,12 +22,12 @@ struct DqShape {
   static constexpr int kStage = 2 * kTile;
   static constexpr int kPitch = D + 4;
   static constexpr int kExchange = KG == 1 ? 0 : 4 * 32 * kPitch * 4;
-  static constexpr int kPerCu = (KG == 4 ? 128 : 256) / D;  // workgroups that a CU holds
+  static constexpr int kPerCu = D == 64 ? (KG == 4 ? 2 : 3) : (KG == 4 ? 1 : 2);  // workgroups a CU
   static constexpr int kLds = 2 * kStage > kExchange ? 2 * kStage : kExchange;
 };
 
 template <class T, int D, int KG>
-__global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_dq(Args a) {
+__global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packed_dq(Args a) {
   using S = DqShape<D, KG>;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   char HK_LDS* const lds = (char HK_LDS*)lds_raw;
@@ -167,11 +167,11 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_dq(Args a) {
 template <int D>
 struct DkvShape {
   static constexpr int kKeys = 128;
-  static constexpr int kRows = 64;  // rows a tile
+  static constexpr int kRows = D == 128 ? 64 : 32;  // rows a tile
   static constexpr int kHalves = D == 128 ? 2 : 1, kThreads = 256 * kHalves;
   static constexpr int kTile = kRows * D * 2;
-  static constexpr int kStage = 2 * kTile + 2 * kRows * 4;  // Q, dO, delta, lse
-  static constexpr int kHeld = kHalves == 2 ? 2 * kKeys * D * 2 : 0;  // K, V
+  static constexpr int kStage = 2 * kTile + 2 * 64 * 4;  // Q, dO, delta, lse (of 64 rows)
+  static constexpr int kHeld = 2 * kKeys * D * 2;  // K, V
   static constexpr int kPitch = D + 4;
   static constexpr int kExchange = kHalves == 2 ? kKeys * kPitch * 4 : 0;
   static constexpr int kLds = kHeld + 2 * kStage > kExchange ? kHeld + 2 * kStage : kExchange;
@@ -185,7 +185,7 @@ __device__ __forceinline__ void copy4_to_lds(const void* addr, unsigned lds_addr
 }
 
 template <class T, int D, bool SPLIT>
-__global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args a) {
+__global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_packed_dkv(Args a) {
   using S = DkvShape<D>;
   constexpr int kWaves = S::kThreads / 64;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args
 
   Seq q;
   int share, kh;
-  if (!find_item(a.cu_k, a.k_tokens, a, 1, S::kKeys, S::kHalves == 2 ? 1 : 2, q, share, kh)) return;
+  if (!find_item(a.cu_k, a.k_tokens, a, 1, S::kKeys, S::kHalves == 2 ? 1 : 3, q, share, kh)) return;
   // under the causal mask the first keys meet the most rows: they go first
   const int k0 = (q.tiles - 1 - q.tile) * S::kKeys;
   const int rows = q.mq * a.group, ahead = q.mk - q.mq;
@@ -236,8 +236,8 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args
       reinterpret_cast<const char*>(a.delta + ((wave & 1) * heads + kh * a.group) * a.q_tokens + q.q0);
   auto fetch = [&](int t) {
     const unsigned to = lds0 + S::kHeld + (t & 1) * S::kStage;
-    if (a.near && (t + 1) * S::kRows <= rows) {
-      const int64_t tok = static_cast<int64_t>(2 * t) * per32;
+    if (a.near && t * S::kRows + 64 <= rows) {
+      const int64_t tok = static_cast<int64_t>(S::kRows / 32 * t) * per32;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         copy16_to_lds(q0p + (tok + i * per32) * a.q.m, off_q, to + 1024 * (wave + kWaves * i));
@@ -259,8 +259,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args
       copy4_to_lds(d0p + 4 * (hd * a.q_tokens + tok), to + 2 * S::kTile + 256 * wave);
     }
   };
-  s16x8_t kx[S::kHalves == 1 ? D / 16 : 1], vx[S::kHalves == 1 ? D / 16 : 1];
-  if constexpr (S::kHalves == 2) {
+  {
     // columns behind the head's last element are zero: those of Q and dO are copies of others
     for (int i = threadIdx.x; i < S::kKeys * kChunks; i += S::kThreads) {
       const int r = i / kChunks, ch = i % kChunks;
@@ -273,22 +272,13 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args
       *reinterpret_cast<u32x4_t HK_LDS*>(lds + at_chunk<D>(r, ch)) = x;
       *reinterpret_cast<u32x4_t HK_LDS*>(lds + S::kHeld / 2 + at_chunk<D>(r, ch)) = y;
     }
-  } else {
-    load_row<D>(a.k.p + (q.k0 + kk) * a.k.m + kh * a.k.h, h, a.d, kx);
-    load_row<D>(a.v.p + (q.k0 + kk) * a.v.m + kh * a.v.h, h, a.d, vx);
   }
   if (t0 < t1) fetch(t0);
 
   const Reads<D> rd(lane);
   const char HK_LDS* const kt = lds + 32 * kb * (2 * D);
-  auto k_of = [&](int i) {
-    if constexpr (S::kHalves == 2) return rd.rows(kt, 0, i);
-    else return kx[i];
-  };
-  auto v_of = [&](int i) {
-    if constexpr (S::kHalves == 2) return rd.rows(kt + S::kHeld / 2, 0, i);
-    else return vx[i];
-  };
+  auto k_of = [&](int i) { return rd.rows(kt, 0, i); };
+  auto v_of = [&](int i) { return rd.rows(kt + S::kHeld / 2, 0, i); };
   const float sc = a.scale * kLog2e;
   const f32x16_t zero = zero_block();
   f32x16_t dk[D / 32], dv[D / 32];
@@ -303,7 +293,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, 2) void attn_packed_dkv(Args
     const char HK_LDS* gt = qt + S::kTile;
     const float HK_LDS* dl = (const float HK_LDS*)(gt + S::kTile);
 #pragma unroll
-    for (int u = 0; u < 2 / S::kHalves; ++u) {
+    for (int u = 0; u < S::kRows / 32 / S::kHalves; ++u) {
       const int n = S::kHalves == 2 ? half : u;
       const int r0 = t * S::kRows + 32 * n;
       if (r0 + 31 < from_lo) continue;  // none of these rows sees the wave's keys
