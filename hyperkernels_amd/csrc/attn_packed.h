@@ -81,7 +81,9 @@ struct Args {
   int causal;
   float scale;
   int tiles;   // slots of row (or key) tiles, all sequences
-  int splits;  // shares of a tile's loop, each with partial results of its own
+  int splits;  // backward: shares of a key tile's rows, each with partial results of its own
+  int chunk, most;  // forward: key tiles a share, and how many shares there are room for
+  int32_t* shares;  // forward: of each row
   int cus;
   int near;  // backward: groups divide 32 rows, which lie within 2^30 bytes
   float* part;   // partial results
@@ -189,6 +191,39 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, con
   q.q0 = of(q0), q.mq = of(q1 - q0), q.k0 = of(k0), q.mk = of(k1 - k0);
   q.tile = lo, q.tiles = of(count);
   share = rest / a.k_heads, head = rest - share * a.k_heads;
+  return true;
+}
+
+// Item L of those that give every row tile's keys in shares of a.chunk tiles of B_k keys, sequence after sequence: shares
+// are alike, so their order is free. At most 64 sequences.
+__device__ __forceinline__ bool find_share(const Args& a, int B, int B_k, int L, Seq& q, int& share, int& shares,
+                                           int& head) {
+  const int lane = threadIdx.x & 63;
+  const int i0 = min(lane, a.n - 1), tq = static_cast<int>(a.q_tokens), tk = static_cast<int>(a.k_tokens);
+  const int cq0 = a.cu_q[i0], cq1 = a.cu_q[i0 + 1], ck0 = a.cu_k[i0], ck1 = a.cu_k[i0 + 1];
+  const int q0 = min(max(cq0, 0), tq), q1 = min(max(cq1, q0), tq);
+  const int k0 = min(max(ck0, 0), tk), k1 = min(max(ck1, k0), tk);
+  const int tiles = static_cast<int>((static_cast<uint32_t>(q1 - q0) * a.group + B - 1) / B);
+  const int parts = max(1, (k1 - k0 + B_k * a.chunk - 1) / (B_k * a.chunk));
+  const int items = lane < a.n ? tiles * parts : 0;
+  int upto = items;  // of the sequences to here
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int below = __shfl_up(upto, d);
+    if (lane >= d) upto += below;
+  }
+  const int x = L / a.k_heads;
+  head = L - x * a.k_heads;
+  const uint64_t behind = __ballot(upto > x);
+  if (behind == 0) return false;
+  const int s = __ffsll(static_cast<unsigned long long>(behind)) - 1;
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+  const int r = x - of(upto - items);
+  shares = of(parts);
+  q.q0 = of(q0), q.mq = of(q1 - q0), q.k0 = of(k0), q.mk = of(k1 - k0);
+  q.tiles = of(tiles);
+  q.tile = r / shares;
+  share = r - q.tile * shares;
   return true;
 }
 

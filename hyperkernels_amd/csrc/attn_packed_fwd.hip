@@ -7,6 +7,8 @@
 // O^T += V^T P^T. P is rounded to 16 bits for that product (half a step of the type, as the inputs are; the sum that
 // divides it is of the fp32 values); scores, maximum, sum and O are fp32.
 // Tiles of keys and values go from memory to LDS past the registers, the next one while this one is used.
+#include <algorithm>
+
 #include "attn_packed.h"
 
 namespace hk {
@@ -27,15 +29,11 @@ struct FwdShape {
   static constexpr int kLds = 2 * kStage > kExchange ? 2 * kStage : kExchange;
 };
 
+// One tile of rows over all of its keys, or (SPLIT) over one share of them.
 template <class T, int D, int KG, bool SPLIT>
-__global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) {
+__device__ __forceinline__ void attend(const Args& a, const Seq& q, int kh, int share, int shares,
+                                       char HK_LDS* const lds) {
   using S = FwdShape<D, KG>;
-  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
-  char HK_LDS* const lds = (char HK_LDS*)lds_raw;
-
-  Seq q;
-  int share, kh;
-  if (!find_item(a.cu_q, a.q_tokens, a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
   const int rows = q.mq * a.group, r0 = q.tile * S::kRows;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -52,9 +50,8 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) 
   const int end = a.causal ? min(q.mk, last_tok / a.group + ahead + 1) : q.mk;
   int t0 = 0, t1 = end > 0 ? (end + S::kKeys - 1) / S::kKeys : 0;
   if (SPLIT) {
-    const int per = (t1 + a.splits - 1) / a.splits;
-    t0 = share * per;
-    t1 = min(t1, t0 + per);
+    t0 = share * a.chunk;
+    t1 = min(t1, t0 + a.chunk);
   }
 
   s16x8_t qx[D / 16];
@@ -184,8 +181,10 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) 
         *reinterpret_cast<u32x2_t*>(op + 2 * col) = u32x2_t{T::pack(x[0] * f, x[1] * f), T::pack(x[2] * f, x[3] * f)};
     }
     if (e0 == 0) {
-      if (SPLIT) a.stat[at] = make_float2(mx, sum);
-      else if (a.lse) a.lse[eh * a.lse_stride + q.q0 + et] = (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+      if constexpr (SPLIT) {
+        a.stat[at] = make_float2(mx, sum);
+        if (share == 0) a.shares[at] = shares;
+      } else if (a.lse) a.lse[eh * a.lse_stride + q.q0 + et] = (mx + __builtin_amdgcn_logf(sum)) * kLn2;
     }
     return;
   }
@@ -194,39 +193,80 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) 
   if (h == 0 && a.lse) a.lse[qh * a.lse_stride + q.q0 + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Joins the shares of each row's keys, one wave a row of one query head.
+template <class T, int D, int KG>
+__global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) {
+  using S = FwdShape<D, KG>;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  Seq q;
+  int share, kh;
+  if (!find_item(a.cu_q, a.q_tokens, a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
+  attend<T, D, KG, false>(a, q, kh, 0, 1, (char HK_LDS*)lds_raw);
+}
+
+// The grid cannot know how many shares there are: workgroups take them in turn.
+template <class T, int D>
+__global__ __launch_bounds__(256, 1) void attn_packed_fwd_shares(Args a) {
+  using S = FwdShape<D, 4>;
+  extern __shared__ __attribute__((aligned(16))) char lds_raw[];
+  Seq q;
+  int share, shares, kh;
+  for (int L = blockIdx.x; find_share(a, S::kRows, S::kKeys, L, q, share, shares, kh); L += gridDim.x) {
+    attend<T, D, 4, true>(a, q, kh, share, shares, (char HK_LDS*)lds_raw);
+    __syncthreads();  // the exchange is read
+  }
+}
+
+// Joins the shares of each row's keys, one wave a row of one query head: a share's maximum and sum a lane, then the
+// values of eight shares at a time.
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_packed_join(Args a) {
   const int64_t rows = a.q_tokens * a.group;  // of one key head
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= rows * a.k_heads) return;
   const int kh = static_cast<int>(i / rows);
-  const int64_t r = i - kh * rows, tok = r / a.group;
+  const int64_t r = i - kh * rows, tok = r / a.group, all = rows * a.k_heads;
   if (tok < a.cu_q[0] || tok >= a.cu_q[a.n]) return;  // of no sequence
   const int qh = kh * a.group + static_cast<int>(r - tok * a.group);
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.stat[s * rows * a.k_heads + i].x);
+  const int lane = threadIdx.x & 63, shares = min(max(a.shares[i], 1), a.most);
+  float m = -INFINITY, l = 0.f;
+  for (int s0 = 0; s0 < shares; s0 += 64)
+    if (s0 + lane < shares) m = fmaxf(m, a.stat[(s0 + lane) * all + i].x);
+  m = wave_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = s * rows * a.k_heads + i;
-    const float2 st = a.stat[at];
-    const float w = __builtin_amdgcn_exp2f(st.x - ref);
-    l += w * st.y;
-    if (D == 128) {
-      const float2 p = reinterpret_cast<const float2*>(a.part + at * D)[lane];
-      x0 += w * p.x, x1 += w * p.y;
-    } else {
-      x0 += w * a.part[at * D + lane];
+  f32x2_t x = {};
+  for (int s0 = 0; s0 < shares; s0 += 64) {
+    float w = 0.f;
+    if (s0 + lane < shares) {
+      const float2 st = a.stat[(s0 + lane) * all + i];
+      w = __builtin_amdgcn_exp2f(st.x - ref);
+      l += w * st.y;
+    }
+    const int here = min(shares - s0, 64);
+    for (int u0 = 0; u0 < here; u0 += 8) {
+      f32x2_t p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        p[u] = f32x2_t{};
+        if (u0 + u < here) {
+          const float* at = a.part + ((s0 + u0 + u) * all + i) * D;
+          if (D == 128) p[u] = reinterpret_cast<const f32x2_t*>(at)[lane];
+          else p[u][0] = at[lane];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (u0 + u) & 63));
+        if (u0 + u < here) x += f * p[u];
+      }
     }
   }
+  l = wave_sum(l);
   const float f = l > 0.f ? 1.f / l : l;
   char* op = a.o.p + tok * a.o.m + qh * a.o.h;
   if (D == 128) {
-    if (2 * lane < a.d) reinterpret_cast<uint32_t*>(op)[lane] = T::pack(x0 * f, x1 * f);
+    if (2 * lane < a.d) reinterpret_cast<uint32_t*>(op)[lane] = T::pack(x[0] * f, x[1] * f);
   } else if (lane < a.d) {
-    T::format::store(reinterpret_cast<uint16_t*>(op), lane, x0 * f);
+    T::format::store(reinterpret_cast<uint16_t*>(op), lane, x[0] * f);
   }
   if (lane == 0 && a.lse) a.lse[qh * a.lse_stride + tok] = (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
@@ -235,31 +275,38 @@ __global__ __launch_bounds__(256) void attn_packed_join(Args a) {
 namespace {
 
 struct Plan {
-  int kg, tiles, splits;
-  int64_t part, stat;  // bytes
+  int kg, tiles, chunk, shares;  // shares: at most, 1 where keys are not shared
+  int64_t part, stat, count;     // bytes
 };
 // 128 rows a workgroup where a sequence fills them and every CU gets two of them; 64, whose keys two waves share, where
 // it gets one (sequences of 2048, 1001 and 333, 16 heads on 4 of 128: 61.3 -> 52.2 us; with two or more 128 are as fast,
 // 13 sequences of 12 heads of 64, or faster, 8192 of 16 heads of 128: 330 against 442); else 32, and where even those
-// leave CUs idle each row's keys are cut into shares.
+// leave CUs idle their keys are cut into equal shares, as many in all as the card takes at once.
 Plan plan(const hk_attn_packed_params* p) {
-  const int group = p->q_heads / p->k_heads, cus = device_cu_count();
-  const int64_t rows = p->q_tokens * group, wide = slots(p->q_tokens, p->num_seqs, group, 128) * p->k_heads;
+  const int group = p->q_heads / p->k_heads, cus = device_cu_count(), n = p->num_seqs;
+  const int64_t rows = p->q_tokens * group, wide = slots(p->q_tokens, n, group, 128) * p->k_heads;
   Plan r{};
-  r.splits = 1;
-  if (rows >= int64_t(96) * p->num_seqs && wide >= cus) {
+  r.shares = 1;
+  if (rows >= int64_t(96) * n && wide >= cus) {
     r.kg = wide < 2 * cus ? 2 : 1;
-    r.tiles = static_cast<int>(slots(p->q_tokens, p->num_seqs, group, 128 / r.kg));
+    r.tiles = static_cast<int>(slots(p->q_tokens, n, group, 128 / r.kg));
     return r;
   }
   r.kg = 4;
-  r.tiles = static_cast<int>(slots(p->q_tokens, p->num_seqs, group, 32));
-  const int64_t wgs = static_cast<int64_t>(r.tiles) * p->k_heads, keys = p->k_tokens / p->num_seqs;
-  const int64_t want = wgs < cus ? ceil_div(2 * cus, wgs) : 1;
-  r.splits = static_cast<int>(clamp64(want, 1, clamp64(keys / 256, 1, 64)));
-  if (r.splits > 1) {
-    const int64_t n = r.splits * p->q_tokens * p->q_heads, D = p->head_dim <= 64 ? 64 : 128;
-    r.part = n * D * 4, r.stat = n * 8;
+  r.tiles = static_cast<int>(slots(p->q_tokens, n, group, 32));
+  const int64_t wgs = static_cast<int64_t>(r.tiles) * p->k_heads;
+  if (wgs < cus && n <= 64 && p->k_tokens >= int64_t(512) * n) {
+    constexpr int kKeys = FwdShape<64, 4>::kKeys;
+    static_assert(kKeys == FwdShape<128, 4>::kKeys, "shares go by one size of tile");
+    const int at_once = p->head_dim <= 64 ? 2 * cus : cus;
+    // key tiles of all row tiles, taken to be spread evenly over the sequences
+    const int64_t work = ceil_div(p->k_tokens, kKeys) * ceil_div(rows, int64_t(32) * n) * p->k_heads;
+    // a sequence's last share is a part of one: all of them have to be under way at once all the same
+    const int64_t whole = std::max<int64_t>(at_once - wgs, at_once / 2);
+    r.chunk = static_cast<int>(std::max<int64_t>(2, ceil_div(work, whole)));
+    r.shares = static_cast<int>(ceil_div(p->k_tokens, int64_t(r.chunk) * kKeys));
+    const int64_t all = p->q_tokens * p->q_heads, D = p->head_dim <= 64 ? 64 : 128;
+    r.part = r.shares * all * D * 4, r.stat = r.shares * all * 8, r.count = ceil_div(all * 4, 16) * 16;
   }
   return r;
 }
@@ -267,10 +314,11 @@ Plan plan(const hk_attn_packed_params* p) {
 template <class T, int D>
 hipError_t run(Args a, const Plan& r, hipStream_t stream) {
   const unsigned x = static_cast<unsigned>(a.tiles) * a.k_heads;
-  if (r.kg == 1) return launch<&attn_packed_fwd<T, D, 1, false>, FwdShape<D, 1>::kLds>(dim3(x), a, stream);
-  if (r.kg == 2) return launch<&attn_packed_fwd<T, D, 2, false>, FwdShape<D, 2>::kLds>(dim3(x), a, stream);
-  if (r.splits == 1) return launch<&attn_packed_fwd<T, D, 4, false>, FwdShape<D, 4>::kLds>(dim3(x), a, stream);
-  HK_RETURN_IF_ERROR((launch<&attn_packed_fwd<T, D, 4, true>, FwdShape<D, 4>::kLds>(dim3(x * r.splits), a, stream)));
+  if (r.kg == 1) return launch<&attn_packed_fwd<T, D, 1>, FwdShape<D, 1>::kLds>(dim3(x), a, stream);
+  if (r.kg == 2) return launch<&attn_packed_fwd<T, D, 2>, FwdShape<D, 2>::kLds>(dim3(x), a, stream);
+  if (r.shares == 1) return launch<&attn_packed_fwd<T, D, 4>, FwdShape<D, 4>::kLds>(dim3(x), a, stream);
+  const unsigned most = x * static_cast<unsigned>(r.shares), grid = static_cast<unsigned>(FwdShape<D, 4>::kPerCu * a.cus);
+  HK_RETURN_IF_ERROR((launch<&attn_packed_fwd_shares<T, D>, FwdShape<D, 4>::kLds>(dim3(std::min(most, grid)), a, stream)));
   const int64_t rows = a.q_tokens * a.group * a.k_heads;
   return launch<&attn_packed_join<T, D>, 0>(dim3(static_cast<unsigned>(ceil_div(rows, 4))), a, stream);
 }
@@ -288,7 +336,7 @@ using namespace hk::packed;
 int64_t hk::packed::forward_workspace(const hk_attn_packed_params* p) {
   if (p->num_seqs == 0 || p->q_tokens == 0) return 0;
   const Plan r = plan(p);
-  return r.part + r.stat;
+  return r.part + r.stat + r.count;
 }
 
 extern "C" hipError_t hk_attn_packed_forward(const hk_attn_packed_params* p, int type, void* ws,
@@ -297,10 +345,11 @@ extern "C" hipError_t hk_attn_packed_forward(const hk_attn_packed_params* p, int
   if (p->num_seqs == 0 || p->q_tokens == 0) return hipSuccess;
   HK_CHECK_ARG(outputs_apart(p, false));
   const Plan r = plan(p);
-  HK_RETURN_IF_ERROR(workspace(r.part + r.stat, ws, workspace_bytes, stream, &ws));
+  HK_RETURN_IF_ERROR(workspace(r.part + r.stat + r.count, ws, workspace_bytes, stream, &ws));
   Args a = make_args(p);
-  a.tiles = r.tiles, a.splits = r.splits;
+  a.tiles = r.tiles, a.chunk = r.chunk, a.most = r.shares;
   a.part = static_cast<float*>(ws);
   a.stat = reinterpret_cast<float2*>(static_cast<char*>(ws) + r.part);
+  a.shares = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + r.part + r.stat);
   return type == HK_TYPE_BF16 ? by_width<TypeBF16>(a, r, stream) : by_width<TypeF16>(a, r, stream);
 }
