@@ -29,6 +29,7 @@ constexpr int kMaxTop = 64;
 constexpr int kMaxPieces = 64;
 constexpr int kList = 1024;  // candidates in LDS
 constexpr int kLanes = 128;  // lanes whose vectors LDS holds
+constexpr int kMostVecs = 14;  // 16-byte vectors a lane: with them 80 registers, three workgroups a CU
 
 struct Row {
   const void* x;
@@ -87,7 +88,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int top, 
 }
 
 template <class F, int THREADS, int V, bool ENT, bool TOP>
-__global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 4) void logprobs_kernel(Row a) {
+__global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kernel(Row a) {
   constexpr int kE = F::kPerVec, W = THREADS / 64;
   using S = typename F::storage;
   __shared__ float red[3][W];
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(256) void logprobs_grad(Grad a) {
 // ---- host --------------------------------------------------------------------------------------------------
 size_t elem(int type) { return type == HK_TYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-constexpr int64_t kMaxVocab = int64_t(1) << 21;
+constexpr int64_t kMaxVocab = int64_t(1) << 20;
 constexpr int64_t kGrid = int64_t(1) << 22;  // workgroups a launch
 
 bool shape_ok(int type, int64_t rows, int64_t vocab, int64_t stride) {
@@ -379,7 +380,7 @@ bool shape_ok(int type, int64_t rows, int64_t vocab, int64_t stride) {
 struct Plan {
   int threads, vecs, pieces, piece;
 };
-// One wave a row where it holds it and there are rows for all, else 512 lanes. Rows are cut where they pass 16 vectors a
+// One wave a row where it holds it and there are rows for all, else 512 lanes. Rows are cut where they pass 14 vectors a
 // lane, and where they leave CUs idle, into pieces of 2048 elements at least.
 Plan plan(int type, int64_t rows, int64_t vocab) {
   const int e = 16 / static_cast<int>(elem(type)), cus = device_cu_count();
@@ -389,7 +390,7 @@ Plan plan(int type, int64_t rows, int64_t vocab) {
     p.threads = 64;
     return p;
   }
-  int64_t pieces = ceil_div(vocab, int64_t(512) * 16 * e);
+  int64_t pieces = ceil_div(vocab, int64_t(512) * kMostVecs * e);
   if (rows < cus) {
     const int64_t fill = ceil_div(cus, rows > 0 ? rows : 1), most = vocab / 2048;
     pieces = pieces > (fill < most ? fill : most) ? pieces : (fill < most ? fill : most);
@@ -398,7 +399,7 @@ Plan plan(int type, int64_t rows, int64_t vocab) {
   p.pieces = static_cast<int>(pieces < 1 ? 1 : pieces);
   p.piece = static_cast<int>(ceil_div(ceil_div(vocab, p.pieces), e) * e);
   p.pieces = static_cast<int>(ceil_div(vocab, p.piece));
-  p.vecs = p.piece <= 512 * 4 * e ? 4 : 16;
+  p.vecs = p.piece <= 512 * 4 * e ? 4 : kMostVecs;
   return p;
 }
 int64_t workspace_bytes_of(const Plan& p, int64_t rows, int top) {
@@ -424,7 +425,7 @@ hipError_t run(Row a, const Plan& p, hipStream_t stream) {
     const int64_t rows = a.rows - a.first < step ? a.rows - a.first : step, blocks = rows * p.pieces;
     HK_RETURN_IF_ERROR(p.threads == 64 ? (launch<F, 64, 4>(a, blocks, stream))
                        : p.vecs == 4   ? (launch<F, 512, 4>(a, blocks, stream))
-                                       : (launch<F, 512, 16>(a, blocks, stream)));
+                                       : (launch<F, 512, kMostVecs>(a, blocks, stream)));
     if (p.pieces > 1) {
       hipLaunchKernelGGL(logprobs_join<F>, dim3(static_cast<unsigned>(rows)), dim3(256),
                          static_cast<size_t>(8) * p.pieces * a.top, stream, a);

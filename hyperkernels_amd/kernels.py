@@ -795,48 +795,75 @@ class AttnPackedParams(ctypes.Structure):
 _PACKED_PACK = struct.Struct("@11P4if?19q").pack
 
 
-def _heads(fn: str, t: torch.Tensor, tokens: int, heads: int, d: int, dt, dev: int) -> tuple[int, int, int]:
+def _heads(fn: str, t: torch.Tensor, shape, dt, dev: int) -> tuple[int, int, int]:
     """(address, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
-    if t.shape != (tokens, heads, d) or t.dtype is not dt or t.get_device() != dev:
-        raise ValueError(f"{fn}: {dt} [{tokens}, {heads}, {d}] of one device expected, "
-                         f"{t.dtype} {tuple(t.shape)} given")
+    if t.shape != shape or t.dtype is not dt or t.get_device() != dev:
+        raise ValueError(f"{fn}: {dt} {list(shape)} of one device expected, {t.dtype} {list(t.shape)} given")
     m, h, one = t.stride()
     if one != 1:
         raise ValueError(f"{fn}: tensors are [tokens, heads, head_dim] with a unit last-dim stride")
     # the stride of a single token or head is never used, whatever it is
-    return t.data_ptr(), m if tokens > 1 else 0, h if heads > 1 else 0
+    return t.data_ptr(), m if shape[0] > 1 else 0, h if shape[1] > 1 else 0
 
 
-def _packed_params(fn, q, k, v, cu_q, cu_k, causal, scale, o, lse, do=None, dq=None, dk=None, dv=None):
-    if q.dim() != 3 or k.dim() != 3 or (q.dtype is not _BF16 and q.dtype is not torch.float16):
+_NO_HEADS = (0, 0, 0)
+
+
+def _like(fn, t, x, sh, dt, dev):
+    """An output of x's shape: the one passed in, checked, or a new contiguous one. (tensor, address, strides)"""
+    if t is not None:
+        return t, _heads(fn, t, sh, dt, dev)
+    t = x.new_empty(sh)
+    return t, (t.data_ptr(), sh[1] * sh[2], sh[2])
+
+
+def _packed(fn, q, k, v, cu_q, cu_k, causal, scale, o, lse, backward=False, do=None, dq=None, dk=None, dv=None):
+    """(parameter block, type, outputs)"""
+    dt, qs, ks = q.dtype, q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or (dt is not _BF16 and dt is not torch.float16):
         raise ValueError(f"{fn}: bf16 or fp16 tensors [tokens, heads, head_dim]")
-    dev, dt = _device(fn, q), q.dtype
-    (tq, hq, d), (tk, hk, _) = q.shape, k.shape
-    cu_k = cu_q if cu_k is None else cu_k
-    n = cu_q.numel() - 1
-    for cu in (cu_q, cu_k):
-        if cu.dtype is not torch.int32 or cu.dim() != 1 or cu.numel() != n + 1 or n < 0 or (
-                cu.get_device() != dev or (n > 0 and cu.stride(0) != 1)):
-            raise ValueError(f"{fn}: cu_q and cu_k are int32 [sequences + 1], contiguous, on the device")
+    dev = _device(fn, q)
+    (tq, hq, d), (tk, hk, _) = qs, ks
     if hk == 0 or hq == 0 or hq % hk or d % 8 or not 8 <= d <= 128:
         raise ValueError(f"{fn}: key heads divide the query heads; head_dim is a multiple of 8, at most 128")
-    Q = _heads(fn, q, tq, hq, d, dt, dev)
-    K, V = _heads(fn, k, tk, hk, d, dt, dev), _heads(fn, v, tk, hk, d, dt, dev)
-    O = _heads(fn, o, tq, hq, d, dt, dev)  # noqa: E741
-    lp = ls = 0
-    if lse is not None:
+    n = cu_q.numel() - 1
+    cq = ck = _starts(fn, cu_q, n, dev)
+    if cu_k is not None:
+        ck = _starts(fn, cu_k, n, dev)
+    Q = _heads(fn, q, qs, dt, dev)
+    ks = (tk, hk, d)
+    K, V = _heads(fn, k, ks, dt, dev), _heads(fn, v, ks, dt, dev)
+    if lse is None:
+        if backward:
+            raise ValueError(f"{fn}: the forward's o and lse are needed")
+        lse = q.new_empty((hq, tq), dtype=_F32)
+        L = lse.data_ptr(), tq
+    else:
         if lse.dtype is not _F32 or lse.shape != (hq, tq) or lse.get_device() != dev or (
                 lse.stride(1) != 1 and tq > 1):
             raise ValueError(f"{fn}: lse is fp32 [heads, tokens] with a unit last-dim stride")
-        lp, ls = lse.data_ptr(), lse.stride(0) if hq > 1 else 0
-    if do is None:
-        G = DQ = DK = DV = (0, 0, 0)
+        L = lse.data_ptr(), lse.stride(0) if hq > 1 else 0
+    if backward:
+        O, G = _heads(fn, o, qs, dt, dev), _heads(fn, do, qs, dt, dev)  # noqa: E741
+        dq, DQ = _like(fn, dq, q, qs, dt, dev)
+        dk, DK = _like(fn, dk, q, ks, dt, dev)
+        dv, DV = _like(fn, dv, q, ks, dt, dev)
+        outs = dq, dk, dv
     else:
-        G, DQ = _heads(fn, do, tq, hq, d, dt, dev), _heads(fn, dq, tq, hq, d, dt, dev)
-        DK, DV = _heads(fn, dk, tk, hk, d, dt, dev), _heads(fn, dv, tk, hk, d, dt, dev)
-    return _PACKED_PACK(Q[0], K[0], V[0], O[0], G[0], DQ[0], DK[0], DV[0], lp, cu_q.data_ptr(), cu_k.data_ptr(),
-                        n, hq, hk, d, d ** -0.5 if scale is None else scale, causal, tq, tk, Q[1], Q[2], K[1],
-                        K[2], V[1], V[2], O[1], O[2], G[1], G[2], DQ[1], DQ[2], DK[1], DK[2], DV[1], DV[2], ls)
+        o, O = _like(fn, o, q, qs, dt, dev)  # noqa: E741
+        G = DQ = DK = DV = _NO_HEADS
+        outs = o, lse
+    return _PACKED_PACK(Q[0], K[0], V[0], O[0], G[0], DQ[0], DK[0], DV[0], L[0], cq, ck, n, hq, hk, d,
+                        d ** -0.5 if scale is None else scale, causal, tq, tk, Q[1], Q[2], K[1], K[2], V[1], V[2],
+                        O[1], O[2], G[1], G[2], DQ[1], DQ[2], DK[1], DK[2], DV[1], DV[2], L[1]), _TYPE[dt], outs
+
+
+def _starts(fn: str, cu: torch.Tensor, n: int, dev: int) -> int:
+    """The address of the sequences' first rows, and the end of the last."""
+    if cu.dtype is not torch.int32 or cu.dim() != 1 or cu.numel() != n + 1 or n < 0 or (
+            cu.get_device() != dev or not cu.is_contiguous()):
+        raise ValueError(f"{fn}: cu_q and cu_k are int32 [sequences + 1], contiguous, on the device")
+    return cu.data_ptr()
 
 
 def attn_packed_forward(q, k, v, cu_q, cu_k=None, causal: bool = True, scale: float | None = None, o=None,
@@ -846,27 +873,18 @@ def attn_packed_forward(q, k, v, cu_q, cu_k=None, causal: bool = True, scale: fl
     None: as cu_q), and query i of m sees key j of n where j <= i + n - m, or all keys. Query head h goes with key
     head h // (q_heads / k_heads). Returns (o, lse): o like q, lse fp32 [q_heads, tokens], 0 and -inf where a
     query sees no key; rows of no sequence are not written."""
-    o = q.new_empty(q.shape) if o is None else o
-    lse = q.new_empty((q.shape[1], q.shape[0]), dtype=_F32) if lse is None and q.dim() == 3 else lse
-    p = _packed_params("attn_packed_forward", q, k, v, cu_q, cu_k, causal, scale, o, lse)
-    kind = _TYPE[q.dtype]
+    p, kind, outs = _packed("attn_packed_forward", q, k, v, cu_q, cu_k, causal, scale, o, lse)
     _call_captured("hk_attn_packed_forward", lambda: lib().hk_attn_packed_workspace(p, kind, 0), p, kind)
-    return o, lse
+    return outs
 
 
 def attn_packed_backward(do, q, k, v, o, lse, cu_q, cu_k=None, causal: bool = True, scale: float | None = None,
                          dq=None, dk=None, dv=None):
     """Gradients (dq, dk, dv) of attn_packed_forward's inputs from that of its output, all of q's type. Written, not
     added to; those of rows of no sequence are not written."""
-    dq = q.new_empty(q.shape) if dq is None else dq
-    dk = k.new_empty(k.shape) if dk is None else dk
-    dv = v.new_empty(v.shape) if dv is None else dv
-    if lse is None:
-        raise ValueError("attn_packed_backward: the forward's lse is needed")
-    p = _packed_params("attn_packed_backward", q, k, v, cu_q, cu_k, causal, scale, o, lse, do, dq, dk, dv)
-    kind = _TYPE[q.dtype]
+    p, kind, outs = _packed("attn_packed_backward", q, k, v, cu_q, cu_k, causal, scale, o, lse, True, do, dq, dk, dv)
     _call_captured("hk_attn_packed_backward", lambda: lib().hk_attn_packed_workspace(p, kind, 1), p, kind)
-    return dq, dk, dv
+    return outs
 
 
 # ----------------------------------------------------------------------------------------------
@@ -919,13 +937,18 @@ def token_logprobs(logits, tokens, entropy=False, top: int = 0, logp=None, lse=N
     dev, rows, vocab, stride = _logits(fn, logits, tokens)
     if not 0 <= top <= min(64, vocab):
         raise ValueError(f"{fn}: top is 64 at most, and the vocabulary")
-    new = lambda dt, *shape: torch.empty(shape, device=logits.device, dtype=dt)  # noqa: E731
-    logp = new(_F32, rows) if logp is None else logp
-    lse = new(_F32, rows) if lse is None else lse
-    ent = new(_F32, rows) if entropy is True else None if entropy is False else entropy
+    entropy = False if entropy is None else entropy
+    ent = None if entropy is True or entropy is False else entropy
+    if logp is None and lse is None and ent is None:  # one allocation for all
+        logp, lse, *more = logits.new_empty((2 + entropy, rows), dtype=_F32).unbind(0)
+        ent = more[0] if more else None
+    else:
+        logp = logits.new_empty((rows,), dtype=_F32) if logp is None else logp
+        lse = logits.new_empty((rows,), dtype=_F32) if lse is None else lse
+        ent = logits.new_empty((rows,), dtype=_F32) if entropy is True else ent
     if top:
-        top_logp = new(_F32, rows, top) if top_logp is None else top_logp
-        top_index = new(torch.int64, rows, top) if top_index is None else top_index
+        top_logp = logits.new_empty((rows, top), dtype=_F32) if top_logp is None else top_logp
+        top_index = logits.new_empty((rows, top), dtype=torch.int64) if top_index is None else top_index
     elif top_logp is not None or top_index is not None:
         raise ValueError(f"{fn}: outputs of alternatives that are not asked for")
     kind = _TYPE[logits.dtype]

@@ -776,7 +776,7 @@ HK_API hipError_t hk_attn_packed_backward(const hk_attn_packed_params* params, i
  * without the first term's one-hot for a token out of range, and NaN for a row without a softmax. grad is of the
  * logits' type, rows grad_stride apart, and may be the logits themselves (with their stride). Sums are fp32; the
  * gradient is rounded once.
- * vocab is 1 .. 2^21, top at most 64 and vocab, rows below 2^31. No output may share memory with anything else of
+ * vocab is 1 .. 2^20, top at most 64 and vocab, rows below 2^31. No output may share memory with anything else of
  * the call. Workspace: hk_token_logprobs_workspace bytes (rows that are cut into pieces; -1: invalid arguments), as
  * for hk_attn_packed_forward.
  * ---------------------------------------------------------------------------------------- */
