@@ -40,6 +40,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // rounding of two fp32 values (to nearest even).
 struct TypeBF16 {
   using format = BF16;
+  static constexpr bool kNarrow = false;  // fp32's exponents
   static __device__ __forceinline__ f32x16_t mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                    __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -53,6 +54,7 @@ struct TypeBF16 {
 };
 struct TypeF16 {
   using format = F16;
+  static constexpr bool kNarrow = true;
   static __device__ __forceinline__ f32x16_t mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
@@ -88,7 +90,7 @@ struct Args {
   int near;  // backward: groups divide 32 rows, which lie within 2^30 bytes
   float* part;   // partial results
   float2* stat;  // forward: (max, sum) of them
-  float* delta;  // backward: rowsum(dout * o), [q head][token]
+  float* delta;  // backward: rowsum(dout * o), log-sum-exp in log 2 and dout's exponent, each [q head][token]
 };
 
 __host__ __device__ inline int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {

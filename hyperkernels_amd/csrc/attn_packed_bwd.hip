@@ -7,11 +7,16 @@
 // dP^T = V dO^T with a row a lane, dS^T the operand of dQ^T += K^T dS^T as it lies) and leaves delta and lse for
 // attn_packed_dkv, which goes by keys: S = Q K^T and dP = dO V^T with a key a lane, P and dS the operands of
 // dV^T += dO^T P and dK^T += Q^T dS as they lie. The rows of a group's heads are one loop there, which sums them.
-// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32.
+// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. dS is as small as P and
+// dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
+// times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
+// where dK is moved to the next when it grows.
 #include "attn_packed.h"
 
 namespace hk {
 namespace packed {
+
+constexpr int kLeast = -40;  // an exponent under any of fp16
 
 template <int D, int KG>
 struct DqShape {
@@ -61,6 +66,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
 
   s16x8_t qx[D / 16], gx[D / 16];
   float delta = 0.f, lse2;
+  int grow = 0;
   {
     const int64_t at = q.q0 + tok;
     load_row<D>(a.q.p + at * a.q.m + qh * a.q.h, h, a.d, qx);
@@ -80,12 +86,31 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
       }
     }
     delta = half32_reduce(delta, AddOp{});
+    if constexpr (T::kNarrow) {
+      float most = 0.f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const u32x4_t y = __builtin_bit_cast(u32x4_t, gx[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2_t w = T::unpack(y[i]);
+          most = fmaxf(most, fmaxf(fabsf(w[0]), fabsf(w[1])));
+        }
+      }
+      // dout is under 2^grow, a row of zeros under any of fp16's
+      most = half32_reduce(most, MaxOp{});
+      grow = most == 0.f ? kLeast : __builtin_amdgcn_frexp_expf(most);
+    }
     if (kg == 0 && h == 0 && row < rows) {
       float* st = a.delta + qh * a.q_tokens + at;
       st[0] = delta;
-      st[static_cast<int64_t>(a.k_heads) * a.group * a.q_tokens] = lse2;
+      const int64_t all = static_cast<int64_t>(a.k_heads) * a.group * a.q_tokens;
+      st[all] = lse2;
+      if (T::kNarrow) st[2 * all] = static_cast<float>(grow);
     }
+    if (T::kNarrow) lse2 += static_cast<float>(grow);
   }
+  const float out = T::kNarrow ? ldexpf(a.scale, grow) : a.scale;
 
   const Reads<D> rd(lane);
   const float sc = a.scale * kLog2e;
@@ -138,7 +163,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4_t HK_LDS*>(ex + (kg * R + w0 - r0 + c) * S::kPitch + 32 * b + 8 * g + 4 * h) =
-            f32x4_t{dq[b][4 * g], dq[b][4 * g + 1], dq[b][4 * g + 2], dq[b][4 * g + 3]};
+            f32x4_t{dq[b][4 * g] * out, dq[b][4 * g + 1] * out, dq[b][4 * g + 2] * out, dq[b][4 * g + 3] * out};
     __syncthreads();
     const int er = threadIdx.x / (2 * KG), e0 = threadIdx.x % (2 * KG);
     if (r0 + er >= rows) return;
@@ -151,14 +176,13 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
 #pragma unroll
       for (int g = 0; g < KG; ++g)
         x += *reinterpret_cast<const f32x4_t HK_LDS*>(ex + (g * R + er) * S::kPitch + col);
-      x *= a.scale;
       if (col < a.d)
         *reinterpret_cast<u32x2_t*>(op + 2 * col) = u32x2_t{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
     }
     return;
   }
   if (row >= rows) return;
-  store_row<T, D>(a.dq.p + (q.q0 + tok) * a.dq.m + qh * a.dq.h, h, a.d, dq, a.scale);
+  store_row<T, D>(a.dq.p + (q.q0 + tok) * a.dq.m + qh * a.dq.h, h, a.d, dq, out);
 }
 
 // A wave takes 32 keys and, of every tile of 64 rows, all or (HALVES = 2, two waves a key block) 32 rows. Heads past 64
@@ -170,7 +194,7 @@ struct DkvShape {
   static constexpr int kRows = D == 128 ? 64 : 32;  // rows a tile
   static constexpr int kHalves = D == 128 ? 2 : 1, kThreads = 256 * kHalves;
   static constexpr int kTile = kRows * D * 2;
-  static constexpr int kStage = 2 * kTile + 2 * 64 * 4;  // Q, dO, delta, lse (of 64 rows)
+  static constexpr int kStage = 2 * kTile + 3 * 64 * 4;  // Q, dO, delta, lse, exponent (of 64 rows)
   static constexpr int kHeld = 2 * kKeys * D * 2;  // K, V
   static constexpr int kPitch = D + 4;
   static constexpr int kExchange = kHalves == 2 ? kKeys * kPitch * 4 : 0;
@@ -221,6 +245,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
   static_assert(kWaves * kCopyRows == 32, "copies are 32 rows apart");
   const int lr = wave * kCopyRows + lane / kChunks;
   const int ch = 16 * min((lane % kChunks) ^ swz<D>(lr), a.d / 8 - 1);
+  constexpr int kStats = T::kNarrow ? 3 : 2;
   int off_q = 0, off_g = 0, off_d = 0, per32 = 0;
   if (a.near) {
     per32 = 32 / a.group;
@@ -233,7 +258,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
   const char* const q0p = a.q.p + q.q0 * a.q.m + kh * a.group * a.q.h;
   const char* const g0p = a.dout.p + q.q0 * a.dout.m + kh * a.group * a.dout.h;
   const char* const d0p =
-      reinterpret_cast<const char*>(a.delta + ((wave & 1) * heads + kh * a.group) * a.q_tokens + q.q0);
+      reinterpret_cast<const char*>(a.delta + ((wave < kStats ? wave : 0) * heads + kh * a.group) * a.q_tokens + q.q0);
   auto fetch = [&](int t) {
     const unsigned to = lds0 + S::kHeld + (t & 1) * S::kStage;
     if (a.near && t * S::kRows + 64 <= rows) {
@@ -243,7 +268,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
         copy16_to_lds(q0p + (tok + i * per32) * a.q.m, off_q, to + 1024 * (wave + kWaves * i));
         copy16_to_lds(g0p + (tok + i * per32) * a.dout.m, off_g, to + S::kTile + 1024 * (wave + kWaves * i));
       }
-      if (wave < 2) copy4_to_lds(d0p + 4 * tok, off_d, to + 2 * S::kTile + 256 * wave);
+      if (wave < kStats) copy4_to_lds(d0p + 4 * tok, off_d, to + 2 * S::kTile + 256 * wave);
       return;
     }
 #pragma unroll
@@ -253,7 +278,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
       copy16_to_lds(q0p + tok * a.q.m + hd * a.q.h + ch, to + 1024 * (wave + kWaves * i));
       copy16_to_lds(g0p + tok * a.dout.m + hd * a.dout.h + ch, to + S::kTile + 1024 * (wave + kWaves * i));
     }
-    if (wave < 2) {
+    if (wave < kStats) {
       const int r = min(t * S::kRows + lane, rows - 1);
       const int tok = r / a.group, hd = r - tok * a.group;
       copy4_to_lds(d0p + 4 * (hd * a.q_tokens + tok), to + 2 * S::kTile + 256 * wave);
@@ -284,6 +309,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
   f32x16_t dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) dk[b] = dv[b] = f32x16_t{};
+  float grow = kLeast;  // exponent of the dout that dk is formed for
 
   for (int t = t0; t < t1; ++t) {
     wait_copies();
@@ -292,6 +318,18 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
     const char HK_LDS* qt = lds + S::kHeld + (t & 1) * S::kStage;
     const char HK_LDS* gt = qt + S::kTile;
     const float HK_LDS* dl = (const float HK_LDS*)(gt + S::kTile);
+    if constexpr (T::kNarrow) {
+      const float g = wave_max(dl[128 + lane]);
+      if (g > grow) {
+        const float f = __builtin_amdgcn_exp2f(grow - g);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[b][i] *= f;
+        grow = g;
+      }
+    }
+    const float shrink = T::kNarrow ? __builtin_amdgcn_exp2f(-grow) : 1.f;
 #pragma unroll
     for (int u = 0; u < S::kRows / 32 / S::kHalves; ++u) {
       const int n = S::kHalves == 2 ? half : u;
@@ -317,7 +355,9 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[4 * g + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + e], sc, -ls[e]));
-          dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - de[e]);
+          dp[4 * g + e] -= de[e];
+          if (T::kNarrow) dp[4 * g + e] *= shrink;
+          dp[4 * g + e] *= s[4 * g + e];
         }
       }
       s16x8_t p[2], ds[2];
@@ -332,6 +372,13 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) dk[b] = T::mfma(rd.cols(qt, 32 * n + 16 * e, b), ds[e], dk[b]);
     }
+  }
+  if constexpr (T::kNarrow) {
+    const float f = __builtin_amdgcn_exp2f(grow);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[b][i] *= f;
   }
   if constexpr (S::kHalves == 2) {
     // the second half's sums, first of dK, then of dV
@@ -423,7 +470,7 @@ Plan plan(const hk_attn_packed_params* p) {
   const int64_t want = wgs < 2 * cus ? ceil_div(3 * cus, wgs) : 1;
   r.splits = static_cast<int>(clamp64(want, 1, clamp64(rows / p->num_seqs / 256, 1, 64)));
   if (r.splits > 1) r.part = r.splits * p->k_tokens * p->k_heads * (p->head_dim <= 64 ? 64 : 128) * 8;
-  r.stat = ceil_div(8 * p->q_tokens * p->q_heads, 16) * 16;
+  r.stat = ceil_div(12 * p->q_tokens * p->q_heads, 16) * 16;
   return r;
 }
 

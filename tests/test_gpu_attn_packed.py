@@ -32,8 +32,8 @@ def cu_of(lens):
     return torch.tensor(at, device=DEV, dtype=torch.int32)
 
 
-def reference(q, k, v, lq, lk, causal, scale, do=None):
-    """Per output its value and tolerance, in 64 bits: {name: (value, tolerance)}."""
+def reference(q, k, v, lq, lk, causal, scale, do=None, step=None):
+    """Per output its value and tolerance, in 64 bits: {name: (value, tolerance)}. step: the absolute one of dS."""
     H, Hk, d = q.shape[1], k.shape[1], q.shape[2]
     e = torch.finfo(q.dtype).eps / 2
     tiny = 2.0 ** -25 if q.dtype is F16 else 2.0 ** -126
@@ -76,7 +76,7 @@ def reference(q, k, v, lq, lk, causal, scale, do=None):
         td = (G.abs() * (to + d * 2.0 ** -23 * o.abs())).sum(2, keepdim=True)
         ds = p * (dp - delta)
         t = p * (td + d * 2.0 ** -23 * (G.abs() @ V.abs().transpose(1, 2))) + ds.abs() * (e * 1.01 + rest)
-        t = torch.where(see, t + tiny * (1 + (dp - delta).abs()), 0.0)
+        t = torch.where(see, t + (tiny * (1 + (dp - delta).abs()) if step is None else step), 0.0)
         dq, tq = scale * ds @ K, scale * t @ K.abs()
         dk, tk = scale * ds.transpose(1, 2) @ Q, scale * t.transpose(1, 2) @ Q.abs()
         # n and m products are summed in fp32
@@ -178,6 +178,24 @@ def test_ranges(hk, std, scale):
     # sharp softmaxes whose maximum moves from tile to tile, and flat ones
     say(std, scale)
     both(hk, [300, 41], [300, 41], 4, 2, 64, BF, True, scale=scale, std=std)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 9])
+@pytest.mark.parametrize("H,Hk,d,lens", [(4, 2, 64, [1500, 70]), (2, 2, 128, [900]), (16, 4, 128, [2048, 600])])
+def test_small_and_large_gradients_in_fp16(hk, size, H, Hk, d, lens):
+    # a dS of P times dout, 1e-3 * 2e-4, is no normal fp16 number: it is held for a dout of 1
+    say(size, H, Hk, d, lens)
+    q, k, v, do = make(lens, lens, H, Hk, d, F16, std=0.3)
+    do = (do * (size / 0.3)).to(F16)
+    do[::3] *= 0.125  # rows of different sizes, and of nothing, as a loss leaves out
+    do[5::7] = 0
+    cq = cu_of(lens)
+    o, lse = hk.attn_packed_forward(q, k, v, cq)
+    dq, dk, dv = hk.attn_packed_backward(do, q, k, v, o, lse, cq)
+    # half a step of fp16's smallest numbers, times the power of two above the largest dout; a result's own is not scaled
+    step = 2.0 ** -24 * float(do.abs().max())
+    want = reference(q, k, v, lens, lens, True, d ** -0.5, do, step)
+    check({"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, want)
 
 
 def test_rows_of_no_sequence_stay(hk):
