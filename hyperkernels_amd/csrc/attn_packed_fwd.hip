@@ -65,6 +65,12 @@ __device__ __forceinline__ void attend(const Args& a, const Seq& q, int kh, int 
     copy_v(t, q.mk, wave, to + S::kTile);
   };
   if (t0 < t1) fetch(t0);
+  if constexpr (KG == 4) {
+    // the compiler waits for the rows here, with the first tile, and not for the second one later
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(qx[i]));
+    if (t0 + 1 < t1) fetch(t0 + 1);
+  }
 
   const Reads<D> rd(lane);
   const float sc = a.scale * kLog2e;
@@ -75,9 +81,22 @@ __device__ __forceinline__ void attend(const Args& a, const Seq& q, int kh, int 
   float m = -INFINITY, l = 0.f;  // in units of log 2
 
   for (int t = t0; t < t1; ++t) {
-    wait_copies();
-    barrier();  // this tile has landed, and every wave is done with the one before it
-    if (t + 1 < t1) fetch(t + 1);
+    if constexpr (KG == 4) {
+      // Few workgroups, bound by memory: the tile after the next is fetched as soon as all waves are done with the last,
+      // whether or not the next has landed (16 tokens over 1 to 4000 keys of 4 heads of 128, with the join: 21.2 -> 19.3 us).
+      if (t > t0) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+        if (t + 1 < t1) fetch(t + 1);
+      }
+      if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * KeyCopy<D, S::kKeys>::kCopies) : "memory");
+      else wait_copies();
+      barrier();  // this tile has landed
+    } else {
+      wait_copies();
+      barrier();  // this tile has landed, and every wave is done with the one before it
+      if (t + 1 < t1) fetch(t + 1);
+    }
     const int key0 = t * S::kKeys + 32 * S::kBlocks * kg;
     if (key0 > lim_hi) continue;  // the wave's rows see none of these
     const char HK_LDS* kt = lds + (t & 1) * S::kStage + 32 * S::kBlocks * kg * (2 * D);
