@@ -940,24 +940,29 @@ def token_logprobs(logits, tokens, entropy=False, top: int = 0, logp=None, lse=N
     entropy = False if entropy is None else entropy
     ent = None if entropy is True or entropy is False else entropy
     if logp is None and lse is None and ent is None:  # one allocation for all
-        logp, lse, *more = logits.new_empty((2 + entropy, rows), dtype=_F32).unbind(0)
+        own = logits.new_empty((2 + entropy, rows), dtype=_F32)
+        logp, lse, *more = own.unbind(0)
         ent = more[0] if more else None
+        p = own.data_ptr()
+        ptrs = p, p + 4 * rows, p + 8 * rows if more else None
     else:
         logp = logits.new_empty((rows,), dtype=_F32) if logp is None else logp
         lse = logits.new_empty((rows,), dtype=_F32) if lse is None else lse
         ent = logits.new_empty((rows,), dtype=_F32) if entropy is True else ent
+        ptrs = (_row_values(fn, "logp", logp, dev, (rows,)), _row_values(fn, "lse", lse, dev, (rows,)),
+                _row_values(fn, "entropy", ent, dev, (rows,)))
+    vp = ip = None
     if top:
         top_logp = logits.new_empty((rows, top), dtype=_F32) if top_logp is None else top_logp
         top_index = logits.new_empty((rows, top), dtype=torch.int64) if top_index is None else top_index
+        vp = _row_values(fn, "top_logp", top_logp, dev, (rows, top))
+        ip = _row_values(fn, "top_index", top_index, dev, (rows, top), torch.int64)
     elif top_logp is not None or top_index is not None:
         raise ValueError(f"{fn}: outputs of alternatives that are not asked for")
     kind = _TYPE[logits.dtype]
     _call_captured("hk_token_logprobs", lambda: lib().hk_token_logprobs_workspace(kind, rows, vocab, top),
-                   logits.data_ptr(), kind, rows, vocab, stride, tokens.data_ptr(), _WIDE[tokens.dtype],
-                   _row_values(fn, "logp", logp, dev, (rows,)), _row_values(fn, "lse", lse, dev, (rows,)),
-                   _row_values(fn, "entropy", ent, dev, (rows,)), top,
-                   _row_values(fn, "top_logp", top_logp, dev, (rows, top)),
-                   _row_values(fn, "top_index", top_index, dev, (rows, top), torch.int64))
+                   logits.data_ptr(), kind, rows, vocab, stride, tokens.data_ptr(), _WIDE[tokens.dtype], *ptrs, top, vp,
+                   ip)
     return TokenLogprobs(logp, lse, ent, top_logp, top_index)
 
 
