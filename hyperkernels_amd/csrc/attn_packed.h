@@ -189,11 +189,12 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, con
   const uint64_t with = __ballot(count > lo);
   const bool it = count > lo && __popcll(with & ((uint64_t(1) << lane) - 1)) == x - above;
   const int s = __ffsll(static_cast<unsigned long long>(__ballot(it))) - 1;
+  if (s < 0) return false;
   auto of = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
   q.q0 = of(q0), q.mq = of(q1 - q0), q.k0 = of(k0), q.mk = of(k1 - k0);
   q.tile = lo, q.tiles = of(count);
   share = rest / a.k_heads, head = rest - share * a.k_heads;
-  return true;
+  return lo >= 0 && lo < q.tiles;  // whatever sequences that overlap add up to
 }
 
 // Item L of those that give every row tile's keys in shares of a.chunk tiles of B_k keys, sequence after sequence: shares
@@ -226,7 +227,7 @@ __device__ __forceinline__ bool find_share(const Args& a, int B, int B_k, int L,
   q.tiles = of(tiles);
   q.tile = r / shares;
   share = r - q.tile * shares;
-  return true;
+  return r >= 0 && q.tile < q.tiles;
 }
 
 // LDS tile: rows of D elements (2 D bytes) as they lie in memory, the 16-byte chunk c of row r at chunk c ^ swz(r).
@@ -383,8 +384,8 @@ inline hipError_t check(const hk_attn_packed_params* p, int type, bool backward)
   HK_CHECK_ARG(p->scale > 0.f && p->scale < INFINITY);
   constexpr int64_t kMost = INT32_MAX / 2;  // rows and keys are counted in 32 bits, a tile's worth behind the last
   HK_CHECK_ARG(p->q_tokens <= kMost / p->q_heads && p->k_tokens <= kMost);
-  // workgroups of one launch: 2^32 threads are more than it takes
-  constexpr int64_t kGrid = int64_t(1) << 23;
+  // workgroups of one launch, of 512 threads at most: 2^32 threads are more than it takes
+  constexpr int64_t kGrid = int64_t(1) << 22;
   HK_CHECK_ARG((slots(p->q_tokens, p->num_seqs, p->q_heads / p->k_heads, 32)) <= kGrid / p->k_heads);
   HK_CHECK_ARG(slots(p->k_tokens, p->num_seqs, 1, 128) <= kGrid / p->k_heads);
   if (p->num_seqs == 0) return hipSuccess;

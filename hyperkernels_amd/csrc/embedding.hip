@@ -115,14 +115,14 @@ struct Grad {
 // Zeros one row of the table: all lanes of a group of `lanes`.
 __device__ __forceinline__ void zero_row(const Grad& a, int64_t row, int lane, int lanes) {
   char* p = static_cast<char*>(a.table) + row * a.table_stride * a.table_elem;
-  const int bytes = a.d * a.table_elem;
+  const int64_t bytes = static_cast<int64_t>(a.d) * a.table_elem;
   const uintptr_t both = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(bytes);
   if ((both & 15) == 0) {
-    for (int i = lane * 16; i < bytes; i += lanes * 16) st_nt(reinterpret_cast<uint4*>(p + i), make_uint4(0, 0, 0, 0));
+    for (int64_t i = lane * 16; i < bytes; i += lanes * 16) st_nt(reinterpret_cast<uint4*>(p + i), make_uint4(0, 0, 0, 0));
   } else if ((both & 3) == 0) {
-    for (int i = lane * 4; i < bytes; i += lanes * 4) *reinterpret_cast<uint32_t*>(p + i) = 0;
+    for (int64_t i = lane * 4; i < bytes; i += lanes * 4) *reinterpret_cast<uint32_t*>(p + i) = 0;
   } else {
-    for (int i = lane * 2; i < bytes; i += lanes * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    for (int64_t i = lane * 2; i < bytes; i += lanes * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
   }
 }
 
@@ -440,6 +440,7 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
     at += __popcll(mask[u]);
   }
   __syncthreads();
+  if (a.accumulate && total == 0) return;  // none of these rows
   for (int r = wave; r < rows; r += 4) {
     bool any = false;
     for (int i = 0; i < total; i += 64) any |= __any(i + lane < total && list[min(i + lane, total - 1)].y == r);

@@ -714,11 +714,12 @@ HK_API hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* params,
  * (HK_TYPE_BF16 or HK_TYPE_F16): any strides of tokens (M) and heads (H) that are multiples of 8 elements, unit
  * last-dim stride, 16-byte aligned; those of tokens of k and v at most 2^23. head_dim is a multiple of 8, 128 at
  * most. lse is fp32 [q_heads, q_tokens], heads lse_strideH elements apart; NULL in the forward pass: not wanted.
- * scale is positive and finite. At most 2^30 rows (q_tokens * q_heads) and 2^23 tiles of 32 rows or 128 keys.
+ * scale is positive and finite. Under 2^30 rows (q_tokens * q_heads) and keys, and at most
+ * 2^22 tiles of 32 rows or 128 keys, counting one a sequence more than they fill, over all key heads.
  * Rows before cu[0] and from cu[num_seqs] on are not written. Starts past the tensors count as their ends and a
  * sequence that would end before it begins as empty: nothing outside the tensors is read or written whatever cu holds.
  * Scores, softmax and sums are fp32; P, and in the backward pass P and dS, are rounded to the call's type for the
- * products over keys or rows. Sums are in a fixed order (no atomics). Elements that are not finite make outputs of
+ * products over keys or rows. Sums are in a fixed order (no atomics). Elements that are not finite, and scores past fp32, make outputs of
  * their own sequence NaN, also those of queries that a mask keeps from them, but of no other sequence.
  * No output may share memory with anything else of the call, nor two of its rows with each other.
  * Workspace: hk_attn_packed_workspace bytes (0: none is needed, -1: invalid arguments), as for

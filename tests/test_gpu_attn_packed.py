@@ -247,6 +247,34 @@ def test_starts_past_the_tensors(hk):
         assert torch.equal(x, y)
 
 
+def test_starts_that_fall_stay_inside(hk):
+    # not what cu may hold: which rows are written is not said, but none outside the tensors is
+    q, k, v, do = make([300], [300], 4, 2, 64, BF)
+    for starts in ([0, 100, 0, 100, 0, 100], [300, 200, 100, 0], [-5, 400, -5, 400], [50, 50, 10, 90, 20, 290]):
+        cu = torch.tensor(starts, device=DEV, dtype=torch.int32)
+        held = [torch.full((t.shape[0] + 20, *t.shape[1:]), 7.0, device=DEV, dtype=BF) for t in (q, q, k, v)]
+        lses = torch.full((4, 340), 7.0, device=DEV)
+        o, dq, dk, dv = (t[10:-10] for t in held)
+        lse = lses[:, 20:320]
+        lse[:] = 0
+        hk.attn_packed_forward(q, k, v, cu, o=o, lse=lse)
+        hk.attn_packed_backward(do, q, k, v, o, lse, cu, dq=dq, dk=dk, dv=dv)
+        torch.cuda.synchronize()
+        for t in held:
+            assert (t[:10] == 7).all() and (t[-10:] == 7).all(), starts
+        assert (lses[:, :20] == 7).all() and (lses[:, 320:] == 7).all(), starts
+
+
+def test_no_keys_and_no_queries(hk):
+    for lq, lk in (([5], [0]), ([0], [7]), ([0, 0], [0, 0])):
+        both(hk, lq, lk, 4, 2, 64, BF, True)
+    # no sequence: nothing is written
+    q, k, v, _ = make([3], [3], 2, 1, 64, F16)
+    o = torch.full_like(q, 7.0)
+    hk.attn_packed_forward(q, k, v, torch.zeros(1, device=DEV, dtype=torch.int32), o=o)
+    assert (o == 7).all()
+
+
 def test_same_bits_and_other_stream(hk):
     lens = [700, 33, 1000]
     a = both(hk, lens, lens, 8, 2, 128, BF, True)

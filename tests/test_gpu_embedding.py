@@ -105,6 +105,15 @@ def test_gradient_of_many_tokens(hk):
         assert torch.equal(out.double(), want)
 
 
+def test_gradient_of_one_row_for_all(hk):
+    # a gradient that was broadcast: one row for all tokens
+    for n in (300, 3000):
+        t = tokens(n, 40, "words")
+        row = torch.randint(-3, 4, (1, 24), device=DEV).float()
+        out = hk.embedding_backward(row.expand(n, 24), t, torch.full((40, 24), 5.0, device=DEV), accumulate=False)
+        assert torch.equal(out, torch.bincount(t, minlength=40)[:, None] * row)
+
+
 def test_gradient_is_the_lookup_s(hk):
     # <lookup(table), g> = <table, gradient(g)>
     for n in (200, 3000):
