@@ -13,9 +13,11 @@
 //
 // The `top` largest: with W waves, the ceil(top / W)-th largest of each wave's 64 lane maxima is reached by that many
 // elements of the wave, so the least of those over the waves is a bound that `top` elements reach and few others do (some
-// 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, where all lanes look them through and
-// collect (value, index) keys, which are ranked by counting the larger ones. Where more pass than these lists take
-// (equal values, or a mask that leaves few), `top` passes over the row find the next largest.
+// 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, 128 lanes at a time, where all lanes
+// look them through and collect (value, index) keys, which are ranked by counting the larger ones. Where more pass
+// than that list takes (equal values), `top` passes over the row find the next largest.
+#include <limits.h>
+
 #include "hk_device.h"
 #include "hk_host.h"
 #include "hk_overlap.h"
@@ -198,26 +200,31 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
       __syncthreads();
       bound = row16_reduce(red[0][lane & (W - 1)], [](float p, float q) { return fminf(p, q); });
     }
+    // A row with fewer than that above -inf has all of those, and then the first at -inf.
+    const bool scarce = bound == -INFINITY && s - s == 0.f;
+    const auto passes = [&](float e) { return scarce ? e > -INFINITY : !(e < bound); };
     auto collect = [&](float e, int i) {
-      if (!(e < bound)) {
+      if (passes(e)) {
         const int at = atomicAdd(&count, 1);
         if (at < kList) list[at] = key_of(e, base + i);
       }
     };
-    if (!(mx < bound)) {
-      const int slot = atomicAdd(&lanes, 1);
-      if (slot < kLanes) {
-        owner[slot] = static_cast<uint16_t>(tid);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v * THREADS + tid < vecs) stash[slot * V + v] = d[v];
-      }
+    int slot = INT_MAX;
+    if (passes(mx)) {
+      slot = atomicAdd(&lanes, 1);
       if (odd >= 0) collect(x0, odd);
     }
     __syncthreads();
     const int held = lanes;
-    if (held <= kLanes) {
-      for (int i = tid; i < held * V; i += THREADS) {
+    for (int from = 0; from < held; from += kLanes) {
+      if (slot >= from && slot < from + kLanes) {
+        owner[slot - from] = static_cast<uint16_t>(tid);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
+      }
+      __syncthreads();
+      for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
         const int at = (i % V) * THREADS + owner[i / V];
         if (at < vecs) {
           float e[kE];
@@ -226,13 +233,26 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
           for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
         }
       }
+      __syncthreads();
+      if (count > kList) break;
     }
     __syncthreads();
     const int found = count;
-    if (held <= kLanes && found <= kList) {
+    if (found <= kList) {
       rank_keys<THREADS>(list, found, a.top, put);
-      // a piece of fewer elements
-      for (int i = found + tid; i < a.top; i += THREADS) put(i, 0);
+      if (tid < 64) {
+        int got = found;
+        if (scarce)
+          for (int i0 = 0; i0 < n && got < a.top; i0 += 64) {
+            const bool it = i0 + lane < n && F::load(x, i0 + lane) == -INFINITY;
+            const uint64_t those = __ballot(it);
+            const int rank = got + __popcll(those & ((uint64_t(1) << lane) - 1));
+            if (it && rank < a.top) put(rank, key_of(-INFINITY, base + i0 + lane));
+            got += __popcll(those);
+          }
+        // a piece of fewer elements
+        for (int i = got + lane; i < a.top; i += 64) put(i, 0);
+      }
     } else {
       uint64_t last = ~uint64_t(0);
       for (int r = 0; r < a.top; ++r) {

@@ -136,6 +136,31 @@ def test_equal_values(hk, rows, vocab):
     check(hk, x, t, 20, grads=False)
 
 
+@pytest.mark.parametrize("rows,vocab,top", [(3000, 20000, 64), (2000, 1500, 64), (400, 50257, 50), (30, 200000, 64)])
+def test_many_rows_and_alternatives(hk, rows, vocab, top):
+    # in some of so many rows the first bound lets many more pass than are asked for
+    say(rows, vocab, top)
+    x, t = make(rows, vocab, F16 if vocab == 1500 else BF, seed=top)
+    check(hk, x, t, top, grads=False)
+
+
+@pytest.mark.parametrize("rows,vocab", [(5, 60000), (600, 1500), (300, 30000)])
+@pytest.mark.parametrize("allowed", [0, 1, 3, 19, 20, 200])
+def test_few_words_allowed(hk, rows, vocab, allowed):
+    say(rows, vocab, allowed)
+    x, t = make(rows, vocab, BF)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    keep = torch.randperm(vocab, generator=g, device=DEV)[:allowed]
+    y = torch.full_like(x, -math.inf)
+    y[:, keep] = x[:, keep]
+    if allowed == 0:
+        p = hk.token_logprobs(y, t, top=20)
+        assert torch.equal(p.top_index, torch.arange(20, device=DEV).expand(rows, 20))
+        return
+    t = keep[torch.arange(rows, device=DEV) % allowed]
+    check(hk, y, t, 20)
+
+
 def test_entropy_left_out(hk):
     x, t = make(5, 3001, BF)
     p = check(hk, x, t, 3, entropy=False)
