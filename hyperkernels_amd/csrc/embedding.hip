@@ -5,10 +5,10 @@
 // few words very often, so rows are neither added atomically nor owned by one workgroup each:
 //   embedding_sort     a workgroup per range of table rows reads all tokens (from L2), counts those below its range, which
 //                      is where its part of the sorted order begins, and places its own by row, in the tokens' order.
-//                      Workgroups behind these clear the table meanwhile: the sort is latency, the clearing bandwidth.
 //   embedding_sum      the sorted order in equal chunks, a wave each and 64 units of columns: rows that lie inside a chunk
 //                      are written, the parts of those that go on across its ends are left as partial sums,
 //   embedding_combine  which are added in order where such a row begins.
+// All three are latency, and clearing the table is bandwidth: each launch clears a part of it beside its own work.
 // Few tokens take one launch: each workgroup finds its rows' tokens and sums them itself.
 #include <algorithm>
 #include <initializer_list>
@@ -102,13 +102,17 @@ struct Grad {
   int d;
   float scale;
   int accumulate;
-  int range;        // table rows a workgroup (sort, few)
+  int range;        // table rows a workgroup that sorts
   int ranges;       // workgroups that sort
-  int clear;        // table rows that each of the others clears
+  int sums;         // workgroups that sum, and that combine
+  int clear;        // table rows that each of the workgroups behind these clears:
+  int64_t clear_sum, clear_sort;  // combine from row 0, sum from clear_sum, sort from clear_sort
+  int few_bits;     // few: workgroup b has rows b, b + 2^few_bits, ..
   int table_elem;   // bytes
   int chunk;        // positions a chunk
   int col_blocks;   // waves a chunk
   uint2* sorted;    // (token's place, its table row) in order of the rows; row ~0 behind the last
+  uint64_t* used;   // a bit for each table row: some token is it
   float* part;      // [chunk][2][d]: of the row that goes on from before, of the one that goes on behind
 };
 
@@ -126,6 +130,15 @@ __device__ __forceinline__ void zero_row(const Grad& a, int64_t row, int lane, i
   }
 }
 
+// Zeros a workgroup's part of the rows from `first` to `end`; without those that have tokens if their bits are known.
+__device__ __forceinline__ void clear_rows(const Grad& a, int block, int64_t first, int64_t end, bool known) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  first += static_cast<int64_t>(block) * a.clear;
+  end = min(end, first + a.clear);
+  for (int64_t r = first + wave; r < end; r += waves)
+    if (!known || !(a.used[r >> 6] >> (r & 63) & 1)) zero_row(a, r, threadIdx.x & 63, 64);
+}
+
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
 constexpr int kRounds = 8;                             // tokens a lane and tile
 constexpr int kTileTokens = kSortThreads * kRounds;    // 4096
@@ -138,8 +151,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   __shared__ int sums[kSortWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   if (static_cast<int>(blockIdx.x) >= a.ranges) {
-    const int64_t first = static_cast<int64_t>(blockIdx.x - a.ranges) * a.clear;
-    for (int r = wave; r < a.clear && first + r < a.vocab; r += kSortWaves) zero_row(a, first + r, lane, 64);
+    clear_rows(a, blockIdx.x - a.ranges, a.clear_sort, a.vocab, false);
     return;
   }
   const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
@@ -168,6 +180,11 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   below = 0;
 #pragma unroll
   for (int w = 0; w < kSortWaves; ++w) below += sums[w];
+  if (!a.accumulate)
+    for (int r = wave * 64; r < rows; r += kSortThreads) {
+      const uint64_t some = __ballot(r + lane < rows && count[min(r + lane, rows - 1)] > 0);
+      if (lane == 0) a.used[(lo + r) >> 6] = some;
+    }
   __syncthreads();
 
   // count[r]: the first place of row r in the sorted order
@@ -310,6 +327,10 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
 
 template <class FG, class FT, int E>
 __global__ __launch_bounds__(256) void embedding_sum(Grad a) {
+  if (static_cast<int>(blockIdx.x) >= a.sums) {
+    clear_rows(a, blockIdx.x - a.sums, a.clear_sum, a.clear_sort, true);
+    return;
+  }
   const Place w(a, E);
   if (w.from >= a.n) return;
   const int lane = threadIdx.x & 63;
@@ -363,6 +384,10 @@ __global__ __launch_bounds__(256) void embedding_sum(Grad a) {
 // The row that begins in a chunk and goes on behind it: its part of this chunk, and of the chunks that it goes on into.
 template <class FT, int E>
 __global__ __launch_bounds__(256) void embedding_combine(Grad a) {
+  if (static_cast<int>(blockIdx.x) >= a.sums) {
+    clear_rows(a, blockIdx.x - a.sums, 0, a.clear_sum, true);
+    return;
+  }
   const Place w(a, E);
   if (w.to >= a.n) return;
   const int lane = threadIdx.x & 63;
@@ -402,26 +427,32 @@ __global__ __launch_bounds__(256) void embedding_combine(Grad a) {
   if (mine) put_row<FT, E>(a, row, w.col, acc);
 }
 
-// Few tokens: a workgroup finds those of its rows and sums them in order.
-constexpr int kFew = 1024;
-template <class FG, class FT, int E>
+// Few tokens: a workgroup finds those of its rows and sums them in order, a wave a row. Frequent words lie side by side in
+// most vocabularies, so a workgroup has rows far apart; and a row of more than kLong tokens, a chain of loads, is summed by
+// all four waves, each every fourth window of the list, and their parts in order.
+constexpr int kFew = 2048, kFewer = 1024;  // tokens: of the two variants, by what a lane holds
+constexpr int kLong = 32;
+template <class FG, class FT, int E, int U>
 __global__ __launch_bounds__(256) void embedding_few(Grad a) {
-  __shared__ uint2 list[kFew];
+  __shared__ uint2 list[U * 256];
+  __shared__ float parts[3][E][64];
   __shared__ int sums[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
-  const int rows = static_cast<int>(min(static_cast<uint64_t>(a.range), static_cast<uint64_t>(a.vocab) - lo));
-  constexpr int kTokens = kFew / 4, kU = kTokens / 64;  // a wave, a lane
-  uint64_t row[kU], mask[kU];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const uint32_t stride = 1u << a.few_bits;
+  const int64_t rows = (a.vocab - blockIdx.x + stride - 1) >> a.few_bits;
+  uint32_t row[U];
+  uint64_t mask[U];
   int found = 0;
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const int at = wave * kTokens + 64 * u + lane;
-    row[u] = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) - lo : ~uint64_t(0);
+  for (int u = 0; u < U; ++u) {
+    const int at = (wave * U + u) * 64 + lane;
+    const uint64_t t = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) : ~uint64_t(0);
+    const bool here = t < static_cast<uint64_t>(a.vocab) && (t & (stride - 1)) == blockIdx.x;
+    row[u] = here ? static_cast<uint32_t>(t >> a.few_bits) : ~0u;
   }
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    mask[u] = __ballot(row[u] < static_cast<uint64_t>(rows));
+  for (int u = 0; u < U; ++u) {
+    mask[u] = __ballot(row[u] != ~0u);
     found += __popcll(mask[u]);
   }
   if (lane == 0) sums[wave] = found;
@@ -433,46 +464,75 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
     total += sums[w];
   }
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    if (row[u] < static_cast<uint64_t>(rows))
-      list[at + __popcll(mask[u] & ((uint64_t(1) << lane) - 1))] =
-          make_uint2(wave * kTokens + 64 * u + lane, static_cast<uint32_t>(row[u]));
+  for (int u = 0; u < U; ++u) {
+    if (row[u] != ~0u)
+      list[at + __popcll(mask[u] & ((uint64_t(1) << lane) - 1))] = make_uint2((wave * U + u) * 64 + lane, row[u]);
     at += __popcll(mask[u]);
   }
   __syncthreads();
   if (a.accumulate && total == 0) return;  // none of these rows
-  for (int r = wave; r < rows; r += 4) {
-    bool any = false;
-    for (int i = 0; i < total; i += 64) any |= __any(i + lane < total && list[min(i + lane, total - 1)].y == r);
-    if (!any) {
-      if (!a.accumulate && blockIdx.y == 0) zero_row(a, static_cast<int64_t>(lo) + r, lane, 64);
-      continue;
+  auto tokens_in = [&](int i, uint32_t r) { return __ballot(i + lane < total && list[min(i + lane, total - 1)].y == r); };
+  auto tokens_of = [&](uint32_t r) {
+    int c = 0;
+    for (int i = 0; i < total; i += 64) c += __popcll(tokens_in(i, r));
+    return c;
+  };
+  // the sum of the row's tokens in every `step`-th window of the list
+  auto sum = [&](uint32_t r, int first, int step, int col, bool mine, float* acc) {
+    for (int i = first * 64; i < total; i += step * 64) {
+      uint64_t of = tokens_in(i, r);
+      while (of) {
+        float x[kAhead][E];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+          if (of) {
+            const int k = __ffsll(static_cast<unsigned long long>(of)) - 1;
+            of &= of - 1;
+            if (mine) load<FG, E>(a.grad, static_cast<int64_t>(list[i + k].x) * a.grad_stride + col, x[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += x[u][e];
+      }
     }
+  };
+  for (int64_t r = wave; r < rows; r += 4) {
+    const int64_t to = (r << a.few_bits) + blockIdx.x;
+    const int of = tokens_of(static_cast<uint32_t>(r));
+    if (of == 0) {
+      if (!a.accumulate && r % gridDim.y == blockIdx.y) zero_row(a, to, lane, 64);
+    } else if (of <= kLong) {
+      for (int c0 = blockIdx.y; c0 < a.col_blocks; c0 += gridDim.y) {
+        const int col = (c0 * 64 + lane) * E;
+        float acc[E] = {};
+        sum(static_cast<uint32_t>(r), 0, 1, col, col < a.d, acc);
+        if (col < a.d) put_row<FT, E>(a, static_cast<uint32_t>(to), col, acc);
+      }
+    }
+  }
+  if (total <= kLong) return;
+  for (int64_t r = 0; r < rows; ++r) {
+    if (tokens_of(static_cast<uint32_t>(r)) <= kLong) continue;
     for (int c0 = blockIdx.y; c0 < a.col_blocks; c0 += gridDim.y) {
       const int col = (c0 * 64 + lane) * E;
-      const bool mine = col < a.d;
       float acc[E] = {};
-      for (int i = 0; i < total; i += 64) {
-        uint64_t of = __ballot(i + lane < total && list[min(i + lane, total - 1)].y == r);
-        while (of) {
-          float x[kAhead][E];
+      sum(static_cast<uint32_t>(r), wave, 4, col, col < a.d, acc);
+      if (wave > 0)
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
+        for (int e = 0; e < E; ++e) parts[wave - 1][e][lane] = acc[e];
+      __syncthreads();
+      if (wave == 0 && col < a.d) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[u][e] = 0.f;
-            if (of) {
-              const int k = __ffsll(static_cast<unsigned long long>(of)) - 1;
-              of &= of - 1;
-              if (mine) load<FG, E>(a.grad, static_cast<int64_t>(list[i + k].x) * a.grad_stride + col, x[u]);
-            }
-          }
+        for (int w = 0; w < 3; ++w)
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += x[u][e];
-        }
+          for (int e = 0; e < E; ++e) acc[e] += parts[w][e][lane];
+        put_row<FT, E>(a, static_cast<uint32_t>((r << a.few_bits) + blockIdx.x), col, acc);
       }
-      if (mine) put_row<FT, E>(a, static_cast<uint32_t>(lo) + r, col, acc);
+      __syncthreads();
     }
   }
 }
@@ -528,41 +588,55 @@ int chunk_of(int64_t n) {
   return c;
 }
 int64_t chunks_of(int64_t n) { return ceil_div(n, chunk_of(n)); }
-int64_t gradient_workspace(int64_t n, int64_t d) {
-  return n <= kFew ? 0 : ceil_div(8 * n, 16) * 16 + chunks_of(n) * 2 * d * 4;
+// One launch: up to 1024 tokens, and up to 2048 over a table that this launch clears as fast as the three (one launch and
+// three: 333 tokens over 1009 x 131 8 and 26 us, 1000 over 50257 x 768 38 and 34, 2048 over 1000 x 64 12 and 28, over 5000
+// x 256 18 and 19, over 50257 x 768 41 and 34, over 131072 x 512 69 and 54).
+bool few(int64_t n, int64_t vocab) { return n <= kFewer || (n <= kFew && vocab <= 32768); }
+struct Workspace {
+  int64_t used, part, bytes;
+};
+Workspace gradient_workspace(int64_t n, int64_t vocab, int64_t d) {
+  if (few(n, vocab)) return {0, 0, 0};
+  const int64_t used = ceil_div(8 * n, 16) * 16, part = used + ceil_div(vocab, 128) * 16;
+  return {used, part, part + chunks_of(n) * 2 * d * 4};
 }
 
 template <class FG, class FT, int E>
 hipError_t gradient(Grad a, hipStream_t stream) {
-  if (a.n <= kFew) {
-    // A wave a row, and workgroups for all CUs; a frequent row is a chain of loads, so its columns go to several (333
-    // tokens, 1009 x 131: 11.7 -> 6.4 us).
-    a.range = static_cast<int>(std::max<int64_t>(4, ceil_div(a.vocab, 2048)));
-    a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
-    hipLaunchKernelGGL((embedding_few<FG, FT, E>),
-                       dim3(static_cast<unsigned>(ceil_div(a.vocab, a.range)), std::min(a.col_blocks, 16)), dim3(256),
-                       0, stream, a);
+  a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
+  if (few(a.n, a.vocab)) {
+    // A wave a row, and workgroups for all CUs; the columns of a frequent row go to several (333 tokens, 1009 x 131: 11.7
+    // -> 6.4 us).
+    int64_t blocks = 1;
+    while (blocks < 2048 && blocks * 4 < a.vocab) blocks *= 2, ++a.few_bits;
+    const dim3 grid(static_cast<unsigned>(std::min(blocks, a.vocab)), std::min(a.col_blocks, 16));
+    if (a.n <= kFewer)
+      hipLaunchKernelGGL((embedding_few<FG, FT, E, kFewer / 256>), grid, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((embedding_few<FG, FT, E, kFew / 256>), grid, dim3(256), 0, stream, a);
     return launch_status();
   }
   // as many ranges as half of the workgroups that the card holds at once
   a.range = 64;
   while (a.range < kMaxRange && ceil_div(a.vocab, a.range) > device_cu_count()) a.range *= 2;
   a.ranges = static_cast<int>(ceil_div(a.vocab, a.range));
-  int64_t blocks = a.ranges;
-  if (!a.accumulate) {
-    // 64 KiB a workgroup, and not more workgroups than a launch takes
-    a.clear = static_cast<int>(std::max<int64_t>({kSortWaves, 65536 / (int64_t(a.d) * a.table_elem), a.vocab >> 20}));
-    blocks += ceil_div(a.vocab, a.clear);
-  }
-  hipLaunchKernelGGL(embedding_sort, dim3(static_cast<unsigned>(blocks)), dim3(kSortThreads), 0, stream, a);
-  HK_RETURN_IF_ERROR(launch_status());
   a.chunk = chunk_of(a.n);
-  a.col_blocks = static_cast<int>(ceil_div(a.d, 64 * E));
-  const int64_t waves = chunks_of(a.n) * a.col_blocks;
-  const dim3 grid(static_cast<unsigned>(ceil_div(waves, 4)));
-  hipLaunchKernelGGL((embedding_sum<FG, FT, E>), grid, dim3(256), 0, stream, a);
+  a.sums = static_cast<int>(ceil_div(chunks_of(a.n) * a.col_blocks, 4));
+  int64_t sort = a.ranges, sum = a.sums, combine = a.sums;
+  if (!a.accumulate) {
+    // 64 KiB a workgroup, and not more workgroups than a launch takes; the three launches' parts by how long they are
+    // without it (8192 tokens, 50257 x 768: all in the first CLEARALL, so CLEARSPLIT us)
+    a.clear = static_cast<int>(std::max<int64_t>({kSortWaves, 65536 / (int64_t(a.d) * a.table_elem), a.vocab >> 20}));
+    a.clear_sum = a.vocab * 3 / 10, a.clear_sort = a.vocab * 6 / 10;
+    combine += ceil_div(a.clear_sum, a.clear);
+    sum += ceil_div(a.clear_sort - a.clear_sum, a.clear);
+    sort += ceil_div(a.vocab - a.clear_sort, a.clear);
+  }
+  hipLaunchKernelGGL(embedding_sort, dim3(static_cast<unsigned>(sort)), dim3(kSortThreads), 0, stream, a);
   HK_RETURN_IF_ERROR(launch_status());
-  hipLaunchKernelGGL((embedding_combine<FT, E>), grid, dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((embedding_sum<FG, FT, E>), dim3(static_cast<unsigned>(sum)), dim3(256), 0, stream, a);
+  HK_RETURN_IF_ERROR(launch_status());
+  hipLaunchKernelGGL((embedding_combine<FT, E>), dim3(static_cast<unsigned>(combine)), dim3(256), 0, stream, a);
   return launch_status();
 }
 template <class FG, class FT>
@@ -614,7 +688,7 @@ extern "C" hipError_t hk_embedding_forward(const void* table, int type, int64_t 
 }
 
 extern "C" int64_t hk_embedding_workspace(int64_t n, int64_t vocab, int64_t d) {
-  return hk::gradient_ok(n, vocab, d) ? hk::gradient_workspace(n, d) : -1;
+  return hk::gradient_ok(n, vocab, d) ? hk::gradient_workspace(n, vocab, d).bytes : -1;
 }
 
 extern "C" hipError_t hk_embedding_backward(const void* grad, int type, int64_t n, int64_t d, int64_t grad_stride,
@@ -631,7 +705,8 @@ extern "C" hipError_t hk_embedding_backward(const void* grad, int type, int64_t 
   const Rows o = Rows(grad_table, et, d).along(vocab, et * table_stride);
   HK_CHECK_ARG(!overlaps_itself(o) && !overlap(o, Rows(grad, eg, d).along(n, eg * grad_stride)) &&
                !overlap(o, Rows(tokens, ei, n)));
-  const int64_t need = gradient_workspace(n, d);
+  const Workspace layout = gradient_workspace(n, vocab, d);
+  const int64_t need = layout.bytes;
   if (need > 0) {
     if (workspace) {
       HK_CHECK_ARG(workspace_bytes >= need && aligned16(workspace));
@@ -646,7 +721,8 @@ extern "C" hipError_t hk_embedding_backward(const void* grad, int type, int64_t 
   a.n = n, a.vocab = vocab, a.grad_stride = grad_stride, a.table_stride = table_stride, a.d = static_cast<int>(d);
   a.scale = scale, a.accumulate = accumulate, a.table_elem = static_cast<int>(et);
   a.sorted = static_cast<uint2*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ceil_div(8 * n, 16) * 16);
+  a.used = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + layout.used);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + layout.part);
   const int e = unit(d, 4, {{grad, grad_stride, eg, n}, {grad_table, table_stride, et, vocab}});
   return type == HK_TYPE_F32    ? gradient_to<F32>(a, e, table_type, stream)
          : type == HK_TYPE_BF16 ? gradient_to<BF16>(a, e, table_type, stream)

@@ -62,7 +62,8 @@ def test_lookup(hk, n, vocab, d, pad, tt, ot):
 @pytest.mark.parametrize("n,vocab,d,pad", [(0, 10, 8, 0), (1, 3, 1, 0), (7, 1009, 131, 0), (512, 300, 64, 0),
                                            (513, 300, 64, 1), (2048, 50, 36, 2), (5000, 5003, 200, 0),
                                            (9000, 1, 16, 0), (20000, 70001, 24, 0), (1024, 700, 52, 0),
-                                           (1025, 701, 52, 0)])
+                                           (1025, 701, 52, 0), (2048, 3, 300, 0), (2048, 9001, 131, 1), (2048, 40000, 36, 0),
+                                           (1500, 2049, 1100, 0), (2049, 2048, 64, 0), (6000, 65, 7, 1)])
 def test_gradient(hk, n, vocab, d, pad, kind, gt, tt):
     say(n, vocab, d, pad, kind, gt, tt)
     grad = torch.randn(n, d + pad, device=DEV).to(gt)[:, :d]

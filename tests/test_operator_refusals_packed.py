@@ -180,7 +180,7 @@ def test_embedding_refuses(L):
 
 
 def test_embedding_backward_refuses(L):
-    good = dict(grad=16 * M, type=BF16, n=2000, d=64, gs=64, tokens=32 * M, wide=1, table=64 * M, tt=F32, vocab=1000,
+    good = dict(grad=16 * M, type=BF16, n=3000, d=64, gs=64, tokens=32 * M, wide=1, table=64 * M, tt=F32, vocab=1000,
                 ts=64, acc=0, ws=128 * M, bytes=1 << 30)
 
     def go(**c):
@@ -196,7 +196,8 @@ def test_embedding_backward_refuses(L):
     assert go(n=0, acc=1, table=0) == 0
     ws = L.hk_embedding_workspace
     assert ws(-1, 10, 4) == -1 and ws(10, 0, 4) == -1 and ws(10, 10, 0) == -1
-    assert ws(1024, 1000, 64) == 0 and ws(1025, 1000, 64) >= 8 * 1025
+    assert ws(1024, 1000, 64) == 0 and ws(2048, 1000, 64) == 0 and ws(2049, 1000, 64) >= 8 * 2049 + 128
+    assert ws(2048, 32769, 64) > 0
 
 
 # ---- the torch front end ---------------------------------------------------------------------------------
