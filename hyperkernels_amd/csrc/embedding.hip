@@ -3,8 +3,9 @@
 //
 // Both are bound by memory. The gradient has to be the same whatever the order in which workgroups run, and texts repeat a
 // few words very often, so rows are neither added atomically nor owned by one workgroup each:
-//   embedding_sort     a workgroup per range of table rows reads all tokens (from L2), counts those below its range, which
-//                      is where its part of the sorted order begins, and places its own by row, in the tokens' order.
+//   embedding_sort     workgroup b of 2^bits has the table rows b, b + 2^bits, .. (frequent words lie side by side in most
+//                      vocabularies). It reads all tokens (from L2), counts those of the workgroups before it, which is
+//                      where its part of the order begins, and places its own by row, in the tokens' order.
 //   embedding_sum      the sorted order in equal chunks, a wave each and 64 units of columns: rows that lie inside a chunk
 //                      are written, the parts of those that go on across its ends are left as partial sums,
 //   embedding_combine  which are added in order where such a row begins.
@@ -102,17 +103,17 @@ struct Grad {
   int d;
   float scale;
   int accumulate;
-  int range;        // table rows a workgroup that sorts
+  int bits;         // workgroup b that sorts (or of `few`) has rows b, b + 2^bits, ..
+  int range;        // their bits in `used`
   int ranges;       // workgroups that sort
   int sums;         // workgroups that sum, and that combine
   int clear;        // table rows that each of the workgroups behind these clears:
   int64_t clear_sum, clear_sort;  // combine from row 0, sum from clear_sum, sort from clear_sort
-  int few_bits;     // few: workgroup b has rows b, b + 2^few_bits, ..
   int table_elem;   // bytes
   int chunk;        // positions a chunk
   int col_blocks;   // waves a chunk
-  uint2* sorted;    // (token's place, its table row) in order of the rows; row ~0 behind the last
-  uint64_t* used;   // a bit for each table row: some token is it
+  uint2* sorted;    // (token's place, its table row), the places of a row side by side; row ~0 behind the last
+  uint64_t* used;   // a bit for each table row, `range` a workgroup: some token is it
   float* part;      // [chunk][2][d]: of the row that goes on from before, of the one that goes on behind
 };
 
@@ -135,8 +136,10 @@ __device__ __forceinline__ void clear_rows(const Grad& a, int block, int64_t fir
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   first += static_cast<int64_t>(block) * a.clear;
   end = min(end, first + a.clear);
-  for (int64_t r = first + wave; r < end; r += waves)
-    if (!known || !(a.used[r >> 6] >> (r & 63) & 1)) zero_row(a, r, threadIdx.x & 63, 64);
+  for (int64_t r = first + wave; r < end; r += waves) {
+    const int64_t bit = (r & ((int64_t(1) << a.bits) - 1)) * a.range + (r >> a.bits);
+    if (!known || !(a.used[bit >> 6] >> (bit & 63) & 1)) zero_row(a, r, threadIdx.x & 63, 64);
+  }
 }
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
@@ -154,8 +157,12 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
     clear_rows(a, blockIdx.x - a.ranges, a.clear_sort, a.vocab, false);
     return;
   }
-  const uint64_t lo = static_cast<uint64_t>(blockIdx.x) * a.range;
-  const int rows = static_cast<int>(min(static_cast<uint64_t>(a.range), static_cast<uint64_t>(a.vocab) - lo));
+  const uint32_t mask_of = (1u << a.bits) - 1, me = blockIdx.x;
+  const int rows = static_cast<int>((a.vocab - me + mask_of) >> a.bits);
+  // the row of one of this workgroup's tokens, ~0 for others
+  auto row_of = [&](uint64_t t) {
+    return t < static_cast<uint64_t>(a.vocab) && (t & mask_of) == me ? static_cast<uint32_t>(t >> a.bits) : ~0u;
+  };
 
   for (int i = tid; i < rows; i += kSortThreads) count[i] = 0;
   __syncthreads();
@@ -169,8 +176,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      below += t[u] < lo;
-      if (t[u] - lo < static_cast<uint64_t>(rows)) atomicAdd(&count[static_cast<int>(t[u] - lo)], 1);
+      below += t[u] < static_cast<uint64_t>(a.vocab) && (t[u] & mask_of) < me;
+      const uint32_t r = row_of(t[u]);
+      if (r != ~0u) atomicAdd(&count[r], 1);
     }
   }
 #pragma unroll
@@ -183,7 +191,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   if (!a.accumulate)
     for (int r = wave * 64; r < rows; r += kSortThreads) {
       const uint64_t some = __ballot(r + lane < rows && count[min(r + lane, rows - 1)] > 0);
-      if (lane == 0) a.used[(lo + r) >> 6] = some;
+      if (lane == 0) a.used[(static_cast<int64_t>(me) * a.range + r) >> 6] = some;
     }
   __syncthreads();
 
@@ -216,7 +224,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
     // the last workgroup knows where the valid tokens end
     int total = below;
     for (int w = 0; w < kSortWaves; ++w) total += sums[w];
-    if (lo + rows == static_cast<uint64_t>(a.vocab))
+    if (static_cast<int>(me) == a.ranges - 1)
       for (int64_t i = total + tid; i < a.n; i += kSortThreads) a.sorted[i] = make_uint2(0, ~0u);
     if (total == below) return;  // none of these rows
   }
@@ -225,17 +233,18 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
   while ((1 << bits) < rows) ++bits;
   for (int64_t base = 0; base < a.n; base += kTileTokens) {
     // this range's tokens of the tile in order: each wave looks through 64 x kRounds of them
-    uint64_t row[kRounds], mask[kRounds];
+    uint32_t row[kRounds];
+    uint64_t mask[kRounds];
     int found = 0;
     const int64_t w0 = base + wave * (64 * kRounds) + lane;
 #pragma unroll
     for (int u = 0; u < kRounds; ++u) {
       const int64_t at = w0 + 64 * u;
-      row[u] = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) - lo : ~uint64_t(0);
+      row[u] = at < a.n ? row_of(static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at))) : ~0u;
     }
 #pragma unroll
     for (int u = 0; u < kRounds; ++u) {
-      mask[u] = __ballot(row[u] < static_cast<uint64_t>(rows));
+      mask[u] = __ballot(row[u] != ~0u);
       found += __popcll(mask[u]);
     }
     __syncthreads();  // the tile before is done with list and sums
@@ -252,8 +261,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
 #pragma unroll
     for (int u = 0; u < kRounds; ++u) {
       const int before = __popcll(mask[u] & ((uint64_t(1) << lane) - 1));
-      if (row[u] < static_cast<uint64_t>(rows))
-        list[at + before] = make_uint2(static_cast<uint32_t>(w0 + 64 * u), static_cast<uint32_t>(row[u]));
+      if (row[u] != ~0u) list[at + before] = make_uint2(static_cast<uint32_t>(w0 + 64 * u), row[u]);
       at += __popcll(mask[u]);
     }
     __syncthreads();
@@ -287,7 +295,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort(Grad a) {
       int place = 0;
       if (some) place = wave_at[wave][e.y] + before;
       if (some && (same >> lane) == 1) wave_at[wave][e.y] = place + 1;  // the last of them
-      if (some) a.sorted[place] = make_uint2(e.x, static_cast<uint32_t>(lo) + e.y);
+      if (some) a.sorted[place] = make_uint2(e.x, (e.y << a.bits) + me);
     }
   }
 }
@@ -438,8 +446,8 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
   __shared__ float parts[3][E][64];
   __shared__ int sums[4];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const uint32_t stride = 1u << a.few_bits;
-  const int64_t rows = (a.vocab - blockIdx.x + stride - 1) >> a.few_bits;
+  const uint32_t stride = 1u << a.bits;
+  const int64_t rows = (a.vocab - blockIdx.x + stride - 1) >> a.bits;
   uint32_t row[U];
   uint64_t mask[U];
   int found = 0;
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
     const int at = (wave * U + u) * 64 + lane;
     const uint64_t t = at < a.n ? static_cast<uint64_t>(token_of(a.tokens, a.wide_tokens, at)) : ~uint64_t(0);
     const bool here = t < static_cast<uint64_t>(a.vocab) && (t & (stride - 1)) == blockIdx.x;
-    row[u] = here ? static_cast<uint32_t>(t >> a.few_bits) : ~0u;
+    row[u] = here ? static_cast<uint32_t>(t >> a.bits) : ~0u;
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -501,7 +509,7 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
     }
   };
   for (int64_t r = wave; r < rows; r += 4) {
-    const int64_t to = (r << a.few_bits) + blockIdx.x;
+    const int64_t to = (r << a.bits) + blockIdx.x;
     const int of = tokens_of(static_cast<uint32_t>(r));
     if (of == 0) {
       if (!a.accumulate && r % gridDim.y == blockIdx.y) zero_row(a, to, lane, 64);
@@ -530,7 +538,7 @@ __global__ __launch_bounds__(256) void embedding_few(Grad a) {
         for (int w = 0; w < 3; ++w)
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[e] += parts[w][e][lane];
-        put_row<FT, E>(a, static_cast<uint32_t>((r << a.few_bits) + blockIdx.x), col, acc);
+        put_row<FT, E>(a, static_cast<uint32_t>((r << a.bits) + blockIdx.x), col, acc);
       }
       __syncthreads();
     }
@@ -592,12 +600,19 @@ int64_t chunks_of(int64_t n) { return ceil_div(n, chunk_of(n)); }
 // three: 333 tokens over 1009 x 131 8 and 26 us, 1000 over 50257 x 768 38 and 34, 2048 over 1000 x 64 12 and 28, over 5000
 // x 256 18 and 19, over 50257 x 768 41 and 34, over 131072 x 512 69 and 54).
 bool few(int64_t n, int64_t vocab) { return n <= kFewer || (n <= kFew && vocab <= 32768); }
+// Half of the workgroups that the card holds at once, of 16 to 1024 rows.
+int sort_bits(int64_t vocab) {
+  int bits = 0;
+  while ((bits < 8 && (vocab >> bits) > 16) || ceil_div(vocab, int64_t(1) << bits) > kMaxRange) ++bits;
+  return bits;
+}
+int used_bits(int64_t vocab) { return static_cast<int>(ceil_div(ceil_div(vocab, int64_t(1) << sort_bits(vocab)), 64) * 64); }
 struct Workspace {
   int64_t used, part, bytes;
 };
 Workspace gradient_workspace(int64_t n, int64_t vocab, int64_t d) {
   if (few(n, vocab)) return {0, 0, 0};
-  const int64_t used = ceil_div(8 * n, 16) * 16, part = used + ceil_div(vocab, 128) * 16;
+  const int64_t used = ceil_div(8 * n, 16) * 16, part = used + ceil_div(int64_t(used_bits(vocab) / 8) << sort_bits(vocab), 16) * 16;
   return {used, part, part + chunks_of(n) * 2 * d * 4};
 }
 
@@ -608,7 +623,7 @@ hipError_t gradient(Grad a, hipStream_t stream) {
     // A wave a row, and workgroups for all CUs; the columns of a frequent row go to several (333 tokens, 1009 x 131: 11.7
     // -> 6.4 us).
     int64_t blocks = 1;
-    while (blocks < 2048 && blocks * 4 < a.vocab) blocks *= 2, ++a.few_bits;
+    while (blocks < 2048 && blocks * 4 < a.vocab) blocks *= 2, ++a.bits;
     const dim3 grid(static_cast<unsigned>(std::min(blocks, a.vocab)), std::min(a.col_blocks, 16));
     if (a.n <= kFewer)
       hipLaunchKernelGGL((embedding_few<FG, FT, E, kFewer / 256>), grid, dim3(256), 0, stream, a);
@@ -616,16 +631,15 @@ hipError_t gradient(Grad a, hipStream_t stream) {
       hipLaunchKernelGGL((embedding_few<FG, FT, E, kFew / 256>), grid, dim3(256), 0, stream, a);
     return launch_status();
   }
-  // as many ranges as half of the workgroups that the card holds at once
-  a.range = 64;
-  while (a.range < kMaxRange && ceil_div(a.vocab, a.range) > device_cu_count()) a.range *= 2;
-  a.ranges = static_cast<int>(ceil_div(a.vocab, a.range));
+  a.bits = sort_bits(a.vocab);
+  a.ranges = static_cast<int>(std::min(int64_t(1) << a.bits, a.vocab));
+  a.range = used_bits(a.vocab);
   a.chunk = chunk_of(a.n);
   a.sums = static_cast<int>(ceil_div(chunks_of(a.n) * a.col_blocks, 4));
   int64_t sort = a.ranges, sum = a.sums, combine = a.sums;
   if (!a.accumulate) {
     // 64 KiB a workgroup, and not more workgroups than a launch takes; the three launches' parts by how long they are
-    // without it (8192 tokens, 50257 x 768: all in the first CLEARALL, so CLEARSPLIT us)
+    // without it (8192 tokens, 50257 x 768: all in the first 46.5, so 43.3 us)
     a.clear = static_cast<int>(std::max<int64_t>({kSortWaves, 65536 / (int64_t(a.d) * a.table_elem), a.vocab >> 20}));
     a.clear_sum = a.vocab * 3 / 10, a.clear_sort = a.vocab * 6 / 10;
     combine += ceil_div(a.clear_sum, a.clear);
