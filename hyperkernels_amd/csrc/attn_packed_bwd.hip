@@ -11,6 +11,10 @@
 // dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
 // times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
 // where dK is moved to the next when it grows.
+//
+// Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 31, dk and dv 43 us; sequences of 2048, 1001 and
+// 333, 16 heads on 4 of 128, fp16: 53, and 85 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
+// need them) at two to three waves a SIMD; one kernel for both that hands ds over took as long (7.6 for delta, then 84).
 #include "attn_packed.h"
 
 namespace hk {

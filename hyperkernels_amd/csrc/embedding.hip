@@ -11,6 +11,10 @@
 //   embedding_combine  which are added in order where such a row begins.
 // All three are latency, and clearing the table is bandwidth: each launch clears a part of it beside its own work.
 // Few tokens take one launch: each workgroup finds its rows' tokens and sums them itself.
+//
+// Measured: 8192 rows of 768 of an fp32 table, added to bf16 rows, 7.8 us; their table's gradient (50257 rows, 154 MB
+// written) 43 us (17 + 15 + 11 as profiled), 6.1 TB/s of it 26: the three are chains of dependent loads; 333 tokens over
+// 1009 x 131 6.0 us, launch and loads.
 #include <algorithm>
 #include <initializer_list>
 

@@ -16,6 +16,10 @@
 // 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, 128 lanes at a time, where all lanes
 // look them through and collect (value, index) keys, which are ranked by counting the larger ones. Where more pass
 // than that list takes (equal values), `top` passes over the row find the next largest.
+//
+// Measured, rows of 50257: 4096 of bf16 with 5 alternatives 76 us (5.4 TB/s, where the bound is the memory); 8192 of bf16
+// without 143 (5.8), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
+// latency: load, maximum, sums, selection one after the other.
 #include <limits.h>
 
 #include "hk_device.h"
