@@ -7,7 +7,10 @@
 // dP^T = V dO^T with a row a lane, dS^T the operand of dQ^T += K^T dS^T as it lies) and leaves delta and lse for
 // attn_packed_dkv, which goes by keys: S = Q K^T and dP = dO V^T with a key a lane, P and dS the operands of
 // dV^T += dO^T P and dK^T += Q^T dS as they lie. The rows of a group's heads are one loop there, which sums them.
-// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. dS is as small as P and
+// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. That makes the norm of the
+// gradients' error sqrt(2) of what rounding them leaves. delta from the o that was rounded adds p (dout . o's error) to
+// dS, 2 / (n - 1) of that rounding's square over n equal keys: rows of few keys, where it would be most of the error,
+// take delta = sum p dp instead, from one more pass over their one or two tiles of keys. dS is as small as P and
 // dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
 // times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
 // where dK is moved to the next when it grows.
@@ -27,6 +30,7 @@ struct DqShape {
   static constexpr int kRows = 128 / KG;
   static constexpr int kKeys = KG == 4 ? 128 : 64;
   static constexpr int kBlocks = kKeys / KG / 32;
+  static constexpr int kFew = 128 / kKeys;  // tiles of keys up to which delta is formed from p and dp
   static constexpr int kTile = kKeys * D * 2;
   static constexpr int kStage = 2 * kTile;
   static constexpr int kPitch = D + 4;
@@ -66,10 +70,29 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     copy_k(t, q.mk, wave, to);
     copy_v(t, q.mk, wave, to + S::kTile);
   };
+  const bool few = t1 <= S::kFew;
   if (t1 > 0) fetch(0);
+  if (few && t1 > 1) fetch(1);
 
+  const Reads<D> rd(lane);
+  const float sc = a.scale * kLog2e;
+  const f32x16_t zero = zero_block();
   s16x8_t qx[D / 16], gx[D / 16];
   float delta = 0.f, lse2;
+  // scores, with -inf where a key is masked, and dp of the 32 keys from key0 on, at kt and vt in LDS
+  auto products = [&](const char HK_LDS* kt, const char HK_LDS* vt, int key0, f32x16_t& s, f32x16_t& dp) {
+    s = T::mfma(rd.rows(kt, 0, 0), qx[0], zero);
+#pragma unroll
+    for (int i = 1; i < D / 16; ++i) s = T::mfma(rd.rows(kt, 0, i), qx[i], s);
+    dp = T::mfma(rd.rows(vt, 0, 0), gx[0], zero);
+#pragma unroll
+    for (int i = 1; i < D / 16; ++i) dp = T::mfma(rd.rows(vt, 0, i), gx[i], dp);
+    if (key0 + 31 > lim_lo) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (key0 + 8 * (i >> 2) + 4 * h + (i & 3) > lim) s[i] = -INFINITY;
+    }
+  };
   int grow = 0;
   {
     const int64_t at = q.q0 + tok;
@@ -78,15 +101,28 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     const float lse = a.lse[qh * a.lse_stride + at];
     // a row that sees nothing has exponentials of 0
     lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
-    s16x8_t ox[D / 16];
-    load_row<D>(a.o.p + at * a.o.m + qh * a.o.h, h, a.d, ox);
+    if (few) {
+      wait_copies();
+      barrier();
+      for (int key0 = 0; key0 < t1 * S::kKeys && key0 <= lim_hi; key0 += 32) {
+        const char HK_LDS* kt = lds + key0 / S::kKeys * S::kStage + key0 % S::kKeys * (2 * D);
+        f32x16_t s, dp;
+        products(kt, kt + S::kTile, key0, s, dp);
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const u32x4_t x = __builtin_bit_cast(u32x4_t, ox[s]), y = __builtin_bit_cast(u32x4_t, gx[s]);
+        for (int i = 0; i < 16; ++i)
+          delta = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, -lse2)), dp[i], delta);
+      }
+    } else {
+      s16x8_t ox[D / 16];
+      load_row<D>(a.o.p + at * a.o.m + qh * a.o.h, h, a.d, ox);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x2_t u = T::unpack(x[i]), w = T::unpack(y[i]);
-        delta += u[0] * w[0] + u[1] * w[1];
+      for (int s = 0; s < D / 16; ++s) {
+        const u32x4_t x = __builtin_bit_cast(u32x4_t, ox[s]), y = __builtin_bit_cast(u32x4_t, gx[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2_t u = T::unpack(x[i]), w = T::unpack(y[i]);
+          delta += u[0] * w[0] + u[1] * w[1];
+        }
       }
     }
     delta = half32_reduce(delta, AddOp{});
@@ -116,9 +152,6 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
   }
   const float out = T::kNarrow ? ldexpf(a.scale, grow) : a.scale;
 
-  const Reads<D> rd(lane);
-  const float sc = a.scale * kLog2e;
-  const f32x16_t zero = zero_block();
   f32x16_t dq[D / 32];
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) dq[b] = f32x16_t{};
@@ -126,24 +159,15 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
   for (int t = 0; t < t1; ++t) {
     wait_copies();
     barrier();
-    if (t + 1 < t1) fetch(t + 1);
+    if (t + 1 < t1 && !few) fetch(t + 1);
     const int key0 = t * S::kKeys + 32 * S::kBlocks * kg;
     const char HK_LDS* kt = lds + (t & 1) * S::kStage + 32 * S::kBlocks * kg * (2 * D);
     const char HK_LDS* vt = kt + S::kTile;
 #pragma unroll
     for (int n = 0; n < S::kBlocks; ++n) {
       if (key0 + 32 * n > lim_hi) break;
-      f32x16_t s = T::mfma(rd.rows(kt, 32 * n, 0), qx[0], zero);
-#pragma unroll
-      for (int i = 1; i < D / 16; ++i) s = T::mfma(rd.rows(kt, 32 * n, i), qx[i], s);
-      f32x16_t dp = T::mfma(rd.rows(vt, 32 * n, 0), gx[0], zero);
-#pragma unroll
-      for (int i = 1; i < D / 16; ++i) dp = T::mfma(rd.rows(vt, 32 * n, i), gx[i], dp);
-      if (key0 + 32 * n + 31 > lim_lo) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3) > lim) s[i] = -INFINITY;
-      }
+      f32x16_t s, dp;
+      products(kt + 32 * n * (2 * D), vt + 32 * n * (2 * D), key0 + 32 * n, s, dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, -lse2)) * (dp[i] - delta);

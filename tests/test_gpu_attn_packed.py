@@ -338,3 +338,24 @@ def test_gradients_against_differences(hk):
         noise = sum(float((r["o"][1] * do.double()).square().sum()) for r in ref) ** 0.5 * 4
         size = float(grads[i].double().square().sum()) ** 0.5 * float((x1 - x0).square().sum()) ** 0.5
         assert abs(along - change) <= noise + 2.0 ** -6 * size, (i, along, change, noise, size)
+
+
+@pytest.mark.parametrize("t", [BF, F16])
+@pytest.mark.parametrize("H,Hk,d", [(4, 4, 64), (8, 2, 128)])
+@pytest.mark.parametrize("lens", [[24, 117, 390, 5, 64], [1300], [16] * 40])
+def test_gradients_are_off_by_little_more_than_their_rounding(hk, lens, H, Hk, d, t):
+    # In the norm: dq and dk have the rounding of dS beside their own, both of the same relative size at random signs:
+    # sqrt(2) of their own. Where delta is formed from the o that was rounded (twice), over 65 keys and more, that adds
+    # at most 2 / 64 to the 2 under the root. A thirtieth for the chance in both.
+    say(lens, H, Hk, d, t)
+    q, k, v, do = make(lens, lens, H, Hk, d, t)
+    cu = cu_of(lens)
+    o, lse = hk.attn_packed_forward(q, k, v, cu)
+    dq, dk, _ = hk.attn_packed_backward(do, q, k, v, o, lse, cu)
+    ref = reference(q, k, v, lens, lens, True, d ** -0.5, do)
+    for name, got in (("dq", dq), ("dk", dk)):
+        want = ref[name][0]
+        least = float((want.to(t).double() - want).norm())
+        off = float((got.double() - want).norm())
+        print("   ", name, off / least, flush=True)
+        assert off <= (2 + 1 / 32) ** 0.5 * (1 + 1 / 30) * least, (name, off / least)
