@@ -15,7 +15,7 @@
 // elements of the wave, so the least of those over the waves is a bound that `top` elements reach and few others do (some
 // 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, 128 lanes at a time, where all lanes
 // look them through and collect (value, index) keys, which are ranked by counting the larger ones. Where more pass
-// than that list takes (equal values), `top` passes over the row find the next largest.
+// than that list takes even without those equal to the bound, `top` passes over the row find the next largest.
 //
 // Measured, rows of 50257: 4096 of bf16 with 5 alternatives 76 us (5.4 TB/s, where the bound is the memory); 8192 of bf16
 // without 143 (5.8), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
@@ -148,13 +148,12 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
     m = row16_reduce(m, MaxOp{});  // W <= 16, and every lane of the row has one of the values
   }
   const float ref = m == -INFINITY ? 0.f : m;  // nothing above -inf: the sums are 0
-  const float r2 = ref * kLog2e;
   float s = 0.f, u = 0.f;
   // as far as the compiler can see these are new: else it keeps the first pass's fp32 values of 16-bit rows
 #pragma unroll
   for (int v = 0; v < V; ++v) asm("" : "+v"(d[v].x), "+v"(d[v].y), "+v"(d[v].z), "+v"(d[v].w));
   auto add = [&](float e) {
-    const float t = __builtin_fmaf(e, kLog2e, -r2);  // log2 of the term
+    const float t = (e - ref) * kLog2e;  // log2 of the term; as one fma it would overflow at fp32's lowest values
     const float p = __builtin_amdgcn_exp2f(t);
     s += p;
     // -inf has p = 0 and counts for nothing; a NaN is in s
@@ -172,15 +171,15 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
     for (int w = 0; w < W; ++w) s += red[1][w], u += red[2][w];
   }
   u *= kLn2;
-  const float lse = ref + __logf(s);
+  const float log_s = __logf(s), lse = ref + log_s;
   if (tid == 0) {
     if (a.pieces > 1) {
       a.part[item] = make_float4(m, s, u, 0.f);
     } else {
       if (a.lse) a.lse[row] = lse;
-      if (ENT) a.entropy[row] = __logf(s) - u / s;
+      if (ENT) a.entropy[row] = log_s - u / s;
       const int64_t t = token_of(a.tokens, a.wide_tokens, row);
-      a.logp[row] = t >= 0 && t < n ? F::load(x, t) - lse : __uint_as_float(0x7fc00000u);
+      a.logp[row] = t >= 0 && t < n ? F::load(x, t) - ref - log_s : __uint_as_float(0x7fc00000u);
     }
   }
   if constexpr (TOP) {
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
       if (a.pieces > 1) {
         a.keys[item * a.top + rank] = key;
       } else {
-        a.top_logp[row * a.top + rank] = key_value(key) - lse;
+        a.top_logp[row * a.top + rank] = key_value(key) - ref - log_s;
         a.top_index[row * a.top + rank] = key_index(key);
       }
     };
@@ -204,54 +203,64 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
       __syncthreads();
       bound = row16_reduce(red[0][lane & (W - 1)], [](float p, float q) { return fminf(p, q); });
     }
-    // A row with fewer than that above -inf has all of those, and then the first at -inf.
-    const bool scarce = bound == -INFINITY && s - s == 0.f;
-    const auto passes = [&](float e) { return scarce ? e > -INFINITY : !(e < bound); };
+    // Where too many are equal to the bound (masked words), those above it are all there are, and then the first of those
+    // equal to it. So it is at -inf from the start: fewer than asked for are above that.
+    bool above = bound == -INFINITY && s - s == 0.f;
+    const bool may = above || bound > -INFINITY;
+    const auto passes = [&](float e) { return above ? e > bound : !(e < bound); };
     auto collect = [&](float e, int i) {
       if (passes(e)) {
         const int at = atomicAdd(&count, 1);
         if (at < kList) list[at] = key_of(e, base + i);
       }
     };
-    int slot = INT_MAX;
-    if (passes(mx)) {
-      slot = atomicAdd(&lanes, 1);
-      if (odd >= 0) collect(x0, odd);
-    }
-    __syncthreads();
-    const int held = lanes;
-    for (int from = 0; from < held; from += kLanes) {
-      if (slot >= from && slot < from + kLanes) {
-        owner[slot - from] = static_cast<uint16_t>(tid);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
+    int found;
+    for (;;) {
+      int slot = INT_MAX;
+      if (passes(mx)) {
+        slot = atomicAdd(&lanes, 1);
+        if (odd >= 0) collect(x0, odd);
       }
       __syncthreads();
-      for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
-        const int at = (i % V) * THREADS + owner[i / V];
-        if (at < vecs) {
-          float e[kE];
-          F::unpack(stash[i], e);
+      const int held = lanes;
+      for (int from = 0; from < held; from += kLanes) {
+        if (slot >= from && slot < from + kLanes) {
+          owner[slot - from] = static_cast<uint16_t>(tid);
 #pragma unroll
-          for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
+          for (int v = 0; v < V; ++v)
+            if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
         }
+        __syncthreads();
+        for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
+          const int at = (i % V) * THREADS + owner[i / V];
+          if (at < vecs) {
+            float e[kE];
+            F::unpack(stash[i], e);
+#pragma unroll
+            for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
+          }
+        }
+        __syncthreads();
+        if (count > kList) break;
       }
       __syncthreads();
-      if (count > kList) break;
+      found = count;
+      if (found <= kList || above || !may) break;
+      above = true;
+      __syncthreads();
+      if (tid == 0) count = lanes = 0;
+      __syncthreads();
     }
-    __syncthreads();
-    const int found = count;
     if (found <= kList) {
       rank_keys<THREADS>(list, found, a.top, put);
       if (tid < 64) {
         int got = found;
-        if (scarce)
+        if (above)
           for (int i0 = 0; i0 < n && got < a.top; i0 += 64) {
-            const bool it = i0 + lane < n && F::load(x, i0 + lane) == -INFINITY;
+            const bool it = i0 + lane < n && F::load(x, i0 + lane) == bound;
             const uint64_t those = __ballot(it);
             const int rank = got + __popcll(those & ((uint64_t(1) << lane) - 1));
-            if (it && rank < a.top) put(rank, key_of(-INFINITY, base + i0 + lane));
+            if (it && rank < a.top) put(rank, key_of(bound, base + i0 + lane));
             got += __popcll(those);
           }
         // a piece of fewer elements
@@ -303,13 +312,12 @@ __global__ __launch_bounds__(512, 8) void logprobs_stream(Row a) {
   float m = odd >= 0 ? F::load(x, odd) : -INFINITY;  // NaN: the sums get it below
   const float x0 = m;
   m = m != m ? -INFINITY : m;
-  float s = 0.f, u = 0.f, r2 = 0.f;
+  float s = 0.f, u = 0.f, r = m == -INFINITY ? 0.f : m;
   auto add = [&](float e) {
-    const float t = __builtin_fmaf(e, kLog2e, -r2), p = __builtin_amdgcn_exp2f(t);
+    const float t = (e - r) * kLog2e, p = __builtin_amdgcn_exp2f(t);
     s += p;
     if (ENT) u = __builtin_fmaf(fmaxf(t, -1000.f), p, u);
   };
-  r2 = m == -INFINITY ? 0.f : m * kLog2e;
   if (odd >= 0) add(x0);
   auto load4 = [&](int v0, uint4 (&d)[kAhead]) {
 #pragma unroll
@@ -327,10 +335,10 @@ __global__ __launch_bounds__(512, 8) void logprobs_stream(Row a) {
       for (int i = 1; i < kE; ++i) top = fmaxf(top, e[i]);
       if (top > m) {
         const float by = (m - top) * kLog2e, f = __builtin_amdgcn_exp2f(by);
-        if (ENT) u = m == -INFINITY ? u : f * __builtin_fmaf(by, s, u);
+        if (ENT) u = m == -INFINITY ? u : f * __builtin_fmaf(fmaxf(by, -1000.f), s, u);
         s = m == -INFINITY ? s : s * f;  // of nothing but a NaN
         m = top;
-        r2 = m * kLog2e;
+        r = m;
       }
 #pragma unroll
       for (int i = 0; i < kE; ++i) add(e[i]);
@@ -364,11 +372,11 @@ __global__ __launch_bounds__(512, 8) void logprobs_stream(Row a) {
     a.part[item] = make_float4(all, s, u, 0.f);
     return;
   }
-  const float lse = ref + __logf(s);
-  if (a.lse) a.lse[row] = lse;
-  if (ENT) a.entropy[row] = __logf(s) - u / s;
+  const float log_s = __logf(s);
+  if (a.lse) a.lse[row] = ref + log_s;
+  if (ENT) a.entropy[row] = log_s - u / s;
   const int64_t t = token_of(a.tokens, a.wide_tokens, row);
-  a.logp[row] = t >= 0 && t < n ? F::load(x, t) - lse : __uint_as_float(0x7fc00000u);
+  a.logp[row] = t >= 0 && t < n ? F::load(x, t) - ref - log_s : __uint_as_float(0x7fc00000u);
 }
 
 // Joins the pieces of a row.
@@ -386,13 +394,13 @@ __global__ __launch_bounds__(256) void logprobs_join(Row a) {
   const float f = p.x == -INFINITY ? 0.f : __expf(p.x - ref);
   const float s = wave_sum(p.x == -INFINITY ? p.y : f * p.y);
   const float u = wave_sum(p.x == -INFINITY ? 0.f : f * __builtin_fmaf(shift, p.y, p.z));
-  const float lse = ref + __logf(s);
+  const float log_s = __logf(s);
   if (tid == 0) {
-    if (a.lse) a.lse[row] = lse;
-    if (a.entropy) a.entropy[row] = __logf(s) - u / s;
+    if (a.lse) a.lse[row] = ref + log_s;
+    if (a.entropy) a.entropy[row] = log_s - u / s;
     using S = typename F::storage;
     const int64_t t = token_of(a.tokens, a.wide_tokens, row);
-    a.logp[row] = t >= 0 && t < a.vocab ? F::load(static_cast<const S*>(a.x) + row * a.stride, t) - lse
+    a.logp[row] = t >= 0 && t < a.vocab ? F::load(static_cast<const S*>(a.x) + row * a.stride, t) - ref - log_s
                                         : __uint_as_float(0x7fc00000u);
     count = 0;
   }
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(256) void logprobs_join(Row a) {
   }
   __syncthreads();
   rank_keys<256>(list, count, a.top, [&](int rank, uint64_t key) {
-    a.top_logp[row * a.top + rank] = key_value(key) - lse;
+    a.top_logp[row * a.top + rank] = key_value(key) - ref - log_s;
     a.top_index[row * a.top + rank] = key_index(key);
   });
 }

@@ -161,6 +161,43 @@ def test_few_words_allowed(hk, rows, vocab, allowed):
     check(hk, y, t, 20)
 
 
+@pytest.mark.parametrize("dt", [BF, F16, F32])
+@pytest.mark.parametrize("rows,vocab", [(5, 20000), (600, 700), (300, 50257), (300, 9000)])
+@pytest.mark.parametrize("allowed", [0, 1, 7, 19, 20, 21, 40])
+def test_words_masked_by_the_lowest_value(hk, rows, vocab, allowed, dt):
+    # all but a few words at the type's lowest value: equal ones rank by their index, behind the few
+    say(rows, vocab, allowed, dt)
+    x, t = make(rows, vocab, dt)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    keep = torch.randperm(vocab, generator=g, device=DEV)[:allowed]
+    y = torch.full_like(x, torch.finfo(dt).min)
+    y[:, keep] = x[:, keep]
+    p = hk.token_logprobs(y, t, entropy=True, top=20)
+    q = hk.token_logprobs(y, t, entropy=True)
+    few, order = torch.sort(y[:, keep].float(), dim=1, descending=True, stable=True)
+    rest = torch.ones(vocab, device=DEV, dtype=torch.bool)
+    rest[keep] = False
+    first = rest.nonzero()[:20, 0]
+    for i in range(min(allowed, 20)):
+        assert torch.equal(y.gather(1, p.top_index[:, i:i + 1])[:, 0].float(), few[:, i])
+    if allowed < 20:
+        assert torch.equal(p.top_index[:, allowed:], first[:20 - allowed].expand(rows, -1))
+    # less the maximum first: beside the lowest value lse has no room for log s
+    z = y.double() - y.double().amax(1, keepdim=True)
+    log_s = z.exp().sum(1, keepdim=True).log()
+    lp = z - log_s
+    prob = lp.exp()
+    ent = -(prob * torch.where(prob > 0, lp, 0.0)).sum(1)
+    tol = lambda want: 2.0 ** -16 + 2.0 ** -21 * (want.abs() + log_s.abs().max() + 8)  # noqa: E731  logits under 16
+    for got, want in ((p.top_logp, lp.gather(1, p.top_index)), (p.logp, lp.gather(1, t[:, None])[:, 0]),
+                      (q.logp, lp.gather(1, t[:, None])[:, 0])):
+        assert bool(((got.double() - want).abs() <= tol(want)).logical_or(got.double() == want.float().double()).all())
+    for r in (p, q):
+        assert bool(((r.entropy.double() - ent).abs() <= 2 * tol(ent)).all())
+        dx = hk.token_logprobs_backward(y, t, r.lse, torch.ones(rows, device=DEV), r.entropy, torch.ones(rows, device=DEV))
+        assert torch.isfinite(dx).all()
+
+
 def test_entropy_left_out(hk):
     x, t = make(5, 3001, BF)
     p = check(hk, x, t, 3, entropy=False)
