@@ -206,7 +206,6 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
     // Where too many are equal to the bound (masked words), those above it are all there are, and then the first of those
     // equal to it. So it is at -inf from the start: fewer than asked for are above that.
     bool above = bound == -INFINITY && s - s == 0.f;
-    const bool may = above || bound > -INFINITY;
     const auto passes = [&](float e) { return above ? e > bound : !(e < bound); };
     auto collect = [&](float e, int i) {
       if (passes(e)) {
@@ -214,42 +213,43 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
         if (at < kList) list[at] = key_of(e, base + i);
       }
     };
-    int found;
-    for (;;) {
-      int slot = INT_MAX;
-      if (passes(mx)) {
-        slot = atomicAdd(&lanes, 1);
-        if (odd >= 0) collect(x0, odd);
+    int slot = INT_MAX;
+    if (passes(mx)) {
+      slot = atomicAdd(&lanes, 1);
+      if (odd >= 0) collect(x0, odd);
+    }
+    __syncthreads();
+    const int held = lanes;
+    for (int from = 0; from < held; from += kLanes) {
+      if (slot >= from && slot < from + kLanes) {
+        owner[slot - from] = static_cast<uint16_t>(tid);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
       }
       __syncthreads();
-      const int held = lanes;
-      for (int from = 0; from < held; from += kLanes) {
-        if (slot >= from && slot < from + kLanes) {
-          owner[slot - from] = static_cast<uint16_t>(tid);
+      for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
+        const int at = (i % V) * THREADS + owner[i / V];
+        if (at < vecs) {
+          float e[kE];
+          F::unpack(stash[i], e);
 #pragma unroll
-          for (int v = 0; v < V; ++v)
-            if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
+          for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
         }
-        __syncthreads();
-        for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
-          const int at = (i % V) * THREADS + owner[i / V];
-          if (at < vecs) {
-            float e[kE];
-            F::unpack(stash[i], e);
-#pragma unroll
-            for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
-          }
-        }
-        __syncthreads();
-        if (count > kList) break;
       }
       __syncthreads();
-      found = count;
-      if (found <= kList || above || !may) break;
+      if (count > kList) break;
+    }
+    __syncthreads();
+    int found = count;
+    if (found > kList && !above && bound > -INFINITY) {
       above = true;
       __syncthreads();
-      if (tid == 0) count = lanes = 0;
+      if (tid == 0) count = 0;
       __syncthreads();
+      for (int i = tid; i < n; i += THREADS) collect(F::load(x, i), i);
+      __syncthreads();
+      found = count;
     }
     if (found <= kList) {
       rank_keys<THREADS>(list, found, a.top, put);
