@@ -17,8 +17,8 @@
 // look them through and collect (value, index) keys, which are ranked by counting the larger ones. Where more pass
 // than that list takes even without those equal to the bound, `top` passes over the row find the next largest.
 //
-// Measured, rows of 50257: 4096 of bf16 with 5 alternatives 76 us (5.4 TB/s, where the bound is the memory); 8192 of bf16
-// without 143 (5.8), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
+// Measured, rows of 50257: 4096 of bf16 with 5 alternatives 78 us (5.3 TB/s, where the bound is the memory); 8192 of bf16
+// without 149 (5.5), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
 // latency: load, maximum, sums, selection one after the other.
 #include <limits.h>
 
@@ -314,6 +314,7 @@ __global__ __launch_bounds__(512, 8) void logprobs_stream(Row a) {
   m = m != m ? -INFINITY : m;
   float s = 0.f, u = 0.f, r = m == -INFINITY ? 0.f : m;
   auto add = [&](float e) {
+    // not one fma: x log2 e may be past fp32, and loses 2^-24 of a large x
     const float t = (e - r) * kLog2e, p = __builtin_amdgcn_exp2f(t);
     s += p;
     if (ENT) u = __builtin_fmaf(fmaxf(t, -1000.f), p, u);
