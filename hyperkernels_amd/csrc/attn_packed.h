@@ -130,11 +130,13 @@ __device__ __forceinline__ int wave_add(int v) {
 // once (per_cu a CU), workgroup L and L + P (P CUs) are likely to meet on one CU, so every other P of them run backwards:
 // a CU gets heavy and light ones. (8192 tokens in 13 documents, 12 heads of 64, sequence by sequence instead: forward
 // 34.6 us against 29.8, dk and dv 59 against 48.)
-// More than 64 sequences, one a lane, are taken one after the other.
-__device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, const Args& a, int group, int B, int per_cu,
-                                          Seq& q, int& share, int& head) {
+// More than 64 sequences, one a lane, are taken one after the other. ByQ: tiles of queries (`group` rows each), else of
+// keys. cu_q and cu_k may be one array over tensors of different lengths, so the starts do not tell.
+template <bool ByQ>
+__device__ __forceinline__ bool find_item(const Args& a, int group, int B, int per_cu, Seq& q, int& share, int& head) {
   const int lane = threadIdx.x & 63, per_tile = a.k_heads * a.splits;
-  const bool by_q = cu == a.cu_q;
+  const int32_t* const cu = ByQ ? a.cu_q : a.cu_k;
+  const int64_t tokens = ByQ ? a.q_tokens : a.k_tokens;
   if (a.n > 64) {
     // slot floor(cu[s] group / B) + s is the first of sequence s, which leaves each the tiles it needs
     const int x = a.tiles - 1 - static_cast<int>(blockIdx.x) / per_tile, rest = blockIdx.x % per_tile;
@@ -153,8 +155,8 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, con
     const int64_t k0 = clamp64(a.cu_k[lo], 0, a.k_tokens), k1 = clamp64(a.cu_k[lo + 1], k0, a.k_tokens);
     q.q0 = q0, q.mq = static_cast<int>(q1 - q0);
     q.k0 = k0, q.mk = static_cast<int>(k1 - k0);
-    q.tile = x - static_cast<int>((by_q ? q0 : k0) * group / B + lo);
-    q.tiles = static_cast<int>(((by_q ? q.mq : q.mk) * static_cast<int64_t>(group) + B - 1) / B);
+    q.tile = x - static_cast<int>((ByQ ? q0 : k0) * group / B + lo);
+    q.tiles = static_cast<int>(((ByQ ? q.mq : q.mk) * static_cast<int64_t>(group) + B - 1) / B);
     share = rest / a.k_heads, head = rest - share * a.k_heads;
     return q.tile >= 0 && q.tile < q.tiles;
   }
@@ -163,7 +165,7 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int64_t tokens, con
   const int cq0 = a.cu_q[i0], cq1 = a.cu_q[i0 + 1], ck0 = a.cu_k[i0], ck1 = a.cu_k[i0 + 1];
   const int q0 = min(max(cq0, 0), tq), q1 = min(max(cq1, q0), tq);
   const int k0 = min(max(ck0, 0), tk), k1 = min(max(ck1, k0), tk);
-  const uint32_t len = static_cast<uint32_t>(by_q ? q1 - q0 : k1 - k0) * group;
+  const uint32_t len = static_cast<uint32_t>(ByQ ? q1 - q0 : k1 - k0) * group;
   const int count = lane < a.n ? static_cast<int>((len + B - 1) / B) : 0;  // the sequence's tiles
   auto over = [&](int t) { return wave_add(max(count - t, 0)); };  // tiles of number t and over
   const int total = over(0) * per_tile;

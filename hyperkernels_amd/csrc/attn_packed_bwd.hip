@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
 
   Seq q;
   int share, kh;
-  if (!find_item(a.cu_q, a.q_tokens, a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
+  if (!find_item<true>(a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
   const int rows = q.mq * a.group, r0 = q.tile * S::kRows;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
 
   Seq q;
   int share, kh;
-  if (!find_item(a.cu_k, a.k_tokens, a, 1, S::kKeys, S::kHalves == 2 ? 1 : 3, q, share, kh)) return;
+  if (!find_item<false>(a, 1, S::kKeys, S::kHalves == 2 ? 1 : 3, q, share, kh)) return;
   // under the causal mask the first keys meet the most rows: they go first
   const int k0 = (q.tiles - 1 - q.tile) * S::kKeys;
   const int rows = q.mq * a.group, ahead = q.mk - q.mq;

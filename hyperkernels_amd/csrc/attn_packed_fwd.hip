@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : 2) void attn_packed_fwd(Args a) 
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   Seq q;
   int share, kh;
-  if (!find_item(a.cu_q, a.q_tokens, a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
+  if (!find_item<true>(a, a.group, S::kRows, S::kPerCu, q, share, kh)) return;
   attend<T, D, KG, false>(a, q, kh, 0, 1, (char HK_LDS*)lds_raw);
 }
 
