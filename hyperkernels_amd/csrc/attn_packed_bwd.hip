@@ -13,7 +13,9 @@
 // take delta = sum p dp instead, from one more pass over their one or two tiles of keys. dS is as small as P and
 // dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
 // times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
-// where dK is moved to the next when it grows.
+// where dK is moved to the next when it grows. Large values could take such a dS past fp16's end: attn_packed_dq looks at each
+// block's largest and moves the row's power, and dQ with it (4096 tokens, 16 heads of 128: 126 -> 131 us; a second pass over such tiles
+// instead, for want of registers, 139); attn_packed_dkv has the sum of a key's |v|, which bounds its dP before the loop.
 //
 // Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 31, dk and dv 43 us; sequences of 2048, 1001 and
 // 333, 16 heads on 4 of 128, fp16: 53, and 85 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
@@ -24,6 +26,10 @@ namespace hk {
 namespace packed {
 
 constexpr int kLeast = -40;  // an exponent under any of fp16
+constexpr float kMost = 65504.f;  // fp16's largest number
+
+// The exponent e of |x| < 2^e, kLeast for 0.
+__device__ __forceinline__ int exponent(float x) { return x == 0.f ? kLeast : __builtin_amdgcn_frexp_expf(x); }
 
 template <int D, int KG>
 struct DqShape {
@@ -137,9 +143,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
           most = fmaxf(most, fmaxf(fabsf(w[0]), fabsf(w[1])));
         }
       }
-      // dout is under 2^grow, a row of zeros under any of fp16's
-      most = half32_reduce(most, MaxOp{});
-      grow = most == 0.f ? kLeast : __builtin_amdgcn_frexp_expf(most);
+      grow = max(exponent(half32_reduce(most, MaxOp{})), exponent(delta) - 14);  // dout under 2^grow, delta under 2^14 of that
     }
     if (kg == 0 && h == 0 && row < rows) {
       float* st = a.delta + qh * a.q_tokens + at;
@@ -150,8 +154,6 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     }
     if (T::kNarrow) lse2 += static_cast<float>(grow);
   }
-  const float out = T::kNarrow ? ldexpf(a.scale, grow) : a.scale;
-
   f32x16_t dq[D / 32];
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) dq[b] = f32x16_t{};
@@ -171,6 +173,23 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, -lse2)) * (dp[i] - delta);
+      if constexpr (T::kNarrow) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
+        if (__any(top > kMost)) {  // of large values: the row's power of two moves, and dq with it
+          top = half32_reduce(top, MaxOp{});
+          const int up = top > kMost && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+          const float f = ldexpf(1.f, -up);
+          grow += up, lse2 += static_cast<float>(up);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] *= f;
+#pragma unroll
+          for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dq[b][i] *= f;
+        }
+      }
       s16x8_t ds[2];
       pack_block<T>(s, ds);
 #pragma unroll
@@ -180,6 +199,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     }
   }
 
+  const float out = T::kNarrow ? ldexpf(a.scale, grow) : a.scale;
   if constexpr (KG > 1) {
     // the sums of the waves that have the same rows
     constexpr int R = S::kRows;
@@ -226,7 +246,8 @@ struct DkvShape {
   static constexpr int kHeld = 2 * kKeys * D * 2;  // K, V
   static constexpr int kPitch = D + 4;
   static constexpr int kExchange = kHalves == 2 ? kKeys * kPitch * 4 : 0;
-  static constexpr int kLds = kHeld + 2 * kStage > kExchange ? kHeld + 2 * kStage : kExchange;
+  static constexpr int kNorms = kHeld + 2 * kStage;  // fp16: of the keys' values
+  static constexpr int kLds = kNorms + 4 * kKeys > kExchange ? kNorms + 4 * kKeys : kExchange;
 };
 
 __device__ __forceinline__ void copy4_to_lds(const void* sbase, int voff, unsigned lds_addr) {
@@ -312,6 +333,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
       copy4_to_lds(d0p + 4 * (hd * a.q_tokens + tok), to + 2 * S::kTile + 256 * wave);
     }
   };
+  float HK_LDS* const norms = (float HK_LDS*)(lds + S::kNorms);
   {
     // columns behind the head's last element are zero: those of Q and dO are copies of others
     for (int i = threadIdx.x; i < S::kKeys * kChunks; i += S::kThreads) {
@@ -324,6 +346,20 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
       }
       *reinterpret_cast<u32x4_t HK_LDS*>(lds + at_chunk<D>(r, ch)) = x;
       *reinterpret_cast<u32x4_t HK_LDS*>(lds + S::kHeld / 2 + at_chunk<D>(r, ch)) = y;
+      if constexpr (T::kNarrow) {
+        // sum |v| of the key: kChunks lanes have it
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x2_t w = T::unpack(y[e]);
+          sum += fabsf(w[0]) + fabsf(w[1]);
+        }
+        sum += detail::dpp<detail::kDppXor1>(sum);
+        sum += detail::dpp<detail::kDppXor2>(sum);
+        sum += detail::dpp<detail::kDppHalfMirror>(sum);
+        if (kChunks == 16) sum += detail::dpp<detail::kDppMirror>(sum);
+        if (ch == 0) norms[r] = sum;
+      }
     }
   }
   if (t0 < t1) fetch(t0);
@@ -337,7 +373,13 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
   f32x16_t dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int b = 0; b < D / 32; ++b) dk[b] = dv[b] = f32x16_t{};
-  float grow = kLeast;  // exponent of the dout that dk is formed for
+  float grow = kLeast;  // exponent of the dout that dk is formed for, and what it is more than that for large values:
+  float more = 0.f;     // |dp| is under sum |v| times 2^grow, which is under 2^(14 + more) times that
+  if constexpr (T::kNarrow) {
+    wait_copies();
+    barrier();
+    more = static_cast<float>(max(exponent(norms[32 * kb + c]) - 14, 0));
+  }
 
   for (int t = t0; t < t1; ++t) {
     wait_copies();
@@ -357,7 +399,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
         grow = g;
       }
     }
-    const float shrink = T::kNarrow ? __builtin_amdgcn_exp2f(-grow) : 1.f;
+    const float shrink = T::kNarrow ? __builtin_amdgcn_exp2f(-grow - more) : 1.f;
 #pragma unroll
     for (int u = 0; u < S::kRows / 32 / S::kHalves; ++u) {
       const int n = S::kHalves == 2 ? half : u;
@@ -402,7 +444,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
     }
   }
   if constexpr (T::kNarrow) {
-    const float f = __builtin_amdgcn_exp2f(grow);
+    const float f = __builtin_amdgcn_exp2f(grow + more);
 #pragma unroll
     for (int b = 0; b < D / 32; ++b)
 #pragma unroll

@@ -1,0 +1,48 @@
+"""Packed attention in fp16 at the ends of its range. Values and tolerances as in test_gpu_attn_packed.py."""
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_attn_packed import DEV, F16, check, cu_of, make, reference, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("H,Hk,d,lens", [(4, 2, 64, [300, 41]), (2, 2, 128, [129, 2, 700]), (8, 8, 64, [4097]),
+                                         (16, 4, 128, [2048, 1001, 333]), (3, 1, 8, [50])])
+def test_large_values_and_small_gradients(hk, H, Hk, d, lens):
+    # dout of 2^-10 along values of up to 2^13 of the same signs: dS is some hundreds, but past fp16 for a dout of 1
+    say(H, Hk, d, lens)
+    q, k, v, do = make(lens, lens, H, Hk, d, F16)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g, device=DEV) * 2.0 - 1  # noqa: E731
+    u = sign(1, 1, d)
+    large = torch.rand(v.shape[0], Hk, 1, generator=g, device=DEV) < 0.7  # and others of 1
+    v = torch.where(large, 2.0 ** 13 * sign(v.shape[0], Hk, 1) * u, v.float()).to(F16)
+    do = (2.0 ** -10 * sign(do.shape[0], H, 1) * u * (0.5 + 0.5 * torch.rand(do.shape, generator=g, device=DEV))).to(F16)
+    do[5::7] = 0
+    cq = cu_of(lens)
+    o, lse = hk.attn_packed_forward(q, k, v, cq)
+    dq, dk, dv = hk.attn_packed_backward(do, q, k, v, o, lse, cq)
+    # dS is held for a dout of at most 2^14: half a step of fp16's smallest numbers times that, and the power of two
+    # above the largest dout
+    want = reference(q, k, v, lens, lens, True, d ** -0.5, do, 2.0 ** -25 * 2.0 ** 14 * 2 * float(do.abs().max()))
+    assert all(torch.isfinite(t[0].to(F16)).all() for n, t in want.items() if n != "lse")
+    check({"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, want)
+
+
+def test_values_at_the_end_of_fp16(hk):
+    # the largest dS that finite inputs of few keys can have: the gradients' own range is the limit
+    lens, d = [2, 3], 128
+    q, k, v, do = make(lens, lens, 2, 2, d, F16, std=2.0 ** -6)
+    v = torch.full_like(v, 65504.0)
+    v[1::2] = -65504.0
+    do = torch.full_like(do, 2.0 ** -8)
+    do[:, :, ::2] *= -0.5
+    cq = cu_of(lens)
+    o, lse = hk.attn_packed_forward(q, k, v, cq)
+    got = dict(zip(("dq", "dk", "dv"), hk.attn_packed_backward(do, q, k, v, o, lse, cq)))
+    want = reference(q, k, v, lens, lens, True, d ** -0.5, do, 2.0 ** -25 * 2.0 ** 14 * 2 * 2.0 ** -8)
+    del want["o"], want["lse"]
+    assert all(torch.isfinite(t[0].to(F16)).all() for t in want.values())
+    check(got, want)
