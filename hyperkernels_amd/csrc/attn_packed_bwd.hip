@@ -15,7 +15,7 @@
 // times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
 // where dK is moved to the next when it grows. Large values could take such a dS past fp16's end: attn_packed_dq looks at each
 // block's largest and moves the row's power, and dQ with it (4096 tokens, 16 heads of 128: 126 -> 131 us; a second pass over such tiles
-// instead, for want of registers, 139); attn_packed_dkv has the sum of a key's |v|, which bounds its dP before the loop.
+// instead, for want of registers, 139); attn_packed_dkv has the sum of a key's |v|, which bounds its dP before the loop. There P, as small as one over a row's keys, is held for a sum of 2^12.
 //
 // Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 31, dk and dv 43 us; sequences of 2048, 1001 and
 // 333, 16 heads on 4 of 128, fp16: 53, and 85 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
@@ -27,6 +27,7 @@ namespace packed {
 
 constexpr int kLeast = -40;  // an exponent under any of fp16
 constexpr float kMost = 65504.f;  // fp16's largest number
+constexpr int kUp = 12;  // fp16: P is held times 2^12, normal numbers to 2^-26: rows of more than 2^14 keys have P under 2^-14
 
 // The exponent e of |x| < 2^e, kLeast for 0.
 __device__ __forceinline__ int exponent(float x) { return x == 0.f ? kLeast : __builtin_amdgcn_frexp_expf(x); }
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
       float* st = a.delta + qh * a.q_tokens + at;
       st[0] = delta;
       const int64_t all = static_cast<int64_t>(a.k_heads) * a.group * a.q_tokens;
-      st[all] = lse2;
+      st[all] = T::kNarrow ? lse2 - kUp : lse2;
       if (T::kNarrow) st[2 * all] = static_cast<float>(grow);
     }
     if (T::kNarrow) lse2 += static_cast<float>(grow);
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
         grow = g;
       }
     }
-    const float shrink = T::kNarrow ? __builtin_amdgcn_exp2f(-grow - more) : 1.f;
+    const float shrink = T::kNarrow ? __builtin_amdgcn_exp2f(-grow - more - kUp) : 1.f;
 #pragma unroll
     for (int u = 0; u < S::kRows / 32 / S::kHalves; ++u) {
       const int n = S::kHalves == 2 ? half : u;
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
 #pragma unroll
     for (int b = 0; b < D / 32; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dk[b][i] *= f;
+      for (int i = 0; i < 16; ++i) dk[b][i] *= f, dv[b][i] *= 1.f / (1 << kUp);
   }
   if constexpr (S::kHalves == 2) {
     // the second half's sums, first of dK, then of dV

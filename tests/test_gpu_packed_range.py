@@ -46,3 +46,27 @@ def test_values_at_the_end_of_fp16(hk):
     del want["o"], want["lse"]
     assert all(torch.isfinite(t[0].to(F16)).all() for t in want.values())
     check(got, want)
+
+
+@pytest.mark.parametrize("n,d,causal", [(208412, 64, False), (120000, 128, True)])
+def test_flat_rows_over_many_keys(hk, n, d, causal):
+    # Equal scores: p = 1 / n, which fp16's own steps of 2^-24 are off by one in 160. dv = p sum of dout, with P's rounding
+    # and the result's, 2^-11 each. In fp32: the sum of n terms (n / 4096 additions one after the other: blocks of 64 keys, 16
+    # of them a lane, in four sums), and the log-sum-exp (under 16), the exponential and 32 products, 2^-18 together.
+    say(n, d, causal)
+    m = 32
+    q, k, v, do = make([m], [n], 1, 1, d, F16)
+    q.zero_()
+    do = (do * 1024).abs()
+    cq, ck = cu_of([m]), cu_of([n])
+    o, lse = hk.attn_packed_forward(q, k, v, cq, ck, causal)
+    _, _, dv = hk.attn_packed_backward(do, q, k, v, o, lse, cq, ck, causal)
+    i = torch.arange(m, device=DEV, dtype=torch.float64)
+    p = 1 / (i + n - m + 1) if causal else torch.full_like(i, 1 / n)
+    x = do.double()[:, 0] * p[:, None]
+    want = x.sum(0).expand(n, d).clone()
+    if causal:  # the last keys are seen by the last queries alone
+        want[n - m:] = x.flip(0).cumsum(0).flip(0)
+    off = (dv.double()[:, 0] - want).abs()
+    tol = (2 * 2.0 ** -11 * 1.01 + n / 4096 * 2.0 ** -24 + 2.0 ** -18) * want + 2.0 ** -25
+    assert bool((off <= tol).all()), float((off / want).max())
