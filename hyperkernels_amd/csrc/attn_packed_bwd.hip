@@ -9,8 +9,8 @@
 // dV^T += dO^T P and dK^T += Q^T dS as they lie. The rows of a group's heads are one loop there, which sums them.
 // P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. That makes the norm of the
 // gradients' error sqrt(2) of what rounding them leaves. delta from the o that was rounded adds p (dout . o's error) to
-// dS, 2 / (n - 1) of that rounding's square over n equal keys: rows of few keys, where it would be most of the error,
-// take delta = sum p dp instead, from one more pass over their one or two tiles of keys. dS is as small as P and
+// dS, 2 / (n - 1) of that rounding's square over n equal keys: rows of up to 128 keys, where it would be most of the error,
+// take delta = sum p dp instead, from one more pass over the first one or two tiles of keys in workgroups that have such rows. dS is as small as P and
 // dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
 // times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
 // where dK is moved to the next when it grows. Large values could take such a dS past fp16's end: attn_packed_dq looks at each
@@ -26,6 +26,7 @@ namespace hk {
 namespace packed {
 
 constexpr int kLeast = -40;  // an exponent under any of fp16
+constexpr int kShort = 128;  // keys of a row up to which delta is formed from p and dp
 constexpr float kMost = 65504.f;  // fp16's largest number
 constexpr int kUp = 12;  // fp16: P is held times 2^12, normal numbers to 2^-26: rows of more than 2^14 keys have P under 2^-14
 
@@ -37,7 +38,7 @@ struct DqShape {
   static constexpr int kRows = 128 / KG;
   static constexpr int kKeys = KG == 4 ? 128 : 64;
   static constexpr int kBlocks = kKeys / KG / 32;
-  static constexpr int kFew = 128 / kKeys;  // tiles of keys up to which delta is formed from p and dp
+  static constexpr int kFew = kShort / kKeys;  // tiles of keys of rows whose delta is formed from p and dp
   static constexpr int kTile = kKeys * D * 2;
   static constexpr int kStage = 2 * kTile;
   static constexpr int kPitch = D + 4;
@@ -77,9 +78,9 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     copy_k(t, q.mk, wave, to);
     copy_v(t, q.mk, wave, to + S::kTile);
   };
-  const bool few = t1 <= S::kFew;
+  const bool few = (a.causal ? r0 / a.group + ahead : q.mk - 1) < kShort;  // the first row, and so some, has few keys
   if (t1 > 0) fetch(0);
-  if (few && t1 > 1) fetch(1);
+  if (few && S::kFew > 1 && t1 > 1) fetch(1);
 
   const Reads<D> rd(lane);
   const float sc = a.scale * kLog2e;
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
     if (few) {
       wait_copies();
       barrier();
-      for (int key0 = 0; key0 < t1 * S::kKeys && key0 <= lim_hi; key0 += 32) {
+      for (int key0 = 0; lim_lo < kShort && key0 < kShort && key0 <= lim_hi; key0 += 32) {
         const char HK_LDS* kt = lds + key0 / S::kKeys * S::kStage + key0 % S::kKeys * (2 * D);
         f32x16_t s, dp;
         products(kt, kt + S::kTile, key0, s, dp);
@@ -119,18 +120,21 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
         for (int i = 0; i < 16; ++i)
           delta = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sc, -lse2)), dp[i], delta);
       }
-    } else {
+    }
+    if (lim_hi >= kShort) {
       s16x8_t ox[D / 16];
       load_row<D>(a.o.p + at * a.o.m + qh * a.o.h, h, a.d, ox);
+      float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
         const u32x4_t x = __builtin_bit_cast(u32x4_t, ox[s]), y = __builtin_bit_cast(u32x4_t, gx[s]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x2_t u = T::unpack(x[i]), w = T::unpack(y[i]);
-          delta += u[0] * w[0] + u[1] * w[1];
+          sum += u[0] * w[0] + u[1] * w[1];
         }
       }
+      delta = lim < kShort ? delta : sum;
     }
     delta = half32_reduce(delta, AddOp{});
     if constexpr (T::kNarrow) {
@@ -162,7 +166,7 @@ __global__ __launch_bounds__(256, KG == 4 ? 1 : D == 64 ? 3 : 2) void attn_packe
   for (int t = 0; t < t1; ++t) {
     wait_copies();
     barrier();
-    if (t + 1 < t1 && !few) fetch(t + 1);
+    if (t + 1 < t1 && (!few || t + 1 >= S::kFew)) fetch(t + 1);
     const int key0 = t * S::kKeys + 32 * S::kBlocks * kg;
     const char HK_LDS* kt = lds + (t & 1) * S::kStage + 32 * S::kBlocks * kg * (2 * D);
     const char HK_LDS* vt = kt + S::kTile;
