@@ -5,6 +5,9 @@
 //   lse = log sum_j exp(x_j),  logp = x_token - lse,  H = -sum p log p = log s - u / s
 //   with m = max x, s = sum exp(x - m), u = sum (x - m) exp(x - m);
 //   dx_j = g ([j = token] - p_j) - h p_j (x_j - lse + H).
+// One fp32 number has no room for log s beside a maximum far from 0: logp takes them off one after the other, and so does the
+// gradient of rows whose lse is past kFar, for which one workgroup a row reads it twice (2048 rows of 50257 fp32 near
+// 1000: 228 us, 140 near 0; 16 of 131072: 94, 12 near 0).
 //
 // Forward: a workgroup holds a row (or a piece of one) in registers, so it is read once whatever follows: the maximum, then
 // both sums against it without any rescaling, then the selection. Rows that are longer than the registers, or too
@@ -21,6 +24,8 @@
 // without 149 (5.5), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
 // latency: load, maximum, sums, selection one after the other.
 #include <limits.h>
+
+#include <type_traits>
 
 #include "hk_device.h"
 #include "hk_host.h"
@@ -436,6 +441,64 @@ struct Grad {
 };
 
 constexpr int kGradVecs = 2;  // 16-byte vectors a lane
+// p = exp(x - lse) is off by half a step of lse, relative. Below these that is a sixteenth of the result's rounding, or 2^-18 of fp32's;
+// past them it has no bound: a row of words at the type's lowest value has an lse with no room for log s.
+template <class F>
+constexpr float kFar = F::kPerVec == 4 ? 128.f : std::is_same_v<F, F16> ? 1024.f : 4096.f;
+
+// Where a row's elements lie: up to 7 before its first 16-byte boundary, vectors, and up to 7 behind them.
+template <class F>
+struct Span {
+  int head, vecs, odd;  // odd: the one of the others that this lane has, or -1
+  __device__ __forceinline__ Span(const typename F::storage* x, int n) {
+    constexpr int kE = F::kPerVec;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(*x)), tid = threadIdx.x;
+    head = min(off ? kE - off : 0, n), vecs = (n - head) / kE;
+    const int tail0 = head + vecs * kE;
+    odd = tid < head ? tid : tid >= 32 && tid - 32 < n - tail0 ? tail0 + tid - 32 : -1;
+  }
+};
+
+// A row's maximum, and the logarithm of its sum of exponentials against that, by all of the workgroup's 256 lanes.
+constexpr int kFarVecs = 4;  // in flight
+template <class F>
+__device__ __forceinline__ void row_parts(const typename F::storage* x, const Span<F>& at, float& ref, float& log_s) {
+  constexpr int kE = F::kPerVec;
+  __shared__ float red[2][4];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + at.head);
+  float m = at.odd >= 0 ? F::load(x, at.odd) : -INFINITY;
+  float s = m == -INFINITY ? 0.f : 1.f;
+  for (int v0 = tid; v0 < at.vecs; v0 += 256 * kFarVecs) {
+    uint4 d[kFarVecs];
+#pragma unroll
+    for (int u = 0; u < kFarVecs; ++u)
+      if (v0 + 256 * u < at.vecs) d[u] = xv[v0 + 256 * u];
+#pragma unroll
+    for (int u = 0; u < kFarVecs; ++u) {
+      if (v0 + 256 * u >= at.vecs) continue;
+      float e[kE], top = m;
+      F::unpack(d[u], e);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) top = fmaxf(top, e[i]);
+      if (top > m) {
+        s *= __builtin_amdgcn_exp2f((m - top) * kLog2e);
+        m = top;
+      }
+      const float r = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) s += __builtin_amdgcn_exp2f((e[i] - r) * kLog2e);
+    }
+  }
+  const float wm = wave_max(m);
+  if (lane == 0) red[0][wave] = wm;
+  __syncthreads();
+  ref = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  s = wave_sum(m == -INFINITY ? s : s * __builtin_amdgcn_exp2f((m - ref) * kLog2e));
+  if (lane == 0) red[1][wave] = s;
+  __syncthreads();
+  log_s = __logf((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
+}
 
 // VEC: rows of x and dx have the same place within 16 bytes, so the vectors of one are vectors of the other.
 template <class F, bool VEC>
@@ -452,35 +515,61 @@ __global__ __launch_bounds__(256) void logprobs_grad(Grad a) {
   const float h = a.h ? a.h[row] : 0.f, ent = a.h ? a.entropy[row] : 0.f;
   // a row without a softmax has no gradient either: what the terms below leave out would hide it
   const float all = lse - lse == 0.f ? g : __uint_as_float(0x7fc00000u);
-  auto one = [&](float e, int i) {
-    const float d = fmaxf(e - lse, -200.f);  // exp of less is 0, and -inf has to be no factor
+  auto from_log = [&](float log_p, int i) {
+    const float d = fmaxf(log_p, -200.f);  // exp of less is 0, and -inf has to be no factor
     const float p = __builtin_amdgcn_exp2f(d * kLog2e);
     const float t = p * __builtin_fmaf(h, d + ent, all);
     return (i == token ? g : 0.f) - t;
   };
+  const Span<F> at(x, a.vocab);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + at.head);
+  uint4* ov = reinterpret_cast<uint4*>(dx + at.head);
+  if (fabsf(lse) >= kFar<F> && fabsf(lse) < INFINITY) {
+    // the row's first workgroup does all of it: what the others would write may lie on what this one reads
+    if (seg > 0) return;
+    float ref, log_s;
+    row_parts<F>(x, at, ref, log_s);
+    auto one = [&](float e, int i) { return from_log((e - ref) - log_s, i); };
+    if (!VEC) {
+      for (int i = tid; i < a.vocab; i += 256) F::store(dx, i, one(F::load(x, i), i));
+      return;
+    }
+    if (at.odd >= 0) F::store(dx, at.odd, one(F::load(x, at.odd), at.odd));
+    for (int v0 = tid; v0 < at.vecs; v0 += 256 * kFarVecs) {
+      uint4 d[kFarVecs];
+#pragma unroll
+      for (int u = 0; u < kFarVecs; ++u)
+        if (v0 + 256 * u < at.vecs) d[u] = xv[v0 + 256 * u];
+#pragma unroll
+      for (int u = 0; u < kFarVecs; ++u) {
+        const int v = v0 + 256 * u;
+        if (v >= at.vecs) continue;
+        float e[kE];
+        F::unpack(d[u], e);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) e[i] = one(e[i], at.head + v * kE + i);
+        st_nt(ov + v, F::pack(e));
+      }
+    }
+    return;
+  }
+  auto one = [&](float e, int i) { return from_log(e - lse, i); };
   if (VEC) {
-    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(S));
-    const int head = min(off ? kE - off : 0, a.vocab), vecs = (a.vocab - head) / kE, tail0 = head + vecs * kE;
-    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-    uint4* ov = reinterpret_cast<uint4*>(dx + head);
     uint4 d[kGradVecs];
     const int v0 = seg * (256 * kGradVecs) + tid;
 #pragma unroll
     for (int v = 0; v < kGradVecs; ++v)
-      if (v0 + 256 * v < vecs) d[v] = ld_nt(xv + v0 + 256 * v);
-    if (seg == 0) {
-      const int odd = tid < head ? tid : tid >= 32 && tid - 32 < a.vocab - tail0 ? tail0 + tid - 32 : -1;
-      if (odd >= 0) F::store(dx, odd, one(F::load(x, odd), odd));
-    }
+      if (v0 + 256 * v < at.vecs) d[v] = ld_nt(xv + v0 + 256 * v);
+    if (seg == 0 && at.odd >= 0) F::store(dx, at.odd, one(F::load(x, at.odd), at.odd));
 #pragma unroll
     for (int v = 0; v < kGradVecs; ++v) {
-      const int at = v0 + 256 * v;
-      if (at < vecs) {
+      const int i0 = v0 + 256 * v;
+      if (i0 < at.vecs) {
         float e[kE];
         F::unpack(d[v], e);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) e[i] = one(e[i], head + at * kE + i);
-        st_nt(ov + at, F::pack(e));
+        for (int i = 0; i < kE; ++i) e[i] = one(e[i], at.head + i0 * kE + i);
+        st_nt(ov + i0, F::pack(e));
       }
     }
   } else {

@@ -769,10 +769,11 @@ HK_API hipError_t hk_attn_packed_backward(const hk_attn_packed_params* params, i
  *   lse = log sum_j exp(x_j),  logp = x[token] - lse,  entropy = -sum_j p_j log p_j  (p = exp(x - lse))
  * and, where top > 0, the `top` largest log probabilities of the row, falling, with their indices (of equal ones the
  * lowest index first; NaN counts as less than everything): [rows, top] each. lse and entropy may be NULL: not
- * wanted. logp is formed from the maximum and the sum, so words masked by the type's lowest value, even a whole row of
- * them, are as exact as others; lse alone has no room for log s beside such a value, and the gradient of a row all of whose
- * words are there, which goes by lse, has p = 1. x = -inf has p = 0 and counts for nothing. A row that holds a NaN or
- * +inf, or nothing above -inf, has no softmax: logp, entropy and top_logp are NaN (indices are as above). A token outside 0 .. vocab - 1 has logp NaN.
+ * wanted. Logits far from 0, and words masked by the type's lowest value, even a whole row of them, are as exact as
+ * others: logp is formed from the maximum and the sum, and the gradient goes by lse only where its rounding is small
+ * beside the result's (|lse| under 128 for fp32, 1024 for fp16, 4096 for bf16) and forms maximum and sum again from the row
+ * past that. x = -inf has p = 0 and counts for nothing. A row that holds a NaN or +inf, or nothing above -inf, has no
+ * softmax: logp, entropy and top_logp are NaN (indices are as above). A token outside 0 .. vocab - 1 has logp NaN.
  * The gradient of the logits, from those of logp and entropy (each may be NULL: zero; grad_entropy needs the forward's
  * entropy) and the forward's lse:
  *   dx_j = grad_logp ([j == token] - p_j) - grad_entropy p_j (x_j - lse + entropy),
