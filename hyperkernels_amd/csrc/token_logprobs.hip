@@ -17,12 +17,16 @@
 // The `top` largest: with W waves, the ceil(top / W)-th largest of each wave's 64 lane maxima is reached by that many
 // elements of the wave, so the least of those over the waves is a bound that `top` elements reach and few others do (some
 // 60 of 50257 for top = 20). The lanes that hold one put their vectors into LDS, 128 lanes at a time, where all lanes
-// look them through and collect (value, index) keys, which are ranked by counting the larger ones. Where more pass
-// than that list takes even without those equal to the bound, `top` passes over the row find the next largest.
+// look them through and collect (value, index) keys, which are ranked by counting the larger ones. A wave of few words (of a
+// short piece, or with most masked) has no such bound or a low one, which many reach: then it is the `top`-th largest of all lane
+// maxima, found bit by bit. Where more reach that than the list takes even without those equal to it, `top` passes over
+// the row find the next largest.
 //
 // Measured, rows of 50257: 4096 of bf16 with 5 alternatives 78 us (5.3 TB/s, where the bound is the memory); 8192 of bf16
 // without 149 (5.5), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
-// latency: load, maximum, sums, selection one after the other.
+// latency: load, maximum, sums, selection one after the other. With waves that have no words: 16 rows of bf16, 20 alternatives,
+// 14.1 us (a pass for each: 40); 600 rows of 3000, 13.0 (52); 300 rows, 5 alternatives, an eighth of the words masked in a wave's
+// share of each 4096, 27 (162).
 #include <limits.h>
 
 #include <type_traits>
@@ -39,6 +43,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 64;
 constexpr int kMaxPieces = 64;
 constexpr int kList = 1024;  // candidates in LDS
+constexpr int kMany = 384;  // candidates that take longer to rank than a better bound does to find
 constexpr int kLanes = 128;  // lanes whose vectors LDS holds
 constexpr int kMostVecs = 14;  // 16-byte vectors a lane: with them 80 registers, three workgroups a CU
 
@@ -65,15 +70,17 @@ __device__ __forceinline__ int64_t token_of(const void* tokens, int wide, int64_
 
 // (value, index) as a number that is larger for larger values, and for the lower index of equal ones; NaN is under
 // all values, and 0 stands for nothing.
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
-  uint32_t b = __float_as_uint(v + 0.f);  // -0 is 0
-  b = v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return (static_cast<uint64_t>(b) << 32) | (0xffffffffu - index);
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);  // -0 is 0
+  return v != v ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t b = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float value_of(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x7fc00000u : (b & 0x80000000u) ? b & 0x7fffffffu : ~b);
 }
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  return (static_cast<uint64_t>(ordered(v)) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ float key_value(uint64_t key) { return value_of(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ int64_t key_index(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
 }
@@ -209,8 +216,9 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
       bound = row16_reduce(red[0][lane & (W - 1)], [](float p, float q) { return fminf(p, q); });
     }
     // Where too many are equal to the bound (masked words), those above it are all there are, and then the first of those
-    // equal to it. So it is at -inf from the start: fewer than asked for are above that.
-    bool above = bound == -INFINITY && s - s == 0.f;
+    // equal to it. So it is at -inf from the start: fewer lanes than are asked for have any word above that.
+    bool searched = W == 1;  // one wave's bound is the `top`-th largest of all
+    bool above = searched && bound == -INFINITY && s - s == 0.f;
     const auto passes = [&](float e) { return above ? e > bound : !(e < bound); };
     auto collect = [&](float e, int i) {
       if (passes(e)) {
@@ -218,41 +226,84 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
         if (at < kList) list[at] = key_of(e, base + i);
       }
     };
-    int slot = INT_MAX;
-    if (passes(mx)) {
-      slot = atomicAdd(&lanes, 1);
-      if (odd >= 0) collect(x0, odd);
-    }
-    __syncthreads();
-    const int held = lanes;
-    for (int from = 0; from < held; from += kLanes) {
-      if (slot >= from && slot < from + kLanes) {
-        owner[slot - from] = static_cast<uint16_t>(tid);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
+    int found = kList + 1;
+    if (searched || bound > -INFINITY) {
+      int slot = INT_MAX;
+      if (passes(mx)) {
+        slot = atomicAdd(&lanes, 1);
+        if (odd >= 0) collect(x0, odd);
       }
       __syncthreads();
-      for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
-        const int at = (i % V) * THREADS + owner[i / V];
-        if (at < vecs) {
-          float e[kE];
-          F::unpack(stash[i], e);
+      const int held = lanes;
+      const bool low = !searched && held > 2 * kLanes;
+      for (int from = 0; !low && from < held; from += kLanes) {
+        if (slot >= from && slot < from + kLanes) {
+          owner[slot - from] = static_cast<uint16_t>(tid);
 #pragma unroll
-          for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
+          for (int v = 0; v < V; ++v)
+            if (v * THREADS + tid < vecs) stash[(slot - from) * V + v] = d[v];
         }
+        __syncthreads();
+        for (int i = tid; i < min(held - from, kLanes) * V; i += THREADS) {
+          const int at = (i % V) * THREADS + owner[i / V];
+          if (at < vecs) {
+            float e[kE];
+            F::unpack(stash[i], e);
+#pragma unroll
+            for (int j = 0; j < kE; ++j) collect(e[j], head + at * kE + j);
+          }
+        }
+        __syncthreads();
+        if (count > kList) break;
       }
       __syncthreads();
-      if (count > kList) break;
+      if (!low) found = count;
     }
-    __syncthreads();
-    int found = count;
-    if (found > kList && !above && bound > -INFINITY) {
-      above = true;
+    while (found > (searched ? kList : kMany)) {
+      if (!searched) {
+        // The `top`-th largest of all lanes' maxima, or a value that a few more reach, four bits at a time: lane t of each
+        // wave counts its lanes that reach the number with t there.
+        int* const counts = reinterpret_cast<int*>(stash);  // two rounds' [wave][16]
+        const uint32_t mine = ordered(mx);
+        uint32_t least = 0;
+        for (int shift = 28; shift >= 0; shift -= 4) {
+          int* const of = counts + (shift & 4) * (4 * W);
+          int reach = 0;
+#pragma unroll 5
+          for (uint32_t t = 1; t < 16; ++t) {
+            const int c = __popcll(__ballot(mine >= (least | t << shift)));
+            reach = lane == static_cast<int>(t) ? c : reach;
+          }
+          if (lane < 16) of[16 * wave + lane] = reach;
+          __syncthreads();
+          reach = 0;
+#pragma unroll
+          for (int w = 0; w < W; ++w) reach += of[16 * w + (lane & 15)];
+          const int digit = __popcll(__ballot(lane > 0 && lane < 16 && reach >= a.top));  // fewer reach more
+          least |= static_cast<uint32_t>(digit) << shift;
+          if (digit > 0 && __builtin_amdgcn_readlane(reach, digit) <= a.top + W) break;
+        }
+        bound = value_of(least);
+        searched = true;
+        above = bound == -INFINITY && s - s == 0.f;
+      } else if (!above && bound > -INFINITY) {
+        above = true;
+      } else {
+        break;
+      }
+      // once more from memory: held until here, the row's registers would spill
+      constexpr int kLoads = 8;
       __syncthreads();
       if (tid == 0) count = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += THREADS) collect(F::load(x, i), i);
+      for (int i0 = tid; i0 < n; i0 += kLoads * THREADS) {
+        float e[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) e[u] = F::load(x, min(i0 + u * THREADS, n - 1));
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+          if (i0 + u * THREADS < n) collect(e[u], i0 + u * THREADS);
+      }
       __syncthreads();
       found = count;
     }
