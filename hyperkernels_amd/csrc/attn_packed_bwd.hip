@@ -19,7 +19,8 @@
 //
 // Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 31, dk and dv 43 us; sequences of 2048, 1001 and
 // 333, 16 heads on 4 of 128, fp16: 53, and 85 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
-// need them) at two to three waves a SIMD; one kernel for both that hands ds over took as long (7.6 for delta, then 84).
+// need them) at two to three waves a SIMD. Both in one launch, every other workgroup a tile of either, took as long (7.6 for delta,
+// then 84). Five products, with dS handed from one to the other, have not been tried.
 #include "attn_packed.h"
 
 namespace hk {
@@ -341,22 +342,28 @@ __global__ __launch_bounds__(DkvShape<D>::kThreads, D == 64 ? 3 : 2) void attn_p
   float HK_LDS* const norms = (float HK_LDS*)(lds + S::kNorms);
   {
     // columns behind the head's last element are zero: those of Q and dO are copies of others
-    for (int i = threadIdx.x; i < S::kKeys * kChunks; i += S::kThreads) {
-      const int r = i / kChunks, ch = i % kChunks;
+    constexpr int kLoads = S::kKeys * kChunks / S::kThreads;
+    u32x4_t x[kLoads] = {}, y[kLoads] = {};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (threadIdx.x + i * S::kThreads) / kChunks, ch = threadIdx.x % kChunks;
       const int64_t tok = q.k0 + min(k0 + r, q.mk - 1);
-      u32x4_t x = {}, y = {};
       if (8 * ch < a.d) {
-        x = *reinterpret_cast<const u32x4_t*>(a.k.p + tok * a.k.m + kh * a.k.h + 16 * ch);
-        y = *reinterpret_cast<const u32x4_t*>(a.v.p + tok * a.v.m + kh * a.v.h + 16 * ch);
+        x[i] = *reinterpret_cast<const u32x4_t*>(a.k.p + tok * a.k.m + kh * a.k.h + 16 * ch);
+        y[i] = *reinterpret_cast<const u32x4_t*>(a.v.p + tok * a.v.m + kh * a.v.h + 16 * ch);
       }
-      *reinterpret_cast<u32x4_t HK_LDS*>(lds + at_chunk<D>(r, ch)) = x;
-      *reinterpret_cast<u32x4_t HK_LDS*>(lds + S::kHeld / 2 + at_chunk<D>(r, ch)) = y;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (threadIdx.x + i * S::kThreads) / kChunks, ch = threadIdx.x % kChunks;
+      *reinterpret_cast<u32x4_t HK_LDS*>(lds + at_chunk<D>(r, ch)) = x[i];
+      *reinterpret_cast<u32x4_t HK_LDS*>(lds + S::kHeld / 2 + at_chunk<D>(r, ch)) = y[i];
       if constexpr (T::kNarrow) {
         // sum |v| of the key: kChunks lanes have it
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const f32x2_t w = T::unpack(y[e]);
+          const f32x2_t w = T::unpack(y[i][e]);
           sum += fabsf(w[0]) + fabsf(w[1]);
         }
         sum += detail::dpp<detail::kDppXor1>(sum);
