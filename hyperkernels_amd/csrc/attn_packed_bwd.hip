@@ -7,18 +7,20 @@
 // dP^T = V dO^T with a row a lane, dS^T the operand of dQ^T += K^T dS^T as it lies) and leaves delta and lse for
 // attn_packed_dkv, which goes by keys: S = Q K^T and dP = dO V^T with a key a lane, P and dS the operands of
 // dV^T += dO^T P and dK^T += Q^T dS as they lie. The rows of a group's heads are one loop there, which sums them.
-// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. That makes the norm of the
-// gradients' error sqrt(2) of what rounding them leaves. delta from the o that was rounded adds p (dout . o's error) to
-// dS, 2 / (n - 1) of that rounding's square over n equal keys: rows of up to 128 keys, where it would be most of the error,
-// take delta = sum p dp instead, from one more pass over the first one or two tiles of keys in workgroups that have such rows. dS is as small as P and
-// dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under fp16's normal range: there it is formed for dout
-// times a power of two, of its row in attn_packed_dq (an addend of the exponent), of the rows so far in attn_packed_dkv,
-// where dK is moved to the next when it grows. Large values could take such a dS past fp16's end: attn_packed_dq looks at each
-// block's largest and moves the row's power, and dQ with it (4096 tokens, 16 heads of 128: 126 -> 131 us; a second pass over such tiles
-// instead, for want of registers, 139); attn_packed_dkv has the sum of a key's |v|, which bounds its dP before the loop. There P, as small as one over a row's keys, is held for a sum of 2^12.
+// P and dS are rounded to 16 bits for the products, as the inputs are; everything else is fp32. That makes the norm of
+// the gradients' error sqrt(2) of what rounding them leaves. delta from the o that was rounded adds p (dout . o's
+// error) to dS, 2 / (n - 1) of that rounding's square over n equal keys: rows of up to 128 keys, where it would be most
+// of the error, take delta = sum p dp instead, from one more pass over the first one or two tiles of keys in workgroups
+// that have such rows. dS is as small as P and dout together (1e-7 for a dout of 1e-3 over 1000 keys), which is under
+// fp16's normal range: there it is formed for dout times a power of two, of its row in attn_packed_dq (an addend of the
+// exponent), of the rows so far in attn_packed_dkv, where dK is moved to the next when it grows. Large values could
+// take such a dS past fp16's end: attn_packed_dq looks at each block's largest and moves the row's power, and dQ with
+// it (4096 tokens, 16 heads of 128: 126 -> 131 us; a second pass over such tiles instead, for want of registers, 139);
+// attn_packed_dkv has the sum of a key's |v|, which bounds its dP before the loop. There P, as small as one over the
+// number of a row's keys, is held times 2^12.
 //
-// Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 31, dk and dv 43 us; sequences of 2048, 1001 and
-// 333, 16 heads on 4 of 128, fp16: 53, and 85 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
+// Measured, causal: 13 documents, 8192 tokens, 12 heads of 64, bf16: dq 32, dk and dv 42 us; sequences of 2048, 1001 and
+// 333, 16 heads on 4 of 128, fp16: 54, and 86 + 17 to join. Bound by each workgroup's chain (products, exponentials, products that
 // need them) at two to three waves a SIMD. Both in one launch, every other workgroup a tile of either, took as long (7.6 for delta,
 // then 84). Five products, with dS handed from one to the other, have not been tried.
 #include "attn_packed.h"

@@ -707,7 +707,8 @@ HK_API hipError_t hk_qk_norm_rope_backward(const hk_qk_norm_rope_params* params,
  * cu_k[s + 1] - 1 (int32 in device memory, num_seqs + 1 each, rising; cu_q itself may be cu_k). Query i of m sees
  * key j of n where is_causal is not set or j <= i + n - m: the last query is level with the last key, so a prompt is
  * m == n, a chunk of one or a new token over a cache m < n, and the first m - n queries see nothing where m > n.
- * Query head h reads key head h / (q_heads / k_heads).
+ * Query head h reads key head h / (q_heads / k_heads). A cache with room behind each sequence has a sequence without
+ * queries between any two, whose keys are the room (dk and dv are 0 there).
  *   forward   o = softmax(scale q k^T) v,  lse = the log of the sum of exp(scale q k^T)  (0 and -inf without a key)
  *   backward  from dout, the gradient of o, and the forward's o and lse: dq, dk, dv (written)
  * q, o, dout, dq are [q_tokens, q_heads, head_dim], k, v, dk, dv [k_tokens, k_heads, head_dim], all of the call's type
