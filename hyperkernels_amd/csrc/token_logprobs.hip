@@ -25,7 +25,7 @@
 // Measured, rows of 50257: 4096 of bf16 with 5 alternatives 78 us (5.3 TB/s, where the bound is the memory); 8192 of bf16
 // without 149 (5.5), their gradient 269 (read and write at 6.1, the copy's rate); 16 of fp32 with 20 alternatives 7.1 + 5.1 us, which is
 // latency: load, maximum, sums, selection one after the other. With waves that have no words: 16 rows of bf16, 20 alternatives,
-// 14.1 us (a pass for each: 40); 600 rows of 3000, 13.0 (52); 300 rows, 5 alternatives, an eighth of the words masked in a wave's
+// 14.4 us (a pass for each: 40); 600 rows of 3000, 13.4 (52); 300 rows, 5 alternatives, an eighth of the words masked in a wave's
 // share of each 4096, 27 (162).
 #include <limits.h>
 
@@ -43,7 +43,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 64;
 constexpr int kMaxPieces = 64;
 constexpr int kList = 1024;  // candidates in LDS
-constexpr int kMany = 384;  // candidates that take longer to rank than a better bound does to find
+constexpr int kMany = 384;  // candidates that take longer to rank than fewer do to find
 constexpr int kLanes = 128;  // lanes whose vectors LDS holds
 constexpr int kMostVecs = 14;  // 16-byte vectors a lane: with them 80 registers, three workgroups a CU
 
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
   __shared__ uint64_t list[TOP ? kList : 1];
   __shared__ uint4 stash[TOP ? kLanes * V : 1];
   __shared__ uint16_t owner[TOP ? kLanes : 1];
-  __shared__ int count, lanes;
+  __shared__ int count, lanes, over;
 
   const int64_t item = blockIdx.x + a.first * a.pieces, row = a.pieces == 1 ? item : item / a.pieces;
   const int pc = static_cast<int>(item - row * a.pieces);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
   each([&](float e, int) { mx = fmaxf(mx, e); });
 
   float m = wave_max(mx);
-  if (TOP && tid == 0) count = lanes = 0;
+  if (TOP && tid == 0) count = lanes = over = 0;
   if (W > 1) {
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
@@ -217,8 +217,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
     }
     // Where too many are equal to the bound (masked words), those above it are all there are, and then the first of those
     // equal to it. So it is at -inf from the start: fewer lanes than are asked for have any word above that.
-    bool searched = W == 1;  // one wave's bound is the `top`-th largest of all
-    bool above = searched && bound == -INFINITY && s - s == 0.f;
+    bool above = bound == -INFINITY && s - s == 0.f;
     const auto passes = [&](float e) { return above ? e > bound : !(e < bound); };
     auto collect = [&](float e, int i) {
       if (passes(e)) {
@@ -226,17 +225,19 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
         if (at < kList) list[at] = key_of(e, base + i);
       }
     };
+    int slot = INT_MAX;
+    if (mx > bound) atomicAdd(&over, 1);
+    if (passes(mx)) {
+      slot = atomicAdd(&lanes, 1);
+      if (odd >= 0) collect(x0, odd);
+    }
+    __syncthreads();
+    // Where fewer lanes are over it, the bound is the `top`-th largest of all lanes' maxima already, as that of one wave is.
+    bool searched = W == 1 || over < a.top;
+    const int held = lanes;
     int found = kList + 1;
-    if (searched || bound > -INFINITY) {
-      int slot = INT_MAX;
-      if (passes(mx)) {
-        slot = atomicAdd(&lanes, 1);
-        if (odd >= 0) collect(x0, odd);
-      }
-      __syncthreads();
-      const int held = lanes;
-      const bool low = !searched && held > 2 * kLanes;
-      for (int from = 0; !low && from < held; from += kLanes) {
+    if (held <= 2 * kLanes) {  // of more there is a better bound, or too many are equal to it
+      for (int from = 0; from < held; from += kLanes) {
         if (slot >= from && slot < from + kLanes) {
           owner[slot - from] = static_cast<uint16_t>(tid);
 #pragma unroll
@@ -257,12 +258,12 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 2 : 6) void logprobs_kerne
         if (count > kList) break;
       }
       __syncthreads();
-      if (!low) found = count;
+      found = count;
     }
-    while (found > (searched ? kList : kMany)) {
+    while (found > kMany) {
       if (!searched) {
-        // The `top`-th largest of all lanes' maxima, or a value that a few more reach, four bits at a time: lane t of each
-        // wave counts its lanes that reach the number with t there.
+        // The `top`-th largest, or a value that a few more reach, four bits at a time: lane t of each wave counts its
+        // lanes that reach the number with t there.
         int* const counts = reinterpret_cast<int*>(stash);  // two rounds' [wave][16]
         const uint32_t mine = ordered(mx);
         uint32_t least = 0;
