@@ -70,3 +70,24 @@ def test_flat_rows_over_many_keys(hk, n, d, causal):
     off = (dv.double()[:, 0] - want).abs()
     tol = (2 * 2.0 ** -11 * 1.01 + n / 4096 * 2.0 ** -24 + 2.0 ** -18) * want + 2.0 ** -25
     assert bool((off <= tol).all()), float((off / want).max())
+
+
+@pytest.mark.parametrize("H,Hk,d", [(4, 2, 64), (4, 4, 128)])
+def test_not_finite_stays_in_its_sequence(hk, H, Hk, d):
+    lens = [65, 130, 40]
+    for bad in (float("nan"), float("inf")):
+        for where in range(4):
+            x = make(lens, lens, H, Hk, d, F16)
+            want = reference(*x[:3], lens, lens, True, d ** -0.5, x[3])
+            x[where][100, 1, 3] = bad
+            q, k, v, do = x
+            cq = cu_of(lens)
+            o, lse = hk.attn_packed_forward(q, k, v, cq)
+            got = dict(zip(("o", "lse", "dq", "dk", "dv"),
+                           (o, lse.t(), *hk.attn_packed_backward(do, q, k, v, o, lse, cq))))
+            want["lse"] = [t.t() for t in want["lse"]]
+            for s in (slice(0, 65), slice(195, 235)):
+                check({n: t[s] for n, t in got.items()}, {n: [t[s] for t in w] for n, w in want.items()})
+            # the gradient of the query that it is in, or that sees the key (through its score, its dP or its delta)
+            reader = 1 if where in (0, 3) else H // Hk  # the first query head of key head 1
+            assert not torch.isfinite(got["dq"][100, reader]).all()
